@@ -196,6 +196,66 @@ int ojx_linattn_prep(const void* proj, const int32_t* hist, const int32_t* rep_p
                      int32_t KD, int32_t VD, int32_t HV, int32_t HK, int32_t HD, int32_t rep_qk, void* q, void* k,
                      void* v, float* g, void* beta, ojx_stream_t stream);
 
+/* Paged key / value cache, written and read by token slots. A cache is kc, vc [pages, HKV, page, D]; fmt says how it
+ * holds values: OJX_KV_BF16 (16-bit patterns, ks and vs NULL) or OJX_KV_E4M3 (OCP e4m3 bytes and one fp32 scale for each
+ * token and head, ks, vs [pages, HKV, page]; a value is byte * scale). slots int64 [N]: token n's place, page index * page
+ * + offset; a slot outside [0, pages * page) is skipped by the write and read back as zeros. D = 128 or 256, page a
+ * multiple of 16, at most 1024.
+ * The write quantises: scale = the smallest power of two 2^e, e >= -126, with max |x| / 2^e <= 448 over the row's finite
+ * values (1 for a row of zeros); stored = e4m3(x / scale), nearest, ties to even; NaN for a value that is not finite. It
+ * touches nothing but the slots named. Two tokens with the same slot leave either's values there, or a mix of both.
+ * k, v bf16 [HKV, N, D], as ojx_fullattn_prep writes them. */
+enum { OJX_KV_BF16 = 0, OJX_KV_E4M3 = 1 };
+int ojx_kv_cache_write(const void* k, const void* v, const int64_t* slots, int64_t N, int32_t HKV, int32_t D,
+                       int32_t fmt, void* kc, void* vc, float* ks, float* vs, int64_t pages, int32_t page,
+                       ojx_stream_t stream);
+int ojx_kv_cache_read(const void* kc, const void* vc, const float* ks, const float* vs, const int64_t* slots, int64_t N,
+                      int32_t HKV, int32_t D, int32_t fmt, void* k, void* v, int64_t pages, int32_t page,
+                      ojx_stream_t stream);
+
+/* Attention of drafted tokens over a paged cache: the full-attention core of a decoding step, with one drafted token, a
+ * line of them or a tree. Sequence b has the query rows q_ptr[b] .. q_ptr[b+1] - 1 (int32 [B + 1], non-decreasing; n_b =
+ * their count, 0 allowed) and ctx[b] tokens before them (int32 [B]). Its cache position t lies in page table[b][t / page]
+ * (int32 [B, max_pages]) at place t % page; drafted token j is at position ctx[b] + j, written there before. Row i of the
+ * sequence sees the positions below ctx[b], and drafted token j where bit j of its bits is set (int64 [N, words], bit j =
+ * bit j % 64 of word j / 64; tokens beyond the words are not seen). bits NULL: it sees drafted tokens 0 .. i.
+ * Positions from ctx[b] + n_b or max_pages * page on, and pages whose table entry is outside [0, pages), are not seen,
+ * whatever lies there. Query head h reads kv head h / (HQ / HKV).
+ *   out[n][h] = sum_t p_t v_t / sum_t p_t, p_t = exp(scale q . k_t), bf16 [N, HQ, D]; lse (may be NULL) = log sum_t p_t,
+ * fp32 [N, HQ]. A row that sees nothing, and a row of no sequence, gives zeros and -infinity.
+ * q bf16 [HQ, N, D] (ojx_fullattn_prep's qt). D = 128 or 256, HQ a multiple of HKV. workspace: ojx_tree_attn_workspace
+ * bytes of device memory, 16-byte aligned (0 = none needed); it depends on sizes only. */
+int64_t ojx_tree_attn_workspace(int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t max_pages,
+                                int32_t page);
+int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const int64_t* bits, int32_t words,
+                  const void* kc, const void* vc, const float* ks, const float* vs, int32_t fmt, const int32_t* table,
+                  int64_t max_pages, int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t pages,
+                  int32_t page, float scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                  ojx_stream_t stream);
+
+/* Linear attention with a decay for each head: the core of the linear-attention layers, on ojx_linattn_prep's outputs.
+ * A value head carries a state S [128 key dims][128 value dims], fp32; a token does
+ *   S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q
+ * (the gated delta rule), or with beta NULL u = v (plain decayed sums). q, k bf16 [R, HK, 128], v bf16 [R, HV, 128],
+ * g fp32 [R, HV] (-infinity clears the state), beta bf16 [R, HV], o bf16 [R, HV, 128]; value head h reads key head
+ * h / (HV / HK).
+ * ojx_linattn_prompt runs whole sequences: sequence s has rows seq_ptr[s] .. seq_ptr[s+1] - 1 (int32 [S + 1],
+ * non-decreasing; none allowed). It starts from state[src[s]] (state fp32 [slots, HV, 128, 128], src int32 [S]; src[s] < 0
+ * = zeros, src[s] >= slots = NaN; src NULL = s itself; state NULL = zeros for all) and leaves its last state in
+ * state_out[s] (fp32 [S, HV, 128, 128], not overlapping state). Rows of no sequence get zeros. workspace:
+ * ojx_linattn_prompt_workspace bytes of device memory, 16-byte aligned (0 = none needed); it depends on sizes only.
+ * ojx_linattn_step runs one token for each of R rows on state[slot[r]], updated in place (slot int32 [R]). A row whose
+ * slot is negative is idle: it gets zeros. A slot of state_slots or more, or one that an earlier row names too, gives NaN
+ * for that row and leaves the states alone. */
+int64_t ojx_linattn_prompt_workspace(int64_t R, int64_t S, int32_t HV, int32_t HK, int32_t delta);
+int ojx_linattn_prompt(const void* q, const void* k, const void* v, const float* g, const void* beta,
+                       const int32_t* seq_ptr, const float* state, const int32_t* src, int64_t state_slots, int64_t R,
+                       int64_t S, int32_t HV, int32_t HK, float scale, void* o, float* state_out, void* workspace,
+                       int64_t workspace_bytes, ojx_stream_t stream);
+int ojx_linattn_step(const void* q, const void* k, const void* v, const float* g, const void* beta, float* state,
+                     const int32_t* slot, int64_t state_slots, int64_t R, int32_t HV, int32_t HK, float scale, void* o,
+                     ojx_stream_t stream);
+
 /* Bytes of the static device scratch behind ojx_gemm_residual_rmsnorm_noalloc (one array per GPU). */
 #define OJX_NOALLOC_SCRATCH_BYTES (32LL << 20)
 

@@ -58,6 +58,15 @@ EXPORTS = {
                                                   _i32, _i32, _i32, _f32, _p]),
     "ojx_linattn_prep": (ctypes.c_int, [_p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32,
                                         _i32, _p, _p, _p, _p, _p, _p]),
+    "ojx_kv_cache_write": (ctypes.c_int, [_p, _p, _p, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _i64, _i32, _p]),
+    "ojx_kv_cache_read": (ctypes.c_int, [_p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _p, _i64, _i32, _p]),
+    "ojx_tree_attn_workspace": (ctypes.c_int64, [_i64, _i32, _i32, _i32, _i32, _i64, _i32]),
+    "ojx_tree_attn": (ctypes.c_int, [_p, _p, _p, _p, _i32, _p, _p, _p, _p, _i32, _p, _i64, _i64, _i32, _i32, _i32, _i32,
+                                     _i64, _i32, _f32, _p, _p, _p, _i64, _p]),
+    "ojx_linattn_prompt_workspace": (ctypes.c_int64, [_i64, _i64, _i32, _i32, _i32]),
+    "ojx_linattn_prompt": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _f32, _p, _p, _p,
+                                          _i64, _p]),
+    "ojx_linattn_step": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _f32, _p, _p]),
     "ojx_add_rmsnorm": (ctypes.c_int, [_p, _p, _p, _p, _f32, _p, _p, _i64, _i64, _p]),
     "ojx_add_rmsnorm_sk": (ctypes.c_int, [_p, _p, _i32, _p, _p, _f32, _p, _p, _i64, _i64, _p]),
     "ojx_silu_mul": (ctypes.c_int, [_p, _p, _i64, _i64, _p]),
@@ -67,6 +76,7 @@ EXPORTS = {
     "ojx_pack_gate_up": (ctypes.c_int, [_p, _p, _p, _i64, _i64, _p]),
 }
 
+KV_BF16, KV_E4M3 = 0, 1
 KIND_PLAIN, KIND_SILU_MUL, KIND_RESIDUAL, KIND_PACKED = 0, 1, 2, 4
 
 _lib = None

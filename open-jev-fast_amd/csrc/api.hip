@@ -854,6 +854,170 @@ int ojx_linattn_prep(const void* proj, const int32_t* hist, const int32_t* rep_p
                                             static_cast<hipStream_t>(stream)), "linear-attention prep launch");
 }
 
+namespace {
+
+// Sizes of a paged cache: the kernels index its rows (tokens of a head) and values with 64 bits, a page's rows with 32.
+int check_cache(int32_t HKV, int32_t D, int32_t fmt, int64_t pages, int32_t page, const void* kc, const void* vc,
+                const float* ks, const float* vs) {
+  if (D != 128 && D != 256) return fail(OJX_ERR_SHAPE, "cache heads are of 128 or 256 (D=%d)", D);
+  if (HKV < 1 || HKV > 1024) return fail(OJX_ERR_SHAPE, "bad head count HKV=%d (1 to 1024)", HKV);
+  if (fmt != OJX_KV_BF16 && fmt != OJX_KV_E4M3) return fail(OJX_ERR_ARG, "unknown cache format %d", fmt);
+  if (page < 16 || page % 16 != 0 || page > 1024)
+    return fail(OJX_ERR_SHAPE, "page=%d must be a multiple of 16, at most 1024", page);
+  if (pages < 0 || pages >= (1LL << 31)) return fail(OJX_ERR_SHAPE, "bad page count %lld", (long long)pages);
+  if (pages > 0 && (kc == nullptr || vc == nullptr)) return fail(OJX_ERR_ARG, "null cache");
+  if (!aligned(kc, 16) || !aligned(vc, 16)) return fail(OJX_ERR_ARG, "the cache must be 16-byte aligned");
+  if (fmt == OJX_KV_E4M3 && pages > 0 && (ks == nullptr || vs == nullptr))
+    return fail(OJX_ERR_ARG, "an e4m3 cache needs its scales");
+  if (fmt == OJX_KV_E4M3 && (!aligned(ks, 16) || !aligned(vs, 16)))
+    return fail(OJX_ERR_ARG, "cache scales must be 16-byte aligned");
+  return OJX_OK;
+}
+
+int check_kv_tokens(const void* k, const void* v, const int64_t* slots, int64_t N) {
+  if (N < 0 || N >= (1LL << 31)) return fail(OJX_ERR_SHAPE, "bad token count N=%lld", (long long)N);
+  if (N == 0) return OJX_OK;
+  if (k == nullptr || v == nullptr || slots == nullptr) return fail(OJX_ERR_ARG, "null k, v or slots");
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 8))
+    return fail(OJX_ERR_ARG, "k and v must be 16-byte aligned, slots 8-byte");
+  return OJX_OK;
+}
+
+int check_tree(int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t max_pages, int32_t page) {
+  if (N < 0 || N >= (1LL << 31) || B < 0 || B > 65536)
+    return fail(OJX_ERR_SHAPE, "bad sizes N=%lld B=%d (B at most 65536)", (long long)N, B);
+  if (D != 128 && D != 256) return fail(OJX_ERR_SHAPE, "attention heads are of 128 or 256 (D=%d)", D);
+  if (HKV < 1 || HKV > 1024 || HQ < HKV || HQ % HKV != 0 || HQ / HKV > 64)
+    return fail(OJX_ERR_SHAPE, "HQ=%d must be a multiple of HKV=%d, at most 64 times it", HQ, HKV);
+  if (page < 16 || page % 16 != 0 || page > 1024)
+    return fail(OJX_ERR_SHAPE, "page=%d must be a multiple of 16, at most 1024", page);
+  if (max_pages < 0 || max_pages * page >= (1LL << 31))
+    return fail(OJX_ERR_SHAPE, "bad max_pages=%lld (at most 2^31 positions)", (long long)max_pages);
+  if (N * HQ >= (1LL << 24))
+    return fail(OJX_ERR_SHAPE, "N=%lld rows of %d heads: too many for one call", (long long)N, HQ);
+  return OJX_OK;
+}
+
+int check_linattn(const void* q, const void* k, const void* v, const float* g, const void* beta, int64_t R, int32_t HV,
+                  int32_t HK, const void* o) {
+  if (HK < 1 || HV < HK || HV % HK != 0 || HV > 1024)
+    return fail(OJX_ERR_SHAPE, "HV=%d must be a multiple of HK=%d, at most 1024", HV, HK);
+  if (R < 0 || R >= (1LL << 31)) return fail(OJX_ERR_SHAPE, "bad row count R=%lld", (long long)R);
+  if (R == 0) return OJX_OK;
+  if (q == nullptr || k == nullptr || v == nullptr || g == nullptr || o == nullptr)
+    return fail(OJX_ERR_ARG, "null q, k, v, g or o");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(o, 16) || !aligned(g, 4) || !aligned(beta, 2))
+    return fail(OJX_ERR_ARG, "q, k, v and o must be 16-byte aligned");
+  return OJX_OK;
+}
+
+}  // namespace
+
+int ojx_kv_cache_write(const void* k, const void* v, const int64_t* slots, int64_t N, int32_t HKV, int32_t D,
+                       int32_t fmt, void* kc, void* vc, float* ks, float* vs, int64_t pages, int32_t page,
+                       ojx_stream_t stream) {
+  OJX_TRY(check_cache(HKV, D, fmt, pages, page, kc, vc, ks, vs));
+  OJX_TRY(check_kv_tokens(k, v, slots, N));
+  if (N == 0 || pages == 0) return OJX_OK;
+  return hip_check(ojx::launch_kv_write(static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), slots, N, HKV,
+                                        D, fmt == OJX_KV_E4M3, kc, vc, ks, vs, pages * page, page,
+                                        static_cast<hipStream_t>(stream)), "cache write launch");
+}
+
+int ojx_kv_cache_read(const void* kc, const void* vc, const float* ks, const float* vs, const int64_t* slots, int64_t N,
+                      int32_t HKV, int32_t D, int32_t fmt, void* k, void* v, int64_t pages, int32_t page,
+                      ojx_stream_t stream) {
+  OJX_TRY(check_cache(HKV, D, fmt, pages, page, kc, vc, ks, vs));
+  OJX_TRY(check_kv_tokens(k, v, slots, N));
+  if (N == 0) return OJX_OK;
+  return hip_check(ojx::launch_kv_read(kc, vc, ks, vs, slots, N, HKV, D, fmt == OJX_KV_E4M3,
+                                       static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), pages * page, page,
+                                       static_cast<hipStream_t>(stream)), "cache read launch");
+}
+
+int64_t ojx_tree_attn_workspace(int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t max_pages,
+                                int32_t page) {
+  if (check_tree(N, B, HQ, HKV, D, max_pages, page) != OJX_OK) return -1;
+  return 0;
+}
+
+int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const int64_t* bits, int32_t words,
+                  const void* kc, const void* vc, const float* ks, const float* vs, int32_t fmt, const int32_t* table,
+                  int64_t max_pages, int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t pages,
+                  int32_t page, float scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                  ojx_stream_t stream) {
+  OJX_TRY(check_tree(N, B, HQ, HKV, D, max_pages, page));
+  OJX_TRY(check_cache(HKV, D, fmt, pages, page, kc, vc, ks, vs));
+  if (bits != nullptr && (words < 1 || words > (1 << 20))) return fail(OJX_ERR_SHAPE, "bad words=%d", words);
+  if (N == 0) return OJX_OK;
+  if (q == nullptr || out == nullptr || q_ptr == nullptr || (B > 0 && ctx == nullptr) ||
+      (B > 0 && max_pages > 0 && table == nullptr))
+    return fail(OJX_ERR_ARG, "null q, q_ptr, ctx, table or out");
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(q_ptr, 4) || !aligned(ctx, 4) || !aligned(table, 4) ||
+      !aligned(lse, 4) || !aligned(bits, 8))
+    return fail(OJX_ERR_ARG, "q and out must be 16-byte aligned, bits 8-byte");
+  const int64_t need = ojx_tree_attn_workspace(N, B, HQ, HKV, D, max_pages, page);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(OJX_ERR_WORKSPACE, "tree attention needs %lld bytes of 16-byte aligned workspace, got %lld",
+                (long long)need, (long long)workspace_bytes);
+  const ojx::TreeParams p{static_cast<const uint16_t*>(q), q_ptr, ctx, bits, bits != nullptr ? words : 0, kc, vc, ks, vs,
+                          table, max_pages, N, pages, B, HQ, HKV, page, scale, static_cast<uint16_t*>(out), lse};
+  return hip_check(ojx::launch_tree_attn(p, D, fmt == OJX_KV_E4M3, static_cast<hipStream_t>(stream)),
+                   "tree attention launch");
+}
+
+int64_t ojx_linattn_prompt_workspace(int64_t R, int64_t S, int32_t HV, int32_t HK, int32_t delta) {
+  (void)delta;
+  // a workgroup of 256 threads per sequence and head at most; a launch has fewer than 2^32 threads
+  if (HK < 1 || HV < HK || HV % HK != 0 || HV > 1024 || R < 0 || R >= (1LL << 31) || S < 0 ||
+      (S + 1) * HV >= (1LL << 24)) {
+    fail(OJX_ERR_SHAPE, "bad sizes R=%lld S=%lld HV=%d HK=%d", (long long)R, (long long)S, HV, HK);
+    return -1;
+  }
+  return 0;
+}
+
+int ojx_linattn_prompt(const void* q, const void* k, const void* v, const float* g, const void* beta,
+                       const int32_t* seq_ptr, const float* state, const int32_t* src, int64_t state_slots, int64_t R,
+                       int64_t S, int32_t HV, int32_t HK, float scale, void* o, float* state_out, void* workspace,
+                       int64_t workspace_bytes, ojx_stream_t stream) {
+  OJX_TRY(check_linattn(q, k, v, g, beta, R, HV, HK, o));
+  const int64_t need = ojx_linattn_prompt_workspace(R, S, HV, HK, beta != nullptr);
+  if (need < 0) return OJX_ERR_SHAPE;
+  if (state_slots < 0 || state_slots >= (1LL << 31))
+    return fail(OJX_ERR_SHAPE, "bad state_slots=%lld", (long long)state_slots);
+  if (R == 0 && S == 0) return OJX_OK;
+  if (seq_ptr == nullptr || (S > 0 && state_out == nullptr)) return fail(OJX_ERR_ARG, "null seq_ptr or state_out");
+  if (!aligned(state, 16) || !aligned(state_out, 16) || !aligned(seq_ptr, 4) || !aligned(src, 4))
+    return fail(OJX_ERR_ARG, "states must be 16-byte aligned");
+  if (state != nullptr && src == nullptr && state_slots < S)
+    return fail(OJX_ERR_SHAPE, "%lld sequences and %lld states", (long long)S, (long long)state_slots);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(OJX_ERR_WORKSPACE, "linear attention needs %lld bytes of 16-byte aligned workspace, got %lld",
+                (long long)need, (long long)workspace_bytes);
+  const ojx::LinParams p{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
+                         static_cast<const uint16_t*>(v), g, static_cast<const uint16_t*>(beta), seq_ptr, state, src,
+                         state_out, static_cast<uint16_t*>(o), R, S, state_slots, HV, HK, scale};
+  return hip_check(ojx::launch_linattn_prompt(p, static_cast<hipStream_t>(stream)), "linear attention launch");
+}
+
+int ojx_linattn_step(const void* q, const void* k, const void* v, const float* g, const void* beta, float* state,
+                     const int32_t* slot, int64_t state_slots, int64_t R, int32_t HV, int32_t HK, float scale, void* o,
+                     ojx_stream_t stream) {
+  OJX_TRY(check_linattn(q, k, v, g, beta, R, HV, HK, o));
+  if (state_slots < 0 || state_slots >= (1LL << 31))
+    return fail(OJX_ERR_SHAPE, "bad state_slots=%lld", (long long)state_slots);
+  if (R * HV >= (1LL << 24)) return fail(OJX_ERR_SHAPE, "R=%lld rows of %d heads: too many for one step", (long long)R, HV);
+  if (R == 0) return OJX_OK;
+  if (slot == nullptr || (state == nullptr && state_slots > 0)) return fail(OJX_ERR_ARG, "null state or slot");
+  if (!aligned(state, 16) || !aligned(slot, 4)) return fail(OJX_ERR_ARG, "states must be 16-byte aligned");
+  const ojx::LinParams p{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
+                         static_cast<const uint16_t*>(v), g, static_cast<const uint16_t*>(beta), nullptr, nullptr,
+                         nullptr, nullptr, static_cast<uint16_t*>(o), R, 0, state_slots, HV, HK, scale};
+  return hip_check(ojx::launch_linattn_step(p, state, slot, static_cast<hipStream_t>(stream)),
+                   "linear attention step launch");
+}
+
 int ojx_gemm_residual_rmsnorm_noalloc(const void* x, const void* w, const void* residual, const float* w1,
                                       const int32_t* rowmask, float eps, void* h_out, void* hn_out, int64_t M,
                                       int64_t N, int64_t K, const ojx_cfg* cfg, ojx_stream_t stream) {

@@ -190,4 +190,44 @@ hipError_t launch_linattn_prep(const uint16_t* proj, const int32_t* hist, const 
 hipError_t launch_pack_weight(const uint16_t* w, uint16_t* wp, int64_t N, int64_t K, hipStream_t st);
 hipError_t launch_unsplit_weight(const uint16_t* wt, uint16_t* w, int64_t K, int64_t N, hipStream_t st);
 
+
+// Paged key / value cache [pages, HKV, page, D] (kvcache.hip); rows = pages * page.
+hipError_t launch_kv_write(const uint16_t* k, const uint16_t* v, const int64_t* slots, int64_t N, int HKV, int D,
+                           bool fp8, void* kc, void* vc, float* ks, float* vs, int64_t rows, int page,
+                           hipStream_t st);
+hipError_t launch_kv_read(const void* kc, const void* vc, const float* ks, const float* vs, const int64_t* slots,
+                          int64_t N, int HKV, int D, bool fp8, uint16_t* k, uint16_t* v, int64_t rows, int page,
+                          hipStream_t st);
+
+// Attention of drafted tokens over a paged cache (tree_attn.hip).
+struct TreeParams {
+  const uint16_t* q;                      // [HQ, N, D]
+  const int32_t* q_ptr; const int32_t* ctx;  // [B + 1], [B]
+  const int64_t* bits; int64_t words;     // [N, words], or null: drafted tokens see their predecessors and themselves
+  const void* kc; const void* vc;         // [pages, HKV, page, D]
+  const float* ks; const float* vs;       // [pages, HKV, page] of an e4m3 cache
+  const int32_t* table; int64_t max_pages;  // [B, max_pages]
+  int64_t N, pages;
+  int B, HQ, HKV, page;
+  float scale;
+  uint16_t* out; float* lse;              // [N, HQ, D]; [N, HQ] or null
+};
+hipError_t launch_tree_attn(const TreeParams& p, int D, bool fp8, hipStream_t st);
+
+// Linear attention with a decay for each head (linattn.hip); heads of 128.
+struct LinParams {
+  const uint16_t* q; const uint16_t* k;   // [R, HK, 128]
+  const uint16_t* v;                      // [R, HV, 128]
+  const float* g; const uint16_t* beta;   // [R, HV]; beta null: no delta rule
+  const int32_t* seq_ptr;                 // [S + 1] (prompts)
+  const float* state; const int32_t* src; // [slots, HV, 128, 128] and [S], or null (prompts)
+  float* state_out;                       // [S, HV, 128, 128] (prompts)
+  uint16_t* o;                            // [R, HV, 128]
+  int64_t R, S, slots;
+  int HV, HK;
+  float scale;
+};
+hipError_t launch_linattn_step(const LinParams& p, float* state, const int32_t* slot, hipStream_t st);
+hipError_t launch_linattn_prompt(const LinParams& p, hipStream_t st);
+
 }  // namespace ojx

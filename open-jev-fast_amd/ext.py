@@ -467,3 +467,219 @@ def mm_fullattn_prep(x, w_qkv, qw1, kw1, cos, sin, HQ, HKV, D, eps, fused=False)
                                            _ptr(sin), _ptr(qt), _ptr(kt), _ptr(vt), _ptr(gate), M, K, HQ, HKV, D,
                                            cos.shape[1], float(eps), _stream()))
     return [qt.unsqueeze(0), kt.unsqueeze(0), vt.unsqueeze(0), gate]
+
+
+# ------------------------------------------------------------------------------------------------ attention cores
+def _one_device(*tensors):
+    """The launches go on the current device's stream: every tensor has to live there."""
+    cur = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != cur:
+            raise RuntimeError(f"all tensors must be on the current device cuda:{cur}, got {t.device}")
+
+
+def _scratch(n, like):
+    """Workspace of one call, from torch's allocator: ordered on the current stream, and in a graph capture part of the
+    graph's own memory, so that no two graphs or streams share it."""
+    return torch.empty(n, dtype=torch.uint8, device=like.device) if n > 0 else None
+
+
+def _heads_rows(t, name):
+    """(heads, rows, D) of a prep output, [heads, N, D] or with the leading batch axis of 1."""
+    _chk(t, name, torch.bfloat16)
+    if t.dim() == 4 and t.shape[0] == 1:
+        return t.shape[1:]
+    if t.dim() != 3:
+        raise RuntimeError(f"{name} must be [heads, N, D] or [1, heads, N, D], got {tuple(t.shape)}")
+    return t.shape
+
+
+def _chk_cache(kc, vc, ks, vs, HKV, D):
+    """(format, pages, page) of a paged cache."""
+    fmt = {torch.bfloat16: _lib.KV_BF16, torch.float8_e4m3fn: _lib.KV_E4M3}.get(kc.dtype)
+    if fmt is None:
+        raise RuntimeError(f"a cache is torch.bfloat16 or torch.float8_e4m3fn, got {kc.dtype}")
+    _chk(kc, "kc")
+    _chk(vc, "vc", kc.dtype)
+    if kc.dim() != 4 or kc.shape != vc.shape or kc.shape[1] != HKV or kc.shape[3] != D:
+        raise RuntimeError(f"kc {tuple(kc.shape)} and vc {tuple(vc.shape)} must both be [pages, HKV={HKV}, page, D={D}]")
+    if fmt == _lib.KV_E4M3:
+        _chk(ks, "ks", torch.float32)
+        _chk(vs, "vs", torch.float32)
+        if ks.shape != kc.shape[:3] or vs.shape != kc.shape[:3]:
+            raise RuntimeError(f"ks {tuple(ks.shape)} and vs {tuple(vs.shape)} must be {tuple(kc.shape[:3])}")
+    elif ks is not None or vs is not None:
+        raise RuntimeError("a bf16 cache has no scales")
+    return fmt, kc.shape[0], kc.shape[2]
+
+
+def kv_cache_write(k, v, slots, kc, vc, ks=None, vs=None):
+    """Writes N tokens' keys and values into a paged cache, in place. k, v bf16 [HKV, N, D] (fullattn_prep2's kt and vt,
+    with or without their batch axis); slots int64 [N], page index * page + place (outside the cache: not written); kc, vc
+    [pages, HKV, page, D], bf16, or float8_e4m3fn with the rows' scales ks, vs fp32 [pages, HKV, page]. The e4m3 form
+    stores x / scale with scale the smallest power of two that brings the row within +-448."""
+    HKV, N, D = _heads_rows(k, "k")
+    if tuple(_heads_rows(v, "v")) != (HKV, N, D):
+        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
+    fmt, pages, page = _chk_cache(kc, vc, ks, vs, HKV, D)
+    _chk(slots, "slots", torch.int64)
+    if slots.numel() != N:
+        raise RuntimeError(f"slots must have N={N} elements, got {slots.numel()}")
+    _one_device(k, v, slots, kc, vc, ks, vs)
+    check(lib().ojx_kv_cache_write(_ptr(k), _ptr(v), _ptr(slots), N, HKV, D, fmt, _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs),
+                                   pages, page, _stream()))
+
+
+def kv_cache_read(kc, vc, slots, ks=None, vs=None):
+    """(k, v) bf16 [HKV, N, D]: the tokens in slots int64 [N] of a paged cache (see kv_cache_write), zeros for a slot
+    outside it."""
+    if kc.dim() != 4:
+        raise RuntimeError(f"kc must be [pages, HKV, page, D], got {tuple(kc.shape)}")
+    HKV, D = kc.shape[1], kc.shape[3]
+    fmt, pages, page = _chk_cache(kc, vc, ks, vs, HKV, D)
+    _chk(slots, "slots", torch.int64)
+    N = slots.numel()
+    _one_device(slots, kc, vc, ks, vs)
+    k = slots.new_empty((HKV, N, D), dtype=torch.bfloat16)
+    v = torch.empty_like(k)
+    check(lib().ojx_kv_cache_read(_ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), _ptr(slots), N, HKV, D, fmt, _ptr(k), _ptr(v),
+                                  pages, page, _stream()))
+    return k, v
+
+
+def tree_bits(parents):
+    """The bits that tree_attn takes, int64 [N, words] on the CPU, for sequences of drafted tokens given by their parents:
+    parents[b][j] is the index within sequence b of token j's parent, smaller than j, or -1 for a token that follows the
+    context. A token sees its ancestors and itself."""
+    words = max([1] + [-(-len(p) // 64) for p in parents])
+    rows = []
+    for b, p in enumerate(parents):
+        seen = []
+        for j, parent in enumerate(p):
+            parent = int(parent)
+            if not -1 <= parent < j:
+                raise RuntimeError(f"parents[{b}][{j}] = {parent} must be -1 or the index of an earlier token")
+            seen.append((seen[parent] if parent >= 0 else 0) | 1 << j)
+        rows += seen
+    flat = [(x >> 64 * w) & ((1 << 64) - 1) for x in rows for w in range(words)]
+    return torch.tensor([x - (1 << 64) if x >> 63 else x for x in flat], dtype=torch.int64).reshape(len(rows), words)
+
+
+def tree_attn(q, kc, vc, table, ctx, q_ptr, bits=None, ks=None, vs=None, scale=None, want_lse=False):
+    """Attention of drafted tokens over a paged cache: out bf16 [N, HQ D], with want_lse (out, lse fp32 [N, HQ]).
+    q bf16 [HQ, N, D] (fullattn_prep2's qt, with or without its batch axis); the cache as in kv_cache_write; table int32
+    [B, max_pages], ctx int32 [B], q_ptr int32 [B + 1]. Sequence b's query rows are q_ptr[b] .. q_ptr[b+1] - 1, its
+    drafted tokens; drafted token j stands in the cache at position ctx[b] + j, written before this call. A row sees the
+    ctx[b] positions before the drafted tokens, and those drafted tokens whose bit is set in its bits int64 [N, words]
+    (tree_bits); with bits=None its predecessors and itself (a plain continuation, or a single token). A row that sees
+    nothing, or belongs to no sequence, gives zeros (lse -inf). scale defaults to D ** -0.5."""
+    HQ, N, D = _heads_rows(q, "q")
+    if kc.dim() != 4 or kc.shape[1] < 1 or HQ % kc.shape[1]:
+        raise RuntimeError(f"kc {tuple(kc.shape)} must be [pages, HKV, page, D] with HKV dividing HQ={HQ}")
+    HKV = kc.shape[1]
+    fmt, pages, page = _chk_cache(kc, vc, ks, vs, HKV, D)
+    for t, nm in ((table, "table"), (ctx, "ctx"), (q_ptr, "q_ptr")):
+        _chk(t, nm, torch.int32)
+    B = ctx.numel()
+    if table.dim() != 2 or table.shape[0] != B or q_ptr.numel() != B + 1:
+        raise RuntimeError(f"table {tuple(table.shape)} must be [B={B}, max_pages] and q_ptr [B + 1], got "
+                           f"{q_ptr.numel()}")
+    words = 0
+    if bits is not None:
+        _chk(bits, "bits", torch.int64)
+        if bits.dim() != 2 or bits.shape[0] != N or bits.shape[1] < 1:
+            raise RuntimeError(f"bits must be [N={N}, words], got {tuple(bits.shape)}")
+        words = bits.shape[1]
+    _one_device(q, kc, vc, ks, vs, table, ctx, q_ptr, bits)
+    out = q.new_empty((N, HQ * D))
+    lse = q.new_empty((N, HQ), dtype=torch.float32) if want_lse else None
+    MP = table.shape[1]
+    n = lib().ojx_tree_attn_workspace(N, B, HQ, HKV, D, MP, page)
+    if n < 0:
+        check(2)
+    ws = _scratch(n, q)
+    check(lib().ojx_tree_attn(_ptr(q), _ptr(q_ptr), _ptr(ctx), _ptr(bits), words, _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs),
+                              fmt, _ptr(table), MP, N, B, HQ, HKV, D, pages, page,
+                              float(D ** -0.5 if scale is None else scale), _ptr(out), _ptr(lse), _ptr(ws), n,
+                              _stream()))
+    return (out, lse) if want_lse else out
+
+
+def _chk_linattn(q, k, v, g, beta):
+    """(R, HV, HK) of the linear-attention operands (linattn_prep_dedup2's outputs)."""
+    _chk(q, "q", torch.bfloat16)
+    _chk(k, "k", torch.bfloat16)
+    _chk(v, "v", torch.bfloat16)
+    _chk(g, "g", torch.float32)
+    if q.dim() != 2 or q.shape != k.shape or q.shape[1] % 128 or q.shape[1] == 0:
+        raise RuntimeError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must both be [R, HK 128]")
+    R, HK = q.shape[0], q.shape[1] // 128
+    if g.dim() != 2 or g.shape[0] != R:
+        raise RuntimeError(f"g must be [R={R}, HV], got {tuple(g.shape)}")
+    HV = g.shape[1]
+    if tuple(v.shape) != (R, HV * 128) or HV % HK or HV == 0:
+        raise RuntimeError(f"v {tuple(v.shape)} must be [R={R}, HV 128] with HV={HV} a multiple of HK={HK}")
+    if beta is not None:
+        _chk(beta, "beta", torch.bfloat16)
+        if beta.shape != g.shape:
+            raise RuntimeError(f"beta {tuple(beta.shape)} must be [R, HV] = {tuple(g.shape)}")
+    return R, HV, HK
+
+
+def _chk_states(state, HV):
+    _chk(state, "state", torch.float32)
+    if state.dim() != 4 or tuple(state.shape[1:]) != (HV, 128, 128):
+        raise RuntimeError(f"state must be [slots, HV={HV}, 128, 128], got {tuple(state.shape)}")
+
+
+def linattn_prompt(q, k, v, g, beta, seq_ptr, state=None, src=None, scale=None):
+    """Linear attention with a decay for each head over whole sequences, on linattn_prep_dedup2's outputs:
+    (o bf16 [R, HV 128], states fp32 [S, HV, 128, 128]). q, k bf16 [R, HK 128], v bf16 [R, HV 128], g fp32 [R, HV] (the
+    decay's logarithm), beta bf16 [R, HV], or None for plain decayed sums without the delta rule. Sequence s is rows
+    seq_ptr[s] .. seq_ptr[s+1] - 1 (int32 [S + 1]; the path slots of the tree layout: seq_ptr = arange(0, R + 1, L2)).
+    It starts from state[src[s]] (state fp32 [slots, HV, 128, 128], src int32 [S], -1 = zeros; src=None: state[s];
+    state=None: zeros), so that paths can go on from a state that they share. scale defaults to 128 ** -0.5."""
+    R, HV, HK = _chk_linattn(q, k, v, g, beta)
+    _chk(seq_ptr, "seq_ptr", torch.int32)
+    S = seq_ptr.numel() - 1
+    if S < 0:
+        raise RuntimeError("seq_ptr must be [S + 1]")
+    slots = 0
+    if state is not None:
+        _chk_states(state, HV)
+        slots = state.shape[0]
+        if src is None and slots != S:
+            raise RuntimeError(f"without src there must be S={S} states, got {slots}")
+    if src is not None:
+        if state is None:
+            raise RuntimeError("src without state")
+        _chk(src, "src", torch.int32)
+        if src.numel() != S:
+            raise RuntimeError(f"src must have S={S} elements, got {src.numel()}")
+    _one_device(q, k, v, g, beta, seq_ptr, state, src)
+    o = torch.empty_like(v)
+    last = q.new_empty((S, HV, 128, 128), dtype=torch.float32)
+    n = lib().ojx_linattn_prompt_workspace(R, S, HV, HK, beta is not None)
+    if n < 0:
+        check(2)
+    ws = _scratch(n, q)
+    check(lib().ojx_linattn_prompt(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(seq_ptr), _ptr(state), _ptr(src),
+                                   slots, R, S, HV, HK, float(128 ** -0.5 if scale is None else scale), _ptr(o),
+                                   _ptr(last), _ptr(ws), n, _stream()))
+    return o, last
+
+
+def linattn_step(q, k, v, g, beta, state, slot, scale=None):
+    """linattn_prompt for single tokens: o bf16 [R, HV 128]; row r's token runs on state[slot[r]] (state fp32 [slots, HV,
+    128, 128], slot int32 [R]), which is updated in place. A negative slot is an idle row (zeros); a slot that is not in
+    state, or that an earlier row names too, gives NaN and no update. Operands as in linattn_prompt."""
+    R, HV, HK = _chk_linattn(q, k, v, g, beta)
+    _chk_states(state, HV)
+    _chk(slot, "slot", torch.int32)
+    if slot.numel() != R:
+        raise RuntimeError(f"slot must have R={R} elements, got {slot.numel()}")
+    _one_device(q, k, v, g, beta, state, slot)
+    o = torch.empty_like(v)
+    check(lib().ojx_linattn_step(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(slot), state.shape[0],
+                                 R, HV, HK, float(128 ** -0.5 if scale is None else scale), _ptr(o), _stream()))
+    return o
