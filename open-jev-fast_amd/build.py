@@ -28,6 +28,11 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
          f"-I{INCLUDE}", f"-I{CSRC}"]
 
 
+# Tree attention keeps outputs that both MFMA and VALU code update: with the products' results in ordinary registers (not
+# the accumulation ones) nothing is copied between the two files on every update, and nothing spills.
+FILE_FLAGS = {"tree_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
+
 def source_files():
     """Every file the library is compiled from: csrc/ (kernels, C-ABI, plan table) and include/ojx.h."""
     files = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC))
@@ -56,7 +61,7 @@ def build(verbose: bool = False) -> str:
     digest = source_digest()
     for s in SOURCES:
         obj = os.path.join(OBJDIR, s.replace(".hip", ".o"))
-        cmd = [HIPCC, *FLAGS, f'-DOJX_SRC_DIGEST="{digest}"', "-c", os.path.join(CSRC, s), "-o", obj]
+        cmd = [HIPCC, *FLAGS, *FILE_FLAGS.get(s, []), f'-DOJX_SRC_DIGEST="{digest}"', "-c", os.path.join(CSRC, s), "-o", obj]
         jobs.append((cmd, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
     errs = []
     for cmd, obj, pr in jobs:

@@ -938,7 +938,9 @@ int ojx_kv_cache_read(const void* kc, const void* vc, const float* ks, const flo
 int64_t ojx_tree_attn_workspace(int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t max_pages,
                                 int32_t page) {
   if (check_tree(N, B, HQ, HKV, D, max_pages, page) != OJX_OK) return -1;
-  return 0;
+  if (N == 0) return 0;
+  const ojx::TreePlan t = ojx::tree_plan(N, B, HQ, HKV, D, max_pages, page);
+  return t.splits > 1 ? N * HQ * t.splits * (D * 4 + 8) : 0;
 }
 
 int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const int64_t* bits, int32_t words,
@@ -960,9 +962,13 @@ int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(OJX_ERR_WORKSPACE, "tree attention needs %lld bytes of 16-byte aligned workspace, got %lld",
                 (long long)need, (long long)workspace_bytes);
+  const ojx::TreePlan t = ojx::tree_plan(N, B, HQ, HKV, D, max_pages, page);
+  float* const part = static_cast<float*>(workspace);
   const ojx::TreeParams p{static_cast<const uint16_t*>(q), q_ptr, ctx, bits, bits != nullptr ? words : 0, kc, vc, ks, vs,
-                          table, max_pages, N, pages, B, HQ, HKV, page, scale, static_cast<uint16_t*>(out), lse};
-  return hip_check(ojx::launch_tree_attn(p, D, fmt == OJX_KV_E4M3, static_cast<hipStream_t>(stream)),
+                          table, max_pages, N, pages, B, HQ, HKV, page, scale, static_cast<uint16_t*>(out), lse,
+                          (int)t.splits, (uint32_t)(((1ULL << 32) + page / 16 - 1) / (page / 16)), part,
+                          reinterpret_cast<float2*>(part + N * HQ * t.splits * D)};
+  return hip_check(ojx::launch_tree_attn(p, t, D, fmt == OJX_KV_E4M3, static_cast<hipStream_t>(stream)),
                    "tree attention launch");
 }
 

@@ -211,8 +211,17 @@ struct TreeParams {
   int B, HQ, HKV, page;
   float scale;
   uint16_t* out; float* lse;              // [N, HQ, D]; [N, HQ] or null
+  int splits;                             // parts of a sequence's positions
+  uint32_t tiles_inv;                     // 2^32 / (page / 16), rounded up; not used for pages of 16
+  float* part; float2* ml;                // [N, HQ, splits, D] sums, [N, HQ, splits] (maximum, base two; sum)
 };
-hipError_t launch_tree_attn(const TreeParams& p, int D, bool fp8, hipStream_t st);
+// Shape of a launch, from sizes alone: packed rows a workgroup takes, workgroups along the rows, parts of the positions.
+struct TreePlan {
+  int rows;
+  int64_t blocks, splits;
+};
+TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, int page);
+hipError_t launch_tree_attn(const TreeParams& p, const TreePlan& t, int D, bool fp8, hipStream_t st);
 
 // Linear attention with a decay for each head (linattn.hip); heads of 128.
 struct LinParams {

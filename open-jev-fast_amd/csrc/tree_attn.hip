@@ -5,91 +5,664 @@
 // below ctx[b] and those drafted tokens whose bit is set in its bits (without bits: its predecessors and itself).
 //   s_p = scale q . k_p,  m = max s_p,  out = sum exp(s_p - m) v_p / sum exp(s_p - m),  lse = m + log sum exp(s_p - m)
 // over the positions seen; a row that sees nothing gives zeros and lse = -inf.
+//
+// Work layout. The G = HQ / HKV query heads of a kv head read the same keys, so their rows (token, head) are packed: a
+// workgroup takes a block of 16 CT packed rows of one sequence and kv head and a part of the positions. Its four waves
+// take the part's units of 32 positions in turn and are independent until the end:
+//   * S^T = K Q^T on 16x16x32 MFMA: the K rows are the A operand, straight from the cache into registers (a lane's 16
+//     bytes are 8 bf16 or 16 e4m3 values of one key; the e4m3 form orders the contraction accordingly, for Q too), Q stays
+//     in registers. A lane then holds one row's scores of 4 positions of each 16.
+//   * the softmax runs per lane: the maximum needs two shuffles, the sum none until the end, and the reference maximum
+//     only moves when it has grown by 2^8 (the weights stay below 2^8, well inside fp32 and bf16), so that the outputs are
+//     rarely rescaled;
+//   * O^T += V^T P^T: P^T is the B operand as the lane holds it, with the contraction in the order 4 of the first 16
+//     positions, 4 of the second; V^T comes from the wave's own LDS rows by transposing reads (ds_read_b64_tr_b16: 16
+//     lanes get 4 x 16 elements column by column), rows padded by 32 bytes so that the reads spread over the banks.
+// The loads of the next unit, keys and values, go into the registers that the present unit has just left and arrive
+// behind its products. P is rounded to bf16 as every operand of these products is (half a step, 2^-8 of each weight); the
+// sum of the weights and the outputs are fp32.
+// Units in which a row may not see every position (drafted ones, the sequence's end, pages outside the cache) also mask,
+// take the values of places that nobody sees as zeros and, where a value is not finite, add position by position, so that
+// a NaN reaches the rows that see it and no other.
+// Where sequences and row blocks are few, the positions are split over more workgroups, whose sums a second launch joins.
 #include "ojx_internal.h"
+
+#include <algorithm>
 
 namespace ojx {
 
 namespace {
 
-template <bool FP8>
-__device__ __forceinline__ float cache_value(const void* c, const float* s, int64_t row, int D, int d) {
-  if (FP8) {
-    const uint8_t* p = static_cast<const uint8_t*>(c) + row * D + d;
-    return __builtin_amdgcn_cvt_f32_fp8(*p, 0) * s[row];
-  }
-  return bf2f(static_cast<const uint16_t*>(c)[row * D + d]);
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(4))) const int32_t* const_ints;  // read-only: scalar loads
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 8.f;  // the reference maximum follows when it is this far behind, base two
+
+__device__ __forceinline__ int64_t clamp_row(int64_t x, int64_t N) { return min(max(x, (int64_t)0), N); }
+
+// Sequence b's first row and row count, whatever its pointers hold.
+__device__ __forceinline__ void seq_rows(const TreeParams& p, int b, int& first, int& n) {
+  const int64_t x = clamp_row(p.q_ptr[b], p.N), y = max(clamp_row(p.q_ptr[b + 1], p.N), x);
+  first = (int)x;
+  n = (int)(y - x);
 }
 
-// One workgroup of four waves per (row, query head); wave w takes positions w, w + 4, ..; a lane holds D / 64 dims.
-template <int D, bool FP8>
-__global__ void __launch_bounds__(256) tree_attn_k(TreeParams p) {
-  constexpr int E = D / 64;
-  const int64_t n = blockIdx.x / p.HQ;
-  const int h = blockIdx.x - (int)(n * p.HQ), hk = h / (p.HQ / p.HKV);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t b = -1, first = 0, end = 0;
-  for (int i = 0; i < p.B; ++i) {
-    const int64_t x = min(max((int64_t)p.q_ptr[i], (int64_t)0), p.N), y = min(max((int64_t)p.q_ptr[i + 1], x), p.N);
-    if (n >= x && n < y) {
-      b = i;
-      first = x;
-      end = y;
+// The sequence of row block rb (blocks of R packed rows, sequence after sequence) and its place in it; false: none.
+__device__ __forceinline__ bool find_block(const TreeParams& p, int rb, int R, int& b, int& first, int& n, int& row0) {
+  const int lane = threadIdx.x & 63, G = p.HQ / p.HKV;
+  for (int base = 0; base < p.B; base += 64) {
+    int x = 0, c = 0;
+    if (base + lane < p.B) seq_rows(p, base + lane, x, c);
+    const int blocks = (c * G + R - 1) / R;
+    int s = blocks;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(s, o);
+      if (lane >= o) s += t;
+    }
+    const int total = __builtin_amdgcn_readlane(s, 63);
+    if (rb < total) {
+      const int j = __builtin_ctzll(__ballot(s > rb));
+      b = base + j;
+      first = __builtin_amdgcn_readlane(x, j);
+      n = __builtin_amdgcn_readlane(c, j);
+      row0 = (rb - __builtin_amdgcn_readlane(s - blocks, j)) * R;
+      return true;
+    }
+    rb -= total;
+  }
+  return false;
+}
+
+// Zeros (and lse -inf) for kv head hk's heads of the rows before the first sequence and behind the last.
+__device__ __forceinline__ void zero_rows(const TreeParams& p, int hk, int D) {
+  int64_t lo = p.B > 0 ? clamp_row(p.q_ptr[0], p.N) : p.N, hi = 0;
+  for (int i = threadIdx.x & 63; i <= p.B; i += 64) hi = max(hi, clamp_row(p.q_ptr[i], p.N));
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) hi = max(hi, (int64_t)__shfl_xor((int)hi, o));
+  hi = max(hi, lo);
+  const int G = p.HQ / p.HKV, per = G * D / 8;
+  const int64_t rows = lo + (p.N - hi);
+  for (int64_t t = threadIdx.x; t < rows * per; t += blockDim.x) {
+    const int64_t i = t / per, n = i < lo ? i : hi + (i - lo);
+    const int c = (int)(t - i * per);
+    *reinterpret_cast<uint4*>(p.out + (n * p.HQ + hk * G) * D + c * 8) = make_uint4(0u, 0u, 0u, 0u);
+    if (p.lse != nullptr && c < G) p.lse[n * p.HQ + hk * G + c] = -INFINITY;
+  }
+}
+
+__device__ __forceinline__ uint32_t cvt_fp8x2(int x, bool hi) {  // two e4m3 values as bf16: exact
+  const bf16x2 r = hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true)
+                      : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false);
+  return __builtin_bit_cast(uint32_t, r);
+}
+__device__ __forceinline__ uint4 cvt_fp8x8(uint32_t a, uint32_t b) {
+  return make_uint4(cvt_fp8x2(a, false), cvt_fp8x2(a, true), cvt_fp8x2(b, false), cvt_fp8x2(b, true));
+}
+__device__ __forceinline__ bool odd2(uint32_t x) {  // either bf16 of x is not finite
+  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+}
+
+// Positions p0 .. p0 + 31 of those that a row of drafted index i sees, as bits; w: its words.
+__device__ __forceinline__ uint32_t seen32(const TreeParams& p, const int64_t* w, int i, int64_t j0) {
+  if (j0 <= -32) return ~0u;
+  if (w == nullptr) {
+    const int64_t c = i - j0 + 1;
+    return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1;
+  }
+  if (j0 < 0) return ((uint32_t)w[0] << -j0) | ((1u << -j0) - 1);
+  const int64_t at = j0 >> 6;
+  const int sh = (int)(j0 & 63);
+  if (at >= p.words) return 0u;
+  uint64_t x = (uint64_t)w[at] >> sh;
+  if (sh > 32 && at + 1 < p.words) x |= (uint64_t)w[at + 1] << (64 - sh);
+  return (uint32_t)x;
+}
+
+// The packed rows that a lane's columns stand for: row0 + 16 ct + lane % 16.
+template <int CT>
+struct Rows {
+  int tok[CT], head[CT];
+  bool live[CT];
+  const int64_t* words[CT];
+  __device__ __forceinline__ Rows(const TreeParams& p, int row0, int rows, int first, int hk) {
+    const int G = p.HQ / p.HKV;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int r = row0 + ct * 16 + (threadIdx.x & 15);
+      live[ct] = r < rows;
+      tok[ct] = live[ct] ? r / G : 0;
+      head[ct] = hk * G + (live[ct] ? r - tok[ct] * G : 0);
+      words[ct] = p.bits != nullptr ? p.bits + (int64_t)(first + tok[ct]) * p.words : nullptr;
     }
   }
-  float q[E], acc[E], m = -INFINITY, l = 0.f;
-  for (int e = 0; e < E; ++e) {
-    q[e] = bf2f(p.q[((int64_t)h * p.N + n) * D + lane * E + e]);
-    acc[e] = 0.f;
+};
+
+// Q as the B operand; an e4m3 cache's 16-byte pieces of a key order the contraction.
+template <int D, bool FP8, int CT>
+__device__ __forceinline__ void load_q(const TreeParams& p, const Rows<CT>& w, int first, bool paired,
+                                       bf16x8 (&qf)[CT][D / 32]) {
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const uint16_t* src = p.q + ((int64_t)w.head[ct] * p.N + first + w.tok[ct]) * D;
+#pragma unroll
+    for (int f = 0; f < D / 32; ++f) {
+      const int d = paired ? (f >> 1) * 64 + g * 16 + (f & 1) * 8 : f * 32 + g * 8;
+      qf[ct][f] = w.live[ct] ? *reinterpret_cast<const bf16x8*>(src + d) : bf16x8{};
+    }
   }
-  if (b >= 0) {
-    const int64_t ctx = max(p.ctx[b], 0);
-    const int64_t total = min(ctx + (end - first), p.max_pages * p.page);
-    for (int64_t pos = wave; pos < total; pos += 4) {
-      const int64_t j = pos - ctx;
-      if (j >= 0) {
-        const bool sees = p.bits == nullptr ? j <= n - first
-                                            : j < 64LL * p.words && ((p.bits[n * p.words + j / 64] >> (j % 64)) & 1);
-        if (!sees) continue;
+}
+
+// One workgroup's part of the positions.
+struct Part {
+  int b, first, n, row0, rows, hk, split, u0, u1;
+  int64_t ctx, total;
+  // false: nothing to do. Blocks and parts of a launch are numbered row block, part, kv head, the last fastest.
+  __device__ __forceinline__ bool find(const TreeParams& p, int R, int D, int step) {
+    const int groups = p.HKV * p.splits;
+    const int rb = blockIdx.x / groups, at = blockIdx.x - rb * groups;
+    split = at / p.HKV;
+    hk = at - split * p.HKV;
+    if (rb == 0 && split == 0) zero_rows(p, hk, D);
+    if (!find_block(p, rb, R, b, first, n, row0)) return false;
+    rows = n * (p.HQ / p.HKV);
+    ctx = max(p.ctx[b], 0);
+    total = p.pages > 0 ? min(ctx + n, p.max_pages * p.page) : 0;
+    const int units = (int)((total + 31) >> 5);
+    const int part = max(step, ((units + p.splits - 1) / p.splits + step - 1) / step * step);
+    u0 = min(units, split * part);
+    u1 = min(units, u0 + part);
+    return true;
+  }
+  __device__ __forceinline__ int64_t head_row(const TreeParams& p, int row) const {  // (row, head) of a packed row
+    const int G = p.HQ / p.HKV, tk = row / G;
+    return (int64_t)(first + tk) * p.HQ + hk * G + (row - tk * G);
+  }
+  // An empty part of a short sequence has no sums: its rows say so.
+  __device__ __forceinline__ void no_sums(const TreeParams& p, int R) const {
+    for (int r = row0 + threadIdx.x; r < min(rows, row0 + R); r += blockDim.x)
+      p.ml[head_row(p, r) * p.splits + split] = make_float2(-INFINITY, 0.f);
+  }
+};
+
+// Row of the cache where the 16 positions of tile t begin, or -1 where there is none.
+struct Table {
+  const_ints at;
+  int64_t max_pages, pages;
+  int tiles, page, HKV, hk;
+  uint32_t inv;
+  __device__ __forceinline__ Table(const TreeParams& p, const Part& w)
+      : at((const_ints)(uintptr_t)(p.table + (int64_t)w.b * p.max_pages)), max_pages(p.max_pages), pages(p.pages),
+        tiles(p.page >> 4), page(p.page), HKV(p.HKV), hk(w.hk), inv(p.tiles_inv) {}
+  __device__ __forceinline__ int64_t row(int t) const {
+    int i = t;  // t / tiles
+    if (tiles > 1) {
+      i = (int)(((uint64_t)(uint32_t)t * inv) >> 32);  // or one more
+      if (i * tiles > t) --i;
+    }
+    if (i >= max_pages) return -1;
+    const int pg = at[i];
+    return pg >= 0 && pg < pages ? ((int64_t)pg * HKV + hk) * page + (t - i * tiles) * 16 : -1;
+  }
+};
+
+// Scores of 32 positions -> weights (the B operand of the outputs' product, and for the rare path as they are), with the
+// rows' reference maxima, sums and outputs brought up to date. edge: `there` and the rows' bits say what is seen.
+template <bool FP8, int DT, int CT>
+__device__ __forceinline__ void soft_weights(const TreeParams& p, const Rows<CT>& rw, const f32x4 (&s)[2][CT], float f2,
+                                             const f32x4 (&kq)[2], const f32x4 (&vq)[2], bool edge, uint32_t there,
+                                             int64_t j0, float (&m)[CT], float (&l)[CT], f32x4 (&acc)[DT][CT],
+                                             float (&w)[CT][8], bf16x8 (&pf)[CT]) {
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    uint32_t see = ~0u;
+    if (edge) see = (rw.live[ct] ? there & seen32(p, rw.words[ct], rw.tok[ct], j0) : 0u) >> (g * 4);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = s[i >> 2][ct][i & 3] * f2;
+      if (FP8) v *= kq[i >> 2][i & 3];
+      if (edge && !(see >> ((i >> 2) * 16 + (i & 3)) & 1)) v = -INFINITY;
+      w[ct][i] = v;
+      top = fmaxf(top, v);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const bool up = top > m[ct] + kSlack;
+    if (__any(up)) {
+      const float a = up ? __builtin_amdgcn_exp2f(m[ct] - top) : 1.f;
+      if (up) m[ct] = top;
+      l[ct] *= a;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d][ct] *= a;
+    }
+    const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float e = __builtin_amdgcn_exp2f(w[ct][i] - ref);
+      l[ct] += e;
+      w[ct][i] = e;
+      if (FP8) w[ct][i] = edge && !(see >> ((i >> 2) * 16 + (i & 3)) & 1) ? 0.f : e * vq[i >> 2][i & 3];
+    }
+    pf[ct] = __builtin_bit_cast(bf16x8, make_uint4(pack2(w[ct][0], w[ct][1]), pack2(w[ct][2], w[ct][3]),
+                                                   pack2(w[ct][4], w[ct][5]), pack2(w[ct][6], w[ct][7])));
+  }
+}
+
+// O^T += V^T P^T over 32 positions from LDS rows of RS values; one by one where a value is not finite, so that a weight of
+// zero takes nothing.
+template <int RS, int DT, int CT>
+__device__ __forceinline__ void add_values(const uint16_t* vl, const float (&w)[CT][8], const bf16x8 (&pf)[CT], bool odd,
+                                           f32x4 (&acc)[DT][CT]) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  if (odd) {
+#pragma unroll 1
+    for (int key = 0; key < 32; ++key) {
+      const int slot = (key >> 4) * 4 + (key & 3), from = ((key >> 2) & 3) * 16 + c;
+      float wk[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float y = w[ct][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) y = slot == i ? w[ct][i] : y;
+        wk[ct] = __shfl(y, from);
       }
-      const int page = p.table[b * p.max_pages + pos / p.page];
-      if (page < 0 || page >= p.pages) continue;
-      const int64_t row = ((int64_t)page * p.HKV + hk) * p.page + pos % p.page;
-      float s = 0.f;
-      for (int e = 0; e < E; ++e) s += q[e] * cache_value<FP8>(p.kc, p.ks, row, D, lane * E + e);
-      s = wave_sum64(s) * p.scale;
-      const float t = fmaxf(m, s), a = m == -INFINITY ? 0.f : expf(m - t), w = expf(s - t);
-      l = l * a + w;
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * a + w * cache_value<FP8>(p.vc, p.vs, row, D, lane * E + e);
-      m = t;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = bf2f(vl[key * RS + d * 16 + g * 4 + r]);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[d][ct][r] += wk[ct] == 0.f ? 0.f : wk[ct] * v;
+        }
     }
+    return;
   }
-  __shared__ float sm[4], sl[4], so[4][D];
-  for (int e = 0; e < E; ++e) so[wave][lane * E + e] = acc[e];
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
+  const uint16_t* const at = vl + (g * 4 + (c >> 2)) * RS + (c & 3) * 4;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    const bf16x4 lo =
+        __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(at + d * 16));
+    const bf16x4 hi =
+        __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(at + 16 * RS + d * 16));
+    const bf16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) acc[d][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pf[ct], acc[d][ct], 0, 0, 0);
+  }
+}
+
+// Which of the 32 positions from p0 exist: below the sequence's end, in pages of the cache.
+__device__ __forceinline__ uint32_t existing(int64_t left, bool ok0, bool ok1) {
+  return (left >= 32 ? ~0u : (1u << left) - 1) & ((ok0 ? 0xffffu : 0u) | (ok1 ? 0xffff0000u : 0u));
+}
+
+// Few rows: 16 packed rows a workgroup, its four waves take the part's units in turn.
+template <int D, bool FP8>
+__global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
+  constexpr int R = 16, KF = D / 32, DT = D / 16, RB = D * (FP8 ? 1 : 2);  // RB: bytes of a cache row
+  constexpr int RS = D + 16;                                 // LDS row of values, in bf16
+  constexpr int KL = RB / 64;                                // 16-byte loads of a key
+  constexpr int VR = RB / 16;                                // lanes of a value row
+  constexpr int VK = 64 / VR, VL = 32 / VK;                  // keys a load, loads of 32 keys
+  constexpr int XS = D + 4;                                  // row of the waves' exchange, in floats
+  __shared__ __attribute__((aligned(16))) uint16_t vbuf[4 * 32 * RS];
+  __shared__ float sm[4][R], sl[4][R];
+  static_assert(sizeof(vbuf) >= 4 * R * XS * 4, "the exchange of sums reuses the value rows");
+
+  Part w;
+  if (!w.find(p, R, D, 4)) return;
+  if (p.splits > 1 && w.u0 >= w.u1) return w.no_sums(p, R);
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Rows<1> rw(p, w.row0, w.rows, w.first, w.hk);
+  const Table table(p, w);
+  bf16x8 qf[1][KF];
+  load_q<D, FP8, 1>(p, rw, w.first, FP8, qf);
+
+  uint4 kx[2][KL], vx[VL];
+  f32x4 ks[2], vs[2];
+  bool ok[2];
+  const auto load = [&](int u) {
+    int64_t row[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      row[t] = table.row(2 * u + t);
+      ok[t] = row[t] >= 0;
+      row[t] = max(row[t], (int64_t)0);  // any row of the cache: its values are not used
+      const uint8_t* kb = static_cast<const uint8_t*>(p.kc) + row[t] * RB;
+#pragma unroll
+      for (int f = 0; f < KL; ++f) kx[t][f] = *reinterpret_cast<const uint4*>(kb + c * RB + f * 64 + g * 16);
+      if (FP8) {
+        ks[t] = *reinterpret_cast<const f32x4*>(p.ks + row[t] + g * 4);
+        vs[t] = *reinterpret_cast<const f32x4*>(p.vs + row[t] + g * 4);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i)
+      vx[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.vc) + row[i / (VL / 2)] * RB +
+                                              (i % (VL / 2)) * 1024 + lane * 16);
+  };
+
+  const float f2 = p.scale * kLog2e;
+  f32x4 acc[DT][1];
+  float m[1] = {-INFINITY}, l[1] = {0.f};
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d][0] = f32x4{};
+  uint16_t* const vl = vbuf + wave * 32 * RS;
+
+  int u = w.u0 + wave;
+  if (u < w.u1) load(u);
+  for (; u < w.u1; u += 4) {
+    f32x4 s[2][1];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t][0] = f32x4{};
+#pragma unroll
+      for (int f = 0; f < KF; ++f) {
+        const uint4 x = kx[t][FP8 ? f >> 1 : f];
+        const bf16x8 a = __builtin_bit_cast(bf16x8, !FP8 ? x : f & 1 ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y));
+        s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[0][f], s[t][0], 0, 0, 0);
+      }
+    }
+    const int64_t p0 = (int64_t)u * 32;
+    const bool edge = !(ok[0] && ok[1]) || p0 + 32 > min(w.ctx, w.total);
+    const uint32_t there = existing(w.total - p0, ok[0], ok[1]);
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int key = i * VK + lane / VR;
+      uint4* const dst = reinterpret_cast<uint4*>(vl + key * RS + (lane % VR) * (FP8 ? 16 : 8));
+#pragma unroll
+      for (int h = 0; h < (FP8 ? 2 : 1); ++h) {
+        uint4 x = vx[i];
+        if (FP8) x = h ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y);
+        if (edge) {
+          if (!(there >> key & 1)) x = make_uint4(0u, 0u, 0u, 0u);
+          odd |= odd2(x.x) || odd2(x.y) || odd2(x.z) || odd2(x.w);
+        }
+        dst[h] = x;
+      }
+    }
+    f32x4 kq[2], vq[2];
+    if (FP8)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        kq[t] = ks[t];
+        vq[t] = vs[t];
+      }
+    if (u + 4 < w.u1) load(u + 4);
+    float wt[1][8];
+    bf16x8 pf[1];
+    soft_weights<FP8, DT, 1>(p, rw, s, f2, kq, vq, edge, there, p0 - w.ctx, m, l, acc, wt, pf);
+    add_values<RS, DT, 1>(vl, wt, pf, edge && __any(odd), acc);
+  }
+
+  // the four waves' sums, each brought to the largest reference
+  l[0] += __shfl_xor(l[0], 16);
+  l[0] += __shfl_xor(l[0], 32);
+  if (g == 0) {
+    sm[wave][c] = m[0];
+    sl[wave][c] = l[0];
   }
   __syncthreads();
-  float mm = -INFINITY, ll = 0.f, f[4];
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w]);
-  for (int w = 0; w < 4; ++w) {
-    f[w] = sm[w] == -INFINITY ? 0.f : expf(sm[w] - mm);
-    ll += f[w] * sl[w];
+  const float all = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
+  const float mine = m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[0] - all);
+  float* const swap = reinterpret_cast<float*>(vbuf);
+#pragma unroll
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(swap + (wave * R + c) * XS + d * 16 + g * 4) = acc[d][0] * mine;
+  __syncthreads();
+  const int r = threadIdx.x >> 4, row = w.row0 + r;
+  if (row >= w.rows) return;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) top = fmaxf(top, sm[k][r]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)  // a wave without a reference has a sum only where every score was NaN
+    sum += sm[k][r] == -INFINITY ? sl[k][r] : sl[k][r] * __builtin_amdgcn_exp2f(sm[k][r] - top);
+  const int64_t nh = w.head_row(p, row), i = nh * p.splits + w.split;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int q = 0; q < D / 64; ++q) {
+    const int d = q * 64 + (threadIdx.x & 15) * 4;
+    f32x4 o{};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o += *reinterpret_cast<const f32x4*>(swap + (k * R + r) * XS + d);
+    if (p.splits > 1)
+      *reinterpret_cast<f32x4*>(p.part + i * D + d) = o;
+    else
+      *reinterpret_cast<uint2*>(p.out + nh * D + d) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
   }
-  if (threadIdx.x < D) {
-    float o = 0.f;
-    for (int w = 0; w < 4; ++w) o += f[w] * so[w][threadIdx.x];
-    p.out[(n * p.HQ + h) * D + threadIdx.x] = (uint16_t)f2bf(ll == 0.f ? 0.f : o / ll);
+  if ((threadIdx.x & 15) != 0) return;
+  if (p.splits > 1)
+    p.ml[i] = make_float2(top, sum);
+  else if (p.lse != nullptr)
+    p.lse[nh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+// Many rows: 64 CT packed rows a workgroup, 16 CT of them a wave; all take the part's units in order, from LDS. A thread
+// loads its 16-byte pieces of the next unit before it works on the present one and stores them, as bf16, to the other half
+// of the LDS after it.
+template <int D, bool FP8, int CT>
+__global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) tree_wide_k(TreeParams p) {
+  constexpr int R = 64 * CT, KF = D / 32, DT = D / 16, RB = D * (FP8 ? 1 : 2);
+  constexpr int KS = D + 8, RS = D + 16;   // LDS rows of keys and values: what spreads each one's reads over the banks
+  constexpr int PL = 32 * RB / 16 / 256;   // pieces of the unit's keys (and of its values) a thread loads
+  constexpr int PR = RB / 16;              // pieces of a row
+  constexpr int TILE = 32 * (KS + RS);
+  __shared__ __attribute__((aligned(16))) uint16_t buf[2][TILE];
+  __shared__ __attribute__((aligned(16))) float sc[2][2][32];
+  __shared__ int odd_at[2];
+
+  Part w;
+  if (!w.find(p, R, D, 1)) return;
+  if (p.splits > 1 && w.u0 >= w.u1) return w.no_sums(p, R);
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wrow = w.row0 + wave * 16 * CT;
+  const Rows<CT> rw(p, wrow, w.rows, w.first, w.hk);
+  const Table table(p, w);
+  bf16x8 qf[CT][KF];
+  load_q<D, FP8, CT>(p, rw, w.first, false, qf);
+
+  uint4 kx[PL], vx[PL];
+  float kq1 = 0.f, vq1 = 0.f;
+  bool ok[2], now[2];
+  const auto load = [&](int u) {
+    int64_t row[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      row[t] = table.row(2 * u + t);
+      ok[t] = row[t] >= 0;
+      row[t] = max(row[t], (int64_t)0);  // any row of the cache: its values are not used
+    }
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      const int piece = i * 256 + threadIdx.x, key = piece / PR;
+      const int64_t at = (key >= 16 ? row[1] : row[0]) * RB + (key & 15) * RB + (piece % PR) * 16;
+      kx[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.kc) + at);
+      vx[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.vc) + at);
+    }
+    if (FP8) {
+      const int64_t at = (threadIdx.x & 16 ? row[1] : row[0]) + (threadIdx.x & 15);
+      kq1 = p.ks[at];
+      vq1 = p.vs[at];
+    }
+  };
+  // the loaded unit u to LDS half h
+  const auto store = [&](int u, int h) {
+    const int64_t p0 = (int64_t)u * 32;
+    const bool edge = !(ok[0] && ok[1]) || p0 + 32 > min(w.ctx, w.total);
+    const uint32_t there = existing(w.total - p0, ok[0], ok[1]);
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      const int piece = i * 256 + threadIdx.x, key = piece / PR, d = (piece % PR) * (FP8 ? 16 : 8);
+      uint4* const kd = reinterpret_cast<uint4*>(buf[h] + key * KS + d);
+      uint4* const vd = reinterpret_cast<uint4*>(buf[h] + 32 * KS + key * RS + d);
+#pragma unroll
+      for (int e = 0; e < (FP8 ? 2 : 1); ++e) {
+        uint4 x = vx[i], y = kx[i];
+        if (FP8) {
+          x = e ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y);
+          y = e ? cvt_fp8x8(y.z, y.w) : cvt_fp8x8(y.x, y.y);
+        }
+        if (edge) {
+          if (!(there >> key & 1)) x = make_uint4(0u, 0u, 0u, 0u);
+          odd |= odd2(x.x) || odd2(x.y) || odd2(x.z) || odd2(x.w);
+        }
+        kd[e] = y;
+        vd[e] = x;
+      }
+    }
+    if (FP8 && threadIdx.x < 32) {
+      sc[h][0][threadIdx.x] = kq1;
+      sc[h][1][threadIdx.x] = vq1;
+    }
+    if (edge && __any(odd) && lane == 0) odd_at[h] = u;
+  };
+
+  const float f2 = p.scale * kLog2e;
+  f32x4 acc[DT][CT];
+  float m[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = -INFINITY;
+    l[ct] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d][ct] = f32x4{};
   }
-  if (p.lse != nullptr && threadIdx.x == 0) p.lse[n * p.HQ + h] = ll == 0.f ? -INFINITY : mm + logf(ll);
+  if (threadIdx.x < 2) odd_at[threadIdx.x] = -1;
+  __syncthreads();
+  if (w.u0 < w.u1) {
+    load(w.u0);
+    store(w.u0, 0);
+  }
+  for (int u = w.u0; u < w.u1; ++u) {
+    const int h = (u - w.u0) & 1;
+    now[0] = ok[0];
+    now[1] = ok[1];
+    __syncthreads();
+    if (u + 1 < w.u1) load(u + 1);
+    const uint16_t* const kl = buf[h] + c * KS + g * 8;
+    f32x4 s[2][CT];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[t][ct] = f32x4{};
+#pragma unroll
+      for (int f = 0; f < KF; ++f) {
+        const bf16x8 a = *reinterpret_cast<const bf16x8*>(kl + t * 16 * KS + f * 32);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[t][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[ct][f], s[t][ct], 0, 0, 0);
+      }
+    }
+    const int64_t p0 = (int64_t)u * 32;
+    const bool edge = !(now[0] && now[1]) || p0 + 32 > min(w.ctx, w.total);
+    f32x4 kq[2], vq[2];
+    if (FP8)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        kq[t] = *reinterpret_cast<const f32x4*>(&sc[h][0][t * 16 + g * 4]);
+        vq[t] = *reinterpret_cast<const f32x4*>(&sc[h][1][t * 16 + g * 4]);
+      }
+    float wt[CT][8];
+    bf16x8 pf[CT];
+    soft_weights<FP8, DT, CT>(p, rw, s, f2, kq, vq, edge, existing(w.total - p0, now[0], now[1]), p0 - w.ctx, m, l, acc, wt,
+                              pf);
+    add_values<RS, DT, CT>(buf[h] + 32 * KS, wt, pf, edge && odd_at[h] == u, acc);
+    if (u + 1 < w.u1) store(u + 1, h ^ 1);
+  }
+
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    l[ct] += __shfl_xor(l[ct], 16);
+    l[ct] += __shfl_xor(l[ct], 32);
+    if (!rw.live[ct]) continue;
+    const int64_t nh = (int64_t)(w.first + rw.tok[ct]) * p.HQ + rw.head[ct], i = nh * p.splits + w.split;
+    const float inv = l[ct] == 0.f ? 0.f : 1.f / l[ct];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const f32x4 o = acc[d][ct];
+      if (p.splits > 1)
+        *reinterpret_cast<f32x4*>(p.part + i * D + d * 16 + g * 4) = o;
+      else
+        *reinterpret_cast<uint2*>(p.out + nh * D + d * 16 + g * 4) =
+            make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
+    }
+    if (g != 0) continue;
+    if (p.splits > 1)
+      p.ml[i] = make_float2(m[ct], l[ct]);
+    else if (p.lse != nullptr)
+      p.lse[nh] = l[ct] == 0.f ? -INFINITY : (m[ct] + log2f(l[ct])) * kLn2;
+  }
+}
+
+// Joins the parts of a row: one wave per (row, head), 4 D / 256 dims a lane.
+template <int D>
+__global__ void __launch_bounds__(256) tree_join_k(TreeParams p) {
+  constexpr int E = D / 64;
+  const int64_t nh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (nh >= p.N * p.HQ) return;
+  const int64_t row = nh / p.HQ;
+  bool mine = false;  // the row belongs to a sequence (the others have their zeros)
+  for (int i = lane; i < p.B; i += 64) {
+    int first, n;
+    seq_rows(p, i, first, n);
+    mine |= row >= first && row < (int64_t)first + n;
+  }
+  if (!__any(mine)) return;
+  const float2* const ml = p.ml + nh * p.splits;
+  float top = -INFINITY, sum = 0.f, o[E] = {};
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[s].x);
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 x = ml[s];
+    if (x.x == -INFINITY && x.y == 0.f) continue;  // nothing seen there; an empty part has no sums either
+    const float f = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - top);
+    sum += f * x.y;
+    const float* const src = p.part + (nh * p.splits + s) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] += f * src[e];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint32_t* const dst = reinterpret_cast<uint32_t*>(p.out + nh * D + lane * E);
+#pragma unroll
+  for (int e = 0; e < E; e += 2) dst[e / 2] = pack2(o[e] * inv, o[e + 1] * inv);
+  if (lane == 0 && p.lse != nullptr) p.lse[nh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 }  // namespace
 
-hipError_t launch_tree_attn(const TreeParams& p, int D, bool fp8, hipStream_t st) {
-  const auto kernel = D == 256 ? (fp8 ? tree_attn_k<256, true> : tree_attn_k<256, false>)
-                               : (fp8 ? tree_attn_k<128, true> : tree_attn_k<128, false>);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(p.N * p.HQ)), dim3(256), 0, st, p);
+TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, int page) {
+  TreePlan t{};
+  const int64_t G = HQ / HKV, seqs = std::max<int64_t>(1, std::min<int64_t>(B, N)), mean = (N * G + seqs - 1) / seqs;
+  t.rows = mean <= 16 ? 16 : mean <= 64 ? 64 : 128;
+  // an upper bound of sum ceil(n_b G / rows) over the sequences with rows, which are `seqs` at most
+  t.blocks = (N * G + seqs * (t.rows - 1)) / t.rows;
+  const int64_t units = (max_pages * page + 31) / 32, base = t.blocks * HKV;
+  t.splits = std::max<int64_t>(1, std::min<int64_t>((512 + base - 1) / base, std::min<int64_t>(units / 8, 64)));
+  return t;
+}
+
+template <int D, bool FP8>
+static void (*tree_kernel(int rows))(TreeParams) {
+  return rows == 16 ? tree_narrow_k<D, FP8> : rows == 64 ? tree_wide_k<D, FP8, 1> : tree_wide_k<D, FP8, 2>;
+}
+
+hipError_t launch_tree_attn(const TreeParams& p, const TreePlan& t, int D, bool fp8, hipStream_t st) {
+  const auto kernel = D == 256 ? (fp8 ? tree_kernel<256, true>(t.rows) : tree_kernel<256, false>(t.rows))
+                               : (fp8 ? tree_kernel<128, true>(t.rows) : tree_kernel<128, false>(t.rows));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(t.blocks * p.HKV * t.splits)), dim3(256), 0, st, p);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess || t.splits == 1) return err;
+  hipLaunchKernelGGL(D == 256 ? tree_join_k<256> : tree_join_k<128>, dim3((unsigned)((p.N * p.HQ + 3) / 4)), dim3(256),
+                     0, st, p);
   return hipGetLastError();
 }
 
