@@ -28,9 +28,9 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
          f"-I{INCLUDE}", f"-I{CSRC}"]
 
 
-# Tree attention keeps outputs that both MFMA and VALU code update: with the products' results in ordinary registers (not
+# The attention cores keep sums that both MFMA and VALU code update: with the products' results in ordinary registers (not
 # the accumulation ones) nothing is copied between the two files on every update, and nothing spills.
-FILE_FLAGS = {"tree_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+FILE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in ("tree_attn.hip", "linattn.hip")}
 
 
 def source_files():

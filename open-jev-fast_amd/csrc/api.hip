@@ -973,14 +973,13 @@ int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const
 }
 
 int64_t ojx_linattn_prompt_workspace(int64_t R, int64_t S, int32_t HV, int32_t HK, int32_t delta) {
-  (void)delta;
   // a workgroup of 256 threads per sequence and head at most; a launch has fewer than 2^32 threads
   if (HK < 1 || HV < HK || HV % HK != 0 || HV > 1024 || R < 0 || R >= (1LL << 31) || S < 0 ||
-      (S + 1) * HV >= (1LL << 24)) {
+      2 * (S + 1) * HV >= (1LL << 24) || ojx::linattn_chunks(R, S) * HV >= (1LL << 24)) {
     fail(OJX_ERR_SHAPE, "bad sizes R=%lld S=%lld HV=%d HK=%d", (long long)R, (long long)S, HV, HK);
     return -1;
   }
-  return 0;
+  return ojx::linattn_work_bytes(R, S, HV, delta != 0);
 }
 
 int ojx_linattn_prompt(const void* q, const void* k, const void* v, const float* g, const void* beta,
@@ -1003,7 +1002,8 @@ int ojx_linattn_prompt(const void* q, const void* k, const void* v, const float*
                 (long long)need, (long long)workspace_bytes);
   const ojx::LinParams p{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
                          static_cast<const uint16_t*>(v), g, static_cast<const uint16_t*>(beta), seq_ptr, state, src,
-                         state_out, static_cast<uint16_t*>(o), R, S, state_slots, HV, HK, scale};
+                         state_out, static_cast<uint16_t*>(o), R, S, state_slots, HV, HK, scale,
+                         static_cast<uint8_t*>(workspace)};
   return hip_check(ojx::launch_linattn_prompt(p, static_cast<hipStream_t>(stream)), "linear attention launch");
 }
 
@@ -1019,7 +1019,7 @@ int ojx_linattn_step(const void* q, const void* k, const void* v, const float* g
   if (!aligned(state, 16) || !aligned(slot, 4)) return fail(OJX_ERR_ARG, "states must be 16-byte aligned");
   const ojx::LinParams p{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
                          static_cast<const uint16_t*>(v), g, static_cast<const uint16_t*>(beta), nullptr, nullptr,
-                         nullptr, nullptr, static_cast<uint16_t*>(o), R, 0, state_slots, HV, HK, scale};
+                         nullptr, nullptr, static_cast<uint16_t*>(o), R, 0, state_slots, HV, HK, scale, nullptr};
   return hip_check(ojx::launch_linattn_step(p, state, slot, static_cast<hipStream_t>(stream)),
                    "linear attention step launch");
 }

@@ -92,6 +92,67 @@ __device__ __forceinline__ void rmsnorm_row8(const float (&v)[8], float4 wa, flo
       make_uint4(pack2(o[0], o[1]), pack2(o[2], o[3]), pack2(o[4], o[5]), pack2(o[6], o[7]));
 }
 
+// Running sum, and running maximum, over the wave's lanes up to and including this one.
+__device__ __forceinline__ int wave_scan_sum(int v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(v, o);
+    if ((int)(threadIdx.x & 63) >= o) v += t;
+  }
+  return v;
+}
+__device__ __forceinline__ int wave_scan_max(int v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v = max(v, __shfl_up(v, o));  // below lane o the lane's own value comes back
+  return v;
+}
+
+// Sequences laid end to end in rows by pointers ptr[0 .. S]: sequence i is rows [m_i, m_(i+1)), m_i the largest of ptr[0 ..
+// i] clamped to [0, rows]. For pointers that never fall that is what they say; whatever they hold, sequences stay within
+// the rows and do not overlap. per(n) says how many units a sequence of n rows takes. The whole wave calls, with uniform
+// arguments.
+struct SeqPlace {
+  int seq, first, n;  // its first row and row count
+  int before;         // units of the sequences before it
+};
+__device__ __forceinline__ int seq_bound(const int32_t* ptr, int64_t i, int64_t rows) {
+  return (int)min(max((int64_t)ptr[i], (int64_t)0), rows);
+}
+// find(done): the first sequence where done(its index, units up to and with it) holds; false where none does.
+template <typename Per, typename Done>
+__device__ __forceinline__ bool seq_find(const int32_t* ptr, int64_t S, int64_t rows, Per per, Done done, SeqPlace& out) {
+  const int lane = threadIdx.x & 63;
+  int carry = 0, before = 0;
+  for (int64_t base = 0; base < S; base += 64) {
+    const int64_t i = base + lane;
+    const int x = max(carry, wave_scan_max(seq_bound(ptr, min(i, S), rows)));
+    const int e = max(x, seq_bound(ptr, min(i + 1, S), rows));
+    const int units = per(e - x);  // 0 rows behind the last sequence: e == x there
+    const int s = before + wave_scan_sum(units);
+    const unsigned long long hit = __ballot(i < S && done((int)i, s));
+    if (hit != 0) {
+      const int j = __builtin_ctzll(hit);
+      out.seq = (int)base + j;
+      out.first = __builtin_amdgcn_readlane(x, j);
+      out.n = __builtin_amdgcn_readlane(e - x, j);
+      out.before = __builtin_amdgcn_readlane(s - units, j);
+      return true;
+    }
+    carry = __builtin_amdgcn_readlane(e, 63);
+    before = __builtin_amdgcn_readlane(s, 63);
+  }
+  return false;
+}
+// The rows before the first sequence, lo, and the first row behind the last, hi >= lo.
+__device__ __forceinline__ void seq_span(const int32_t* ptr, int64_t S, int64_t rows, int& lo, int& hi) {
+  const int lane = threadIdx.x & 63;
+  lo = seq_bound(ptr, 0, rows);
+  hi = lo;
+  for (int64_t i = lane; i <= S; i += 64) hi = max(hi, seq_bound(ptr, i, rows));
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) hi = max(hi, __shfl_xor(hi, o));
+}
+
 // ----------------------------------------------------------------------------------------------------------------
 // GEMM epilogue modes (what a workgroup does with its fp32 accumulator tile)
 enum Epi : int {
@@ -235,7 +296,10 @@ struct LinParams {
   int64_t R, S, slots;
   int HV, HK;
   float scale;
+  uint8_t* work;                          // linattn_work_bytes (prompts)
 };
+int64_t linattn_chunks(int64_t R, int64_t S);  // of 64 tokens, at most
+int64_t linattn_work_bytes(int64_t R, int64_t S, int HV, bool delta);
 hipError_t launch_linattn_step(const LinParams& p, float* state, const int32_t* slot, hipStream_t st);
 hipError_t launch_linattn_prompt(const LinParams& p, hipStream_t st);
 

@@ -42,53 +42,14 @@ typedef __attribute__((address_space(4))) const int32_t* const_ints;  // read-on
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;  // the reference maximum follows when it is this far behind, base two
 
-__device__ __forceinline__ int64_t clamp_row(int64_t x, int64_t N) { return min(max(x, (int64_t)0), N); }
-
-// Sequence b's first row and row count, whatever its pointers hold.
-__device__ __forceinline__ void seq_rows(const TreeParams& p, int b, int& first, int& n) {
-  const int64_t x = clamp_row(p.q_ptr[b], p.N), y = max(clamp_row(p.q_ptr[b + 1], p.N), x);
-  first = (int)x;
-  n = (int)(y - x);
-}
-
-// The sequence of row block rb (blocks of R packed rows, sequence after sequence) and its place in it; false: none.
-__device__ __forceinline__ bool find_block(const TreeParams& p, int rb, int R, int& b, int& first, int& n, int& row0) {
-  const int lane = threadIdx.x & 63, G = p.HQ / p.HKV;
-  for (int base = 0; base < p.B; base += 64) {
-    int x = 0, c = 0;
-    if (base + lane < p.B) seq_rows(p, base + lane, x, c);
-    const int blocks = (c * G + R - 1) / R;
-    int s = blocks;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int t = __shfl_up(s, o);
-      if (lane >= o) s += t;
-    }
-    const int total = __builtin_amdgcn_readlane(s, 63);
-    if (rb < total) {
-      const int j = __builtin_ctzll(__ballot(s > rb));
-      b = base + j;
-      first = __builtin_amdgcn_readlane(x, j);
-      n = __builtin_amdgcn_readlane(c, j);
-      row0 = (rb - __builtin_amdgcn_readlane(s - blocks, j)) * R;
-      return true;
-    }
-    rb -= total;
-  }
-  return false;
-}
-
 // Zeros (and lse -inf) for kv head hk's heads of the rows before the first sequence and behind the last.
 __device__ __forceinline__ void zero_rows(const TreeParams& p, int hk, int D) {
-  int64_t lo = p.B > 0 ? clamp_row(p.q_ptr[0], p.N) : p.N, hi = 0;
-  for (int i = threadIdx.x & 63; i <= p.B; i += 64) hi = max(hi, clamp_row(p.q_ptr[i], p.N));
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) hi = max(hi, (int64_t)__shfl_xor((int)hi, o));
-  hi = max(hi, lo);
+  int lo, hi;
+  seq_span(p.q_ptr, p.B, p.N, lo, hi);
   const int G = p.HQ / p.HKV, per = G * D / 8;
-  const int64_t rows = lo + (p.N - hi);
+  const int64_t rows = lo + p.N - hi;
   for (int64_t t = threadIdx.x; t < rows * per; t += blockDim.x) {
-    const int64_t i = t / per, n = i < lo ? i : hi + (i - lo);
+    const int64_t i = t / per, n = i < lo ? i : i - lo + hi;
     const int c = (int)(t - i * per);
     *reinterpret_cast<uint4*>(p.out + (n * p.HQ + hk * G) * D + c * 8) = make_uint4(0u, 0u, 0u, 0u);
     if (p.lse != nullptr && c < G) p.lse[n * p.HQ + hk * G + c] = -INFINITY;
@@ -169,8 +130,16 @@ struct Part {
     split = at / p.HKV;
     hk = at - split * p.HKV;
     if (rb == 0 && split == 0) zero_rows(p, hk, D);
-    if (!find_block(p, rb, R, b, first, n, row0)) return false;
-    rows = n * (p.HQ / p.HKV);
+    const int G = p.HQ / p.HKV;
+    SeqPlace at_seq;
+    if (!seq_find(
+            p.q_ptr, p.B, p.N, [=](int m) { return (m * G + R - 1) / R; }, [=](int, int upto) { return upto > rb; }, at_seq))
+      return false;
+    b = at_seq.seq;
+    first = at_seq.first;
+    n = at_seq.n;
+    row0 = (rb - at_seq.before) * R;
+    rows = n * G;
     ctx = max(p.ctx[b], 0);
     total = p.pages > 0 ? min(ctx + n, p.max_pages * p.page) : 0;
     const int units = (int)((total + 31) >> 5);
@@ -611,13 +580,9 @@ __global__ void __launch_bounds__(256) tree_join_k(TreeParams p) {
   const int lane = threadIdx.x & 63;
   if (nh >= p.N * p.HQ) return;
   const int64_t row = nh / p.HQ;
-  bool mine = false;  // the row belongs to a sequence (the others have their zeros)
-  for (int i = lane; i < p.B; i += 64) {
-    int first, n;
-    seq_rows(p, i, first, n);
-    mine |= row >= first && row < (int64_t)first + n;
-  }
-  if (!__any(mine)) return;
+  int lo, hi;
+  seq_span(p.q_ptr, p.B, p.N, lo, hi);
+  if (row < lo || row >= hi) return;  // of no sequence: it has its zeros
   const float2* const ml = p.ml + nh * p.splits;
   float top = -INFINITY, sum = 0.f, o[E] = {};
   for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[s].x);

@@ -479,6 +479,49 @@ def test_linattn_long_and_many(ext, C, dev):
     _check_lin(C, args, lengths, None, o, last, 128 ** -0.5)
 
 
+def test_falling_pointers_do_not_multiply_rows(ext, C, dev):
+    """Pointers that fall give sequences that begin where those before them ended: no row twice, no more chunks or row
+    blocks than there are rows for."""
+    R = 130
+    args = _lin_case(R, 1, 2, True, seed=31)
+    up = [0, R, 0, R, 5, R, 0, R, 129, R]
+    o, last = ext.linattn_prompt(*_put(dev, *args, torch.tensor(up, dtype=torch.int32)))
+    _check_lin(C, args, [R] + [0] * 8, None, o, last, 128 ** -0.5)
+    up = [0, 70, 10, 90, 20, 130]
+    o, last = ext.linattn_prompt(*_put(dev, *args, torch.tensor(up, dtype=torch.int32)))
+    _check_lin(C, args, [70, 0, 20, 0, 40], None, o, last, 128 ** -0.5)
+    c = _tree_case([40], [30], 1, 2, 128, 16, "bf16", dev, seed=31, ext=ext)
+    c["table"] = c["table"].repeat(4, 1).contiguous()
+    c["ctx"] = c["ctx"].repeat(4).contiguous()
+    want = dict(c, q_ptr=torch.tensor([0, 40, 40, 40, 40], dtype=torch.int32))
+    c["q_ptr"] = torch.tensor([0, 40, 0, 40, 0], dtype=torch.int32)
+    out, lse = _run_tree(ext, c, dev)
+    _check_tree(C, want, out, lse, 128 ** -0.5)
+
+
+def test_linattn_prompt_without_rows(ext, dev):
+    """Sequences without rows hand their states on."""
+    args = _put(dev, *_lin_case(0, 1, 2, True, seed=1))
+    pool = torch.randn(3, 2, 128, 128, device=dev)
+    o, last = ext.linattn_prompt(*args, torch.zeros(3, dtype=torch.int32, device=dev), pool,
+                                 torch.tensor([2, -1], dtype=torch.int32, device=dev))
+    assert tuple(o.shape) == (0, 256) and torch.equal(last[0], pool[2]) and bool((last[1] == 0).all())
+
+
+def test_linattn_is_causal_in_what_is_not_finite(ext, dev):
+    """NaN and infinities reach no token before theirs, in their own chunk as little as in others."""
+    args = _lin_case(150, 1, 2, True, seed=33)
+    ptr = torch.tensor([0, 150], dtype=torch.int32)
+    clean = ext.linattn_prompt(*_put(dev, *args, ptr))[0].float()
+    for t, which, value in ((20, 0, math.nan), (100, 1, math.inf), (64, 2, -math.inf), (63, 3, math.nan), (127, 4, math.nan)):
+        bad = [x.clone() for x in args]
+        bad[which][t] = value
+        o = ext.linattn_prompt(*_put(dev, *bad, ptr))[0].float()
+        err = (o[:t] - clean[:t]).abs()
+        assert bool((err <= 2.0 ** -6 * clean[:t].abs().amax()).all()), which
+        assert not bool(torch.isfinite(o[t]).all())
+
+
 # ---------------------------------------------------------------------------------------------------- as they are used
 def _layers(ext, dev, seed):
     """One decoding step's calls of a full- and a linear-attention layer, on inputs that are overwritten between calls."""
