@@ -4,9 +4,10 @@
 // logarithm g of its decay and, with the delta rule, a strength beta:
 //   S <- e^g S;  u = beta (v - S^T k)  (without the delta rule u = v);  S <- S + k u^T;  o = scale S^T q
 // Value head h reads key head h / (HV / HK).
-#include "ojx_internal.h"
+#include "gemm_common.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cstddef>
 
 namespace ojx {
@@ -141,40 +142,44 @@ __global__ void __launch_bounds__(256) linattn_step_k(LinParams p, float* state,
 // ------------------------------------------------------------------------------------------------------------- prompts
 // A chunk of C = 64 tokens at once. With G_i the sum of g up to token i of the chunk and S0 the state before it,
 //   A_ij = beta_i e^(G_i - G_j) k_i . k_j (j < i),  P_ij = e^(G_i - G_j) q_i . k_j (j <= i),  T = (I + A)^-1 diag(beta),
-//   U = T (V - diag(e^G) K S0)  (without the delta rule U = V),
-//   O = scale (diag(e^G) Q S0 + P U),  S = e^(G_C) S0 + K^T diag(e^(G_C - G)) U.
-// T and P need no state: linattn_chunk_k makes them for all chunks at once. linattn_prompt_k then goes through a
-// sequence's chunks in order.
+//   X = V - diag(e^G) K S0,  U = T X,
+//   O = scale (diag(e^G) Q S0 + P U),  S = e^(G_C) S0 + K^T diag(e^(G_C - G)) U;
+// without the delta rule U = V. T and P need no state: linattn_chunk_k makes, for all chunks at once, scale P T and
+// diag(e^(G_C - G)) T, the two products in which T is used. linattn_prompt_k then goes through a sequence's chunks in order.
 //
-// Precision. The states are fp32, and so is what makes them: a factor that is not a bf16 input (S0, T, U, V - ..) enters
-// its products as two bf16 pieces, hi + lo, which keep 16 bits and more (K and Q are bf16 already; hi lo and lo hi are
-// taken, lo lo is not). Differences of G are taken in 64 bits before they are rounded: after a long decay G is large, and
-// its fp32 steps would show in e^(G_i - G_j). Outputs are rounded to bf16, so what only they need is taken in bf16: S0 for
-// Q S0, P and U for P U.
+// Precision. The states are fp32, and so is what makes them: a factor that is not a bf16 input (S0, X, U, the products with
+// T) enters its products as two bf16 pieces, hi + lo, which keep 16 bits and more (K, Q and V are bf16 already).
+// Differences of G are taken in 64 bits before they are rounded: after a long decay G is large, and its fp32 steps would
+// show in e^(G_i - G_j).
 // A chunk with a value that is not finite, or a decay above 1, goes token by token (the same recurrence), so that nothing
 // reaches the tokens before it: in the products a zero above the diagonal times NaN would.
 
 constexpr int kChunk = 64;
 constexpr float kMinDecay = -200.f;  // e^-200 is 0 in fp32: -infinity does no worse, and differences of sums stay numbers
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(4))) const int32_t* const_ints;
 
-// What a chunk of a head leaves for linattn_prompt_k: A operands of 16 x 32 products, one lane's 8 values after the other.
-// The operand (it, ks) covers tokens 16 it .. + 15 against tokens 32 ks .. + 31, the latter in the order in which a lane
-// holds the other factor: 4 of the first 16, 4 of the second. Those above the diagonal are left out: (0, 0), (1, 0),
-// (2, 0), (2, 1), (3, 0), (3, 1).
+// Rows t0 .. t0 + cnt - 1 of one head of x [R, heads, 128] as a buffer: rows behind them read as zeros, and what is stored
+// there goes nowhere, without a branch.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t head_rows(const void* x, int64_t t0, int cnt, int heads, int h) {
+  return make_rsrc(static_cast<const uint16_t*>(x) + (t0 * heads + h) * kHD, ((int64_t)(cnt - 1) * heads + 1) * kHD * 2);
+}
+
+// What a chunk of a head leaves for linattn_prompt_k, in the order in which it goes to LDS. The matrices are A operands of
+// 16 x 32 products, one lane's 8 values after the other, hi and lo: operand (it, ks) covers tokens 16 it .. + 15 against
+// tokens 32 ks .. + 31, the latter in the order in which a lane holds the other factor: 4 of the first 16, 4 of the
+// second. Those above the diagonal are left out: (0, 0), (1, 0), (2, 0), (2, 1), (3, 0), (3, 1) are here.
 struct ChunkWork {
-  uint16_t P[6][64][8];
-  float from[kChunk], to[kChunk];  // e^G, e^(G_C - G)
-  float all;                       // e^(G_C)
-  int32_t odd;                     // token by token
-  int32_t pad[2];
-  uint16_t T[2][6][64][8];         // hi, lo; the delta rule's last part
+  float from[kChunk], out[kChunk], to[kChunk];  // e^G, scale e^G, e^(G_C - G)
+  float all;                                    // e^(G_C)
+  int32_t odd;                                  // token by token
+  int32_t pad[62];
+  uint16_t P[2][6][64][8];                      // scale P T (without the delta rule scale P)
+  uint16_t T[2][6][64][8];                      // diag(to) T; the delta rule's last part
 };
-constexpr int64_t kPlainBytes = (int64_t)offsetof(ChunkWork, T);
-__host__ __device__ constexpr int64_t chunk_bytes(bool delta) { return delta ? (int64_t)sizeof(ChunkWork) : kPlainBytes; }
+static_assert(offsetof(ChunkWork, P) == 1024, "whole 1-KB pieces");
+constexpr int chunk_bytes(bool delta) { return delta ? (int)sizeof(ChunkWork) : (int)offsetof(ChunkWork, T); }
 __device__ __forceinline__ constexpr int frag(int it, int ks) { return it < 2 ? it : 2 * it - 2 + ks; }
 
 __device__ __forceinline__ int seq_chunks(int n) { return (n + kChunk - 1) / kChunk; }
@@ -185,14 +190,11 @@ __device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8& h
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float x = i < 2 ? a[2 * i] : b[2 * i - 4], y = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
-    h[i] = pack2(x, y);
-    l[i] = pack2(x - __uint_as_float(h[i] << 16), y - __uint_as_float(h[i] & 0xffff0000u));
+    h[i] = cvt_pk2(x, y);
+    l[i] = cvt_pk2(x - __uint_as_float(h[i] << 16), y - __uint_as_float(h[i] & 0xffff0000u));
   }
   hi = __builtin_bit_cast(bf16x8, make_uint4(h[0], h[1], h[2], h[3]));
   lo = __builtin_bit_cast(bf16x8, make_uint4(l[0], l[1], l[2], l[3]));
-}
-__device__ __forceinline__ bf16x8 round8(const f32x4& a, const f32x4& b) {
-  return __builtin_bit_cast(bf16x8, make_uint4(pack2(a[0], a[1]), pack2(a[2], a[3]), pack2(b[0], b[1]), pack2(b[2], b[3])));
 }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -215,7 +217,8 @@ template <bool DELTA>
 __global__ void __launch_bounds__(256) linattn_chunk_k(LinParams p) {
   constexpr int LD = 68;  // LDS row of 64 floats
   __shared__ __attribute__((aligned(16))) float Pt[64 * LD], At[DELTA ? 64 * LD : 1], Tt[DELTA ? 64 * LD : 1];
-  __shared__ int odd_at[4];
+  __shared__ float to_end[64];
+  __shared__ int odd_at;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t chunk = blockIdx.x / p.HV;
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(256) linattn_chunk_k(LinParams p) {
   SeqPlace at;
   if (!seq_find(p.seq_ptr, p.S, p.R, seq_chunks, [=](int, int upto) { return upto > (int)chunk; }, at)) return;
   const int t0 = at.first + ((int)chunk - at.before) * kChunk, cnt = min(kChunk, at.first + at.n - t0);
-  ChunkWork* const out = reinterpret_cast<ChunkWork*>(p.work + (chunk * p.HV + h) * chunk_bytes(DELTA));
+  ChunkWork* const out = reinterpret_cast<ChunkWork*>(p.work + (chunk * p.HV + h) * (int64_t)chunk_bytes(DELTA));
 
   // a token a lane: decays and strengths; tokens behind the end add nothing
   const bool on = lane < cnt;
@@ -237,19 +240,27 @@ __global__ void __launch_bounds__(256) linattn_chunk_k(LinParams p) {
     const double t = __shfl_up(G, o);
     if (lane >= o) G += t;
   }
+  if (w == 0) {
+    to_end[lane] = expf((float)(__shfl(G, 63) - G));
+    if (lane == 0) odd_at = 0;
+  }
 
-  const auto rows = [&](const uint16_t* x, int tile, int s) {
-    const int t = tile * 16 + c;
-    return t < cnt ? *reinterpret_cast<const bf16x8*>(x + ((int64_t)(t0 + t) * p.HK + hk) * kHD + s * 32 + g * 8)
-                   : bf16x8{};
+  const __amdgpu_buffer_rsrc_t kr = head_rows(p.k, t0, cnt, p.HK, hk), qr = head_rows(p.q, t0, cnt, p.HK, hk);
+  const auto rows = [&](__amdgpu_buffer_rsrc_t x, int tile, int s) {
+    return __builtin_bit_cast(bf16x8, bload(x, (uint32_t)(tile * 16 + c) * (p.HK * kHD * 2) + s * 64 + g * 16));
   };
-  bf16x8 ka[4], qa[4];
+  bf16x8 ka[4], qa[4], kb[4][4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
-    ka[s] = rows(p.k, w, s);
-    qa[s] = rows(p.q, w, s);
-    odd |= odd8(ka[s]) || odd8(qa[s]);
+    ka[s] = rows(kr, w, s);
+    qa[s] = rows(qr, w, s);
   }
+#pragma unroll
+  for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) kb[jt][s] = rows(kr, jt, s);
+#pragma unroll
+  for (int s = 0; s < 4; ++s) odd |= odd8(ka[s]) || odd8(qa[s]);
   double Gi[4];
   float bi[4];
 #pragma unroll
@@ -268,9 +279,8 @@ __global__ void __launch_bounds__(256) linattn_chunk_k(LinParams p) {
     f32x4 kk{}, qk{};
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const bf16x8 kb = rows(p.k, jt, s);
-      if (DELTA) kk = mfma(ka[s], kb, kk);
-      qk = mfma(qa[s], kb, qk);
+      if (DELTA) kk = mfma(ka[s], kb[jt][s], kk);
+      qk = mfma(qa[s], kb[jt][s], qk);
     }
     const double Gj = __shfl(G, jt * 16 + c);
 #pragma unroll
@@ -318,54 +328,103 @@ __global__ void __launch_bounds__(256) linattn_chunk_k(LinParams p) {
         t[i] = -neg;
       }
     }
+    // scale P T and diag(to) T, block column w
     const float bj = __shfl(beta, w * 16 + c);
-    __syncthreads();  // the diagonal blocks have been read
+    f32x4 pt[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t[i] *= bj;
+      pt[i] = f32x4{};
+#pragma unroll
+      for (int k = 0; k <= i; ++k) {
+        if (k < w) continue;
+        const f32x4 a = *reinterpret_cast<const f32x4*>(Pt + (i * 16 + c) * LD + k * 16 + g * 4);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) pt[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], t[k][s], pt[i], 0, 0, 0);
+      }
+    }
+    __syncthreads();  // A, P and the diagonal blocks have been read
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float v = t[i][r] * bj;
-        odd |= !(fabsf(v) < INFINITY);
-        Tt[(i * 16 + g * 4 + r) * LD + w * 16 + c] = v;
+        const int row = i * 16 + g * 4 + r;
+        odd |= !(fabsf(t[i][r]) < INFINITY) || !(fabsf(pt[i][r]) < INFINITY);
+        Tt[row * LD + w * 16 + c] = t[i][r] * to_end[row];
+        Pt[row * LD + w * 16 + c] = pt[i][r];
       }
   }
-  if (lane == 0) odd_at[w] = 0;
-  if (__any(odd) && lane == 0) odd_at[w] = 1;
+  if (!DELTA) __syncthreads();
+  if (__any(odd) && lane == 0) atomicOr(&odd_at, 1);
   __syncthreads();
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
     if (ks > (w >> 1)) continue;
     const int at = (w * 16 + c) * LD + ks * 32 + g * 4;
-    const f32x4 a = *reinterpret_cast<const f32x4*>(Pt + at), b = *reinterpret_cast<const f32x4*>(Pt + at + 16);
-    *reinterpret_cast<bf16x8*>(out->P[frag(w, ks)][lane]) = round8(a, b);
+    bf16x8 hi, lo;
+    split8(*reinterpret_cast<const f32x4*>(Pt + at) * p.scale, *reinterpret_cast<const f32x4*>(Pt + at + 16) * p.scale, hi,
+           lo);
+    *reinterpret_cast<bf16x8*>(out->P[0][frag(w, ks)][lane]) = hi;
+    *reinterpret_cast<bf16x8*>(out->P[1][frag(w, ks)][lane]) = lo;
     if (DELTA) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(Tt + at), y = *reinterpret_cast<const f32x4*>(Tt + at + 16);
-      bf16x8 hi, lo;
-      split8(x, y, hi, lo);
+      split8(*reinterpret_cast<const f32x4*>(Tt + at), *reinterpret_cast<const f32x4*>(Tt + at + 16), hi, lo);
       *reinterpret_cast<bf16x8*>(out->T[0][frag(w, ks)][lane]) = hi;
       *reinterpret_cast<bf16x8*>(out->T[1][frag(w, ks)][lane]) = lo;
     }
   }
   if (w != 0) return;
-  const double last = __shfl(G, 63);
-  out->from[lane] = expf((float)G);
-  out->to[lane] = expf((float)(last - G));
-  if (lane == 0) {
-    out->all = expf((float)last);
-    out->odd = odd_at[0] | odd_at[1] | odd_at[2] | odd_at[3];
+  const float e = expf((float)G);
+  out->from[lane] = e;
+  out->out[lane] = p.scale * e;
+  out->to[lane] = to_end[lane];
+  if (lane == 63) {
+    out->all = e;
+    out->odd = odd_at;
   }
 }
 
 // The chunks of one sequence and value head in order. A wave has 16 CT value dims of the state, all 128 key dims: 8 CT
-// accumulators, lane (c, g) holding key dims 16 d + 4 g .. + 3 of value dim c. As the B operand of K S0 and Q S0 that is the
-// contraction in the order 4 of one 16, 4 of the next, so K and Q come as two 8-byte pieces, and nothing of the state, of
-// U or of V - .. ever leaves its lane: the waves share only K and Q, through LDS, and meet once a chunk. K^T comes from
-// the same LDS rows by transposing reads. Every operand of the next chunk is loaded where the present one's has been used.
+// accumulators, d of them with key dims key_dim(d, g) .. + 3 in the lanes (c, g) of value dim c. Two of them together are
+// then the B operand of K S0 and Q S0 for 32 key dims in order, and nothing of the state, of X or of U ever leaves its
+// lane. What the waves share, K, Q, V and the chunk's matrices, comes by LDS DMA one chunk ahead; they meet once a chunk.
+// K^T and V's columns come from the same rows by transposing reads (16 lanes get 4 rows x 16 columns column by column,
+// the columns in any groups of 4). 16-byte piece x of a row r of K and Q lies at x ^ swizzle(r), so that both kinds of
+// reads spread over the banks.
+__device__ __forceinline__ constexpr int key_dim(int d, int g) { return (d >> 1) * 32 + g * 8 + (d & 1) * 4; }
+__device__ __forceinline__ constexpr int swizzle(int r) { return (r & 7) << 1 | (r >> 3 & 1); }
+
+// Eight transposing reads, at a + x and b + x for four x. (The builtin makes the compiler wait for every LDS DMA in flight,
+// the next chunk's among them; the wait for the reads themselves is in the block, so that the registers are filled when it
+// ends.)
+template <int X0, int X1, int X2, int X3>
+__device__ __forceinline__ void tr_read8(const uint8_t* pa, const uint8_t* pb, bf16x4 (&a)[4], bf16x4 (&b)[4]) {
+  const uint32_t x = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)pa;
+  const uint32_t y = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)pb;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %4, %9 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %6, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(b[0]), "=&v"(b[1]), "=&v"(b[2]), "=&v"(b[3])
+      : "v"(x), "v"(y), "n"(X0), "n"(X1), "n"(X2), "n"(X3)
+      : "memory");
+}
+// Every wave's LDS reads of the stage before are done, and what its own wait has seen land is there for all; global loads
+// and DMAs stay in flight.
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 template <bool DELTA, int CT>
 __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
-  constexpr int LD = kHD + 8;  // LDS row
-  __shared__ __attribute__((aligned(16))) uint16_t kq[2][2][kChunk * LD];
-  constexpr int SL = 2 / CT;  // workgroups of a head
+  constexpr int SL = 2 / CT;             // workgroups of a head
+  constexpr int VB = 128 * CT;           // bytes of a V row: the workgroup's 64 CT value dims
+  constexpr int WB = chunk_bytes(DELTA);
+  constexpr int KO = WB, QO = KO + kChunk * 256, VO = QO + kChunk * 256, STAGE = VO + kChunk * VB;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t sq = blockIdx.x / (p.HV * SL);
@@ -382,106 +441,112 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   if (!seq_find(p.seq_ptr, p.S, p.R, seq_chunks, [=](int i, int) { return i == (int)sq; }, place)) return;
   const int first = place.first, n = place.n;
   const int chunks = seq_chunks(n);
-  const int dv = ((hs % SL) * 4 + wave) * 16 * CT + c;  // + 16 ct
+  const int dv0 = (hs % SL) * 64 * CT, dv = dv0 + wave * 16 * CT + c;  // + 16 ct
+
+  // the next chunk to an LDS stage: this wave's 16 rows of K and Q, its part of V and of the chunk's matrices
+  const uint8_t* work = p.work + ((int64_t)place.before * p.HV + h) * (int64_t)WB;
+  const int64_t next_work = (int64_t)p.HV * WB;
+  uint32_t koff[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * i + g;
+    koff[i] = (uint32_t)(wave * 16 + r) * (p.HK * kHD * 2) + (c ^ swizzle(r)) * 16;
+  }
+  constexpr int VL = VB / 16;  // lanes of a V row
+  const uint32_t voff = (uint32_t)(wave * 16 + lane / VL) * (p.HV * kHD * 2) + (lane % VL) * 16;
+  const auto fetch = [&](int t, uint8_t* stage) {  // first token of the chunk
+    const int cnt = min(kChunk, n - t);
+    const __amdgpu_buffer_rsrc_t kr = head_rows(p.k, first + t, cnt, p.HK, hk);
+    const __amdgpu_buffer_rsrc_t qr = head_rows(p.q, first + t, cnt, p.HK, hk);
+    const __amdgpu_buffer_rsrc_t vr = make_rsrc(p.v + ((int64_t)(first + t) * p.HV + h) * kHD + dv0,
+                                                ((int64_t)(cnt - 1) * p.HV * kHD + 64 * CT) * 2);
+    const __amdgpu_buffer_rsrc_t wr = make_rsrc(work, WB);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      dma16(kr, stage + KO + wave * 4096 + i * 1024, koff[i]);
+      dma16(qr, stage + QO + wave * 4096 + i * 1024, koff[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * CT; ++i)
+      dma16(vr, stage + VO + wave * (16 * VB) + i * 1024, voff + (uint32_t)(i * 64 / VL) * (p.HV * kHD * 2));
+#pragma unroll
+    for (int i = 0; i < (WB / 1024 + 3) / 4; ++i) {
+      const int at = min(i * 4 + wave, WB / 1024 - 1) * 1024;  // past the last piece: that one again
+      dma16(wr, stage + at, at + lane * 16);
+    }
+    work += next_work;
+  };
+  if (chunks > 0) fetch(0, smem);
 
   f32x4 st[8][CT];
   {
     int64_t at = -1;
     if (p.state != nullptr) at = p.src != nullptr ? (int64_t)p.src[sq] : sq;
-    const bool have = at >= 0 && at < p.slots;
     const float fill = at >= p.slots ? __uint_as_float(0x7fc00000u) : 0.f;
+    if (at >= 0 && at < p.slots) {
 #pragma unroll
-    for (int d = 0; d < 8; ++d)
+      for (int d = 0; d < 8; ++d)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+        for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          st[d][ct][r] =
-              have ? p.state[(at * p.HV + h) * (kHD * kHD) + (d * 16 + g * 4 + r) * kHD + dv + ct * 16] : fill;
-  }
-  const uint8_t* work = p.work + ((int64_t)place.before * p.HV + h) * chunk_bytes(DELTA);
-  const int64_t next_work = p.HV * chunk_bytes(DELTA);
-
-  // K and Q rows of a chunk: 16-byte pieces, zeros behind the sequence's end
-  uint4 kx[4], qx[4];
-  const auto load_kq = [&](int t) {  // first token of the chunk
+          for (int r = 0; r < 4; ++r)
+            st[d][ct][r] = p.state[(at * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv + ct * 16];
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int piece = i * 256 + threadIdx.x, r = t + (piece >> 4);
-      const int64_t at = ((int64_t)(first + r) * p.HK + hk) * kHD + (piece & 15) * 8;
-      kx[i] = r < n ? *reinterpret_cast<const uint4*>(p.k + at) : make_uint4(0u, 0u, 0u, 0u);
-      qx[i] = r < n ? *reinterpret_cast<const uint4*>(p.q + at) : make_uint4(0u, 0u, 0u, 0u);
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) st[d][ct] = f32x4{fill, fill, fill, fill};
     }
-  };
-  const auto store_kq = [&](int half) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int piece = i * 256 + threadIdx.x, at = (piece >> 4) * LD + (piece & 15) * 8;
-      *reinterpret_cast<uint4*>(kq[half][0] + at) = kx[i];
-      *reinterpret_cast<uint4*>(kq[half][1] + at) = qx[i];
-    }
-  };
-  uint32_t vx[4][4][CT];
-  const auto load_v = [&](int t) {
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const int tk = t + it * 16 + g * 4 + r;
-          vx[it][r][ct] = tk < n ? p.v[((int64_t)(first + tk) * p.HV + h) * kHD + dv + ct * 16] : 0u;
-        }
-  };
-  bf16x8 T[2][6], P[6];
-  f32x4 from[4], to[4];
-  float all = 0.f;
-  int odd = 0;
-  const auto cw = [&](const uint8_t* at) { return reinterpret_cast<const ChunkWork*>(at); };
-  const auto load_T = [&](const ChunkWork* x) {
-    if (DELTA)
-#pragma unroll
-      for (int f = 0; f < 6; ++f) {
-        T[0][f] = *reinterpret_cast<const bf16x8*>(x->T[0][f][lane]);
-        T[1][f] = *reinterpret_cast<const bf16x8*>(x->T[1][f][lane]);
-      }
-  };
-  const auto load_P = [&](const ChunkWork* x) {
-#pragma unroll
-    for (int f = 0; f < 6; ++f) P[f] = *reinterpret_cast<const bf16x8*>(x->P[f][lane]);
-#pragma unroll
-    for (int it = 0; it < 4; ++it) from[it] = *reinterpret_cast<const f32x4*>(x->from + it * 16 + g * 4);
-  };
-  const auto load_to = [&](const ChunkWork* x) {
-#pragma unroll
-    for (int it = 0; it < 4; ++it) to[it] = *reinterpret_cast<const f32x4*>(x->to + it * 16 + g * 4);
-    all = x->all;
-    odd = x->odd;
-  };
-
-  if (chunks > 0) {
-    load_kq(0);
-    load_v(0);
-    load_T(cw(work));
-    load_P(cw(work));
-    load_to(cw(work));
-    store_kq(0);
   }
+
+  // LDS offsets of this lane: rows c of K and Q, key dims 32 s .. + 31; K's rows read transposed, the same key dims
+  int aoff[4], toff[4];
+  const int trow = g * 4 + (c >> 2);
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    aoff[s] = c * 256 + ((s * 4 + g) ^ swizzle(c)) * 16;
+    toff[s] = KO + trow * 256 + ((s * 4 + (c & 3)) ^ swizzle(trow)) * 16;
+  }
+  const int vtoff = trow * VB + wave * 32 * CT + (c & 3) * 8;  // + 32 ct + row * VB
+  const auto rd16 = [](const uint8_t* a) { return *reinterpret_cast<const bf16x8*>(a); };
+  const auto join = [](bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); };
+
+  // vmcnt(0), as the compiler knows it: the state is there, and no wait for it, which would take the DMAs along, is left
+  // for the loop
+  __builtin_amdgcn_s_waitcnt(0x0f70);
   for (int ch = 0; ch < chunks; ++ch) {
-    const int t0 = ch * kChunk, half = ch & 1, cnt = min(kChunk, n - t0);
-    const bool more = ch + 1 < chunks;
-    const ChunkWork* const next = cw(work + next_work);
-    const uint16_t* const kl = kq[half][0];
-    const uint16_t* const ql = kq[half][1];
-    __syncthreads();
-    if (more) load_kq(t0 + kChunk);
-    bool slow = odd != 0;
+    const int t0 = ch * kChunk, cnt = min(kChunk, n - t0);
+    const uint8_t* const stage = smem + (ch & 1) * STAGE;
+    const ChunkWork& cw = *reinterpret_cast<const ChunkWork*>(stage);
+    if (ch > 0) wait_vmcnt<16 * CT>();  // all but the last chunk's output stores
+    stage_barrier();          // the stage has landed, and every wave is done with the other one
+    if (ch + 1 < chunks) fetch(t0 + kChunk, smem + ((ch + 1) & 1) * STAGE);
+
+    // V's columns: X's accumulators' places, and its B operand
+    bf16x4 vt[CT][4];
+    {
+      const uint8_t* const va = stage + VO + vtoff;
+      if constexpr (CT == 2) {
+        tr_read8<0, 16 * VB, 32 * VB, 48 * VB>(va, va + 32, vt[0], vt[1]);
+      } else {
+        bf16x4 a[4], b[4];
+        tr_read8<0, 8, 16 * VB, 16 * VB + 8>(va, va + 32 * VB, a, b);
+        vt[0][0] = a[0], vt[0][1] = a[2], vt[0][2] = b[0], vt[0][3] = b[2];
+      }
+    }
+    uint32_t top = 0;
 #pragma unroll
     for (int it = 0; it < 4; ++it)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) slow |= (vx[it][r][ct] & 0x7f80u) == 0x7f80u;
+      for (int ct = 0; ct < CT; ++ct) {
+        const uint2 x = __builtin_bit_cast(uint2, vt[ct][it]);
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                                     __builtin_bit_cast(u16x2, x.x & 0x7fff7fffu)));
+        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                                     __builtin_bit_cast(u16x2, x.y & 0x7fff7fffu)));
+      }
+    const bool slow = cw.odd != 0 || (top & 0xffffu) >= 0x7f80u || top >= 0x7f800000u;
     if (__any(slow)) {
       for (int t = 0; t < cnt; ++t) {
         const int64_t row = (int64_t)(first + t0 + t) * p.HV + h;
@@ -489,8 +554,9 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         bf16x4 kt[8], qt[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          kt[d] = *reinterpret_cast<const bf16x4*>(kl + t * LD + d * 16 + g * 4);
-          qt[d] = *reinterpret_cast<const bf16x4*>(ql + t * LD + d * 16 + g * 4);
+          const uint8_t* const x = stage + t * 256 + (((d >> 1) * 4 + g) ^ swizzle(t & 15)) * 16 + (d & 1) * 8;
+          kt[d] = *reinterpret_cast<const bf16x4*>(x + KO);
+          qt[d] = *reinterpret_cast<const bf16x4*>(x + QO);
         }
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
@@ -516,123 +582,148 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
           if (g == 0) p.o[row * kHD + dv + ct * 16] = (uint16_t)f2bf(p.scale * o);
         }
       }
-      if (more) {
-        load_v(t0 + kChunk);
-        load_T(next);
-        load_P(next);
-        load_to(next);
-      }
-    } else {
-      bf16x8 sh[4][CT], sl[4][CT];
+      wait_vmcnt<0>();
+      continue;
+    }
+
+    bf16x8 sh[4][CT], sl[4][CT];
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) split8(st[2 * s][ct], st[2 * s + 1][ct], sh[s][ct], sl[s][ct]);
-      f32x4 ks[4][CT], qs[4][CT];
+      for (int ct = 0; ct < CT; ++ct) split8(st[2 * s][ct], st[2 * s + 1][ct], sh[s][ct], sl[s][ct]);
+    bf16x8 xh[2][CT], xl[2][CT];  // X, or V itself
+    if (DELTA) {
+      f32x4 x[4][CT];
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) ks[it][ct] = qs[it][ct] = f32x4{};
+        for (int ct = 0; ct < CT; ++ct) x[it][ct] = f32x4{};
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const int at = (it * 16 + c) * LD + s * 32 + g * 4;
-          if (DELTA) {
-            const bf16x8 a = __builtin_shufflevector(*reinterpret_cast<const bf16x4*>(kl + at),
-                                                     *reinterpret_cast<const bf16x4*>(kl + at + 16), 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              ks[it][ct] = mfma(a, sh[s][ct], ks[it][ct]);
-              ks[it][ct] = mfma(a, sl[s][ct], ks[it][ct]);
-            }
-          }
-          const bf16x8 b = __builtin_shufflevector(*reinterpret_cast<const bf16x4*>(ql + at),
-                                                   *reinterpret_cast<const bf16x4*>(ql + at + 16), 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) qs[it][ct] = mfma(b, sh[s][ct], qs[it][ct]);
-        }
-      }
-      f32x4 u[4][CT];
-#pragma unroll
-      for (int it = 0; it < 4; ++it)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float v = bf2f(vx[it][r][ct]);
-            u[it][ct][r] = DELTA ? v - from[it][r] * ks[it][ct][r] : v;
-          }
-      if (more) load_v(t0 + kChunk);
-      if (DELTA) {
-        bf16x8 rh[2][CT], rl[2][CT];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) split8(u[2 * k][ct], u[2 * k + 1][ct], rh[k][ct], rl[k][ct]);
-#pragma unroll
-        for (int it = 0; it < 4; ++it)
+          const bf16x8 a = rd16(stage + KO + it * 4096 + aoff[s]);
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {
-            f32x4 x{};
-#pragma unroll
-            for (int k = 0; k <= it / 2; ++k) {
-              x = mfma(T[0][frag(it, k)], rh[k][ct], x);
-              x = mfma(T[0][frag(it, k)], rl[k][ct], x);
-              x = mfma(T[1][frag(it, k)], rh[k][ct], x);
-            }
-            u[it][ct] = x;
+            x[it][ct] = mfma(a, sh[s][ct], x[it][ct]);
+            x[it][ct] = mfma(a, sl[s][ct], x[it][ct]);
           }
-        if (more) load_T(next);
+        }
+        const f32x4 f = *reinterpret_cast<const f32x4*>(cw.from + it * 16 + g * 4);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const uint2 v = __builtin_bit_cast(uint2, vt[ct][it]);
+          x[it][ct] = f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                            __uint_as_float(v.y & 0xffff0000u)} -
+                      f * x[it][ct];
+        }
       }
-      // the state
-      bf16x8 uh[2][CT], ul[2][CT], ub[2][CT];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          ub[k][ct] = round8(u[2 * k][ct], u[2 * k + 1][ct]);
-          split8(u[2 * k][ct] * to[2 * k], u[2 * k + 1][ct] * to[2 * k + 1], uh[k][ct], ul[k][ct]);
-        }
-      const uint16_t* const kt = kl + (g * 4 + (c >> 2)) * LD + (c & 3) * 4;
+        for (int ct = 0; ct < CT; ++ct) split8(x[2 * k][ct], x[2 * k + 1][ct], xh[k][ct], xl[k][ct]);
+    } else {
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) st[d][ct] *= all;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-              (__attribute__((address_space(3))) bf16x4*)(kt + k * 32 * LD + d * 16));
-          const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-              (__attribute__((address_space(3))) bf16x4*)(kt + (k * 32 + 16) * LD + d * 16));
-          const bf16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            st[d][ct] = mfma(a, uh[k][ct], st[d][ct]);
-            st[d][ct] = mfma(a, ul[k][ct], st[d][ct]);
-          }
-        }
-      }
-      // the outputs
+        for (int ct = 0; ct < CT; ++ct) xh[k][ct] = join(vt[ct][2 * k], vt[ct][2 * k + 1]);
+    }
+    // the decayed U, and the state
+    bf16x8 uh[2][CT], ul[2][CT];
+    {
+      f32x4 u[4][CT];
 #pragma unroll
       for (int it = 0; it < 4; ++it)
+        if (DELTA) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          f32x4 x = qs[it][ct] * from[it];
+          for (int ct = 0; ct < CT; ++ct) u[it][ct] = f32x4{};
 #pragma unroll
-          for (int k = 0; k <= it / 2; ++k) x = mfma(P[frag(it, k)], ub[k][ct], x);
+          for (int k = 0; k <= it / 2; ++k) {
+            const bf16x8 th = rd16(reinterpret_cast<const uint8_t*>(cw.T[0][frag(it, k)][lane]));
+            const bf16x8 tl = rd16(reinterpret_cast<const uint8_t*>(cw.T[1][frag(it, k)][lane]));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int tk = it * 16 + g * 4 + r;
-            if (tk < cnt)
-              p.o[((int64_t)(first + t0 + tk) * p.HV + h) * kHD + dv + ct * 16] = (uint16_t)f2bf(p.scale * x[r]);
+            for (int ct = 0; ct < CT; ++ct) {
+              u[it][ct] = mfma(th, xh[k][ct], u[it][ct]);
+              u[it][ct] = mfma(th, xl[k][ct], u[it][ct]);
+              u[it][ct] = mfma(tl, xh[k][ct], u[it][ct]);
+              u[it][ct] = mfma(tl, xl[k][ct], u[it][ct]);
+            }
+          }
+        } else {
+          const f32x4 f = *reinterpret_cast<const f32x4*>(cw.to + it * 16 + g * 4);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            const uint2 v = __builtin_bit_cast(uint2, vt[ct][it]);
+            u[it][ct] = f * f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u),
+                                  __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
           }
         }
-      if (more) {
-        load_P(next);
-        load_to(next);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) split8(u[2 * k][ct], u[2 * k + 1][ct], uh[k][ct], ul[k][ct]);
+    }
+    const float all = cw.all;
+    bf16x4 ka[2][4], kb[2][4];
+    tr_read8<0, 4096, 8192, 12288>(stage + toff[0], stage + toff[0] + 8, ka[0], kb[0]);
+#pragma unroll
+    for (int d = 0; d < 8; d += 2) {
+      const int now = d / 2 & 1;
+      if (d < 6) {
+        const uint8_t* const ta = stage + toff[d < 6 ? d / 2 + 1 : 0];
+        tr_read8<0, 4096, 8192, 12288>(ta, ta + 8, ka[now ^ 1], kb[now ^ 1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) st[d + e][ct] *= all;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const bf16x8 a = e == 0 ? join(ka[now][2 * k], ka[now][2 * k + 1]) : join(kb[now][2 * k], kb[now][2 * k + 1]);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            st[d + e][ct] = mfma(a, uh[k][ct], st[d + e][ct]);
+            st[d + e][ct] = mfma(a, ul[k][ct], st[d + e][ct]);
+          }
+        }
       }
     }
-    if (more) store_kq(half ^ 1);
-    work += next_work;
+    // the outputs
+    const __amdgpu_buffer_rsrc_t orow = head_rows(p.o, first + t0, cnt, p.HV, h);
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      f32x4 x[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) x[ct] = f32x4{};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const bf16x8 a = rd16(stage + QO + it * 4096 + aoff[s]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          x[ct] = mfma(a, sh[s][ct], x[ct]);
+          x[ct] = mfma(a, sl[s][ct], x[ct]);
+        }
+      }
+      const f32x4 f = *reinterpret_cast<const f32x4*>(cw.out + it * 16 + g * 4);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) x[ct] *= f;
+#pragma unroll
+      for (int k = 0; k <= it / 2; ++k) {
+        const bf16x8 ph = rd16(reinterpret_cast<const uint8_t*>(cw.P[0][frag(it, k)][lane]));
+        const bf16x8 pl = rd16(reinterpret_cast<const uint8_t*>(cw.P[1][frag(it, k)][lane]));
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          x[ct] = mfma(ph, xh[k][ct], x[ct]);
+          x[ct] = mfma(pl, xh[k][ct], x[ct]);
+          if (DELTA) x[ct] = mfma(ph, xl[k][ct], x[ct]);
+        }
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)f2bf(x[ct][r]), orow,
+                                                (uint32_t)(it * 16 + g * 4 + r) * (p.HV * kHD * 2) + (dv + ct * 16) * 2, 0,
+                                                0);
+    }
   }
 #pragma unroll
   for (int d = 0; d < 8; ++d)
@@ -640,8 +731,10 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        p.state_out[(sq * p.HV + h) * (kHD * kHD) + (d * 16 + g * 4 + r) * kHD + dv + ct * 16] = st[d][ct][r];
+        p.state_out[(sq * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv + ct * 16] = st[d][ct][r];
 }
+
+constexpr int prompt_lds(bool delta, int ct) { return 2 * (chunk_bytes(delta) + kChunk * (512 + 128 * ct)); }
 
 }  // namespace
 
@@ -654,7 +747,7 @@ hipError_t launch_linattn_step(const LinParams& p, float* state, const int32_t* 
 int64_t linattn_chunks(int64_t R, int64_t S) { return R / kChunk + std::min(R, S); }
 
 int64_t linattn_work_bytes(int64_t R, int64_t S, int HV, bool delta) {
-  return linattn_chunks(R, S) * HV * chunk_bytes(delta);
+  return linattn_chunks(R, S) * HV * (int64_t)chunk_bytes(delta);
 }
 
 hipError_t launch_linattn_prompt(const LinParams& p, hipStream_t st) {
@@ -672,7 +765,19 @@ hipError_t launch_linattn_prompt(const LinParams& p, hipStream_t st) {
   const bool wide = p.S * p.HV >= 256;
   const auto kernel = delta ? (wide ? linattn_prompt_k<true, 2> : linattn_prompt_k<true, 1>)
                             : (wide ? linattn_prompt_k<false, 2> : linattn_prompt_k<false, 1>);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.S + 1) * p.HV * (wide ? 1 : 2))), dim3(256), 0, st, p);
+  const int lds = prompt_lds(delta, wide ? 2 : 1);
+  // once for each device and kernel; a second thread that comes meanwhile sets the same again
+  static std::atomic<bool> set[64][4];
+  int dev = 0;
+  hipError_t err = hipGetDevice(&dev);
+  if (err != hipSuccess) return err;
+  std::atomic<bool>* const done = dev >= 0 && dev < 64 ? &set[dev][delta * 2 + wide] : nullptr;
+  if (done == nullptr || !done->load(std::memory_order_acquire)) {
+    err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (err != hipSuccess) return err;
+    if (done != nullptr) done->store(true, std::memory_order_release);
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.S + 1) * p.HV * (wide ? 1 : 2))), dim3(256), lds, st, p);
   return hipGetLastError();
 }
 

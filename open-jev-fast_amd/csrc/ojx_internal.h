@@ -24,6 +24,14 @@ __device__ __forceinline__ float sigmoid_f(float x) { return 1.0f / (1.0f + expf
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) { return f2bf(a) | (f2bf(b) << 16); }
 
+// The same pair as one conversion (the compiler does not join pack2's two; the attention cores convert their operands in
+// the inner loops).
+__device__ __forceinline__ uint32_t cvt_pk2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
 // Sum over the wave's 64 lanes, in every lane: the xor butterfly 32, 16, 8, 4, 2, 1 without its six LDS round trips
 // (a __shfl_xor each). The lane swaps give each lane its partner's half; from step 8 down the values repeat every
 // 16, 8, 4, 2 lanes of a row, so that a rotation within the row of 16 brings the xor partner's value. Every addition

@@ -25,7 +25,7 @@
 // take the values of places that nobody sees as zeros and, where a value is not finite, add position by position, so that
 // a NaN reaches the rows that see it and no other.
 // Where sequences and row blocks are few, the positions are split over more workgroups, whose sums a second launch joins.
-#include "ojx_internal.h"
+#include "gemm_common.h"
 
 #include <algorithm>
 
@@ -33,10 +33,8 @@ namespace ojx {
 
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(4))) const int32_t* const_ints;  // read-only: scalar loads
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -114,7 +112,7 @@ __device__ __forceinline__ void load_q(const TreeParams& p, const Rows<CT>& w, i
 #pragma unroll
     for (int f = 0; f < D / 32; ++f) {
       const int d = paired ? (f >> 1) * 64 + g * 16 + (f & 1) * 8 : f * 32 + g * 8;
-      qf[ct][f] = w.live[ct] ? *reinterpret_cast<const bf16x8*>(src + d) : bf16x8{};
+      qf[ct][f] = *reinterpret_cast<const bf16x8*>(src + d);  // a column without a row repeats the first one's
     }
   }
 }
@@ -219,8 +217,8 @@ __device__ __forceinline__ void soft_weights(const TreeParams& p, const Rows<CT>
       w[ct][i] = e;
       if (FP8) w[ct][i] = edge && !(see >> ((i >> 2) * 16 + (i & 3)) & 1) ? 0.f : e * vq[i >> 2][i & 3];
     }
-    pf[ct] = __builtin_bit_cast(bf16x8, make_uint4(pack2(w[ct][0], w[ct][1]), pack2(w[ct][2], w[ct][3]),
-                                                   pack2(w[ct][4], w[ct][5]), pack2(w[ct][6], w[ct][7])));
+    pf[ct] = __builtin_bit_cast(bf16x8, make_uint4(cvt_pk2(w[ct][0], w[ct][1]), cvt_pk2(w[ct][2], w[ct][3]),
+                                                   cvt_pk2(w[ct][4], w[ct][5]), cvt_pk2(w[ct][6], w[ct][7])));
   }
 }
 
@@ -516,7 +514,7 @@ __global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) tree_wide_k(TreeParams p
     const int h = (u - w.u0) & 1;
     now[0] = ok[0];
     now[1] = ok[1];
-    __syncthreads();
+    lds_barrier();
     if (u + 1 < w.u1) load(u + 1);
     const uint16_t* const kl = buf[h] + c * KS + g * 8;
     f32x4 s[2][CT];
