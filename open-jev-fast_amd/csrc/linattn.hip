@@ -199,24 +199,50 @@ __device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8& h
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ bool odd8(bf16x8 x) {  // one of them is not finite
-  const uint4 u = __builtin_bit_cast(uint4, x);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  bool r = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
-  return r;
+// The sum of x over the lanes up to and including this one, in 64 bits, by lane shifts within rows of 16 and the rows' last
+// lanes handed on (a lane outside reads as zero).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)b, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+  return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+__device__ __forceinline__ double scan64(double x) {
+  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+  x = dpp_add<0x143, 0xc>(x);
+  return x;
+}
+// The largest magnitude of bf16 bits, two at a time.
+__device__ __forceinline__ uint32_t top2(uint32_t top, uint32_t x) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                                __builtin_bit_cast(u16x2, x & 0x7fff7fffu)));
+}
+__device__ __forceinline__ uint32_t top8(uint32_t top, bf16x8 x) {
+  const uint4 u = __builtin_bit_cast(uint4, x);
+  return top2(top2(top2(top2(top, u.x), u.y), u.z), u.w);
+}
+__device__ __forceinline__ bool odd_top(uint32_t top) { return (top & 0xffffu) >= 0x7f80u || top >= 0x7f800000u; }
 
 // T and P of one chunk and value head; wave w has the tokens 16 w .. + 15 as rows.
 //   * k . k and q . k on bf16 MFMA from the rows as they lie in memory;
 //   * (I + A)^-1 in blocks of 16: the diagonal ones by forward substitution, a column a lane; then block column w by wave
 //     w, T_iw = -T_ii (sum_k A_ik T_kw), on fp32 MFMA (16x16x4), whose B operand is the accumulator of the product before
-//     when the contraction runs in its order.
+//     when the contraction runs in its order; P T likewise.
+// LDS holds the ten lower blocks of each matrix, rows of 20 floats (so that 16 rows' 16-byte reads meet every bank once).
+// What bounds it: the chain of one chunk (loads, scan, substitution, up to 19 block products on one wave), so what counts
+// is how many workgroups a CU holds: four, by LDS and registers.
 template <bool DELTA>
-__global__ void __launch_bounds__(256) linattn_chunk_k(LinParams p) {
-  constexpr int LD = 68;  // LDS row of 64 floats
-  __shared__ __attribute__((aligned(16))) float Pt[64 * LD], At[DELTA ? 64 * LD : 1], Tt[DELTA ? 64 * LD : 1];
+__global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
+  constexpr int LD = 20, BLK = 16 * LD;
+  const auto lower = [](int i, int k) { return (i * (i + 1) / 2 + k) * BLK; };
+  __shared__ __attribute__((aligned(16))) float Pb[10 * BLK], Ab[DELTA ? 10 * BLK : 4], Db[DELTA ? 4 * BLK : 4];
+  __shared__ double Gs[4][64];  // every wave's own
   __shared__ float to_end[64];
   __shared__ int odd_at;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -228,83 +254,80 @@ __global__ void __launch_bounds__(256) linattn_chunk_k(LinParams p) {
   const int t0 = at.first + ((int)chunk - at.before) * kChunk, cnt = min(kChunk, at.first + at.n - t0);
   ChunkWork* const out = reinterpret_cast<ChunkWork*>(p.work + (chunk * p.HV + h) * (int64_t)chunk_bytes(DELTA));
 
-  // a token a lane: decays and strengths; tokens behind the end add nothing
-  const bool on = lane < cnt;
-  float gv = on ? p.g[(int64_t)(t0 + lane) * p.HV + h] : 0.f;
-  const float beta = DELTA && on ? bf2f(p.beta[(int64_t)(t0 + lane) * p.HV + h]) : 0.f;
-  bool odd = !(gv <= 0.f) || !(fabsf(beta) < INFINITY);
-  gv = gv < kMinDecay ? kMinDecay : gv;
-  double G = gv;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double t = __shfl_up(G, o);
-    if (lane >= o) G += t;
-  }
-  if (w == 0) {
-    to_end[lane] = expf((float)(__shfl(G, 63) - G));
-    if (lane == 0) odd_at = 0;
-  }
-
   const __amdgpu_buffer_rsrc_t kr = head_rows(p.k, t0, cnt, p.HK, hk), qr = head_rows(p.q, t0, cnt, p.HK, hk);
   const auto rows = [&](__amdgpu_buffer_rsrc_t x, int tile, int s) {
     return __builtin_bit_cast(bf16x8, bload(x, (uint32_t)(tile * 16 + c) * (p.HK * kHD * 2) + s * 64 + g * 16));
   };
-  bf16x8 ka[4], qa[4], kb[4][4];
+  bf16x8 ka[4], qa[4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     ka[s] = rows(kr, w, s);
     qa[s] = rows(qr, w, s);
   }
+  // a token a lane: decays, to base two, and strengths; tokens behind the end add nothing
+  const int64_t tok = (int64_t)(t0 + min(lane, cnt - 1)) * p.HV + h;
+  float gv = p.g[tok], beta = DELTA ? bf2f(p.beta[tok]) : 0.f;
+  if (lane >= cnt) gv = beta = 0.f;
+  bool odd = !(gv <= 0.f) || !(fabsf(beta) < INFINITY);
+  gv = gv < kMinDecay ? kMinDecay : gv;
+  const double G = scan64((double)gv * 1.4426950408889634074);
+  Gs[w][lane] = G;
+  if (w == 0) {
+    const double last = Gs[0][63];
+    to_end[lane] = __builtin_amdgcn_exp2f((float)(last - G));
+    if (lane == 0) odd_at = 0;
+  }
+  uint32_t top = 0;
 #pragma unroll
-  for (int jt = 0; jt < 4; ++jt)
-#pragma unroll
-    for (int s = 0; s < 4; ++s) kb[jt][s] = rows(kr, jt, s);
-#pragma unroll
-  for (int s = 0; s < 4; ++s) odd |= odd8(ka[s]) || odd8(qa[s]);
+  for (int s = 0; s < 4; ++s) top = top8(top8(top, ka[s]), qa[s]);
+  odd |= odd_top(top);
+
   double Gi[4];
   float bi[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    Gi[r] = __shfl(G, w * 16 + g * 4 + r);
-    bi[r] = __shfl(beta, w * 16 + g * 4 + r);
+    Gi[r] = Gs[w][w * 16 + g * 4 + r];
+    bi[r] = DELTA ? __shfl(beta, w * 16 + g * 4 + r) : 0.f;
   }
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt) {
-    if (jt > w) {  // the operands of a pair of tiles reach one tile above the diagonal
-      if (jt == (w | 1))
-#pragma unroll
-        for (int r = 0; r < 4; ++r) Pt[(w * 16 + g * 4 + r) * LD + jt * 16 + c] = 0.f;
-      continue;
-    }
+    if (jt > w) continue;
     f32x4 kk{}, qk{};
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      if (DELTA) kk = mfma(ka[s], kb[jt][s], kk);
-      qk = mfma(qa[s], kb[jt][s], qk);
+      const bf16x8 kb = rows(kr, jt, s);
+      if (DELTA) kk = mfma(ka[s], kb, kk);
+      qk = mfma(qa[s], kb, qk);
     }
-    const double Gj = __shfl(G, jt * 16 + c);
+    const double Gj = Gs[w][jt * 16 + c];
+    f32x4 a;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = w * 16 + g * 4 + r, j = jt * 16 + c;
-      const float e = j <= i ? expf((float)(Gi[r] - Gj)) : 0.f;
-      Pt[i * LD + j] = j <= i ? e * qk[r] : 0.f;
-      if (DELTA) At[i * LD + j] = j < i ? bi[r] * (e * kk[r]) : 0.f;
+      const float e = j <= i ? __builtin_amdgcn_exp2f((float)(Gi[r] - Gj)) : 0.f;
+      Pb[lower(w, jt) + (g * 4 + r) * LD + c] = j <= i ? e * qk[r] : 0.f;
+      a[r] = DELTA && j < i ? bi[r] * (e * kk[r]) : 0.f;
+      if (DELTA && jt < w) Ab[lower(w, jt) + (g * 4 + r) * LD + c] = a[r];
     }
+    if (DELTA && jt == w) *reinterpret_cast<f32x4*>(Db + w * BLK + c * LD + g * 4) = a;  // columns of A as rows
   }
   if (DELTA) {
-    // column c of the diagonal block's inverse
+    // column c of the diagonal block's inverse: a row known, its multiples leave the rows below
     float x[16];
-    const float* const blk = At + w * 16 * LD + w * 16;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float a = i == c ? 1.f : 0.f;
+    for (int i = 0; i < 16; ++i) x[i] = i == c ? 1.f : 0.f;
 #pragma unroll
-      for (int m = 0; m < i; ++m) a -= blk[i * LD + m] * x[m];
-      x[i] = a;
-    }
+    for (int i = 0; i < 15; ++i)
+#pragma unroll
+      for (int q = (i + 1) / 4; q < 4; ++q) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(Db + w * BLK + i * LD + q * 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (q * 4 + r > i) x[q * 4 + r] -= a[r] * x[i];
+      }
     if (g == 0)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) Tt[(w * 16 + i) * LD + w * 16 + c] = x[i];
+      for (int i = 0; i < 16; ++i) Ab[lower(w, w) + i * LD + c] = x[i];
     __syncthreads();
     f32x4 t[4];
 #pragma unroll
@@ -312,68 +335,75 @@ __global__ void __launch_bounds__(256) linattn_chunk_k(LinParams p) {
       t[i] = f32x4{};
       if (i == w) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[i][r] = Tt[(i * 16 + g * 4 + r) * LD + i * 16 + c];
+        for (int r = 0; r < 4; ++r) t[i][r] = Ab[lower(i, i) + (g * 4 + r) * LD + c];
       } else if (i > w) {
         f32x4 sum{}, neg{};
 #pragma unroll
         for (int k = 0; k < i; ++k) {
           if (k < w) continue;
-          const f32x4 a = *reinterpret_cast<const f32x4*>(At + (i * 16 + c) * LD + k * 16 + g * 4);
+          const f32x4 a = *reinterpret_cast<const f32x4*>(Ab + lower(i, k) + c * LD + g * 4);
 #pragma unroll
           for (int s = 0; s < 4; ++s) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], t[k][s], sum, 0, 0, 0);
         }
-        const f32x4 a = *reinterpret_cast<const f32x4*>(Tt + (i * 16 + c) * LD + i * 16 + g * 4);
+        const f32x4 a = *reinterpret_cast<const f32x4*>(Ab + lower(i, i) + c * LD + g * 4);
 #pragma unroll
         for (int s = 0; s < 4; ++s) neg = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], sum[s], neg, 0, 0, 0);
         t[i] = -neg;
       }
     }
-    // scale P T and diag(to) T, block column w
+    // P T and diag(to) T, block column w
     const float bj = __shfl(beta, w * 16 + c);
     f32x4 pt[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       t[i] *= bj;
       pt[i] = f32x4{};
+    }
 #pragma unroll
-      for (int k = 0; k <= i; ++k) {
-        if (k < w) continue;
-        const f32x4 a = *reinterpret_cast<const f32x4*>(Pt + (i * 16 + c) * LD + k * 16 + g * 4);
+    for (int k = 0; k < 4; ++k) {
+      if (k < w) continue;
+#pragma unroll
+      for (int i = k; i < 4; ++i) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(Pb + lower(i, k) + c * LD + g * 4);
 #pragma unroll
         for (int s = 0; s < 4; ++s) pt[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], t[k][s], pt[i], 0, 0, 0);
       }
     }
     __syncthreads();  // A, P and the diagonal blocks have been read
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      if (i < w) continue;
+      const f32x4 e = *reinterpret_cast<const f32x4*>(to_end + i * 16 + g * 4);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int row = i * 16 + g * 4 + r;
-        odd |= !(fabsf(t[i][r]) < INFINITY) || !(fabsf(pt[i][r]) < INFINITY);
-        Tt[row * LD + w * 16 + c] = t[i][r] * to_end[row];
-        Pt[row * LD + w * 16 + c] = pt[i][r];
+        odd |= !(fabsf(t[i][r]) + fabsf(pt[i][r]) < INFINITY);
+        Ab[lower(i, w) + (g * 4 + r) * LD + c] = t[i][r] * e[r];
+        Pb[lower(i, w) + (g * 4 + r) * LD + c] = pt[i][r];
       }
+    }
   }
   if (!DELTA) __syncthreads();
   if (__any(odd) && lane == 0) atomicOr(&odd_at, 1);
   __syncthreads();
+  // operands: row w, the tokens of two tiles; the one above the diagonal is zeros
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
     if (ks > (w >> 1)) continue;
-    const int at = (w * 16 + c) * LD + ks * 32 + g * 4;
+    const bool both = 2 * ks + 1 <= w;
+    const int x = lower(w, 2 * ks) + c * LD + g * 4, y = both ? lower(w, 2 * ks + 1) + c * LD + g * 4 : x;
+    const float on = both ? p.scale : 0.f;
     bf16x8 hi, lo;
-    split8(*reinterpret_cast<const f32x4*>(Pt + at) * p.scale, *reinterpret_cast<const f32x4*>(Pt + at + 16) * p.scale, hi,
-           lo);
+    split8(*reinterpret_cast<const f32x4*>(Pb + x) * p.scale, *reinterpret_cast<const f32x4*>(Pb + y) * on, hi, lo);
     *reinterpret_cast<bf16x8*>(out->P[0][frag(w, ks)][lane]) = hi;
     *reinterpret_cast<bf16x8*>(out->P[1][frag(w, ks)][lane]) = lo;
     if (DELTA) {
-      split8(*reinterpret_cast<const f32x4*>(Tt + at), *reinterpret_cast<const f32x4*>(Tt + at + 16), hi, lo);
+      split8(*reinterpret_cast<const f32x4*>(Ab + x), *reinterpret_cast<const f32x4*>(Ab + y) * (both ? 1.f : 0.f), hi, lo);
       *reinterpret_cast<bf16x8*>(out->T[0][frag(w, ks)][lane]) = hi;
       *reinterpret_cast<bf16x8*>(out->T[1][frag(w, ks)][lane]) = lo;
     }
   }
   if (w != 0) return;
-  const float e = expf((float)G);
+  const float e = __builtin_amdgcn_exp2f((float)G);
   out->from[lane] = e;
   out->out[lane] = p.scale * e;
   out->to[lane] = to_end[lane];
@@ -392,6 +422,63 @@ __global__ void __launch_bounds__(256) linattn_chunk_k(LinParams p) {
 // reads spread over the banks.
 __device__ __forceinline__ constexpr int key_dim(int d, int g) { return (d >> 1) * 32 + g * 8 + (d & 1) * 4; }
 __device__ __forceinline__ constexpr int swizzle(int r) { return (r & 7) << 1 | (r >> 3 & 1); }
+
+// x = the 64 rows at `rows` (aoff: a lane's place in a row of 16 for key dims 32 s ..) times the state's two pieces.
+template <int CT>
+__device__ __forceinline__ void rows_times(const uint8_t* rows, const int (&aoff)[4], const bf16x8 (&sh)[4][CT],
+                                           const bf16x8 (&sl)[4][CT], f32x4 (&x)[4][CT]) {
+#pragma unroll
+  for (int it = 0; it < 4; ++it)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) x[it][ct] = f32x4{};
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    bf16x8 a[4];
+#pragma unroll
+    for (int it = 0; it < 4; ++it) a[it] = *reinterpret_cast<const bf16x8*>(rows + it * 4096 + aoff[s]);
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) x[it][ct] = mfma(a[it], part == 0 ? sh[s][ct] : sl[s][ct], x[it][ct]);
+  }
+}
+
+// x (+)= m b, m a chunk's lower triangular matrix in two pieces, b in two or one (exact).
+template <bool ALL, int CT>
+__device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], int lane, const bf16x8 (&bh)[2][CT],
+                                            const bf16x8 (&bl)[2][CT], f32x4 (&x)[4][CT]) {
+  if (ALL)
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) x[it][ct] = f32x4{};
+#pragma unroll
+  for (int part = 0; part < (ALL ? 4 : 3); ++part)  // hi hi, hi lo, lo hi, lo lo
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int it = 2 * k; it < 4; ++it) {
+        const bf16x8 a = *reinterpret_cast<const bf16x8*>(m[part >> 1][frag(it, k)][lane]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) x[it][ct] = mfma(a, part & 1 ? bl[k][ct] : bh[k][ct], x[it][ct]);
+      }
+}
+template <int CT>
+__device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], int lane, const bf16x8 (&b)[2][CT],
+                                            f32x4 (&x)[4][CT]) {
+#pragma unroll
+  for (int part = 0; part < 2; ++part)
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int it = 2 * k; it < 4; ++it) {
+        const bf16x8 a = *reinterpret_cast<const bf16x8*>(m[part][frag(it, k)][lane]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) x[it][ct] = mfma(a, b[k][ct], x[it][ct]);
+      }
+}
 
 // Eight transposing reads, at a + x and b + x for four x. (The builtin makes the compiler wait for every LDS DMA in flight,
 // the next chunk's among them; the wait for the reads themselves is in the block, so that the registers are filled when it
@@ -508,7 +595,6 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
     toff[s] = KO + trow * 256 + ((s * 4 + (c & 3)) ^ swizzle(trow)) * 16;
   }
   const int vtoff = trow * VB + wave * 32 * CT + (c & 3) * 8;  // + 32 ct + row * VB
-  const auto rd16 = [](const uint8_t* a) { return *reinterpret_cast<const bf16x8*>(a); };
   const auto join = [](bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); };
 
   // vmcnt(0), as the compiler knows it: the state is there, and no wait for it, which would take the DMAs along, is left
@@ -540,13 +626,9 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         const uint2 x = __builtin_bit_cast(uint2, vt[ct][it]);
-        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
-                                                                     __builtin_bit_cast(u16x2, x.x & 0x7fff7fffu)));
-        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
-                                                                     __builtin_bit_cast(u16x2, x.y & 0x7fff7fffu)));
+        top = top2(top2(top, x.x), x.y);
       }
-    const bool slow = cw.odd != 0 || (top & 0xffffu) >= 0x7f80u || top >= 0x7f800000u;
+    const bool slow = cw.odd != 0 || odd_top(top);
     if (__any(slow)) {
       for (int t = 0; t < cnt; ++t) {
         const int64_t row = (int64_t)(first + t0 + t) * p.HV + h;
@@ -591,22 +673,14 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) split8(st[2 * s][ct], st[2 * s + 1][ct], sh[s][ct], sl[s][ct]);
+    // Products on one accumulator follow each other with others between them: a product waits for the one before on its
+    // accumulator twice as long as it occupies the unit.
     bf16x8 xh[2][CT], xl[2][CT];  // X, or V itself
     if (DELTA) {
       f32x4 x[4][CT];
+      rows_times(stage + KO, aoff, sh, sl, x);
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) x[it][ct] = f32x4{};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const bf16x8 a = rd16(stage + KO + it * 4096 + aoff[s]);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            x[it][ct] = mfma(a, sh[s][ct], x[it][ct]);
-            x[it][ct] = mfma(a, sl[s][ct], x[it][ct]);
-          }
-        }
         const f32x4 f = *reinterpret_cast<const f32x4*>(cw.from + it * 16 + g * 4);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
@@ -630,24 +704,11 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
     bf16x8 uh[2][CT], ul[2][CT];
     {
       f32x4 u[4][CT];
+      if (DELTA) {
+        lower_times<true>(cw.T, lane, xh, xl, u);
+      } else {
 #pragma unroll
-      for (int it = 0; it < 4; ++it)
-        if (DELTA) {
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) u[it][ct] = f32x4{};
-#pragma unroll
-          for (int k = 0; k <= it / 2; ++k) {
-            const bf16x8 th = rd16(reinterpret_cast<const uint8_t*>(cw.T[0][frag(it, k)][lane]));
-            const bf16x8 tl = rd16(reinterpret_cast<const uint8_t*>(cw.T[1][frag(it, k)][lane]));
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              u[it][ct] = mfma(th, xh[k][ct], u[it][ct]);
-              u[it][ct] = mfma(th, xl[k][ct], u[it][ct]);
-              u[it][ct] = mfma(tl, xh[k][ct], u[it][ct]);
-              u[it][ct] = mfma(tl, xl[k][ct], u[it][ct]);
-            }
-          }
-        } else {
+        for (int it = 0; it < 4; ++it) {
           const f32x4 f = *reinterpret_cast<const f32x4*>(cw.to + it * 16 + g * 4);
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {
@@ -656,74 +717,55 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
                                   __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
           }
         }
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) split8(u[2 * k][ct], u[2 * k + 1][ct], uh[k][ct], ul[k][ct]);
     }
     const float all = cw.all;
-    bf16x4 ka[2][4], kb[2][4];
-    tr_read8<0, 4096, 8192, 12288>(stage + toff[0], stage + toff[0] + 8, ka[0], kb[0]);
 #pragma unroll
-    for (int d = 0; d < 8; d += 2) {
-      const int now = d / 2 & 1;
-      if (d < 6) {
-        const uint8_t* const ta = stage + toff[d < 6 ? d / 2 + 1 : 0];
-        tr_read8<0, 4096, 8192, 12288>(ta, ta + 8, ka[now ^ 1], kb[now ^ 1]);
-      }
+    for (int d = 0; d < 8; d += 4) {
+      bf16x4 kt[4][4];  // key dims d .. d + 3, tokens 16 t + 4 g ..
+      tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2], stage + toff[d / 2] + 8, kt[0], kt[1]);
+      tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2 + 1], stage + toff[d / 2 + 1] + 8, kt[2], kt[3]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) st[d + e][ct] *= all;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const bf16x8 a = e == 0 ? join(ka[now][2 * k], ka[now][2 * k + 1]) : join(kb[now][2 * k], kb[now][2 * k + 1]);
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            st[d + e][ct] = mfma(a, uh[k][ct], st[d + e][ct]);
-            st[d + e][ct] = mfma(a, ul[k][ct], st[d + e][ct]);
-          }
-        }
-      }
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              st[d + e][ct] = mfma(join(kt[e][2 * k], kt[e][2 * k + 1]), part == 0 ? uh[k][ct] : ul[k][ct], st[d + e][ct]);
     }
     // the outputs
     const __amdgpu_buffer_rsrc_t orow = head_rows(p.o, first + t0, cnt, p.HV, h);
+    f32x4 x[4][CT];
+    rows_times(stage + QO, aoff, sh, sl, x);
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      f32x4 x[CT];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) x[ct] = f32x4{};
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const bf16x8 a = rd16(stage + QO + it * 4096 + aoff[s]);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          x[ct] = mfma(a, sh[s][ct], x[ct]);
-          x[ct] = mfma(a, sl[s][ct], x[ct]);
-        }
-      }
       const f32x4 f = *reinterpret_cast<const f32x4*>(cw.out + it * 16 + g * 4);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) x[ct] *= f;
+      for (int ct = 0; ct < CT; ++ct) x[it][ct] *= f;
+    }
+    if (DELTA)
+      lower_times<false>(cw.P, lane, xh, xl, x);
+    else
+      lower_times(cw.P, lane, xh, x);
 #pragma unroll
-      for (int k = 0; k <= it / 2; ++k) {
-        const bf16x8 ph = rd16(reinterpret_cast<const uint8_t*>(cw.P[0][frag(it, k)][lane]));
-        const bf16x8 pl = rd16(reinterpret_cast<const uint8_t*>(cw.P[1][frag(it, k)][lane]));
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          x[ct] = mfma(ph, xh[k][ct], x[ct]);
-          x[ct] = mfma(pl, xh[k][ct], x[ct]);
-          if (DELTA) x[ct] = mfma(ph, xl[k][ct], x[ct]);
-        }
-      }
+    for (int it = 0; it < 4; ++it)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)f2bf(x[ct][r]), orow,
+          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)f2bf(x[it][ct][r]), orow,
                                                 (uint32_t)(it * 16 + g * 4 + r) * (p.HV * kHD * 2) + (dv + ct * 16) * 2, 0,
                                                 0);
-    }
   }
 #pragma unroll
   for (int d = 0; d < 8; ++d)
