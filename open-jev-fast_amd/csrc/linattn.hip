@@ -199,6 +199,10 @@ __device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8& h
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
+// 16-byte piece x of a row r of K or Q lies at x ^ swizzle(r) in LDS: the reads of 16 rows' pieces, and the transposing ones
+// of 4 pieces of 8 rows, then spread over the banks.
+__device__ __forceinline__ constexpr int swizzle(int r) { return (r & 7) << 1 | (r >> 3 & 1); }
+
 // The sum of x over the lanes up to and including this one, in 64 bits, by lane shifts within rows of 16 and the rows' last
 // lanes handed on (a lane outside reads as zero).
 template <int CTRL, int ROWS>
@@ -241,7 +245,11 @@ template <bool DELTA>
 __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
   constexpr int LD = 20, BLK = 16 * LD;
   const auto lower = [](int i, int k) { return (i * (i + 1) / 2 + k) * BLK; };
-  __shared__ __attribute__((aligned(16))) float Pb[10 * BLK], Ab[DELTA ? 10 * BLK : 4], Db[DELTA ? 4 * BLK : 4];
+  __shared__ __attribute__((aligned(16))) float mem[DELTA ? 24 * BLK : 64 * 64];
+  float* const Pb = mem;              // ten blocks
+  float* const Ab = mem + 10 * BLK;   // ten blocks
+  float* const Db = mem + 20 * BLK;   // four
+  uint8_t* const Kb = reinterpret_cast<uint8_t*>(mem);  // before them: the chunk's rows of K
   __shared__ double Gs[4][64];  // every wave's own
   __shared__ float to_end[64];
   __shared__ int odd_at;
@@ -255,14 +263,12 @@ __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
   ChunkWork* const out = reinterpret_cast<ChunkWork*>(p.work + (chunk * p.HV + h) * (int64_t)chunk_bytes(DELTA));
 
   const __amdgpu_buffer_rsrc_t kr = head_rows(p.k, t0, cnt, p.HK, hk), qr = head_rows(p.q, t0, cnt, p.HK, hk);
-  const auto rows = [&](__amdgpu_buffer_rsrc_t x, int tile, int s) {
-    return __builtin_bit_cast(bf16x8, bload(x, (uint32_t)(tile * 16 + c) * (p.HK * kHD * 2) + s * 64 + g * 16));
-  };
   bf16x8 ka[4], qa[4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
-    ka[s] = rows(kr, w, s);
-    qa[s] = rows(qr, w, s);
+    const uint32_t x = (uint32_t)(w * 16 + c) * (p.HK * kHD * 2) + s * 64 + g * 16;
+    ka[s] = __builtin_bit_cast(bf16x8, bload(kr, x));
+    qa[s] = __builtin_bit_cast(bf16x8, bload(qr, x));
   }
   // a token a lane: decays, to base two, and strengths; tokens behind the end add nothing
   const int64_t tok = (int64_t)(t0 + min(lane, cnt - 1)) * p.HV + h;
@@ -278,9 +284,28 @@ __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
     if (lane == 0) odd_at = 0;
   }
   uint32_t top = 0;
+  int koff[4];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) top = top8(top8(top, ka[s]), qa[s]);
+  for (int s = 0; s < 4; ++s) {
+    koff[s] = c * 256 + ((s * 4 + g) ^ swizzle(c)) * 16;
+    *reinterpret_cast<bf16x8*>(Kb + w * 4096 + koff[s]) = ka[s];
+    top = top8(top8(top, ka[s]), qa[s]);
+  }
   odd |= odd_top(top);
+  __syncthreads();
+  f32x4 kk[4], qk[4];
+#pragma unroll
+  for (int jt = 0; jt < 4; ++jt) {
+    kk[jt] = qk[jt] = f32x4{};
+    if (jt > w) continue;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const bf16x8 kb = *reinterpret_cast<const bf16x8*>(Kb + jt * 4096 + koff[s]);
+      if (DELTA) kk[jt] = mfma(ka[s], kb, kk[jt]);
+      qk[jt] = mfma(qa[s], kb, qk[jt]);
+    }
+  }
+  __syncthreads();  // K has been read
 
   double Gi[4];
   float bi[4];
@@ -292,21 +317,14 @@ __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt) {
     if (jt > w) continue;
-    f32x4 kk{}, qk{};
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const bf16x8 kb = rows(kr, jt, s);
-      if (DELTA) kk = mfma(ka[s], kb, kk);
-      qk = mfma(qa[s], kb, qk);
-    }
     const double Gj = Gs[w][jt * 16 + c];
     f32x4 a;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = w * 16 + g * 4 + r, j = jt * 16 + c;
       const float e = j <= i ? __builtin_amdgcn_exp2f((float)(Gi[r] - Gj)) : 0.f;
-      Pb[lower(w, jt) + (g * 4 + r) * LD + c] = j <= i ? e * qk[r] : 0.f;
-      a[r] = DELTA && j < i ? bi[r] * (e * kk[r]) : 0.f;
+      Pb[lower(w, jt) + (g * 4 + r) * LD + c] = j <= i ? e * qk[jt][r] : 0.f;
+      a[r] = DELTA && j < i ? bi[r] * (e * kk[jt][r]) : 0.f;
       if (DELTA && jt < w) Ab[lower(w, jt) + (g * 4 + r) * LD + c] = a[r];
     }
     if (DELTA && jt == w) *reinterpret_cast<f32x4*>(Db + w * BLK + c * LD + g * 4) = a;  // columns of A as rows
@@ -418,10 +436,8 @@ __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
 // then the B operand of K S0 and Q S0 for 32 key dims in order, and nothing of the state, of X or of U ever leaves its
 // lane. What the waves share, K, Q, V and the chunk's matrices, comes by LDS DMA one chunk ahead; they meet once a chunk.
 // K^T and V's columns come from the same rows by transposing reads (16 lanes get 4 rows x 16 columns column by column,
-// the columns in any groups of 4). 16-byte piece x of a row r of K and Q lies at x ^ swizzle(r), so that both kinds of
-// reads spread over the banks.
+// the columns in any groups of 4).
 __device__ __forceinline__ constexpr int key_dim(int d, int g) { return (d >> 1) * 32 + g * 8 + (d & 1) * 4; }
-__device__ __forceinline__ constexpr int swizzle(int r) { return (r & 7) << 1 | (r >> 3 & 1); }
 
 // x = the 64 rows at `rows` (aoff: a lane's place in a row of 16 for key dims 32 s ..) times the state's two pieces.
 template <int CT>

@@ -100,20 +100,26 @@ __device__ __forceinline__ void rmsnorm_row8(const float (&v)[8], float4 wa, flo
       make_uint4(pack2(o[0], o[1]), pack2(o[2], o[3]), pack2(o[4], o[5]), pack2(o[6], o[7]));
 }
 
-// Running sum, and running maximum, over the wave's lanes up to and including this one.
+// Running sum, and running maximum of values that are not negative, over the wave's lanes up to and including this one: by
+// lane shifts of 1, 2, 4, 8 within rows of 16, then the rows' last lanes handed on (a lane outside reads as zero).
+#define OJX_DPP(x, ctrl, rows) __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false)
 __device__ __forceinline__ int wave_scan_sum(int v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(v, o);
-    if ((int)(threadIdx.x & 63) >= o) v += t;
-  }
-  return v;
+  v += OJX_DPP(v, 0x111, 0xf);
+  v += OJX_DPP(v, 0x112, 0xf);
+  v += OJX_DPP(v, 0x114, 0xf);
+  v += OJX_DPP(v, 0x118, 0xf);
+  v += OJX_DPP(v, 0x142, 0xa);
+  return v + OJX_DPP(v, 0x143, 0xc);
 }
 __device__ __forceinline__ int wave_scan_max(int v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v = max(v, __shfl_up(v, o));  // below lane o the lane's own value comes back
-  return v;
+  v = max(v, OJX_DPP(v, 0x111, 0xf));
+  v = max(v, OJX_DPP(v, 0x112, 0xf));
+  v = max(v, OJX_DPP(v, 0x114, 0xf));
+  v = max(v, OJX_DPP(v, 0x118, 0xf));
+  v = max(v, OJX_DPP(v, 0x142, 0xa));
+  return max(v, OJX_DPP(v, 0x143, 0xc));
 }
+#undef OJX_DPP
 
 // Sequences laid end to end in rows by pointers ptr[0 .. S]: sequence i is rows [m_i, m_(i+1)), m_i the largest of ptr[0 ..
 // i] clamped to [0, rows]. For pointers that never fall that is what they say; whatever they hold, sequences stay within
