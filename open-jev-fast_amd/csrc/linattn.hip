@@ -557,29 +557,26 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   }
   constexpr int VL = VB / 16;  // lanes of a V row
   const uint32_t voff = (uint32_t)(wave * 16 + lane / VL) * (p.HV * kHD * 2) + (lane % VL) * 16;
-  const auto fetch = [&](int t, uint8_t* stage) {  // first token of the chunk
+  // quarter i of the chunk that begins at token t
+  const auto fetch = [&](int i, int t, uint8_t* stage) {
     const int cnt = min(kChunk, n - t);
     const __amdgpu_buffer_rsrc_t kr = head_rows(p.k, first + t, cnt, p.HK, hk);
     const __amdgpu_buffer_rsrc_t qr = head_rows(p.q, first + t, cnt, p.HK, hk);
     const __amdgpu_buffer_rsrc_t vr = make_rsrc(p.v + ((int64_t)(first + t) * p.HV + h) * kHD + dv0,
                                                 ((int64_t)(cnt - 1) * p.HV * kHD + 64 * CT) * 2);
-    const __amdgpu_buffer_rsrc_t wr = make_rsrc(work, WB);
+    const __amdgpu_buffer_rsrc_t wr = make_rsrc(work + (int64_t)(t / kChunk) * next_work, WB);
+    dma16(kr, stage + KO + wave * 4096 + i * 1024, koff[i]);
+    dma16(qr, stage + QO + wave * 4096 + i * 1024, koff[i]);
+    if (i < 2 * CT) dma16(vr, stage + VO + wave * (16 * VB) + i * 1024, voff + (uint32_t)(i * 64 / VL) * (p.HV * kHD * 2));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      dma16(kr, stage + KO + wave * 4096 + i * 1024, koff[i]);
-      dma16(qr, stage + QO + wave * 4096 + i * 1024, koff[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * CT; ++i)
-      dma16(vr, stage + VO + wave * (16 * VB) + i * 1024, voff + (uint32_t)(i * 64 / VL) * (p.HV * kHD * 2));
-#pragma unroll
-    for (int i = 0; i < (WB / 1024 + 3) / 4; ++i) {
-      const int at = min(i * 4 + wave, WB / 1024 - 1) * 1024;  // past the last piece: that one again
+    for (int j = i; j < (WB / 1024 + 3) / 4; j += 4) {
+      const int at = min(j * 4 + wave, WB / 1024 - 1) * 1024;  // past the last piece: that one again
       dma16(wr, stage + at, at + lane * 16);
     }
-    work += next_work;
   };
-  if (chunks > 0) fetch(0, smem);
+  if (chunks > 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fetch(i, 0, smem);
 
   f32x4 st[8][CT];
   {
@@ -622,7 +619,10 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
     const ChunkWork& cw = *reinterpret_cast<const ChunkWork*>(stage);
     if (ch > 0) wait_vmcnt<16 * CT>();  // all but the last chunk's output stores
     stage_barrier();          // the stage has landed, and every wave is done with the other one
-    if (ch + 1 < chunks) fetch(t0 + kChunk, smem + ((ch + 1) & 1) * STAGE);
+    // the next chunk's DMAs go out in quarters between the products: all at once they would hold up the wave
+    const bool more = ch + 1 < chunks;
+    uint8_t* const other = smem + ((ch + 1) & 1) * STAGE;
+    if (more) fetch(0, t0 + kChunk, other);
 
     // V's columns: X's accumulators' places, and its B operand
     bf16x4 vt[CT][4];
@@ -646,6 +646,9 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
       }
     const bool slow = cw.odd != 0 || odd_top(top);
     if (__any(slow)) {
+      if (more)
+#pragma unroll
+        for (int i = 1; i < 4; ++i) fetch(i, t0 + kChunk, other);
       for (int t = 0; t < cnt; ++t) {
         const int64_t row = (int64_t)(first + t0 + t) * p.HV + h;
         const float a = expf(p.g[row]), b = DELTA ? bf2f(p.beta[row]) : 1.f;
@@ -689,6 +692,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) split8(st[2 * s][ct], st[2 * s + 1][ct], sh[s][ct], sl[s][ct]);
+    if (more) fetch(1, t0 + kChunk, other);
     // Products on one accumulator follow each other with others between them: a product waits for the one before on its
     // accumulator twice as long as it occupies the unit.
     bf16x8 xh[2][CT], xl[2][CT];  // X, or V itself
@@ -716,6 +720,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) xh[k][ct] = join(vt[ct][2 * k], vt[ct][2 * k + 1]);
     }
+    if (more) fetch(2, t0 + kChunk, other);
     // the decayed U, and the state
     bf16x8 uh[2][CT], ul[2][CT];
     {
@@ -739,6 +744,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) split8(u[2 * k][ct], u[2 * k + 1][ct], uh[k][ct], ul[k][ct]);
     }
+    if (more) fetch(3, t0 + kChunk, other);
     const float all = cw.all;
 #pragma unroll
     for (int d = 0; d < 8; d += 4) {
