@@ -975,7 +975,7 @@ int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const
 int64_t ojx_linattn_prompt_workspace(int64_t R, int64_t S, int32_t HV, int32_t HK, int32_t delta) {
   // a workgroup of 256 threads per sequence and head at most; a launch has fewer than 2^32 threads
   if (HK < 1 || HV < HK || HV % HK != 0 || HV > 1024 || R < 0 || R >= (1LL << 31) || S < 0 ||
-      2 * (S + 1) * HV >= (1LL << 24) || ojx::linattn_chunks(R, S) * HV >= (1LL << 24)) {
+      4 * (S + 1) * HV >= (1LL << 24) || ojx::linattn_chunks(R, S) * HV >= (1LL << 24)) {
     fail(OJX_ERR_SHAPE, "bad sizes R=%lld S=%lld HV=%d HK=%d", (long long)R, (long long)S, HV, HK);
     return -1;
   }

@@ -431,12 +431,16 @@ __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
   }
 }
 
-// The chunks of one sequence and value head in order. A wave has 16 CT value dims of the state, all 128 key dims: 8 CT
+// The chunks of one sequence and value head in order. A slice is 16 value dims of the state with all 128 key dims: 8
 // accumulators, d of them with key dims key_dim(d, g) .. + 3 in the lanes (c, g) of value dim c. Two of them together are
-// then the B operand of K S0 and Q S0 for 32 key dims in order, and nothing of the state, of X or of U ever leaves its
-// lane. What the waves share, K, Q, V and the chunk's matrices, comes by LDS DMA one chunk ahead; they meet once a chunk.
-// K^T and V's columns come from the same rows by transposing reads (16 lanes get 4 rows x 16 columns column by column,
-// the columns in any groups of 4).
+// then the B operand of K S0 and Q S0 for 32 key dims in order, and nothing of the state, of X or of U has to change its
+// lane. A workgroup takes two slices with two waves each:
+//   * the slice's first wave has the state: X, U, the new state. This is the chain that bounds a long sequence (a chunk's
+//     products wait for each other, and the next chunk for this one), so nothing else is on it;
+//   * the second has the rest: the outputs, from the pieces of S0 and X that the first hands over through LDS, and the DMAs.
+// K, Q, V and the chunk's matrices come to LDS one chunk ahead. K^T and V's columns are read transposed from the rows (16
+// lanes get 4 rows x 16 columns column by column, the columns in any groups of 4). Two barriers a chunk: S0's pieces and
+// the stage are there; X's pieces are there.
 __device__ __forceinline__ constexpr int key_dim(int d, int g) { return (d >> 1) * 32 + g * 8 + (d & 1) * 4; }
 
 // x = the 64 rows at `rows` (aoff: a lane's place in a row of 16 for key dims 32 s ..) times the state's two pieces.
@@ -521,15 +525,16 @@ __device__ __forceinline__ void tr_read8(const uint8_t* pa, const uint8_t* pb, b
 // and DMAs stay in flight.
 __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <bool DELTA, int CT>
+template <bool DELTA>
 __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
-  constexpr int SL = 2 / CT;             // workgroups of a head
-  constexpr int VB = 128 * CT;           // bytes of a V row: the workgroup's 64 CT value dims
+  constexpr int SL = 4;                  // workgroups of a head
+  constexpr int VB = 64;                 // bytes of a V row: the workgroup's 32 value dims
   constexpr int WB = chunk_bytes(DELTA);
   constexpr int KO = WB, QO = KO + kChunk * 256, VO = QO + kChunk * 256, STAGE = VO + kChunk * VB;
+  constexpr int SO = 2 * STAGE, XO = SO + 2 * 8192, FO = XO + 2 * 4096;  // handed over: S0's pieces, X's, token by token
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = wave & 1;
   const int64_t sq = blockIdx.x / (p.HV * SL);
   const int hs = blockIdx.x - (int)(sq * p.HV * SL), h = hs / SL, hk = h / (p.HV / p.HK);
   if (sq == p.S) {  // the rows of no sequence
@@ -544,41 +549,105 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   if (!seq_find(p.seq_ptr, p.S, p.R, seq_chunks, [=](int i, int) { return i == (int)sq; }, place)) return;
   const int first = place.first, n = place.n;
   const int chunks = seq_chunks(n);
-  const int dv0 = (hs % SL) * 64 * CT, dv = dv0 + wave * 16 * CT + c;  // + 16 ct
+  const int dv0 = (hs % SL) * 32, dv = dv0 + slice * 16 + c;
+  // LDS offsets of this lane: rows c of K and Q, key dims 32 s .. + 31; its slice's pieces of S0 and X
+  int aoff[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) aoff[s] = c * 256 + ((s * 4 + g) ^ swizzle(c)) * 16;
+  bf16x8* const s0 = reinterpret_cast<bf16x8*>(smem + SO + slice * 8192) + lane;
+  bf16x8* const x0 = reinterpret_cast<bf16x8*>(smem + XO + slice * 4096) + lane;
+  int32_t* const by_token = reinterpret_cast<int32_t*>(smem + FO) + slice;
 
-  // the next chunk to an LDS stage: this wave's 16 rows of K and Q, its part of V and of the chunk's matrices
-  const uint8_t* work = p.work + ((int64_t)place.before * p.HV + h) * (int64_t)WB;
-  const int64_t next_work = (int64_t)p.HV * WB;
-  uint32_t koff[4];
+  if (wave >= 2) {
+    // ------------------------------------------------------------------------------------------ DMAs and outputs
+    const int64_t next_work = (int64_t)p.HV * WB;
+    const uint8_t* const work = p.work + ((int64_t)place.before * p.HV + h) * (int64_t)WB;
+    uint32_t koff[4];  // rows 4 i + g of 16
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 4 * i + g;
-    koff[i] = (uint32_t)(wave * 16 + r) * (p.HK * kHD * 2) + (c ^ swizzle(r)) * 16;
-  }
-  constexpr int VL = VB / 16;  // lanes of a V row
-  const uint32_t voff = (uint32_t)(wave * 16 + lane / VL) * (p.HV * kHD * 2) + (lane % VL) * 16;
-  // quarter i of the chunk that begins at token t
-  const auto fetch = [&](int i, int t, uint8_t* stage) {
-    const int cnt = min(kChunk, n - t);
-    const __amdgpu_buffer_rsrc_t kr = head_rows(p.k, first + t, cnt, p.HK, hk);
-    const __amdgpu_buffer_rsrc_t qr = head_rows(p.q, first + t, cnt, p.HK, hk);
-    const __amdgpu_buffer_rsrc_t vr = make_rsrc(p.v + ((int64_t)(first + t) * p.HV + h) * kHD + dv0,
-                                                ((int64_t)(cnt - 1) * p.HV * kHD + 64 * CT) * 2);
-    const __amdgpu_buffer_rsrc_t wr = make_rsrc(work + (int64_t)(t / kChunk) * next_work, WB);
-    dma16(kr, stage + KO + wave * 4096 + i * 1024, koff[i]);
-    dma16(qr, stage + QO + wave * 4096 + i * 1024, koff[i]);
-    if (i < 2 * CT) dma16(vr, stage + VO + wave * (16 * VB) + i * 1024, voff + (uint32_t)(i * 64 / VL) * (p.HV * kHD * 2));
+    for (int i = 0; i < 4; ++i) koff[i] = (uint32_t)(4 * i + g) * (p.HK * kHD * 2) + (c ^ swizzle(4 * i + g)) * 16;
+    const uint32_t voff = (uint32_t)(lane >> 2) * (p.HV * kHD * 2) + (lane & 3) * 16;
+    // quarter i of the chunk that begins at token t: 16 rows of K, Q and V, a part of the matrices, between the two waves
+    const auto fetch = [&](int i, int t, uint8_t* stage) {
+      const int cnt = min(kChunk, n - t);
+      const __amdgpu_buffer_rsrc_t kr = head_rows(p.k, first + t, cnt, p.HK, hk);
+      const __amdgpu_buffer_rsrc_t qr = head_rows(p.q, first + t, cnt, p.HK, hk);
+      const __amdgpu_buffer_rsrc_t vr = make_rsrc(p.v + ((int64_t)(first + t) * p.HV + h) * kHD + dv0,
+                                                  ((int64_t)(cnt - 1) * p.HV * kHD + 32) * 2);
+      const __amdgpu_buffer_rsrc_t wr = make_rsrc(work + (int64_t)(t / kChunk) * next_work, WB);
 #pragma unroll
-    for (int j = i; j < (WB / 1024 + 3) / 4; j += 4) {
-      const int at = min(j * 4 + wave, WB / 1024 - 1) * 1024;  // past the last piece: that one again
-      dma16(wr, stage + at, at + lane * 16);
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t at = (uint32_t)(i * 16) * (p.HK * kHD * 2) + koff[j];
+        dma16(slice == 0 ? kr : qr, stage + (slice == 0 ? KO : QO) + i * 4096 + j * 1024, at);
+      }
+      if (slice == (i & 1)) dma16(vr, stage + VO + i * 1024, (uint32_t)(i * 16) * (p.HV * kHD * 2) + voff);
+      constexpr int PW = (WB / 1024 + 1) / 2;  // pieces of the matrices a wave
+#pragma unroll
+      for (int j = i; j < PW; j += 4) {
+        const int at = min(j * 2 + slice, WB / 1024 - 1) * 1024;  // past the last piece: that one again
+        dma16(wr, stage + at, at + lane * 16);
+      }
+    };
+    if (chunks > 0)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fetch(i, 0, smem);
+    for (int ch = 0; ch < chunks; ++ch) {
+      const int t0 = ch * kChunk, cnt = min(kChunk, n - t0);
+      const uint8_t* const stage = smem + (ch & 1) * STAGE;
+      const ChunkWork& cw = *reinterpret_cast<const ChunkWork*>(stage);
+      if (ch > 0)
+        wait_vmcnt<16>();  // all but the last chunk's output stores
+      else
+        wait_vmcnt<0>();
+      stage_barrier();
+      const bool more = ch + 1 < chunks;
+      uint8_t* const other = smem + ((ch + 1) & 1) * STAGE;
+      bf16x8 sh[4][1], sl[4][1];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        sh[s][0] = s0[(2 * s) * 64];
+        sl[s][0] = s0[(2 * s + 1) * 64];
+      }
+      // the next chunk's DMAs go out in quarters: all at once they would hold up the wave
+      if (more) {
+        fetch(0, t0 + kChunk, other);
+        fetch(1, t0 + kChunk, other);
+      }
+      f32x4 x[4][1];
+      rows_times(stage + QO, aoff, sh, sl, x);
+#pragma unroll
+      for (int it = 0; it < 4; ++it) x[it][0] *= *reinterpret_cast<const f32x4*>(cw.out + it * 16 + g * 4);
+      if (more) {
+        fetch(2, t0 + kChunk, other);
+        fetch(3, t0 + kChunk, other);
+      }
+      stage_barrier();
+      if (*by_token != 0) {  // the first wave writes the outputs
+        wait_vmcnt<0>();
+        continue;
+      }
+      bf16x8 xh[2][1], xl[2][1];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        xh[k][0] = x0[(2 * k) * 64];
+        if (DELTA) xl[k][0] = x0[(2 * k + 1) * 64];
+      }
+      if (DELTA)
+        lower_times<false>(cw.P, lane, xh, xl, x);
+      else
+        lower_times(cw.P, lane, xh, x);
+      const __amdgpu_buffer_rsrc_t orow = head_rows(p.o, first + t0, cnt, p.HV, h);
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)f2bf(x[it][0][r]), orow,
+                                                (uint32_t)(it * 16 + g * 4 + r) * (p.HV * kHD * 2) + dv * 2, 0, 0);
     }
-  };
-  if (chunks > 0)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) fetch(i, 0, smem);
+    return;
+  }
 
-  f32x4 st[8][CT];
+  // -------------------------------------------------------------------------------------------------- the state
+  f32x4 st[8][1];
   {
     int64_t at = -1;
     if (p.state != nullptr) at = p.src != nullptr ? (int64_t)p.src[sq] : sq;
@@ -587,68 +656,48 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 #pragma unroll
       for (int d = 0; d < 8; ++d)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            st[d][ct][r] = p.state[(at * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv + ct * 16];
+        for (int r = 0; r < 4; ++r)
+          st[d][0][r] = p.state[(at * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv];
     } else {
 #pragma unroll
-      for (int d = 0; d < 8; ++d)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) st[d][ct] = f32x4{fill, fill, fill, fill};
+      for (int d = 0; d < 8; ++d) st[d][0] = f32x4{fill, fill, fill, fill};
     }
   }
-
-  // LDS offsets of this lane: rows c of K and Q, key dims 32 s .. + 31; K's rows read transposed, the same key dims
-  int aoff[4], toff[4];
+  int toff[4];  // K's rows read transposed, key dims 32 s .. + 31
   const int trow = g * 4 + (c >> 2);
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    aoff[s] = c * 256 + ((s * 4 + g) ^ swizzle(c)) * 16;
-    toff[s] = KO + trow * 256 + ((s * 4 + (c & 3)) ^ swizzle(trow)) * 16;
-  }
-  const int vtoff = trow * VB + wave * 32 * CT + (c & 3) * 8;  // + 32 ct + row * VB
+  for (int s = 0; s < 4; ++s) toff[s] = KO + trow * 256 + ((s * 4 + (c & 3)) ^ swizzle(trow)) * 16;
+  const int vtoff = VO + trow * VB + slice * 32 + (c & 3) * 8;
   const auto join = [](bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); };
-
-  // vmcnt(0), as the compiler knows it: the state is there, and no wait for it, which would take the DMAs along, is left
-  // for the loop
-  __builtin_amdgcn_s_waitcnt(0x0f70);
+  bf16x8 sh[4][1], sl[4][1];
   for (int ch = 0; ch < chunks; ++ch) {
     const int t0 = ch * kChunk, cnt = min(kChunk, n - t0);
     const uint8_t* const stage = smem + (ch & 1) * STAGE;
     const ChunkWork& cw = *reinterpret_cast<const ChunkWork*>(stage);
-    if (ch > 0) wait_vmcnt<16 * CT>();  // all but the last chunk's output stores
-    stage_barrier();          // the stage has landed, and every wave is done with the other one
-    // the next chunk's DMAs go out in quarters between the products: all at once they would hold up the wave
-    const bool more = ch + 1 < chunks;
-    uint8_t* const other = smem + ((ch + 1) & 1) * STAGE;
-    if (more) fetch(0, t0 + kChunk, other);
-
-    // V's columns: X's accumulators' places, and its B operand
-    bf16x4 vt[CT][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      split8(st[2 * s][0], st[2 * s + 1][0], sh[s][0], sl[s][0]);
+      s0[(2 * s) * 64] = sh[s][0];
+      s0[(2 * s + 1) * 64] = sl[s][0];
+    }
+    stage_barrier();
+    bf16x4 vt[4];  // V's columns: X's accumulators' places, and its B operand
     {
-      const uint8_t* const va = stage + VO + vtoff;
-      if constexpr (CT == 2) {
-        tr_read8<0, 16 * VB, 32 * VB, 48 * VB>(va, va + 32, vt[0], vt[1]);
-      } else {
-        bf16x4 a[4], b[4];
-        tr_read8<0, 8, 16 * VB, 16 * VB + 8>(va, va + 32 * VB, a, b);
-        vt[0][0] = a[0], vt[0][1] = a[2], vt[0][2] = b[0], vt[0][3] = b[2];
-      }
+      const uint8_t* const va = stage + vtoff;
+      bf16x4 a[4], b[4];
+      tr_read8<0, 8, 16 * VB, 16 * VB + 8>(va, va + 32 * VB, a, b);
+      vt[0] = a[0], vt[1] = a[2], vt[2] = b[0], vt[3] = b[2];
     }
     uint32_t top = 0;
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const uint2 x = __builtin_bit_cast(uint2, vt[ct][it]);
-        top = top2(top2(top, x.x), x.y);
-      }
-    const bool slow = cw.odd != 0 || odd_top(top);
-    if (__any(slow)) {
-      if (more)
-#pragma unroll
-        for (int i = 1; i < 4; ++i) fetch(i, t0 + kChunk, other);
+    for (int it = 0; it < 4; ++it) {
+      const uint2 x = __builtin_bit_cast(uint2, vt[it]);
+      top = top2(top2(top, x.x), x.y);
+    }
+    const bool slow = __any(cw.odd != 0 || odd_top(top));
+    if (lane == 0) *by_token = slow;
+    if (slow) {
+      stage_barrier();
       for (int t = 0; t < cnt; ++t) {
         const int64_t row = (int64_t)(first + t0 + t) * p.HV + h;
         const float a = expf(p.g[row]), b = DELTA ? bf2f(p.beta[row]) : 1.f;
@@ -659,146 +708,99 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
           kt[d] = *reinterpret_cast<const bf16x4*>(x + KO);
           qt[d] = *reinterpret_cast<const bf16x4*>(x + QO);
         }
+        float u = bf2f(p.v[row * kHD + dv]), x = 0.f, o = 0.f;
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          float u = bf2f(p.v[row * kHD + dv + ct * 16]), x = 0.f, o = 0.f;
+        for (int d = 0; d < 8; ++d) {
+          st[d][0] *= a;
 #pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            st[d][ct] *= a;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x += st[d][ct][r] * (float)kt[d][r];
-          }
-          x += __shfl_xor(x, 16);
-          x += __shfl_xor(x, 32);
-          if (DELTA) u = b * (u - x);
-#pragma unroll
-          for (int d = 0; d < 8; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              st[d][ct][r] += (float)kt[d][r] * u;
-              o += st[d][ct][r] * (float)qt[d][r];
-            }
-          o += __shfl_xor(o, 16);
-          o += __shfl_xor(o, 32);
-          if (g == 0) p.o[row * kHD + dv + ct * 16] = (uint16_t)f2bf(p.scale * o);
+          for (int r = 0; r < 4; ++r) x += st[d][0][r] * (float)kt[d][r];
         }
+        x += __shfl_xor(x, 16);
+        x += __shfl_xor(x, 32);
+        if (DELTA) u = b * (u - x);
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            st[d][0][r] += (float)kt[d][r] * u;
+            o += st[d][0][r] * (float)qt[d][r];
+          }
+        o += __shfl_xor(o, 16);
+        o += __shfl_xor(o, 32);
+        if (g == 0) p.o[row * kHD + dv] = (uint16_t)f2bf(p.scale * o);
       }
-      wait_vmcnt<0>();
       continue;
     }
 
-    bf16x8 sh[4][CT], sl[4][CT];
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) split8(st[2 * s][ct], st[2 * s + 1][ct], sh[s][ct], sl[s][ct]);
-    if (more) fetch(1, t0 + kChunk, other);
     // Products on one accumulator follow each other with others between them: a product waits for the one before on its
     // accumulator twice as long as it occupies the unit.
-    bf16x8 xh[2][CT], xl[2][CT];  // X, or V itself
+    bf16x8 xh[2][1], xl[2][1];  // X, or V itself
     if (DELTA) {
-      f32x4 x[4][CT];
+      f32x4 x[4][1];
       rows_times(stage + KO, aoff, sh, sl, x);
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         const f32x4 f = *reinterpret_cast<const f32x4*>(cw.from + it * 16 + g * 4);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const uint2 v = __builtin_bit_cast(uint2, vt[ct][it]);
-          x[it][ct] = f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
-                            __uint_as_float(v.y & 0xffff0000u)} -
-                      f * x[it][ct];
-        }
+        const uint2 v = __builtin_bit_cast(uint2, vt[it]);
+        x[it][0] = f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                         __uint_as_float(v.y & 0xffff0000u)} -
+                   f * x[it][0];
       }
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) split8(x[2 * k][ct], x[2 * k + 1][ct], xh[k][ct], xl[k][ct]);
+      for (int k = 0; k < 2; ++k) split8(x[2 * k][0], x[2 * k + 1][0], xh[k][0], xl[k][0]);
     } else {
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) xh[k][ct] = join(vt[ct][2 * k], vt[ct][2 * k + 1]);
+      for (int k = 0; k < 2; ++k) xh[k][0] = join(vt[2 * k], vt[2 * k + 1]);
     }
-    if (more) fetch(2, t0 + kChunk, other);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      x0[(2 * k) * 64] = xh[k][0];
+      if (DELTA) x0[(2 * k + 1) * 64] = xl[k][0];
+    }
+    stage_barrier();
     // the decayed U, and the state
-    bf16x8 uh[2][CT], ul[2][CT];
+    bf16x8 uh[2], ul[2];
     {
-      f32x4 u[4][CT];
+      f32x4 u[4][1];
       if (DELTA) {
         lower_times<true>(cw.T, lane, xh, xl, u);
       } else {
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
           const f32x4 f = *reinterpret_cast<const f32x4*>(cw.to + it * 16 + g * 4);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            const uint2 v = __builtin_bit_cast(uint2, vt[ct][it]);
-            u[it][ct] = f * f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u),
-                                  __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
-          }
+          const uint2 v = __builtin_bit_cast(uint2, vt[it]);
+          u[it][0] = f * f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                               __uint_as_float(v.y & 0xffff0000u)};
         }
       }
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) split8(u[2 * k][ct], u[2 * k + 1][ct], uh[k][ct], ul[k][ct]);
+      for (int k = 0; k < 2; ++k) split8(u[2 * k][0], u[2 * k + 1][0], uh[k], ul[k]);
     }
-    if (more) fetch(3, t0 + kChunk, other);
     const float all = cw.all;
 #pragma unroll
     for (int d = 0; d < 8; d += 4) {
-      bf16x4 kt[4][4];  // key dims d .. d + 3, tokens 16 t + 4 g ..
+      bf16x4 kt[4][4];  // key dims of d .. d + 3, tokens 16 t + 4 g ..
       tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2], stage + toff[d / 2] + 8, kt[0], kt[1]);
       tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2 + 1], stage + toff[d / 2 + 1] + 8, kt[2], kt[3]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) st[d + e][ct] *= all;
+      for (int e = 0; e < 4; ++e) st[d + e][0] *= all;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int part = 0; part < 2; ++part)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
-              st[d + e][ct] = mfma(join(kt[e][2 * k], kt[e][2 * k + 1]), part == 0 ? uh[k][ct] : ul[k][ct], st[d + e][ct]);
+            st[d + e][0] = mfma(join(kt[e][2 * k], kt[e][2 * k + 1]), part == 0 ? uh[k] : ul[k], st[d + e][0]);
     }
-    // the outputs
-    const __amdgpu_buffer_rsrc_t orow = head_rows(p.o, first + t0, cnt, p.HV, h);
-    f32x4 x[4][CT];
-    rows_times(stage + QO, aoff, sh, sl, x);
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const f32x4 f = *reinterpret_cast<const f32x4*>(cw.out + it * 16 + g * 4);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) x[it][ct] *= f;
-    }
-    if (DELTA)
-      lower_times<false>(cw.P, lane, xh, xl, x);
-    else
-      lower_times(cw.P, lane, xh, x);
-#pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)f2bf(x[it][ct][r]), orow,
-                                                (uint32_t)(it * 16 + g * 4 + r) * (p.HV * kHD * 2) + (dv + ct * 16) * 2, 0,
-                                                0);
   }
 #pragma unroll
   for (int d = 0; d < 8; ++d)
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        p.state_out[(sq * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv + ct * 16] = st[d][ct][r];
+    for (int r = 0; r < 4; ++r)
+      p.state_out[(sq * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv] = st[d][0][r];
 }
 
-constexpr int prompt_lds(bool delta, int ct) { return 2 * (chunk_bytes(delta) + kChunk * (512 + 128 * ct)); }
+constexpr int prompt_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * (512 + 64)) + 2 * (8192 + 4096) + 16; }
 
 }  // namespace
 
@@ -826,22 +828,20 @@ hipError_t launch_linattn_prompt(const LinParams& p, hipStream_t st) {
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  const bool wide = p.S * p.HV >= 256;
-  const auto kernel = delta ? (wide ? linattn_prompt_k<true, 2> : linattn_prompt_k<true, 1>)
-                            : (wide ? linattn_prompt_k<false, 2> : linattn_prompt_k<false, 1>);
-  const int lds = prompt_lds(delta, wide ? 2 : 1);
+  const auto kernel = delta ? linattn_prompt_k<true> : linattn_prompt_k<false>;
+  const int lds = prompt_lds(delta);
   // once for each device and kernel; a second thread that comes meanwhile sets the same again
-  static std::atomic<bool> set[64][4];
+  static std::atomic<bool> set[64][2];
   int dev = 0;
   hipError_t err = hipGetDevice(&dev);
   if (err != hipSuccess) return err;
-  std::atomic<bool>* const done = dev >= 0 && dev < 64 ? &set[dev][delta * 2 + wide] : nullptr;
+  std::atomic<bool>* const done = dev >= 0 && dev < 64 ? &set[dev][delta] : nullptr;
   if (done == nullptr || !done->load(std::memory_order_acquire)) {
     err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (err != hipSuccess) return err;
     if (done != nullptr) done->store(true, std::memory_order_release);
   }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.S + 1) * p.HV * (wide ? 1 : 2))), dim3(256), lds, st, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.S + 1) * p.HV * 4)), dim3(256), lds, st, p);
   return hipGetLastError();
 }
 
