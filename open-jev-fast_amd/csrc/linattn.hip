@@ -196,6 +196,11 @@ __device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8& h
   hi = __builtin_bit_cast(bf16x8, make_uint4(h[0], h[1], h[2], h[3]));
   lo = __builtin_bit_cast(bf16x8, make_uint4(l[0], l[1], l[2], l[3]));
 }
+__device__ __forceinline__ f32x4 widen(bf16x4 x) {
+  const uint2 v = __builtin_bit_cast(uint2, x);
+  return f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+               __uint_as_float(v.y & 0xffff0000u)};
+}
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -500,27 +505,6 @@ __device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], in
       }
 }
 
-// Eight transposing reads, at a + x and b + x for four x. (The builtin makes the compiler wait for every LDS DMA in flight,
-// the next chunk's among them; the wait for the reads themselves is in the block, so that the registers are filled when it
-// ends.)
-template <int X0, int X1, int X2, int X3>
-__device__ __forceinline__ void tr_read8(const uint8_t* pa, const uint8_t* pb, bf16x4 (&a)[4], bf16x4 (&b)[4]) {
-  const uint32_t x = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)pa;
-  const uint32_t y = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)pb;
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%10\n\t"
-      "ds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
-      "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %4, %9 offset:%10\n\t"
-      "ds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
-      "ds_read_b64_tr_b16 %6, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(b[0]), "=&v"(b[1]), "=&v"(b[2]), "=&v"(b[3])
-      : "v"(x), "v"(y), "n"(X0), "n"(X1), "n"(X2), "n"(X3)
-      : "memory");
-}
 // Every wave's LDS reads of the stage before are done, and what its own wait has seen land is there for all; global loads
 // and DMAs stay in flight.
 __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -607,7 +591,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         sh[s][0] = s0[(2 * s) * 64];
         sl[s][0] = s0[(2 * s + 1) * 64];
       }
-      // the next chunk's DMAs go out in quarters: all at once they would hold up the wave
+      // the next chunk's DMAs, in two lots: all at once they would hold up the wave
       if (more) {
         fetch(0, t0 + kChunk, other);
         fetch(1, t0 + kChunk, other);
@@ -647,7 +631,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   }
 
   // -------------------------------------------------------------------------------------------------- the state
-  f32x4 st[8][1];
+  f32x4 st[8];
   {
     int64_t at = -1;
     if (p.state != nullptr) at = p.src != nullptr ? (int64_t)p.src[sq] : sq;
@@ -657,10 +641,10 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
       for (int d = 0; d < 8; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          st[d][0][r] = p.state[(at * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv];
+          st[d][r] = p.state[(at * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv];
     } else {
 #pragma unroll
-      for (int d = 0; d < 8; ++d) st[d][0] = f32x4{fill, fill, fill, fill};
+      for (int d = 0; d < 8; ++d) st[d] = f32x4{fill, fill, fill, fill};
     }
   }
   int toff[4];  // K's rows read transposed, key dims 32 s .. + 31
@@ -669,51 +653,96 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   for (int s = 0; s < 4; ++s) toff[s] = KO + trow * 256 + ((s * 4 + (c & 3)) ^ swizzle(trow)) * 16;
   const int vtoff = VO + trow * VB + slice * 32 + (c & 3) * 8;
   const auto join = [](bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); };
-  bf16x8 sh[4][1], sl[4][1];
+  // Every step is taken in halves, so that one half's conversions run behind the other's products; products on one
+  // accumulator are two apart (one waits for the one before it twice as long as it occupies the unit); what the second part
+  // of a chunk reads from LDS is read in the first.
+  bf16x8 sh[4], sl[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) split8(st[2 * s], st[2 * s + 1], sh[s], sl[s]);
   for (int ch = 0; ch < chunks; ++ch) {
     const int t0 = ch * kChunk, cnt = min(kChunk, n - t0);
     const uint8_t* const stage = smem + (ch & 1) * STAGE;
     const ChunkWork& cw = *reinterpret_cast<const ChunkWork*>(stage);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      split8(st[2 * s][0], st[2 * s + 1][0], sh[s][0], sl[s][0]);
-      s0[(2 * s) * 64] = sh[s][0];
-      s0[(2 * s + 1) * 64] = sl[s][0];
+      s0[(2 * s) * 64] = sh[s];
+      s0[(2 * s + 1) * 64] = sl[s];
     }
     stage_barrier();
-    bf16x4 vt[4];  // V's columns: X's accumulators' places, and its B operand
-    {
-      const uint8_t* const va = stage + vtoff;
-      bf16x4 a[4], b[4];
-      tr_read8<0, 8, 16 * VB, 16 * VB + 8>(va, va + 32 * VB, a, b);
-      vt[0] = a[0], vt[1] = a[2], vt[2] = b[0], vt[3] = b[2];
+    const auto tr = [](const uint8_t* a) {
+      return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)a);
+    };
+    // The order of the reads from LDS is fixed (sched_barrier): each goes out while the products before its use run.
+    f32x4 x[4], from[4], to[4];
+    bf16x8 ka[2][4][2], T[2][6];
+    bf16x4 vt[4], kt[8][4];  // V's columns (X's accumulators' places); K^T: accumulator d's key dims, tokens 16 t + 4 g ..
+    if (DELTA) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            ka[half][s][e] = *reinterpret_cast<const bf16x8*>(stage + KO + half * 8192 + e * 4096 + aoff[s]);
     }
+    const auto keys_times_state = [&](int half) {
+      x[2 * half] = x[2 * half + 1] = f32x4{};
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) x[2 * half + e] = mfma(ka[half][s][e], part == 0 ? sh[s] : sl[s], x[2 * half + e]);
+    };
+    __builtin_amdgcn_sched_barrier(0);
+    if (DELTA) keys_times_state(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      vt[it] = tr(stage + vtoff + it * 16 * VB);
+      if (DELTA)
+        from[it] = *reinterpret_cast<const f32x4*>(cw.from + it * 16 + g * 4);
+      else
+        to[it] = *reinterpret_cast<const f32x4*>(cw.to + it * 16 + g * 4);
+    }
+    const int odd = cw.odd;
+    const float all = cw.all;
+    __builtin_amdgcn_sched_barrier(0);
+    if (DELTA) keys_times_state(1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (DELTA)
+#pragma unroll
+      for (int f = 0; f < 6; ++f) {
+        T[0][f] = *reinterpret_cast<const bf16x8*>(cw.T[0][f][lane]);
+        T[1][f] = *reinterpret_cast<const bf16x8*>(cw.T[1][f][lane]);
+      }
+    __builtin_amdgcn_sched_barrier(0);
     uint32_t top = 0;
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      const uint2 x = __builtin_bit_cast(uint2, vt[it]);
-      top = top2(top2(top, x.x), x.y);
+      const uint2 v = __builtin_bit_cast(uint2, vt[it]);
+      top = top2(top2(top, v.x), v.y);
     }
-    const bool slow = __any(cw.odd != 0 || odd_top(top));
+    const bool slow = __any(odd != 0 || odd_top(top));
     if (lane == 0) *by_token = slow;
     if (slow) {
       stage_barrier();
       for (int t = 0; t < cnt; ++t) {
         const int64_t row = (int64_t)(first + t0 + t) * p.HV + h;
         const float a = expf(p.g[row]), b = DELTA ? bf2f(p.beta[row]) : 1.f;
-        bf16x4 kt[8], qt[8];
+        bf16x4 kr[8], qr[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
           const uint8_t* const x = stage + t * 256 + (((d >> 1) * 4 + g) ^ swizzle(t & 15)) * 16 + (d & 1) * 8;
-          kt[d] = *reinterpret_cast<const bf16x4*>(x + KO);
-          qt[d] = *reinterpret_cast<const bf16x4*>(x + QO);
+          kr[d] = *reinterpret_cast<const bf16x4*>(x + KO);
+          qr[d] = *reinterpret_cast<const bf16x4*>(x + QO);
         }
         float u = bf2f(p.v[row * kHD + dv]), x = 0.f, o = 0.f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          st[d][0] *= a;
+          st[d] *= a;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x += st[d][0][r] * (float)kt[d][r];
+          for (int r = 0; r < 4; ++r) x += st[d][r] * (float)kr[d][r];
         }
         x += __shfl_xor(x, 16);
         x += __shfl_xor(x, 32);
@@ -722,82 +751,82 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         for (int d = 0; d < 8; ++d)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            st[d][0][r] += (float)kt[d][r] * u;
-            o += st[d][0][r] * (float)qt[d][r];
+            st[d][r] += (float)kr[d][r] * u;
+            o += st[d][r] * (float)qr[d][r];
           }
         o += __shfl_xor(o, 16);
         o += __shfl_xor(o, 32);
         if (g == 0) p.o[row * kHD + dv] = (uint16_t)f2bf(p.scale * o);
       }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) split8(st[2 * s], st[2 * s + 1], sh[s], sl[s]);
       continue;
     }
 
-    // Products on one accumulator follow each other with others between them: a product waits for the one before on its
-    // accumulator twice as long as it occupies the unit.
-    bf16x8 xh[2][1], xl[2][1];  // X, or V itself
-    if (DELTA) {
-      f32x4 x[4][1];
-      rows_times(stage + KO, aoff, sh, sl, x);
-#pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const f32x4 f = *reinterpret_cast<const f32x4*>(cw.from + it * 16 + g * 4);
-        const uint2 v = __builtin_bit_cast(uint2, vt[it]);
-        x[it][0] = f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
-                         __uint_as_float(v.y & 0xffff0000u)} -
-                   f * x[it][0];
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) split8(x[2 * k][0], x[2 * k + 1][0], xh[k][0], xl[k][0]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) xh[k][0] = join(vt[2 * k], vt[2 * k + 1]);
-    }
+    bf16x8 xh[2], xl[2];  // X, or V itself
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      x0[(2 * k) * 64] = xh[k][0];
-      if (DELTA) x0[(2 * k + 1) * 64] = xl[k][0];
-    }
-    stage_barrier();
-    // the decayed U, and the state
-    bf16x8 uh[2], ul[2];
-    {
-      f32x4 u[4][1];
       if (DELTA) {
-        lower_times<true>(cw.T, lane, xh, xl, u);
-      } else {
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          const f32x4 f = *reinterpret_cast<const f32x4*>(cw.to + it * 16 + g * 4);
-          const uint2 v = __builtin_bit_cast(uint2, vt[it]);
-          u[it][0] = f * f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
-                               __uint_as_float(v.y & 0xffff0000u)};
+        for (int it = 2 * k; it < 2 * k + 2; ++it) {
+          x[it] = widen(vt[it]) - from[it] * x[it];
         }
+        split8(x[2 * k], x[2 * k + 1], xh[k], xl[k]);
+        x0[(2 * k + 1) * 64] = xl[k];
+      } else {
+        xh[k] = join(vt[2 * k], vt[2 * k + 1]);
       }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) split8(u[2 * k][0], u[2 * k + 1][0], uh[k], ul[k]);
+      x0[(2 * k) * 64] = xh[k];
     }
-    const float all = cw.all;
 #pragma unroll
-    for (int d = 0; d < 8; d += 4) {
-      bf16x4 kt[4][4];  // key dims of d .. d + 3, tokens 16 t + 4 g ..
-      tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2], stage + toff[d / 2] + 8, kt[0], kt[1]);
-      tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2 + 1], stage + toff[d / 2 + 1] + 8, kt[2], kt[3]);
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) st[d + e][0] *= all;
+      for (int t = 0; t < 4; ++t) {
+        kt[2 * s][t] = tr(stage + toff[s] + t * 4096);
+        kt[2 * s + 1][t] = tr(stage + toff[s] + t * 4096 + 8);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    stage_barrier();
+    // U, decayed to the chunk's end
+    f32x4 u[4];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+    for (int half = 0; half < 2; ++half)
+      if (DELTA) {
+        u[2 * half] = u[2 * half + 1] = f32x4{};
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+        for (int k = 0; k <= half; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            st[d + e][0] = mfma(join(kt[e][2 * k], kt[e][2 * k + 1]), part == 0 ? uh[k] : ul[k], st[d + e][0]);
+          for (int part = 0; part < 4; ++part)
+#pragma unroll
+            for (int it = 2 * half; it < 2 * half + 2; ++it)
+              u[it] = mfma(T[part >> 1][frag(it, k)], part & 1 ? xl[k] : xh[k], u[it]);
+      } else {
+        u[2 * half] = to[2 * half] * widen(vt[2 * half]);
+        u[2 * half + 1] = to[2 * half + 1] * widen(vt[2 * half + 1]);
+      }
+    // the state
+#pragma unroll
+    for (int d = 0; d < 8; ++d) st[d] *= all;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      bf16x8 uh, ul;
+      split8(u[2 * k], u[2 * k + 1], uh, ul);
+#pragma unroll
+      for (int d = 0; d < 8; d += 2) {
+        const bf16x8 a = join(kt[d][2 * k], kt[d][2 * k + 1]), b = join(kt[d + 1][2 * k], kt[d + 1][2 * k + 1]);
+        st[d] = mfma(a, uh, st[d]);
+        st[d + 1] = mfma(b, uh, st[d + 1]);
+        st[d] = mfma(a, ul, st[d]);
+        st[d + 1] = mfma(b, ul, st[d + 1]);
+        if (k == 1) split8(st[d], st[d + 1], sh[d / 2], sl[d / 2]);
+      }
     }
   }
 #pragma unroll
   for (int d = 0; d < 8; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      p.state_out[(sq * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv] = st[d][0][r];
+      p.state_out[(sq * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv] = st[d][r];
 }
 
 constexpr int prompt_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * (512 + 64)) + 2 * (8192 + 4096) + 16; }
