@@ -470,25 +470,24 @@ __device__ __forceinline__ void rows_times(const uint8_t* rows, const int (&aoff
   }
 }
 
-// x (+)= m b, m a chunk's lower triangular matrix in two pieces, b in two or one (exact).
-template <bool ALL, int CT>
+// x += m b, m a chunk's lower triangular matrix in two pieces, b in two or one (exact).
+template <int CT>
 __device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], int lane, const bf16x8 (&bh)[2][CT],
                                             const bf16x8 (&bl)[2][CT], f32x4 (&x)[4][CT]) {
-  if (ALL)
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
+  for (int part = 0; part < 2; ++part)  // hi (hi, lo), lo hi
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) x[it][ct] = f32x4{};
+    for (int k = 0; k < 2; ++k) {
+      bf16x8 a[4];
 #pragma unroll
-  for (int part = 0; part < (ALL ? 4 : 3); ++part)  // hi hi, hi lo, lo hi, lo lo
+      for (int it = 2 * k; it < 4; ++it) a[it] = *reinterpret_cast<const bf16x8*>(m[part][frag(it, k)][lane]);
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+      for (int piece = 0; piece < 2 - part; ++piece)
 #pragma unroll
-      for (int it = 2 * k; it < 4; ++it) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(m[part >> 1][frag(it, k)][lane]);
+        for (int it = 2 * k; it < 4; ++it)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) x[it][ct] = mfma(a, part & 1 ? bl[k][ct] : bh[k][ct], x[it][ct]);
-      }
+          for (int ct = 0; ct < CT; ++ct) x[it][ct] = mfma(a[it], piece == 0 ? bh[k][ct] : bl[k][ct], x[it][ct]);
+    }
 }
 template <int CT>
 __device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], int lane, const bf16x8 (&b)[2][CT],
@@ -616,7 +615,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         if (DELTA) xl[k][0] = x0[(2 * k + 1) * 64];
       }
       if (DELTA)
-        lower_times<false>(cw.P, lane, xh, xl, x);
+        lower_times(cw.P, lane, xh, xl, x);
       else
         lower_times(cw.P, lane, xh, x);
       const __amdgpu_buffer_rsrc_t orow = head_rows(p.o, first + t0, cnt, p.HV, h);
@@ -796,7 +795,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 #pragma unroll
         for (int k = 0; k <= half; ++k)
 #pragma unroll
-          for (int part = 0; part < 4; ++part)
+          for (int part = 0; part < 3; ++part)  // hi hi, hi lo, lo hi
 #pragma unroll
             for (int it = 2 * half; it < 2 * half + 2; ++it)
               u[it] = mfma(T[part >> 1][frag(it, k)], part & 1 ? xl[k] : xh[k], u[it]);
@@ -818,9 +817,10 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         st[d + 1] = mfma(b, uh, st[d + 1]);
         st[d] = mfma(a, ul, st[d]);
         st[d + 1] = mfma(b, ul, st[d + 1]);
-        if (k == 1) split8(st[d], st[d + 1], sh[d / 2], sl[d / 2]);
+        if (k == 1 && d >= 2) split8(st[d - 2], st[d - 1], sh[d / 2 - 1], sl[d / 2 - 1]);
       }
     }
+    split8(st[6], st[7], sh[3], sl[3]);
   }
 #pragma unroll
   for (int d = 0; d < 8; ++d)
