@@ -436,6 +436,15 @@ __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
   }
 }
 
+// Zeros in value head h of the rows of no sequence.
+__device__ __forceinline__ void zero_rows(const LinParams& p, int h) {
+  int lo, hi;
+  seq_span(p.seq_ptr, p.S, p.R, lo, hi);
+  for (int64_t r = threadIdx.x >> 4; r < lo + (p.R - hi); r += blockDim.x >> 4)
+    *reinterpret_cast<uint4*>(p.o + ((r < lo ? r : r - lo + hi) * p.HV + h) * kHD + (threadIdx.x & 15) * 8) =
+        make_uint4(0u, 0u, 0u, 0u);
+}
+
 // The chunks of one sequence and value head in order. A slice is 16 value dims of the state with all 128 key dims: 8
 // accumulators, d of them with key dims key_dim(d, g) .. + 3 in the lanes (c, g) of value dim c. Two of them together are
 // then the B operand of K S0 and Q S0 for 32 key dims in order, and nothing of the state, of X or of U has to change its
@@ -449,13 +458,12 @@ __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
 __device__ __forceinline__ constexpr int key_dim(int d, int g) { return (d >> 1) * 32 + g * 8 + (d & 1) * 4; }
 
 // x = the 64 rows at `rows` (aoff: a lane's place in a row of 16 for key dims 32 s ..) times the state's two pieces.
-template <int CT>
-__device__ __forceinline__ void rows_times(const uint8_t* rows, const int (&aoff)[4], const bf16x8 (&sh)[4][CT],
-                                           const bf16x8 (&sl)[4][CT], f32x4 (&x)[4][CT]) {
+// Products on one accumulator follow each other with others between them: one waits for the one before on its accumulator
+// twice as long as it occupies the unit.
+__device__ __forceinline__ void rows_times(const uint8_t* rows, const int (&aoff)[4], const bf16x8 (&sh)[4],
+                                           const bf16x8 (&sl)[4], f32x4 (&x)[4]) {
 #pragma unroll
-  for (int it = 0; it < 4; ++it)
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) x[it][ct] = f32x4{};
+  for (int it = 0; it < 4; ++it) x[it] = f32x4{};
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     bf16x8 a[4];
@@ -464,44 +472,111 @@ __device__ __forceinline__ void rows_times(const uint8_t* rows, const int (&aoff
 #pragma unroll
     for (int part = 0; part < 2; ++part)
 #pragma unroll
-      for (int it = 0; it < 4; ++it)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) x[it][ct] = mfma(a[it], part == 0 ? sh[s][ct] : sl[s][ct], x[it][ct]);
+      for (int it = 0; it < 4; ++it) x[it] = mfma(a[it], part == 0 ? sh[s] : sl[s], x[it]);
   }
 }
 
-// x += m b, m a chunk's lower triangular matrix in two pieces, b in two or one (exact).
-template <int CT>
-__device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], int lane, const bf16x8 (&bh)[2][CT],
-                                            const bf16x8 (&bl)[2][CT], f32x4 (&x)[4][CT]) {
+// x += m b, m a chunk's lower triangular matrix in two pieces, b in two (lo lo is left out) or, exact, in one.
+template <bool TWO>
+__device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], int lane, const bf16x8 (&bh)[2],
+                                            const bf16x8 (&bl)[2], f32x4 (&x)[4]) {
 #pragma unroll
-  for (int part = 0; part < 2; ++part)  // hi (hi, lo), lo hi
+  for (int part = 0; part < 2; ++part)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       bf16x8 a[4];
 #pragma unroll
       for (int it = 2 * k; it < 4; ++it) a[it] = *reinterpret_cast<const bf16x8*>(m[part][frag(it, k)][lane]);
 #pragma unroll
-      for (int piece = 0; piece < 2 - part; ++piece)
+      for (int piece = 0; piece < (TWO && part == 0 ? 2 : 1); ++piece)
 #pragma unroll
-        for (int it = 2 * k; it < 4; ++it)
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) x[it][ct] = mfma(a[it], piece == 0 ? bh[k][ct] : bl[k][ct], x[it][ct]);
+        for (int it = 2 * k; it < 4; ++it) x[it] = mfma(a[it], piece == 0 ? bh[k] : bl[k], x[it]);
     }
 }
-template <int CT>
-__device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], int lane, const bf16x8 (&b)[2][CT],
-                                            f32x4 (&x)[4][CT]) {
+
+// The state that sequence sq starts from: value dim dv, this lane's key dims.
+__device__ __forceinline__ void load_state(const LinParams& p, int64_t sq, int h, int g, int dv, f32x4 (&st)[8]) {
+  int64_t at = -1;
+  if (p.state != nullptr) at = p.src != nullptr ? (int64_t)p.src[sq] : sq;
+  if (at >= 0 && at < p.slots) {
 #pragma unroll
-  for (int part = 0; part < 2; ++part)
+    for (int d = 0; d < 8; ++d)
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+      for (int r = 0; r < 4; ++r) st[d][r] = p.state[(at * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv];
+  } else {
+    const float fill = at >= p.slots ? __uint_as_float(0x7fc00000u) : 0.f;
 #pragma unroll
-      for (int it = 2 * k; it < 4; ++it) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(m[part][frag(it, k)][lane]);
+    for (int d = 0; d < 8; ++d) st[d] = f32x4{fill, fill, fill, fill};
+  }
+}
+__device__ __forceinline__ void store_state(const LinParams& p, int64_t sq, int h, int g, int dv, const f32x4 (&st)[8]) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) x[it][ct] = mfma(a, b[k][ct], x[it][ct]);
+  for (int d = 0; d < 8; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      p.state_out[(sq * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv] = st[d][r];
+}
+
+// cnt tokens from row t0 one by one, K and Q from LDS: state and outputs.
+template <bool DELTA>
+__device__ __forceinline__ void by_tokens(const LinParams& p, const uint8_t* krows, const uint8_t* qrows, int64_t t0, int cnt,
+                                          int h, int g, int dv, f32x4 (&st)[8]) {
+#pragma unroll 1
+  for (int t = 0; t < cnt; ++t) {
+    const int64_t row = (t0 + t) * p.HV + h;
+    const float a = expf(p.g[row]), b = DELTA ? bf2f(p.beta[row]) : 1.f;
+    bf16x4 k[8], q[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const int at = t * 256 + (((d >> 1) * 4 + g) ^ swizzle(t & 15)) * 16 + (d & 1) * 8;
+      k[d] = *reinterpret_cast<const bf16x4*>(krows + at);
+      q[d] = *reinterpret_cast<const bf16x4*>(qrows + at);
+    }
+    float u = bf2f(p.v[row * kHD + dv]), x = 0.f, o = 0.f;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      st[d] *= a;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x += st[d][r] * (float)k[d][r];
+    }
+    x += __shfl_xor(x, 16);
+    x += __shfl_xor(x, 32);
+    if (DELTA) u = b * (u - x);
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        st[d][r] += (float)k[d][r] * u;
+        o += st[d][r] * (float)q[d][r];
       }
+    o += __shfl_xor(o, 16);
+    o += __shfl_xor(o, 32);
+    if (g == 0) p.o[row * kHD + dv] = (uint16_t)f2bf(p.scale * o);
+  }
+}
+
+// A chunk's outputs in value dim dv; rows: its rows of head h.
+__device__ __forceinline__ void store_out(const LinParams& p, __amdgpu_buffer_rsrc_t rows, int g, int dv,
+                                          const f32x4 (&x)[4]) {
+#pragma unroll
+  for (int it = 0; it < 4; ++it)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      __builtin_amdgcn_raw_buffer_store_b16((uint16_t)f2bf(x[it][r]), rows,
+                                            (uint32_t)(it * 16 + g * 4 + r) * (p.HV * kHD * 2) + dv * 2, 0, 0);
+}
+
+__device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ bool odd_values(const bf16x4 (&v)[4]) {  // one of them is not finite
+  uint32_t top = 0;
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const uint2 x = __builtin_bit_cast(uint2, v[it]);
+    top = top2(top2(top, x.x), x.y);
+  }
+  return odd_top(top);
 }
 
 // Every wave's LDS reads of the stage before are done, and what its own wait has seen land is there for all; global loads
@@ -520,12 +595,8 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = wave & 1;
   const int64_t sq = blockIdx.x / (p.HV * SL);
   const int hs = blockIdx.x - (int)(sq * p.HV * SL), h = hs / SL, hk = h / (p.HV / p.HK);
-  if (sq == p.S) {  // the rows of no sequence
-    int lo, hi;
-    seq_span(p.seq_ptr, p.S, p.R, lo, hi);
-    for (int64_t r = threadIdx.x >> 4; r < lo + (p.R - hi) && hs % SL == 0; r += 16)
-      *reinterpret_cast<uint4*>(p.o + ((r < lo ? r : r - lo + hi) * p.HV + h) * kHD + (threadIdx.x & 15) * 8) =
-          make_uint4(0u, 0u, 0u, 0u);
+  if (sq == p.S) {
+    if (hs % SL == 0) zero_rows(p, h);
     return;
   }
   SeqPlace place;
@@ -584,21 +655,21 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
       stage_barrier();
       const bool more = ch + 1 < chunks;
       uint8_t* const other = smem + ((ch + 1) & 1) * STAGE;
-      bf16x8 sh[4][1], sl[4][1];
+      bf16x8 sh[4], sl[4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        sh[s][0] = s0[(2 * s) * 64];
-        sl[s][0] = s0[(2 * s + 1) * 64];
+        sh[s] = s0[(2 * s) * 64];
+        sl[s] = s0[(2 * s + 1) * 64];
       }
       // the next chunk's DMAs, in two lots: all at once they would hold up the wave
       if (more) {
         fetch(0, t0 + kChunk, other);
         fetch(1, t0 + kChunk, other);
       }
-      f32x4 x[4][1];
+      f32x4 x[4];
       rows_times(stage + QO, aoff, sh, sl, x);
 #pragma unroll
-      for (int it = 0; it < 4; ++it) x[it][0] *= *reinterpret_cast<const f32x4*>(cw.out + it * 16 + g * 4);
+      for (int it = 0; it < 4; ++it) x[it] *= *reinterpret_cast<const f32x4*>(cw.out + it * 16 + g * 4);
       if (more) {
         fetch(2, t0 + kChunk, other);
         fetch(3, t0 + kChunk, other);
@@ -608,50 +679,26 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         wait_vmcnt<0>();
         continue;
       }
-      bf16x8 xh[2][1], xl[2][1];
+      bf16x8 xh[2], xl[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        xh[k][0] = x0[(2 * k) * 64];
-        if (DELTA) xl[k][0] = x0[(2 * k + 1) * 64];
+        xh[k] = x0[(2 * k) * 64];
+        if (DELTA) xl[k] = x0[(2 * k + 1) * 64];
       }
-      if (DELTA)
-        lower_times(cw.P, lane, xh, xl, x);
-      else
-        lower_times(cw.P, lane, xh, x);
-      const __amdgpu_buffer_rsrc_t orow = head_rows(p.o, first + t0, cnt, p.HV, h);
-#pragma unroll
-      for (int it = 0; it < 4; ++it)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)f2bf(x[it][0][r]), orow,
-                                                (uint32_t)(it * 16 + g * 4 + r) * (p.HV * kHD * 2) + dv * 2, 0, 0);
+      lower_times<DELTA>(cw.P, lane, xh, xl, x);
+      store_out(p, head_rows(p.o, first + t0, cnt, p.HV, h), g, dv, x);
     }
     return;
   }
 
   // -------------------------------------------------------------------------------------------------- the state
   f32x4 st[8];
-  {
-    int64_t at = -1;
-    if (p.state != nullptr) at = p.src != nullptr ? (int64_t)p.src[sq] : sq;
-    const float fill = at >= p.slots ? __uint_as_float(0x7fc00000u) : 0.f;
-    if (at >= 0 && at < p.slots) {
-#pragma unroll
-      for (int d = 0; d < 8; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          st[d][r] = p.state[(at * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv];
-    } else {
-#pragma unroll
-      for (int d = 0; d < 8; ++d) st[d] = f32x4{fill, fill, fill, fill};
-    }
-  }
+  load_state(p, sq, h, g, dv, st);
   int toff[4];  // K's rows read transposed, key dims 32 s .. + 31
   const int trow = g * 4 + (c >> 2);
 #pragma unroll
   for (int s = 0; s < 4; ++s) toff[s] = KO + trow * 256 + ((s * 4 + (c & 3)) ^ swizzle(trow)) * 16;
   const int vtoff = VO + trow * VB + slice * 32 + (c & 3) * 8;
-  const auto join = [](bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); };
   // Every step is taken in halves, so that one half's conversions run behind the other's products; products on one
   // accumulator are two apart (one waits for the one before it twice as long as it occupies the unit); what the second part
   // of a chunk reads from LDS is read in the first.
@@ -716,47 +763,11 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         T[1][f] = *reinterpret_cast<const bf16x8*>(cw.T[1][f][lane]);
       }
     __builtin_amdgcn_sched_barrier(0);
-    uint32_t top = 0;
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const uint2 v = __builtin_bit_cast(uint2, vt[it]);
-      top = top2(top2(top, v.x), v.y);
-    }
-    const bool slow = __any(odd != 0 || odd_top(top));
+    const bool slow = __any(odd != 0 || odd_values(vt));
     if (lane == 0) *by_token = slow;
     if (slow) {
       stage_barrier();
-      for (int t = 0; t < cnt; ++t) {
-        const int64_t row = (int64_t)(first + t0 + t) * p.HV + h;
-        const float a = expf(p.g[row]), b = DELTA ? bf2f(p.beta[row]) : 1.f;
-        bf16x4 kr[8], qr[8];
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const uint8_t* const x = stage + t * 256 + (((d >> 1) * 4 + g) ^ swizzle(t & 15)) * 16 + (d & 1) * 8;
-          kr[d] = *reinterpret_cast<const bf16x4*>(x + KO);
-          qr[d] = *reinterpret_cast<const bf16x4*>(x + QO);
-        }
-        float u = bf2f(p.v[row * kHD + dv]), x = 0.f, o = 0.f;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          st[d] *= a;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x += st[d][r] * (float)kr[d][r];
-        }
-        x += __shfl_xor(x, 16);
-        x += __shfl_xor(x, 32);
-        if (DELTA) u = b * (u - x);
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            st[d][r] += (float)kr[d][r] * u;
-            o += st[d][r] * (float)qr[d][r];
-          }
-        o += __shfl_xor(o, 16);
-        o += __shfl_xor(o, 32);
-        if (g == 0) p.o[row * kHD + dv] = (uint16_t)f2bf(p.scale * o);
-      }
+      by_tokens<DELTA>(p, stage + KO, stage + QO, first + t0, cnt, h, g, dv, st);
 #pragma unroll
       for (int s = 0; s < 4; ++s) split8(st[2 * s], st[2 * s + 1], sh[s], sl[s]);
       continue;
@@ -822,13 +833,180 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
     }
     split8(st[6], st[7], sh[3], sl[3]);
   }
-#pragma unroll
-  for (int d = 0; d < 8; ++d)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      p.state_out[(sq * p.HV + h) * (kHD * kHD) + (key_dim(d, g) + r) * kHD + dv] = st[d][r];
+  store_state(p, sq, h, g, dv, st);
 }
 
+// Many sequences: a workgroup of eight waves per sequence and value head, each with one slice and all of its work, so that
+// two waves a SIMD fill each other's gaps and what they share is loaded once a head. (Here the waves that read K^T and V
+// transposed have DMAs in flight, and the builtin makes the compiler wait for those: the reads are written out, with the
+// wait for themselves in the same block, so that the registers are filled when it ends.)
+template <int X0, int X1, int X2, int X3>
+__device__ __forceinline__ void tr_read4(const uint8_t* pa, bf16x4 (&a)[4]) {
+  const uint32_t x = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)pa;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4 offset:%5\n\t"
+      "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+      "ds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
+      "ds_read_b64_tr_b16 %3, %4 offset:%8\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3])
+      : "v"(x), "n"(X0), "n"(X1), "n"(X2), "n"(X3)
+      : "memory");
+}
+template <int X0, int X1, int X2, int X3>
+__device__ __forceinline__ void tr_read8(const uint8_t* pa, const uint8_t* pb, bf16x4 (&a)[4], bf16x4 (&b)[4]) {
+  const uint32_t x = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)pa;
+  const uint32_t y = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)pb;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %4, %9 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %6, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(b[0]), "=&v"(b[1]), "=&v"(b[2]), "=&v"(b[3])
+      : "v"(x), "v"(y), "n"(X0), "n"(X1), "n"(X2), "n"(X3)
+      : "memory");
+}
+
+template <bool DELTA>
+__global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
+  constexpr int WB = chunk_bytes(DELTA);
+  constexpr int KO = WB, QO = KO + kChunk * 256, VO = QO + kChunk * 256, STAGE = VO + kChunk * 256;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t sq = blockIdx.x / p.HV;
+  const int h = blockIdx.x - (int)(sq * p.HV), hk = h / (p.HV / p.HK);
+  if (sq == p.S) return zero_rows(p, h);
+  SeqPlace place;
+  if (!seq_find(p.seq_ptr, p.S, p.R, seq_chunks, [=](int i, int) { return i == (int)sq; }, place)) return;
+  const int first = place.first, n = place.n;
+  const int chunks = seq_chunks(n);
+  const int dv = wave * 16 + c;
+
+  // a chunk to an LDS stage: this wave's 8 rows of K, Q and V, its part of the chunk's matrices, in two halves
+  const uint8_t* const work = p.work + ((int64_t)place.before * p.HV + h) * (int64_t)WB;
+  const int64_t next_work = (int64_t)p.HV * WB;
+  uint32_t koff[2], voff[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = wave * 8 + 4 * i + g;
+    koff[i] = (uint32_t)r * (p.HK * kHD * 2) + (c ^ swizzle(r & 15)) * 16;
+    voff[i] = (uint32_t)r * (p.HV * kHD * 2) + (c ^ swizzle(r & 15)) * 16;
+  }
+  const auto fetch = [&](int i, int t, uint8_t* stage) {
+    const int cnt = min(kChunk, n - t);
+    const __amdgpu_buffer_rsrc_t kr = head_rows(p.k, first + t, cnt, p.HK, hk);
+    const __amdgpu_buffer_rsrc_t qr = head_rows(p.q, first + t, cnt, p.HK, hk);
+    const __amdgpu_buffer_rsrc_t vr = head_rows(p.v, first + t, cnt, p.HV, h);
+    const __amdgpu_buffer_rsrc_t wr = make_rsrc(work + (int64_t)(t / kChunk) * next_work, WB);
+    dma16(kr, stage + KO + wave * 2048 + i * 1024, koff[i]);
+    dma16(qr, stage + QO + wave * 2048 + i * 1024, koff[i]);
+    dma16(vr, stage + VO + wave * 2048 + i * 1024, voff[i]);
+#pragma unroll
+    for (int j = i; j < (WB / 1024 + 7) / 8; j += 2) {
+      const int at = min(j * 8 + wave, WB / 1024 - 1) * 1024;  // past the last piece: that one again
+      dma16(wr, stage + at, at + lane * 16);
+    }
+  };
+  if (chunks > 0) {
+    fetch(0, 0, smem);
+    fetch(1, 0, smem);
+  }
+  f32x4 st[8];
+  load_state(p, sq, h, g, dv, st);
+
+  // LDS offsets of this lane: rows c of K and Q, key dims 32 s .. + 31; the same of K's rows, and V's, read transposed
+  int aoff[4], toff[4];
+  const int trow = g * 4 + (c >> 2);
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    aoff[s] = c * 256 + ((s * 4 + g) ^ swizzle(c)) * 16;
+    toff[s] = KO + trow * 256 + ((s * 4 + (c & 3)) ^ swizzle(trow)) * 16;
+  }
+  const int vtoff = VO + trow * 256 + ((wave * 2 + (c >> 1 & 1)) ^ swizzle(trow)) * 16 + (c & 1) * 8;
+
+  // vmcnt(0), as the compiler knows it: the state is there, and no wait for it, which would take the DMAs along, is left
+  // for the loop
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  for (int ch = 0; ch < chunks; ++ch) {
+    const int t0 = ch * kChunk, cnt = min(kChunk, n - t0);
+    const uint8_t* const stage = smem + (ch & 1) * STAGE;
+    const ChunkWork& cw = *reinterpret_cast<const ChunkWork*>(stage);
+    if (ch > 0) wait_vmcnt<16>();  // all but the last chunk's output stores
+    stage_barrier();               // the stage has landed, and every wave is done with the other one
+    const bool more = ch + 1 < chunks;
+    uint8_t* const other = smem + ((ch + 1) & 1) * STAGE;
+    if (more) fetch(0, t0 + kChunk, other);
+    bf16x4 vt[4];  // V's columns: X's accumulators' places, and its B operand
+    tr_read4<0, 4096, 8192, 12288>(stage + vtoff, vt);
+    if (__any(cw.odd != 0 || odd_values(vt))) {
+      if (more) fetch(1, t0 + kChunk, other);
+      by_tokens<DELTA>(p, stage + KO, stage + QO, first + t0, cnt, h, g, dv, st);
+      wait_vmcnt<0>();
+      continue;
+    }
+    bf16x8 sh[4], sl[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) split8(st[2 * s], st[2 * s + 1], sh[s], sl[s]);
+    if (more) fetch(1, t0 + kChunk, other);
+    bf16x8 xh[2], xl[2];  // X, or V itself
+    if (DELTA) {
+      f32x4 x[4];
+      rows_times(stage + KO, aoff, sh, sl, x);
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+        x[it] = widen(vt[it]) - *reinterpret_cast<const f32x4*>(cw.from + it * 16 + g * 4) * x[it];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) split8(x[2 * k], x[2 * k + 1], xh[k], xl[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) xh[k] = join(vt[2 * k], vt[2 * k + 1]);
+    }
+    // U, decayed to the chunk's end, and the state
+    bf16x8 uh[2], ul[2];
+    {
+      f32x4 u[4];
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+        u[it] = DELTA ? f32x4{} : *reinterpret_cast<const f32x4*>(cw.to + it * 16 + g * 4) * widen(vt[it]);
+      if (DELTA) lower_times<true>(cw.T, lane, xh, xl, u);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) split8(u[2 * k], u[2 * k + 1], uh[k], ul[k]);
+    }
+    const float all = cw.all;
+#pragma unroll
+    for (int d = 0; d < 8; d += 4) {
+      bf16x4 kt[4][4];  // key dims of d .. d + 3, tokens 16 t + 4 g ..
+      tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2], stage + toff[d / 2] + 8, kt[0], kt[1]);
+      tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2 + 1], stage + toff[d / 2 + 1] + 8, kt[2], kt[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[d + e] *= all;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            st[d + e] = mfma(join(kt[e][2 * k], kt[e][2 * k + 1]), part == 0 ? uh[k] : ul[k], st[d + e]);
+    }
+    f32x4 x[4];
+    rows_times(stage + QO, aoff, sh, sl, x);
+#pragma unroll
+    for (int it = 0; it < 4; ++it) x[it] *= *reinterpret_cast<const f32x4*>(cw.out + it * 16 + g * 4);
+    lower_times<DELTA>(cw.P, lane, xh, xl, x);
+    store_out(p, head_rows(p.o, first + t0, cnt, p.HV, h), g, dv, x);
+  }
+  store_state(p, sq, h, g, dv, st);
+}
+
+constexpr int many_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * 768); }
+// Sequences times value heads up to which the workgroups of two slices run (four of them a head).
+constexpr int64_t kFew = 64;
 constexpr int prompt_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * (512 + 64)) + 2 * (8192 + 4096) + 16; }
 
 }  // namespace
@@ -857,20 +1035,22 @@ hipError_t launch_linattn_prompt(const LinParams& p, hipStream_t st) {
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  const auto kernel = delta ? linattn_prompt_k<true> : linattn_prompt_k<false>;
-  const int lds = prompt_lds(delta);
+  const bool many = p.S * p.HV > kFew;
+  const auto kernel = many ? (delta ? linattn_many_k<true> : linattn_many_k<false>)
+                           : (delta ? linattn_prompt_k<true> : linattn_prompt_k<false>);
+  const int lds = many ? many_lds(delta) : prompt_lds(delta);
   // once for each device and kernel; a second thread that comes meanwhile sets the same again
-  static std::atomic<bool> set[64][2];
+  static std::atomic<bool> set[64][4];
   int dev = 0;
   hipError_t err = hipGetDevice(&dev);
   if (err != hipSuccess) return err;
-  std::atomic<bool>* const done = dev >= 0 && dev < 64 ? &set[dev][delta] : nullptr;
+  std::atomic<bool>* const done = dev >= 0 && dev < 64 ? &set[dev][2 * many + delta] : nullptr;
   if (done == nullptr || !done->load(std::memory_order_acquire)) {
     err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (err != hipSuccess) return err;
     if (done != nullptr) done->store(true, std::memory_order_release);
   }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.S + 1) * p.HV * 4)), dim3(256), lds, st, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.S + 1) * p.HV * (many ? 1 : 4))), dim3(many ? 512 : 256), lds, st, p);
   return hipGetLastError();
 }
 
