@@ -1005,8 +1005,9 @@ __global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
 }
 
 constexpr int many_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * 768); }
-// Sequences times value heads up to which the workgroups of two slices run (four of them a head).
-constexpr int64_t kFew = 64;
+// Sequences times value heads up to which the workgroups of two slices run (four of them a head). Both kernels, 500 tokens
+// a sequence: 48 heads 33 us with slices, 47 with eight waves a head; 96 43-49 and 49-51; 144 59 and 54; 288 87 and 63.
+constexpr int64_t kFew = 96;
 constexpr int prompt_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * (512 + 64)) + 2 * (8192 + 4096) + 16; }
 
 }  // namespace

@@ -266,7 +266,7 @@ __device__ __forceinline__ void add_values(const uint16_t* vl, const float (&w)[
 
 // Which of the 32 positions from p0 exist: below the sequence's end, in pages of the cache.
 __device__ __forceinline__ uint32_t existing(int64_t left, bool ok0, bool ok1) {
-  return (left >= 32 ? ~0u : (1u << left) - 1) & ((ok0 ? 0xffffu : 0u) | (ok1 ? 0xffff0000u : 0u));
+  return (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1) & ((ok0 ? 0xffffu : 0u) | (ok1 ? 0xffff0000u : 0u));
 }
 
 // Few rows: 16 packed rows a workgroup, its four waves take the part's units in turn.
@@ -412,90 +412,80 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
     p.lse[nh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-// Many rows: 64 CT packed rows a workgroup, 16 CT of them a wave; all take the part's units in order, from LDS. A thread
-// loads its 16-byte pieces of the next unit before it works on the present one and stores them, as bf16, to the other half
-// of the LDS after it.
+// More rows: 16 CT packed rows a workgroup, 128 positions at a time. A wave takes 32 of the positions for the scores, with
+// their keys straight from the cache as in the narrow kernel, and a quarter of the dims for the outputs, with that quarter
+// of the 128 values in LDS rows of its own: keys and values are read once a workgroup, however many rows it has. What the
+// waves exchange is the weights (a lane's eight are the B operand for its 32 positions as they are) and the maxima. The
+// steps of two lots overlap, so that one barrier a lot is enough: behind it a wave
+//   adds the values of lot i - 1 with the weights of all four waves,
+//   takes lot i's maxima, brings its sums to a new reference where one has grown, makes its weights of lot i,
+//   makes its scores of lot i + 1 and leaves their maxima.
+// All waves see the same maxima and so hold the same references.
 template <int D, bool FP8, int CT>
-__global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) tree_wide_k(TreeParams p) {
-  constexpr int R = 64 * CT, KF = D / 32, DT = D / 16, RB = D * (FP8 ? 1 : 2);
-  constexpr int KS = D + 8, RS = D + 16;   // LDS rows of keys and values: what spreads each one's reads over the banks
-  constexpr int PL = 32 * RB / 16 / 256;   // pieces of the unit's keys (and of its values) a thread loads
-  constexpr int PR = RB / 16;              // pieces of a row
-  constexpr int TILE = 32 * (KS + RS);
-  __shared__ __attribute__((aligned(16))) uint16_t buf[2][TILE];
-  __shared__ __attribute__((aligned(16))) float sc[2][2][32];
-  __shared__ int odd_at[2];
+__global__ void __launch_bounds__(256, 1) tree_wide_k(TreeParams p) {
+  constexpr int R = 16 * CT, KF = D / 32, RB = D * (FP8 ? 1 : 2);  // RB: bytes of a cache row
+  constexpr int DS = D / 4, DT = DS / 16;                          // dims of a wave
+  constexpr int VS = DS + 16;                                      // LDS row of values, in bf16
+  constexpr int KL = RB / 64;                                      // 16-byte loads of a key
+  constexpr int VR = RB / 64, VK = 64 / VR, VL = 128 / VK;         // lanes of a value row's quarter, rows a load, loads
+  __shared__ __attribute__((aligned(16))) uint16_t vbuf[4][128 * VS];
+  __shared__ __attribute__((aligned(16))) uint4 pbuf[2][4][CT][64];
+  __shared__ float sm[2][4][R], sl[4][R];
 
   Part w;
-  if (!w.find(p, R, D, 1)) return;
+  if (!w.find(p, R, D, 4)) return;
   if (p.splits > 1 && w.u0 >= w.u1) return w.no_sums(p, R);
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wrow = w.row0 + wave * 16 * CT;
-  const Rows<CT> rw(p, wrow, w.rows, w.first, w.hk);
+  const Rows<CT> rw(p, w.row0, w.rows, w.first, w.hk);
   const Table table(p, w);
   bf16x8 qf[CT][KF];
-  load_q<D, FP8, CT>(p, rw, w.first, false, qf);
+  load_q<D, FP8, CT>(p, rw, w.first, FP8, qf);
 
-  uint4 kx[PL], vx[PL];
-  float kq1 = 0.f, vq1 = 0.f;
-  bool ok[2], now[2];
-  const auto load = [&](int u) {
-    int64_t row[2];
+  // keys of unit u (32 positions) and values of the lot that begins there; which of their tiles of 16 are in the cache
+  uint4 kx[2][KL], vx[VL];
+  f32x4 ks[2], vs[2];
+  const auto load_k = [&](int u) -> int {
+    int ok = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      row[t] = table.row(2 * u + t);
-      ok[t] = row[t] >= 0;
-      row[t] = max(row[t], (int64_t)0);  // any row of the cache: its values are not used
-    }
+      const int64_t r = table.row(2 * u + t), row = max(r, (int64_t)0);  // any row of the cache: it is not used
+      ok |= (r >= 0) << t;
+      const uint8_t* kb = static_cast<const uint8_t*>(p.kc) + row * RB;
 #pragma unroll
-    for (int i = 0; i < PL; ++i) {
-      const int piece = i * 256 + threadIdx.x, key = piece / PR;
-      const int64_t at = (key >= 16 ? row[1] : row[0]) * RB + (key & 15) * RB + (piece % PR) * 16;
-      kx[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.kc) + at);
-      vx[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.vc) + at);
-    }
-    if (FP8) {
-      const int64_t at = (threadIdx.x & 16 ? row[1] : row[0]) + (threadIdx.x & 15);
-      kq1 = p.ks[at];
-      vq1 = p.vs[at];
-    }
-  };
-  // the loaded unit u to LDS half h
-  const auto store = [&](int u, int h) {
-    const int64_t p0 = (int64_t)u * 32;
-    const bool edge = !(ok[0] && ok[1]) || p0 + 32 > min(w.ctx, w.total);
-    const uint32_t there = existing(w.total - p0, ok[0], ok[1]);
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < PL; ++i) {
-      const int piece = i * 256 + threadIdx.x, key = piece / PR, d = (piece % PR) * (FP8 ? 16 : 8);
-      uint4* const kd = reinterpret_cast<uint4*>(buf[h] + key * KS + d);
-      uint4* const vd = reinterpret_cast<uint4*>(buf[h] + 32 * KS + key * RS + d);
-#pragma unroll
-      for (int e = 0; e < (FP8 ? 2 : 1); ++e) {
-        uint4 x = vx[i], y = kx[i];
-        if (FP8) {
-          x = e ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y);
-          y = e ? cvt_fp8x8(y.z, y.w) : cvt_fp8x8(y.x, y.y);
-        }
-        if (edge) {
-          if (!(there >> key & 1)) x = make_uint4(0u, 0u, 0u, 0u);
-          odd |= odd2(x.x) || odd2(x.y) || odd2(x.z) || odd2(x.w);
-        }
-        kd[e] = y;
-        vd[e] = x;
+      for (int f = 0; f < KL; ++f) kx[t][f] = *reinterpret_cast<const uint4*>(kb + c * RB + f * 64 + g * 16);
+      if (FP8) {
+        ks[t] = *reinterpret_cast<const f32x4*>(p.ks + row + g * 4);
+        vs[t] = *reinterpret_cast<const f32x4*>(p.vs + row + g * 4);
       }
     }
-    if (FP8 && threadIdx.x < 32) {
-      sc[h][0][threadIdx.x] = kq1;
-      sc[h][1][threadIdx.x] = vq1;
-    }
-    if (edge && __any(odd) && lane == 0) odd_at[h] = u;
+    return ok;
   };
+  const auto load_v = [&](int u) -> int {
+    int64_t row[8];
+    int ok = 0;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const int64_t r = table.row(2 * u + t);
+      row[t] = max(r, (int64_t)0);
+      ok |= (r >= 0) << t;
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int key = lane / VR;  // of this load's VK
+      int64_t at;
+      if constexpr (VK == 32)
+        at = (key >= 16 ? row[2 * i + 1] : row[2 * i]) + (key & 15);
+      else
+        at = row[i * VK / 16] + (i * VK) % 16 + key;
+      vx[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.vc) + at * RB + wave * (RB / 4) + (lane % VR) * 16);
+    }
+    return ok;
+  };
+  const int64_t plain = min(w.ctx, w.total);  // positions below are seen by every row, if they are in the cache
 
   const float f2 = p.scale * kLog2e;
-  f32x4 acc[DT][CT];
+  f32x4 acc[DT][CT], s[2][CT], vq[2];
   float m[CT], l[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -504,69 +494,189 @@ __global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) tree_wide_k(TreeParams p
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d][ct] = f32x4{};
   }
-  if (threadIdx.x < 2) odd_at[threadIdx.x] = -1;
-  __syncthreads();
-  if (w.u0 < w.u1) {
-    load(w.u0);
-    store(w.u0, 0);
-  }
-  for (int u = w.u0; u < w.u1; ++u) {
-    const int h = (u - w.u0) & 1;
-    now[0] = ok[0];
-    now[1] = ok[1];
-    lds_barrier();
-    if (u + 1 < w.u1) load(u + 1);
-    const uint16_t* const kl = buf[h] + c * KS + g * 8;
-    f32x4 s[2][CT];
+  bool edge_s = false;  // of the scores in s
+  // scores of the loaded unit u, masked, to base two; their maxima to sm[half]
+  const auto scores = [&](int u, int ok, int half) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) s[t][ct] = f32x4{};
 #pragma unroll
       for (int f = 0; f < KF; ++f) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(kl + t * 16 * KS + f * 32);
+        const uint4 x = kx[t][FP8 ? f >> 1 : f];
+        const bf16x8 a = __builtin_bit_cast(bf16x8, !FP8 ? x : f & 1 ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y));
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) s[t][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[ct][f], s[t][ct], 0, 0, 0);
       }
     }
     const int64_t p0 = (int64_t)u * 32;
-    const bool edge = !(now[0] && now[1]) || p0 + 32 > min(w.ctx, w.total);
-    f32x4 kq[2], vq[2];
-    if (FP8)
+    edge_s = ok != 3 || p0 + 32 > plain;
+    const uint32_t there = edge_s ? existing(w.total - p0, ok & 1, ok >> 1) : ~0u;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float top = -INFINITY;
+      uint32_t see = ~0u;
+      if (edge_s) see = (rw.live[ct] ? there & seen32(p, rw.words[ct], rw.tok[ct], p0 - w.ctx) : 0u) >> (g * 4);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        kq[t] = *reinterpret_cast<const f32x4*>(&sc[h][0][t * 16 + g * 4]);
-        vq[t] = *reinterpret_cast<const f32x4*>(&sc[h][1][t * 16 + g * 4]);
+        s[t][ct] *= f2;
+        if (FP8) s[t][ct] *= ks[t];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (edge_s && !(see >> (t * 16 + r) & 1)) s[t][ct][r] = -INFINITY;
+          top = fmaxf(top, s[t][ct][r]);
+        }
       }
-    float wt[CT][8];
-    bf16x8 pf[CT];
-    soft_weights<FP8, DT, CT>(p, rw, s, f2, kq, vq, edge, existing(w.total - p0, now[0], now[1]), p0 - w.ctx, m, l, acc, wt,
-                              pf);
-    add_values<RS, DT, CT>(buf[h] + 32 * KS, wt, pf, edge && odd_at[h] == u, acc);
-    if (u + 1 < w.u1) store(u + 1, h ^ 1);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (g == 0) sm[half][wave][ct * 16 + c] = top;
+    }
+    if (FP8) {
+      vq[0] = vs[0];
+      vq[1] = vs[1];
+    }
+  };
+  // weights of the scores in s, with the maxima in sm[half], to pbuf[half]
+  const auto weights = [&](int half) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int r = ct * 16 + c;
+      const float top = fmaxf(fmaxf(sm[half][0][r], sm[half][1][r]), fmaxf(sm[half][2][r], sm[half][3][r]));
+      const bool up = top > m[ct] + kSlack;
+      if (__any(up)) {
+        const float a = up ? __builtin_amdgcn_exp2f(m[ct] - top) : 1.f;
+        if (up) m[ct] = top;
+        l[ct] *= a;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d][ct] *= a;
+      }
+      const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = s[i >> 2][ct][i & 3];
+        e[i] = __builtin_amdgcn_exp2f(x - ref);
+        l[ct] += e[i];
+        if (FP8) e[i] = edge_s && x == -INFINITY ? 0.f : e[i] * vq[i >> 2][i & 3];
+      }
+      pbuf[half][wave][ct][lane] =
+          make_uint4(cvt_pk2(e[0], e[1]), cvt_pk2(e[2], e[3]), cvt_pk2(e[4], e[5]), cvt_pk2(e[6], e[7]));
+    }
+  };
+  uint16_t* const vl = vbuf[wave];
+  // the loaded values of the lot that begins at unit u to LDS, zeros where there is no position; whether one is not finite
+  const auto store_v = [&](int u, int ok) -> bool {
+    const int64_t p0 = (int64_t)u * 32;
+    const bool edge = ok != 255 || p0 + 128 > plain;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int key = i * VK + lane / VR;
+      uint4* const dst = reinterpret_cast<uint4*>(vl + key * VS + (lane % VR) * (FP8 ? 16 : 8));
+#pragma unroll
+      for (int h = 0; h < (FP8 ? 2 : 1); ++h) {
+        uint4 x = vx[i];
+        if (FP8) x = h ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y);
+        if (edge) {
+          if (!(ok >> (key >> 4) & 1) || p0 + key >= w.total) x = make_uint4(0u, 0u, 0u, 0u);
+          odd |= odd2(x.x) || odd2(x.y) || odd2(x.z) || odd2(x.w);
+        }
+        dst[h] = x;
+      }
+    }
+    return edge && __any(odd);
+  };
+  const auto add_lot = [&](int half, bool odd) {
+    if (odd) {  // one by one, so that a weight of zero takes nothing
+#pragma unroll 1
+      for (int key = 0; key < 128; ++key) {
+        const int from = ((key >> 2) & 3) * 16 + c, at = (key >> 4 & 1) * 4 + (key & 3);
+        float wk[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          wk[ct] = bf2f(reinterpret_cast<const uint16_t*>(&pbuf[half][key >> 5][ct][from])[at]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float v = bf2f(vl[key * VS + d * 16 + g * 4 + r]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) acc[d][ct][r] += wk[ct] == 0.f ? 0.f : wk[ct] * v;
+          }
+      }
+      return;
+    }
+    const uint16_t* const at = vl + (g * 4 + (c >> 2)) * VS + (c & 3) * 4;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      bf16x8 pf[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) pf[ct] = __builtin_bit_cast(bf16x8, pbuf[half][k][ct][lane]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+            (__attribute__((address_space(3))) bf16x4*)(at + k * 32 * VS + d * 16));
+        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+            (__attribute__((address_space(3))) bf16x4*)(at + (k * 32 + 16) * VS + d * 16));
+        const bf16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          acc[d][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pf[ct], acc[d][ct], 0, 0, 0);
+      }
+    }
+  };
+
+  const int lots = (w.u1 - w.u0 + 3) >> 2;
+  int kok = 0, vok = 0;
+  bool odd = false;
+  if (lots > 0) {
+    kok = load_k(w.u0 + wave);
+    vok = load_v(w.u0);
+    scores(w.u0 + wave, kok, 0);
+    if (lots > 1) kok = load_k(w.u0 + 4 + wave);
   }
+  for (int i = 0; i < lots; ++i) {
+    const int u = w.u0 + 4 * i, half = i & 1;
+    lds_barrier();
+    if (i > 0) add_lot(half ^ 1, odd);
+    odd = store_v(u, vok);
+    if (i + 1 < lots) vok = load_v(u + 4);
+    weights(half);
+    if (i + 1 < lots) {
+      scores(u + 4 + wave, kok, half ^ 1);
+      if (i + 2 < lots) kok = load_k(u + 8 + wave);
+    }
+  }
+  lds_barrier();
+  if (lots > 0) add_lot((lots - 1) & 1, odd);
 
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     l[ct] += __shfl_xor(l[ct], 16);
     l[ct] += __shfl_xor(l[ct], 32);
+    if (g == 0) sl[wave][ct * 16 + c] = l[ct];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
     if (!rw.live[ct]) continue;
+    const int r = ct * 16 + c;
+    const float sum = (sl[0][r] + sl[1][r]) + (sl[2][r] + sl[3][r]), inv = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t nh = (int64_t)(w.first + rw.tok[ct]) * p.HQ + rw.head[ct], i = nh * p.splits + w.split;
-    const float inv = l[ct] == 0.f ? 0.f : 1.f / l[ct];
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const f32x4 o = acc[d][ct];
+      const int at = wave * DS + d * 16 + g * 4;
       if (p.splits > 1)
-        *reinterpret_cast<f32x4*>(p.part + i * D + d * 16 + g * 4) = o;
+        *reinterpret_cast<f32x4*>(p.part + i * D + at) = o;
       else
-        *reinterpret_cast<uint2*>(p.out + nh * D + d * 16 + g * 4) =
-            make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
+        *reinterpret_cast<uint2*>(p.out + nh * D + at) = make_uint2(cvt_pk2(o[0] * inv, o[1] * inv), cvt_pk2(o[2] * inv, o[3] * inv));
     }
-    if (g != 0) continue;
+    if (g != 0 || wave != 0) continue;
     if (p.splits > 1)
-      p.ml[i] = make_float2(m[ct], l[ct]);
+      p.ml[i] = make_float2(m[ct], sum);
     else if (p.lse != nullptr)
-      p.lse[nh] = l[ct] == 0.f ? -INFINITY : (m[ct] + log2f(l[ct])) * kLn2;
+      p.lse[nh] = sum == 0.f ? -INFINITY : (m[ct] + log2f(sum)) * kLn2;
   }
 }
 
@@ -605,7 +715,7 @@ __global__ void __launch_bounds__(256) tree_join_k(TreeParams p) {
 TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, int page) {
   TreePlan t{};
   const int64_t G = HQ / HKV, seqs = std::max<int64_t>(1, std::min<int64_t>(B, N)), mean = (N * G + seqs - 1) / seqs;
-  t.rows = mean <= 16 ? 16 : mean <= 64 ? 64 : 128;
+  t.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
   // an upper bound of sum ceil(n_b G / rows) over the sequences with rows, which are `seqs` at most
   t.blocks = (N * G + seqs * (t.rows - 1)) / t.rows;
   const int64_t units = (max_pages * page + 31) / 32, base = t.blocks * HKV;
@@ -615,7 +725,7 @@ TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, 
 
 template <int D, bool FP8>
 static void (*tree_kernel(int rows))(TreeParams) {
-  return rows == 16 ? tree_narrow_k<D, FP8> : rows == 64 ? tree_wide_k<D, FP8, 1> : tree_wide_k<D, FP8, 2>;
+  return rows == 16 ? tree_narrow_k<D, FP8> : rows == 32 ? tree_wide_k<D, FP8, 2> : tree_wide_k<D, FP8, 4>;
 }
 
 hipError_t launch_tree_attn(const TreeParams& p, const TreePlan& t, int D, bool fp8, hipStream_t st) {
