@@ -63,7 +63,11 @@ __device__ __forceinline__ uint4 cvt_fp8x8(uint32_t a, uint32_t b) {
   return make_uint4(cvt_fp8x2(a, false), cvt_fp8x2(a, true), cvt_fp8x2(b, false), cvt_fp8x2(b, true));
 }
 __device__ __forceinline__ bool odd2(uint32_t x) {  // either bf16 of x is not finite
-  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+  return ((x & 0x7f80u) == 0x7f80u) | ((x & 0x7f800000u) == 0x7f800000u);
+}
+__device__ __forceinline__ uint32_t even2(uint32_t x) {  // with zeros for those
+  x = (x & 0x7f80u) == 0x7f80u ? x & 0xffff0000u : x;
+  return (x & 0x7f800000u) == 0x7f800000u ? x & 0xffffu : x;
 }
 
 // Positions p0 .. p0 + 31 of those that a row of drafted index i sees, as bits; w: its words.
@@ -82,38 +86,29 @@ __device__ __forceinline__ uint32_t seen32(const TreeParams& p, const int64_t* w
   return (uint32_t)x;
 }
 
-// The packed rows that a lane's columns stand for: row0 + 16 ct + lane % 16.
-template <int CT>
-struct Rows {
-  int tok[CT], head[CT];
-  bool live[CT];
-  const int64_t* words[CT];
-  __device__ __forceinline__ Rows(const TreeParams& p, int row0, int rows, int first, int hk) {
-    const int G = p.HQ / p.HKV;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int r = row0 + ct * 16 + (threadIdx.x & 15);
-      live[ct] = r < rows;
-      tok[ct] = live[ct] ? r / G : 0;
-      head[ct] = hk * G + (live[ct] ? r - tok[ct] * G : 0);
-      words[ct] = p.bits != nullptr ? p.bits + (int64_t)(first + tok[ct]) * p.words : nullptr;
-    }
+// The packed row that a lane's column stands for: row0 + lane % 16 (column).
+struct Row {
+  int tok, head;
+  bool live;
+  const int64_t* words;
+  __device__ __forceinline__ Row(const TreeParams& p, int row0, int rows, int first, int hk, int column) {
+    const int G = p.HQ / p.HKV, r = row0 + column;
+    live = r < rows;
+    tok = live ? r / G : 0;
+    head = hk * G + (live ? r - tok * G : 0);
+    words = p.bits != nullptr ? p.bits + (int64_t)(first + tok) * p.words : nullptr;
   }
 };
 
-// Q as the B operand; an e4m3 cache's 16-byte pieces of a key order the contraction.
-template <int D, bool FP8, int CT>
-__device__ __forceinline__ void load_q(const TreeParams& p, const Rows<CT>& w, int first, bool paired,
-                                       bf16x8 (&qf)[CT][D / 32]) {
+// Q as the B operand; an e4m3 cache's 16-byte pieces of a key order the contraction (paired).
+template <int D>
+__device__ __forceinline__ void load_q(const TreeParams& p, const Row& w, int first, bool paired, bf16x8 (&qf)[D / 32]) {
   const int g = (threadIdx.x & 63) >> 4;
+  const uint16_t* src = p.q + ((int64_t)w.head * p.N + first + w.tok) * D;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const uint16_t* src = p.q + ((int64_t)w.head[ct] * p.N + first + w.tok[ct]) * D;
-#pragma unroll
-    for (int f = 0; f < D / 32; ++f) {
-      const int d = paired ? (f >> 1) * 64 + g * 16 + (f & 1) * 8 : f * 32 + g * 8;
-      qf[ct][f] = *reinterpret_cast<const bf16x8*>(src + d);  // a column without a row repeats the first one's
-    }
+  for (int f = 0; f < D / 32; ++f) {
+    const int d = paired ? (f >> 1) * 64 + g * 16 + (f & 1) * 8 : f * 32 + g * 8;
+    qf[f] = *reinterpret_cast<const bf16x8*>(src + d);  // a column without a row repeats the first one's
   }
 }
 
@@ -157,97 +152,97 @@ struct Part {
   }
 };
 
-// Row of the cache where the 16 positions of tile t begin, or -1 where there is none.
+// Row of the cache where the 16 positions of tile t begin, or -1 where there is none (a sequence with positions has pages).
 struct Table {
   const_ints at;
-  int64_t max_pages, pages;
-  int tiles, page, HKV, hk;
-  uint32_t inv;
+  int max_pages, tiles, page, HKV, hk;
+  uint32_t inv, pages;
   __device__ __forceinline__ Table(const TreeParams& p, const Part& w)
-      : at((const_ints)(uintptr_t)(p.table + (int64_t)w.b * p.max_pages)), max_pages(p.max_pages), pages(p.pages),
-        tiles(p.page >> 4), page(p.page), HKV(p.HKV), hk(w.hk), inv(p.tiles_inv) {}
+      : at((const_ints)(uintptr_t)(p.table + (int64_t)w.b * p.max_pages)), max_pages((int)p.max_pages), tiles(p.page >> 4),
+        page(p.page), HKV(p.HKV), hk(w.hk), inv(p.tiles_inv), pages((uint32_t)p.pages) {}
+  // without a branch: a tile behind the table reads its last entry, and counts as none
   __device__ __forceinline__ int64_t row(int t) const {
-    int i = t;  // t / tiles
-    if (tiles > 1) {
-      i = (int)(((uint64_t)(uint32_t)t * inv) >> 32);  // or one more
-      if (i * tiles > t) --i;
-    }
-    if (i >= max_pages) return -1;
-    const int pg = at[i];
-    return pg >= 0 && pg < pages ? ((int64_t)pg * HKV + hk) * page + (t - i * tiles) * 16 : -1;
+    int i = (int)(((uint64_t)(uint32_t)t * inv) >> 32);  // t / tiles, or one more
+    i = tiles > 1 ? i - (i * tiles > t) : t;
+    const int pg = at[min(i, max_pages - 1)];
+    const int64_t r = ((int64_t)pg * HKV + hk) * page + (t - i * tiles) * 16;
+    return (i < max_pages) & ((uint32_t)pg < pages) ? r : -1;
   }
 };
 
+// The largest of lanes l, l ^ 16, l ^ 32, l ^ 48, by swaps of rows of 16 and halves of 32: no trip through LDS.
+__device__ __forceinline__ float quarters_max(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t v = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // Scores of 32 positions -> weights (the B operand of the outputs' product, and for the rare path as they are), with the
-// rows' reference maxima, sums and outputs brought up to date. edge: `there` and the rows' bits say what is seen.
-template <bool FP8, int DT, int CT>
-__device__ __forceinline__ void soft_weights(const TreeParams& p, const Rows<CT>& rw, const f32x4 (&s)[2][CT], float f2,
-                                             const f32x4 (&kq)[2], const f32x4 (&vq)[2], bool edge, uint32_t there,
-                                             int64_t j0, float (&m)[CT], float (&l)[CT], f32x4 (&acc)[DT][CT],
-                                             float (&w)[CT][8], bf16x8 (&pf)[CT]) {
+// rows' reference maxima, sums and outputs brought up to date. edge: seen() says which of the positions the row sees.
+template <bool FP8, int DT, typename Seen>
+__device__ __forceinline__ void soft_weights(const f32x4 (&s)[2], float f2, const f32x4 (&kq)[2], const f32x4 (&vq)[2],
+                                             bool edge, Seen seen, float& m, float& l, f32x4 (&acc)[DT], bf16x8& pf) {
+  float w[8];
   const int g = (threadIdx.x & 63) >> 4;
+  uint32_t see = ~0u;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    uint32_t see = ~0u;
-    if (edge) see = (rw.live[ct] ? there & seen32(p, rw.words[ct], rw.tok[ct], j0) : 0u) >> (g * 4);
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v = s[i >> 2][ct][i & 3] * f2;
-      if (FP8) v *= kq[i >> 2][i & 3];
-      if (edge && !(see >> ((i >> 2) * 16 + (i & 3)) & 1)) v = -INFINITY;
-      w[ct][i] = v;
-      top = fmaxf(top, v);
-    }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const bool up = top > m[ct] + kSlack;
-    if (__any(up)) {
-      const float a = up ? __builtin_amdgcn_exp2f(m[ct] - top) : 1.f;
-      if (up) m[ct] = top;
-      l[ct] *= a;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) acc[d][ct] *= a;
-    }
-    const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float e = __builtin_amdgcn_exp2f(w[ct][i] - ref);
-      l[ct] += e;
-      w[ct][i] = e;
-      if (FP8) w[ct][i] = edge && !(see >> ((i >> 2) * 16 + (i & 3)) & 1) ? 0.f : e * vq[i >> 2][i & 3];
-    }
-    pf[ct] = __builtin_bit_cast(bf16x8, make_uint4(cvt_pk2(w[ct][0], w[ct][1]), cvt_pk2(w[ct][2], w[ct][3]),
-                                                   cvt_pk2(w[ct][4], w[ct][5]), cvt_pk2(w[ct][6], w[ct][7])));
+  for (int i = 0; i < 8; ++i) {
+    w[i] = s[i >> 2][i & 3] * f2;
+    if (FP8) w[i] *= kq[i >> 2][i & 3];
   }
+  if (edge) {
+    see = seen() >> (g * 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = see >> ((i >> 2) * 16 + (i & 3)) & 1 ? w[i] : -INFINITY;
+  }
+  float top = w[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, w[i]);
+  top = quarters_max(top);
+  const bool up = top > m + kSlack;
+  if (__any(up)) {
+    const float a = up ? __builtin_amdgcn_exp2f(m - top) : 1.f;
+    if (up) m = top;
+    l *= a;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] *= a;
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = __builtin_amdgcn_exp2f(w[i] - ref);
+    l += w[i];
+    if (FP8) w[i] *= vq[i >> 2][i & 3];
+  }
+  if (FP8 && edge)  // a scale that nobody sees may be anything
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = see >> ((i >> 2) * 16 + (i & 3)) & 1 ? w[i] : 0.f;
+  pf = __builtin_bit_cast(bf16x8, make_uint4(cvt_pk2(w[0], w[1]), cvt_pk2(w[2], w[3]), cvt_pk2(w[4], w[5]), cvt_pk2(w[6], w[7])));
+}
+
+// One of a row's 32 weights, from the lane that holds it.
+__device__ __forceinline__ float weight_of(bf16x8 pf, int key) {
+  const int slot = (key >> 4) * 4 + (key & 3), from = ((key >> 2) & 3) * 16 + (threadIdx.x & 15);
+  const uint4 y = __builtin_bit_cast(uint4, pf);
+  const uint32_t z = slot < 2 ? y.x : slot < 4 ? y.y : slot < 6 ? y.z : y.w;
+  return bf2f((uint32_t)__shfl((int)(slot & 1 ? z >> 16 : z & 0xffffu), from));
 }
 
 // O^T += V^T P^T over 32 positions from LDS rows of RS values; one by one where a value is not finite, so that a weight of
 // zero takes nothing.
-template <int RS, int DT, int CT>
-__device__ __forceinline__ void add_values(const uint16_t* vl, const float (&w)[CT][8], const bf16x8 (&pf)[CT], bool odd,
-                                           f32x4 (&acc)[DT][CT]) {
+template <int RS, int DT>
+__device__ __forceinline__ void add_values(const uint16_t* vl, bf16x8 pf, bool odd, f32x4 (&acc)[DT]) {
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   if (odd) {
 #pragma unroll 1
     for (int key = 0; key < 32; ++key) {
-      const int slot = (key >> 4) * 4 + (key & 3), from = ((key >> 2) & 3) * 16 + c;
-      float wk[CT];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        float y = w[ct][0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) y = slot == i ? w[ct][i] : y;
-        wk[ct] = __shfl(y, from);
-      }
+      const float wk = weight_of(pf, key);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float v = bf2f(vl[key * RS + d * 16 + g * 4 + r]);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[d][ct][r] += wk[ct] == 0.f ? 0.f : wk[ct] * v;
-        }
+        for (int r = 0; r < 4; ++r) acc[d][r] += wk == 0.f ? 0.f : wk * bf2f(vl[key * RS + d * 16 + g * 4 + r]);
     }
     return;
   }
@@ -258,9 +253,7 @@ __device__ __forceinline__ void add_values(const uint16_t* vl, const float (&w)[
         __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(at + d * 16));
     const bf16x4 hi =
         __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(at + 16 * RS + d * 16));
-    const bf16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) acc[d][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pf[ct], acc[d][ct], 0, 0, 0);
+    acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf, acc[d], 0, 0, 0);
   }
 }
 
@@ -287,10 +280,10 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
   if (p.splits > 1 && w.u0 >= w.u1) return w.no_sums(p, R);
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Rows<1> rw(p, w.row0, w.rows, w.first, w.hk);
+  const Row rw(p, w.row0, w.rows, w.first, w.hk, c);
   const Table table(p, w);
-  bf16x8 qf[1][KF];
-  load_q<D, FP8, 1>(p, rw, w.first, FP8, qf);
+  bf16x8 qf[KF];
+  load_q<D>(p, rw, w.first, FP8, qf);
 
   uint4 kx[2][KL], vx[VL];
   f32x4 ks[2], vs[2];
@@ -317,44 +310,49 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
   };
 
   const float f2 = p.scale * kLog2e;
-  f32x4 acc[DT][1];
-  float m[1] = {-INFINITY}, l[1] = {0.f};
+  f32x4 acc[DT];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int d = 0; d < DT; ++d) acc[d][0] = f32x4{};
+  for (int d = 0; d < DT; ++d) acc[d] = f32x4{};
   uint16_t* const vl = vbuf + wave * 32 * RS;
 
   int u = w.u0 + wave;
   if (u < w.u1) load(u);
   for (; u < w.u1; u += 4) {
-    f32x4 s[2][1];
+    f32x4 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      s[t][0] = f32x4{};
+      s[t] = f32x4{};
 #pragma unroll
       for (int f = 0; f < KF; ++f) {
         const uint4 x = kx[t][FP8 ? f >> 1 : f];
         const bf16x8 a = __builtin_bit_cast(bf16x8, !FP8 ? x : f & 1 ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y));
-        s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[0][f], s[t][0], 0, 0, 0);
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[f], s[t], 0, 0, 0);
       }
     }
     const int64_t p0 = (int64_t)u * 32;
     const bool edge = !(ok[0] && ok[1]) || p0 + 32 > min(w.ctx, w.total);
     const uint32_t there = existing(w.total - p0, ok[0], ok[1]);
     bool odd = false;
+    const auto piece = [&](int i, int h) {
+      return !FP8 ? vx[i] : h ? cvt_fp8x8(vx[i].z, vx[i].w) : cvt_fp8x8(vx[i].x, vx[i].y);
+    };
+    uint4* const dst = reinterpret_cast<uint4*>(vl + lane / VR * RS + (lane % VR) * (FP8 ? 16 : 8));
+    constexpr int STEP = VK * RS / 8;  // from one load's rows to the next's
+    if (!edge) {
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int key = i * VK + lane / VR;
-      uint4* const dst = reinterpret_cast<uint4*>(vl + key * RS + (lane % VR) * (FP8 ? 16 : 8));
+      for (int i = 0; i < VL; ++i)
 #pragma unroll
-      for (int h = 0; h < (FP8 ? 2 : 1); ++h) {
-        uint4 x = vx[i];
-        if (FP8) x = h ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y);
-        if (edge) {
-          if (!(there >> key & 1)) x = make_uint4(0u, 0u, 0u, 0u);
-          odd |= odd2(x.x) || odd2(x.y) || odd2(x.z) || odd2(x.w);
+        for (int h = 0; h < (FP8 ? 2 : 1); ++h) dst[i * STEP + h] = piece(i, h);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VL; ++i)
+#pragma unroll
+        for (int h = 0; h < (FP8 ? 2 : 1); ++h) {
+          const uint4 x = there >> (i * VK + lane / VR) & 1 ? piece(i, h) : make_uint4(0u, 0u, 0u, 0u);
+          odd |= odd2(x.x) | odd2(x.y) | odd2(x.z) | odd2(x.w);
+          dst[i * STEP + h] = x;
         }
-        dst[h] = x;
-      }
     }
     f32x4 kq[2], vq[2];
     if (FP8)
@@ -364,25 +362,25 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
         vq[t] = vs[t];
       }
     if (u + 4 < w.u1) load(u + 4);
-    float wt[1][8];
-    bf16x8 pf[1];
-    soft_weights<FP8, DT, 1>(p, rw, s, f2, kq, vq, edge, there, p0 - w.ctx, m, l, acc, wt, pf);
-    add_values<RS, DT, 1>(vl, wt, pf, edge && __any(odd), acc);
+    bf16x8 pf;
+    soft_weights<FP8, DT>(
+        s, f2, kq, vq, edge, [&] { return rw.live ? there & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u; }, m, l, acc, pf);
+    add_values<RS, DT>(vl, pf, edge && __any(odd), acc);
   }
 
   // the four waves' sums, each brought to the largest reference
-  l[0] += __shfl_xor(l[0], 16);
-  l[0] += __shfl_xor(l[0], 32);
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
   if (g == 0) {
-    sm[wave][c] = m[0];
-    sl[wave][c] = l[0];
+    sm[wave][c] = m;
+    sl[wave][c] = l;
   }
   __syncthreads();
   const float all = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
-  const float mine = m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[0] - all);
+  const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - all);
   float* const swap = reinterpret_cast<float*>(vbuf);
 #pragma unroll
-  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(swap + (wave * R + c) * XS + d * 16 + g * 4) = acc[d][0] * mine;
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(swap + (wave * R + c) * XS + d * 16 + g * 4) = acc[d] * mine;
   __syncthreads();
   const int r = threadIdx.x >> 4, row = w.row0 + r;
   if (row >= w.rows) return;
@@ -412,271 +410,294 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
     p.lse[nh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-// More rows: 16 CT packed rows a workgroup, 128 positions at a time. A wave takes 32 of the positions for the scores, with
-// their keys straight from the cache as in the narrow kernel, and a quarter of the dims for the outputs, with that quarter
-// of the 128 values in LDS rows of its own: keys and values are read once a workgroup, however many rows it has. What the
-// waves exchange is the weights (a lane's eight are the B operand for its 32 positions as they are) and the maxima. The
-// steps of two lots overlap, so that one barrier a lot is enough: behind it a wave
-//   adds the values of lot i - 1 with the weights of all four waves,
-//   takes lot i's maxima, brings its sums to a new reference where one has grown, makes its weights of lot i,
-//   makes its scores of lot i + 1 and leaves their maxima.
-// All waves see the same maxima and so hold the same references.
+// Values of 4 tiles of 16 dims as the A operand (lo: the first 16 of 32 positions, hi: the others) from LDS. Written out
+// with the wait in the same block, because the builtin makes the compiler wait for the DMAs in flight, too.
+template <int LO, int HI>
+__device__ __forceinline__ void values4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, bf16x4 (&lo)[4], bf16x4 (&hi)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3])
+      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(LO), "n"(HI)
+      : "memory");
+}
+
+// The lane, in a way that keeps what is made of it from being kept over a loop: there, every register is the outputs'.
+__device__ __forceinline__ int lane_anew() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+// Many rows: 64 CT packed rows a workgroup, 16 CT of them a wave; all take the part's units of 32 positions in order, from
+// LDS, where a wave brings 8 of a unit's rows of keys and of values. Rows are not padded: the 16-byte chunk j of key r lies
+// at place j ^ r % 8 of its row, the pair of chunks j of value r at j ^ r % 8, which spreads both kinds of reads over the
+// banks. A bf16 cache's unit is fetched by LDS DMA (each lane fetches the chunk that belongs where the DMA puts it) an
+// iteration ahead, an e4m3 cache's through registers, where it becomes bf16.
 template <int D, bool FP8, int CT>
-__global__ void __launch_bounds__(256, 1) tree_wide_k(TreeParams p) {
-  constexpr int R = 16 * CT, KF = D / 32, RB = D * (FP8 ? 1 : 2);  // RB: bytes of a cache row
-  constexpr int DS = D / 4, DT = DS / 16;                          // dims of a wave
-  constexpr int VS = DS + 16;                                      // LDS row of values, in bf16
-  constexpr int KL = RB / 64;                                      // 16-byte loads of a key
-  constexpr int VR = RB / 64, VK = 64 / VR, VL = 128 / VK;         // lanes of a value row's quarter, rows a load, loads
-  __shared__ __attribute__((aligned(16))) uint16_t vbuf[4][128 * VS];
-  __shared__ __attribute__((aligned(16))) uint4 pbuf[2][4][CT][64];
-  __shared__ float sm[2][4][R], sl[4][R];
+__global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
+  constexpr int R = 64 * CT, KF = D / 32, DT = D / 16, SB = D * (FP8 ? 1 : 2), RB = D * 2;  // bytes of a row: cache, LDS
+  constexpr int PR = SB / 16, RL = 64 / PR, PL = 8 / RL;  // 16-byte pieces of a row, rows a wave's load takes, loads of 8 rows
+  constexpr int TILE = 32 * RB;
+  __shared__ __attribute__((aligned(1024))) uint8_t buf[2][2][TILE];  // keys, values
+  __shared__ __attribute__((aligned(16))) float sc[2][2][32];
+  __shared__ int odd_any;
 
   Part w;
-  if (!w.find(p, R, D, 4)) return;
+  if (!w.find(p, R, D, 1)) return;
   if (p.splits > 1 && w.u0 >= w.u1) return w.no_sums(p, R);
-  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Rows<CT> rw(p, w.row0, w.rows, w.first, w.hk);
+  const int wrow = w.row0 + wave * 16 * CT;
   const Table table(p, w);
+  const int64_t plain = min(w.ctx, w.total);  // positions below are seen by every row, if they are in the cache
   bf16x8 qf[CT][KF];
-  load_q<D, FP8, CT>(p, rw, w.first, FP8, qf);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+    load_q<D>(p, Row(p, wrow + ct * 16, w.rows, w.first, w.hk, threadIdx.x & 15), w.first, false, qf[ct]);
 
-  // keys of unit u (32 positions) and values of the lot that begins there; which of their tiles of 16 are in the cache
-  uint4 kx[2][KL], vx[VL];
-  f32x4 ks[2], vs[2];
-  const auto load_k = [&](int u) -> int {
-    int ok = 0;
+  struct Pieces {
+    uint4 k[PL], v[PL];
+    float ks, vs;
+  };
+  // the unit's rows of the cache and whether they are: of its first 16 positions, of the others
+  int64_t r0, r1;
+  const auto rows_of = [&](int u) {
+    r0 = table.row(2 * u);
+    r1 = table.row(2 * u + 1);
+  };
+  const auto is_edge = [&](int u, bool ok) { return !ok || (int64_t)u * 32 + 32 > plain; };
+  const auto dma = [&](int h) {  // rows_of()'s rows to half h
+    const int lane = lane_anew(), sub = lane / PR, pc = lane % PR;  // row and piece of a lane in a load
+    const int64_t row = wave >> 1 ? r1 : r0;
+    const auto kr = make_rsrc(static_cast<const uint8_t*>(p.kc) + row * SB, 16 * SB);
+    const auto vr = make_rsrc(static_cast<const uint8_t*>(p.vc) + row * SB, 16 * SB);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int64_t r = table.row(2 * u + t), row = max(r, (int64_t)0);  // any row of the cache: it is not used
-      ok |= (r >= 0) << t;
-      const uint8_t* kb = static_cast<const uint8_t*>(p.kc) + row * RB;
+    for (int i = 0; i < PL; ++i) {
+      const int r = i * RL + sub, at = ((wave & 1) * 8 + r) * SB;
+      dma16(kr, &buf[h][0][(wave * 8 + i * RL) * RB], at + (pc ^ r) * 16);
+      dma16(vr, &buf[h][1][(wave * 8 + i * RL) * RB], at + (pc ^ r * 2) * 16);
+    }
+  };
+  const auto fetch = [&](Pieces& x) {  // or to registers
+    const int lane = lane_anew(), sub = lane / PR, pc = lane % PR;
+    const int64_t row = max(wave >> 1 ? r1 : r0, (int64_t)0);  // any row of the cache: it is not used
+    const auto kr = make_rsrc(static_cast<const uint8_t*>(p.kc) + row * SB, 16 * SB);
+    const auto vr = make_rsrc(static_cast<const uint8_t*>(p.vc) + row * SB, 16 * SB);
 #pragma unroll
-      for (int f = 0; f < KL; ++f) kx[t][f] = *reinterpret_cast<const uint4*>(kb + c * RB + f * 64 + g * 16);
-      if (FP8) {
-        ks[t] = *reinterpret_cast<const f32x4*>(p.ks + row + g * 4);
-        vs[t] = *reinterpret_cast<const f32x4*>(p.vs + row + g * 4);
+    for (int i = 0; i < PL; ++i) {
+      const int at = ((wave & 1) * 8 + i * RL + sub) * SB + pc * 16;
+      x.k[i] = bload(kr, at);
+      x.v[i] = bload(vr, at);
+    }
+    if (FP8) {
+      x.ks = p.ks[row + (wave & 1) * 8 + (lane & 7)];
+      x.vs = p.vs[row + (wave & 1) * 8 + (lane & 7)];
+    }
+  };
+  const auto store = [&](Pieces& x, int u, int h, bool ok0, bool ok1) {  // the fetched unit u to LDS half h
+    const int lane = lane_anew(), sub = lane / PR, pc = lane % PR;
+    const bool edge = is_edge(u, ok0 && ok1);
+    const uint32_t there = existing(w.total - (int64_t)u * 32, ok0, ok1);
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      const int r = i * RL + sub;
+      uint8_t* const kd = &buf[h][0][(wave * 8 + r) * RB];
+      uint8_t* const vd = &buf[h][1][(wave * 8 + r) * RB];
+      if (edge && !(there >> (wave * 8 + r) & 1)) x.v[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int e = 0; e < (FP8 ? 2 : 1); ++e) {
+        const uint4 y = !FP8 ? x.k[i] : e ? cvt_fp8x8(x.k[i].z, x.k[i].w) : cvt_fp8x8(x.k[i].x, x.k[i].y);
+        uint4 z = !FP8 ? x.v[i] : e ? cvt_fp8x8(x.v[i].z, x.v[i].w) : cvt_fp8x8(x.v[i].x, x.v[i].y);
+        if (edge) {
+          odd |= odd2(z.x) | odd2(z.y) | odd2(z.z) | odd2(z.w);
+          z = make_uint4(even2(z.x), even2(z.y), even2(z.z), even2(z.w));
+        }
+        const int j = FP8 ? pc * 2 + e : pc;
+        *reinterpret_cast<uint4*>(kd + (j ^ r) * 16) = y;
+        *reinterpret_cast<uint4*>(vd + (j ^ r * 2) * 16) = z;
       }
     }
-    return ok;
-  };
-  const auto load_v = [&](int u) -> int {
-    int64_t row[8];
-    int ok = 0;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      const int64_t r = table.row(2 * u + t);
-      row[t] = max(r, (int64_t)0);
-      ok |= (r >= 0) << t;
+    if (FP8) {  // the same from eight lanes
+      sc[h][0][wave * 8 + (lane & 7)] = x.ks;
+      sc[h][1][wave * 8 + (lane & 7)] = x.vs;
     }
-#pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int key = lane / VR;  // of this load's VK
-      int64_t at;
-      if constexpr (VK == 32)
-        at = (key >= 16 ? row[2 * i + 1] : row[2 * i]) + (key & 15);
-      else
-        at = row[i * VK / 16] + (i * VK) % 16 + key;
-      vx[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.vc) + at * RB + wave * (RB / 4) + (lane % VR) * 16);
-    }
-    return ok;
+    if (edge && __any(odd)) odd_any = 1;
   };
-  const int64_t plain = min(w.ctx, w.total);  // positions below are seen by every row, if they are in the cache
 
   const float f2 = p.scale * kLog2e;
-  f32x4 acc[DT][CT], s[2][CT], vq[2];
+  f32x4 acc[CT][DT];
   float m[CT], l[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     m[ct] = -INFINITY;
     l[ct] = 0.f;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) acc[d][ct] = f32x4{};
+    for (int d = 0; d < DT; ++d) acc[ct][d] = f32x4{};
   }
-  bool edge_s = false;  // of the scores in s
-  // scores of the loaded unit u, masked, to base two; their maxima to sm[half]
-  const auto scores = [&](int u, int ok, int half) {
+  if (threadIdx.x == 0) odd_any = 0;
+  __syncthreads();
+  bool ok0 = false, ok1 = false;  // of the unit at hand
+  if (w.u0 < w.u1) {
+    rows_of(w.u0);
+    ok0 = r0 >= 0;
+    ok1 = r1 >= 0;
+    if (FP8 || is_edge(w.u0, ok0 && ok1)) {
+      Pieces x;
+      fetch(x);
+      store(x, w.u0, 0, ok0, ok1);
+    } else {
+      dma(0);
+    }
+    rows_of(w.u0 + 1);
+  }
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&buf[0][0][0];
+  for (int u = w.u0; u < w.u1; ++u) {
+    const int h = (u - w.u0) & 1;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows are there
+    lds_barrier();
+    const bool more = u + 1 < w.u1, ok2 = r0 >= 0, ok3 = r1 >= 0;
+    Pieces next;
+    if (FP8) {
+      if (more) fetch(next);
+    } else if (more) {
+      if (is_edge(u + 1, ok2 && ok3)) {
+        Pieces x;
+        fetch(x);
+        store(x, u + 1, h ^ 1, ok2, ok3);
+      } else {
+        dma(h ^ 1);
+      }
+    }
+    if (more) rows_of(u + 2);
+    if (wrow < w.rows) {
+      const int lane = lane_anew(), g = lane >> 4, c = lane & 15, vrow = g * 4 + (c >> 2);
+      const uint8_t* const kl = &buf[h][0][c * RB + (g ^ (c & 7)) * 16];
+      const uint8_t* const kl4 = &buf[h][0][c * RB + (g ^ 4 ^ (c & 7)) * 16];
+      f32x4 s[CT][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) s[t][ct] = f32x4{};
+      for (int ct = 0; ct < CT; ++ct) s[ct][0] = s[ct][1] = f32x4{};
+      bf16x8 a[2][2];
+      const auto keys = [&](int f) {
+        const uint8_t* const at = (f & 1 ? kl4 : kl) + (f >> 1) * 128;
+        a[f & 1][0] = *reinterpret_cast<const bf16x8*>(at);
+        a[f & 1][1] = *reinterpret_cast<const bf16x8*>(at + 16 * RB);
+      };
+      keys(0);
 #pragma unroll
       for (int f = 0; f < KF; ++f) {
-        const uint4 x = kx[t][FP8 ? f >> 1 : f];
-        const bf16x8 a = __builtin_bit_cast(bf16x8, !FP8 ? x : f & 1 ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y));
+        if (f + 1 < KF) keys(f + 1);
+        __builtin_amdgcn_sched_barrier(0);  // one step ahead: more would take the outputs' registers
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) s[t][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[ct][f], s[t][ct], 0, 0, 0);
-      }
-    }
-    const int64_t p0 = (int64_t)u * 32;
-    edge_s = ok != 3 || p0 + 32 > plain;
-    const uint32_t there = edge_s ? existing(w.total - p0, ok & 1, ok >> 1) : ~0u;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float top = -INFINITY;
-      uint32_t see = ~0u;
-      if (edge_s) see = (rw.live[ct] ? there & seen32(p, rw.words[ct], rw.tok[ct], p0 - w.ctx) : 0u) >> (g * 4);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        s[t][ct] *= f2;
-        if (FP8) s[t][ct] *= ks[t];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (edge_s && !(see >> (t * 16 + r) & 1)) s[t][ct][r] = -INFINITY;
-          top = fmaxf(top, s[t][ct][r]);
+        for (int ct = 0; ct < CT; ++ct) {
+          s[ct][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[f & 1][0], qf[ct][f], s[ct][0], 0, 0, 0);
+          s[ct][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[f & 1][1], qf[ct][f], s[ct][1], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (g == 0) sm[half][wave][ct * 16 + c] = top;
-    }
-    if (FP8) {
-      vq[0] = vs[0];
-      vq[1] = vs[1];
-    }
-  };
-  // weights of the scores in s, with the maxima in sm[half], to pbuf[half]
-  const auto weights = [&](int half) {
+      const int64_t p0 = (int64_t)u * 32;
+      const bool edge = is_edge(u, ok0 && ok1);
+      f32x4 kq[2], vq[2];
+      if (FP8)
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int r = ct * 16 + c;
-      const float top = fmaxf(fmaxf(sm[half][0][r], sm[half][1][r]), fmaxf(sm[half][2][r], sm[half][3][r]));
-      const bool up = top > m[ct] + kSlack;
-      if (__any(up)) {
-        const float a = up ? __builtin_amdgcn_exp2f(m[ct] - top) : 1.f;
-        if (up) m[ct] = top;
-        l[ct] *= a;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d][ct] *= a;
-      }
-      const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
-      float e[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = s[i >> 2][ct][i & 3];
-        e[i] = __builtin_amdgcn_exp2f(x - ref);
-        l[ct] += e[i];
-        if (FP8) e[i] = edge_s && x == -INFINITY ? 0.f : e[i] * vq[i >> 2][i & 3];
-      }
-      pbuf[half][wave][ct][lane] =
-          make_uint4(cvt_pk2(e[0], e[1]), cvt_pk2(e[2], e[3]), cvt_pk2(e[4], e[5]), cvt_pk2(e[6], e[7]));
-    }
-  };
-  uint16_t* const vl = vbuf[wave];
-  // the loaded values of the lot that begins at unit u to LDS, zeros where there is no position; whether one is not finite
-  const auto store_v = [&](int u, int ok) -> bool {
-    const int64_t p0 = (int64_t)u * 32;
-    const bool edge = ok != 255 || p0 + 128 > plain;
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int key = i * VK + lane / VR;
-      uint4* const dst = reinterpret_cast<uint4*>(vl + key * VS + (lane % VR) * (FP8 ? 16 : 8));
-#pragma unroll
-      for (int h = 0; h < (FP8 ? 2 : 1); ++h) {
-        uint4 x = vx[i];
-        if (FP8) x = h ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y);
-        if (edge) {
-          if (!(ok >> (key >> 4) & 1) || p0 + key >= w.total) x = make_uint4(0u, 0u, 0u, 0u);
-          odd |= odd2(x.x) || odd2(x.y) || odd2(x.z) || odd2(x.w);
+        for (int t = 0; t < 2; ++t) {
+          kq[t] = *reinterpret_cast<const f32x4*>(&sc[h][0][t * 16 + g * 4]);
+          vq[t] = *reinterpret_cast<const f32x4*>(&sc[h][1][t * 16 + g * 4]);
         }
-        dst[h] = x;
-      }
-    }
-    return edge && __any(odd);
-  };
-  const auto add_lot = [&](int half, bool odd) {
-    if (odd) {  // one by one, so that a weight of zero takes nothing
-#pragma unroll 1
-      for (int key = 0; key < 128; ++key) {
-        const int from = ((key >> 2) & 3) * 16 + c, at = (key >> 4 & 1) * 4 + (key & 3);
-        float wk[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          wk[ct] = bf2f(reinterpret_cast<const uint16_t*>(&pbuf[half][key >> 5][ct][from])[at]);
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float v = bf2f(vl[key * VS + d * 16 + g * 4 + r]);
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) acc[d][ct][r] += wk[ct] == 0.f ? 0.f : wk[ct] * v;
-          }
-      }
-      return;
-    }
-    const uint16_t* const at = vl + (g * 4 + (c >> 2)) * VS + (c & 3) * 4;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
       bf16x8 pf[CT];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) pf[ct] = __builtin_bit_cast(bf16x8, pbuf[half][k][ct][lane]);
+      for (int ct = 0; ct < CT; ++ct)
+        soft_weights<FP8, DT>(
+            s[ct], f2, kq, vq, edge,
+            [&] {
+              const Row rw(p, wrow + ct * 16, w.rows, w.first, w.hk, lane_anew() & 15);
+              return rw.live ? existing(w.total - p0, ok0, ok1) & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u;
+            },
+            m[ct], l[ct], acc[ct], pf[ct]);
+      const uint32_t at = lds + (h * 2 + 1) * TILE + vrow * RB + (vrow & 7) * 32 + (c & 3) * 8;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-            (__attribute__((address_space(3))) bf16x4*)(at + k * 32 * VS + d * 16));
-        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-            (__attribute__((address_space(3))) bf16x4*)(at + (k * 32 + 16) * VS + d * 16));
-        const bf16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      for (int d0 = 0; d0 < DT; d0 += 4) {
+        bf16x4 lo[4], hi[4];
+        const uint32_t b = at ^ (d0 & 7) * 32;
+        if (d0 < 8)
+          values4<0, 16 * RB>(b, b ^ 32, b ^ 64, b ^ 96, lo, hi);
+        else
+          values4<256, 16 * RB + 256>(b, b ^ 32, b ^ 64, b ^ 96, lo, hi);
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          acc[d][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pf[ct], acc[d][ct], 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+          const bf16x8 a = __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            acc[ct][d0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pf[ct], acc[ct][d0 + i], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-  };
-
-  const int lots = (w.u1 - w.u0 + 3) >> 2;
-  int kok = 0, vok = 0;
-  bool odd = false;
-  if (lots > 0) {
-    kok = load_k(w.u0 + wave);
-    vok = load_v(w.u0);
-    scores(w.u0 + wave, kok, 0);
-    if (lots > 1) kok = load_k(w.u0 + 4 + wave);
+    if (FP8 && more) store(next, u + 1, h ^ 1, ok2, ok3);
+    ok0 = ok2;
+    ok1 = ok3;
   }
-  for (int i = 0; i < lots; ++i) {
-    const int u = w.u0 + 4 * i, half = i & 1;
-    lds_barrier();
-    if (i > 0) add_lot(half ^ 1, odd);
-    odd = store_v(u, vok);
-    if (i + 1 < lots) vok = load_v(u + 4);
-    weights(half);
-    if (i + 1 < lots) {
-      scores(u + 4 + wave, kok, half ^ 1);
-      if (i + 2 < lots) kok = load_k(u + 8 + wave);
-    }
-  }
-  lds_barrier();
-  if (lots > 0) add_lot((lots - 1) & 1, odd);
 
+  const int lane = lane_anew(), g = lane >> 4, c = lane & 15;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     l[ct] += __shfl_xor(l[ct], 16);
     l[ct] += __shfl_xor(l[ct], 32);
-    if (g == 0) sl[wave][ct * 16 + c] = l[ct];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    if (!rw.live[ct]) continue;
-    const int r = ct * 16 + c;
-    const float sum = (sl[0][r] + sl[1][r]) + (sl[2][r] + sl[3][r]), inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int64_t nh = (int64_t)(w.first + rw.tok[ct]) * p.HQ + rw.head[ct], i = nh * p.splits + w.split;
+    const Row rw(p, wrow + ct * 16, w.rows, w.first, w.hk, c);
+    if (!rw.live) continue;
+    const int64_t nh = (int64_t)(w.first + rw.tok) * p.HQ + rw.head, i = nh * p.splits + w.split;
+    const float inv = l[ct] == 0.f ? 0.f : 1.f / l[ct];
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const f32x4 o = acc[d][ct];
-      const int at = wave * DS + d * 16 + g * 4;
+      const f32x4 o = acc[ct][d];
       if (p.splits > 1)
-        *reinterpret_cast<f32x4*>(p.part + i * D + at) = o;
+        *reinterpret_cast<f32x4*>(p.part + i * D + d * 16 + g * 4) = o;
       else
-        *reinterpret_cast<uint2*>(p.out + nh * D + at) = make_uint2(cvt_pk2(o[0] * inv, o[1] * inv), cvt_pk2(o[2] * inv, o[3] * inv));
+        *reinterpret_cast<uint2*>(p.out + nh * D + d * 16 + g * 4) = make_uint2(cvt_pk2(o[0] * inv, o[1] * inv), cvt_pk2(o[2] * inv, o[3] * inv));
     }
-    if (g != 0 || wave != 0) continue;
+    if (g != 0) continue;
     if (p.splits > 1)
-      p.ml[i] = make_float2(m[ct], sum);
+      p.ml[i] = make_float2(m[ct], l[ct]);
     else if (p.lse != nullptr)
-      p.lse[nh] = sum == 0.f ? -INFINITY : (m[ct] + log2f(sum)) * kLn2;
+      p.lse[nh] = l[ct] == 0.f ? -INFINITY : (m[ct] + log2f(l[ct])) * kLn2;
+  }
+
+  if (odd_any == 0) return;
+#pragma unroll 1
+  for (int ct = 0; ct < CT; ++ct) {
+    const Row rw(p, wrow + ct * 16, w.rows, w.first, w.hk, c);
+    if (!rw.live) continue;
+    const int64_t nh = (int64_t)(w.first + rw.tok) * p.HQ + rw.head;
+#pragma unroll 1
+    for (int u = w.u0; u < w.u1; ++u) {
+      rows_of(u);
+      if (!is_edge(u, r0 >= 0 && r1 >= 0)) continue;
+      const int64_t p0 = (int64_t)u * 32;
+      const uint32_t see = existing(w.total - p0, r0 >= 0, r1 >= 0) & seen32(p, rw.words, rw.tok, p0 - w.ctx);
+#pragma unroll 1
+      for (int key = 0; key < 32; ++key) {
+        if (!(see >> key & 1)) continue;
+        const int64_t v = ((key >> 4 ? r1 : r0) + (key & 15)) * D;
+#pragma unroll 1
+        for (int i = 0; i < D / 4; ++i) {
+          const int d = (i >> 2) * 16 + g * 4 + (i & 3);  // what this lane has written
+          const float x = FP8 ? bf2f(cvt_fp8x2(static_cast<const uint8_t*>(p.vc)[v + d], false) & 0xffffu)
+                              : bf2f(static_cast<const uint16_t*>(p.vc)[v + d]);
+          if (fabsf(x) < INFINITY) continue;
+          if (p.splits > 1)
+            p.part[(nh * p.splits + w.split) * D + d] += x;
+          else
+            p.out[nh * D + d] = (uint16_t)f2bf(bf2f(p.out[nh * D + d]) + x);
+        }
+      }
+    }
   }
 }
 
@@ -715,7 +736,7 @@ __global__ void __launch_bounds__(256) tree_join_k(TreeParams p) {
 TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, int page) {
   TreePlan t{};
   const int64_t G = HQ / HKV, seqs = std::max<int64_t>(1, std::min<int64_t>(B, N)), mean = (N * G + seqs - 1) / seqs;
-  t.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+  t.rows = mean <= 16 ? 16 : mean <= 64 ? 64 : 128;
   // an upper bound of sum ceil(n_b G / rows) over the sequences with rows, which are `seqs` at most
   t.blocks = (N * G + seqs * (t.rows - 1)) / t.rows;
   const int64_t units = (max_pages * page + 31) / 32, base = t.blocks * HKV;
@@ -725,7 +746,7 @@ TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, 
 
 template <int D, bool FP8>
 static void (*tree_kernel(int rows))(TreeParams) {
-  return rows == 16 ? tree_narrow_k<D, FP8> : rows == 32 ? tree_wide_k<D, FP8, 2> : tree_wide_k<D, FP8, 4>;
+  return rows == 16 ? tree_narrow_k<D, FP8> : rows == 64 ? tree_wide_k<D, FP8, 1> : tree_wide_k<D, FP8, 2>;
 }
 
 hipError_t launch_tree_attn(const TreeParams& p, const TreePlan& t, int D, bool fp8, hipStream_t st) {
