@@ -895,6 +895,9 @@ int check_tree(int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t
     return fail(OJX_ERR_SHAPE, "bad max_pages=%lld (at most 2^31 positions)", (long long)max_pages);
   if (N * HQ >= (1LL << 24))
     return fail(OJX_ERR_SHAPE, "N=%lld rows of %d heads: too many for one call", (long long)N, HQ);
+  // workgroups of 256 threads; a launch has fewer than 2^32 threads
+  if (N > 0 && ojx::tree_plan(N, B, HQ, HKV, D, max_pages, page).shares * HKV >= (1LL << 24))
+    return fail(OJX_ERR_SHAPE, "N=%lld rows of B=%d sequences: too many for one call", (long long)N, B);
   return OJX_OK;
 }
 
@@ -940,7 +943,7 @@ int64_t ojx_tree_attn_workspace(int64_t N, int32_t B, int32_t HQ, int32_t HKV, i
   if (check_tree(N, B, HQ, HKV, D, max_pages, page) != OJX_OK) return -1;
   if (N == 0) return 0;
   const ojx::TreePlan t = ojx::tree_plan(N, B, HQ, HKV, D, max_pages, page);
-  return t.splits > 1 ? N * HQ * t.splits * (D * 4 + 8) : 0;
+  return t.target > 0 ? t.slots * (D * 4 + 8) + N * HQ * 8 : 0;
 }
 
 int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const int64_t* bits, int32_t words,
@@ -964,10 +967,11 @@ int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const
                 (long long)need, (long long)workspace_bytes);
   const ojx::TreePlan t = ojx::tree_plan(N, B, HQ, HKV, D, max_pages, page);
   float* const part = static_cast<float*>(workspace);
+  float2* const ml = reinterpret_cast<float2*>(part + t.slots * D);
   const ojx::TreeParams p{static_cast<const uint16_t*>(q), q_ptr, ctx, bits, bits != nullptr ? words : 0, kc, vc, ks, vs,
                           table, max_pages, N, pages, B, HQ, HKV, page, scale, static_cast<uint16_t*>(out), lse,
-                          (int)t.splits, (uint32_t)(((1ULL << 32) + page / 16 - 1) / (page / 16)), part,
-                          reinterpret_cast<float2*>(part + N * HQ * t.splits * D)};
+                          t.target, t.least, (uint32_t)(((1ULL << 32) + page / 16 - 1) / (page / 16)), part, ml,
+                          reinterpret_cast<uint2*>(ml + t.slots)};
   return hip_check(ojx::launch_tree_attn(p, t, D, fmt == OJX_KV_E4M3, static_cast<hipStream_t>(stream)),
                    "tree attention launch");
 }

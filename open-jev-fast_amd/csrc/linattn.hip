@@ -182,7 +182,7 @@ static_assert(offsetof(ChunkWork, P) == 1024, "whole 1-KB pieces");
 constexpr int chunk_bytes(bool delta) { return delta ? (int)sizeof(ChunkWork) : (int)offsetof(ChunkWork, T); }
 __device__ __forceinline__ constexpr int frag(int it, int ks) { return it < 2 ? it : 2 * it - 2 + ks; }
 
-__device__ __forceinline__ int seq_chunks(int n) { return (n + kChunk - 1) / kChunk; }
+__device__ __forceinline__ int seq_chunks(int, int n) { return (n + kChunk - 1) / kChunk; }
 
 // Two bf16 pieces of 8 values: x = hi + lo to 16 bits.
 __device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8& hi, bf16x8& lo) {
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   SeqPlace place;
   if (!seq_find(p.seq_ptr, p.S, p.R, seq_chunks, [=](int i, int) { return i == (int)sq; }, place)) return;
   const int first = place.first, n = place.n;
-  const int chunks = seq_chunks(n);
+  const int chunks = seq_chunks(0, n);
   const int dv0 = (hs % SL) * 32, dv = dv0 + slice * 16 + c;
   // LDS offsets of this lane: rows c of K and Q, key dims 32 s .. + 31; its slice's pieces of S0 and X
   int aoff[4];
@@ -885,7 +885,7 @@ __global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
   SeqPlace place;
   if (!seq_find(p.seq_ptr, p.S, p.R, seq_chunks, [=](int i, int) { return i == (int)sq; }, place)) return;
   const int first = place.first, n = place.n;
-  const int chunks = seq_chunks(n);
+  const int chunks = seq_chunks(0, n);
   const int dv = wave * 16 + c;
 
   // a chunk to an LDS stage: this wave's 8 rows of K, Q and V, its part of the chunk's matrices, in two halves

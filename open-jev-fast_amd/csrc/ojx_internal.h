@@ -123,7 +123,7 @@ __device__ __forceinline__ int wave_scan_max(int v) {
 
 // Sequences laid end to end in rows by pointers ptr[0 .. S]: sequence i is rows [m_i, m_(i+1)), m_i the largest of ptr[0 ..
 // i] clamped to [0, rows]. For pointers that never fall that is what they say; whatever they hold, sequences stay within
-// the rows and do not overlap. per(n) says how many units a sequence of n rows takes. The whole wave calls, with uniform
+// the rows and do not overlap. per(i, n) says how many units sequence i of n rows takes (i >= S: n is 0). The whole wave calls, with uniform
 // arguments.
 struct SeqPlace {
   int seq, first, n;  // its first row and row count
@@ -141,7 +141,7 @@ __device__ __forceinline__ bool seq_find(const int32_t* ptr, int64_t S, int64_t 
     const int64_t i = base + lane;
     const int x = max(carry, wave_scan_max(seq_bound(ptr, min(i, S), rows)));
     const int e = max(x, seq_bound(ptr, min(i + 1, S), rows));
-    const int units = per(e - x);  // 0 rows behind the last sequence: e == x there
+    const int units = per((int)i, e - x);  // 0 rows behind the last sequence: e == x there
     const int s = before + wave_scan_sum(units);
     const unsigned long long hit = __ballot(i < S && done((int)i, s));
     if (hit != 0) {
@@ -286,14 +286,18 @@ struct TreeParams {
   int B, HQ, HKV, page;
   float scale;
   uint16_t* out; float* lse;              // [N, HQ, D]; [N, HQ] or null
-  int splits;                             // parts of a sequence's positions
+  int target, least;                      // of tree_plan
   uint32_t tiles_inv;                     // 2^32 / (page / 16), rounded up; not used for pages of 16
-  float* part; float2* ml;                // [N, HQ, splits, D] sums, [N, HQ, splits] (maximum, base two; sum)
+  float* part; float2* ml;                // [slots, D] sums, [slots] (maximum, base two; sum)
+  uint2* joins;                           // [N, HQ] slot of a row's first part, parts
 };
-// Shape of a launch, from sizes alone: packed rows a workgroup takes, workgroups along the rows, parts of the positions.
+// Shape of a launch, from sizes alone: packed rows a workgroup takes, workgroups of a kv head, rows of workspace; the work
+// that they share out (tree_attn.hip): the workgroups of a kv head that run at once (0: positions stay in one part), the
+// fewest units of a part.
 struct TreePlan {
   int rows;
-  int64_t blocks, splits;
+  int64_t shares, slots;
+  int target, least;
 };
 TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, int page);
 hipError_t launch_tree_attn(const TreeParams& p, const TreePlan& t, int D, bool fp8, hipStream_t st);

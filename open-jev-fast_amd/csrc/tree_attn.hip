@@ -50,7 +50,9 @@ __device__ __forceinline__ void zero_rows(const TreeParams& p, int hk, int D) {
     const int64_t i = t / per, n = i < lo ? i : i - lo + hi;
     const int c = (int)(t - i * per);
     *reinterpret_cast<uint4*>(p.out + (n * p.HQ + hk * G) * D + c * 8) = make_uint4(0u, 0u, 0u, 0u);
-    if (p.lse != nullptr && c < G) p.lse[n * p.HQ + hk * G + c] = -INFINITY;
+    if (c >= G) continue;
+    if (p.lse != nullptr) p.lse[n * p.HQ + hk * G + c] = -INFINITY;
+    if (p.target > 0) p.joins[n * p.HQ + hk * G + c] = make_uint2(0u, 0u);
   }
 }
 
@@ -61,6 +63,10 @@ __device__ __forceinline__ uint32_t cvt_fp8x2(int x, bool hi) {  // two e4m3 val
 }
 __device__ __forceinline__ uint4 cvt_fp8x8(uint32_t a, uint32_t b) {
   return make_uint4(cvt_fp8x2(a, false), cvt_fp8x2(a, true), cvt_fp8x2(b, false), cvt_fp8x2(b, true));
+}
+template <bool FP8>
+__device__ __forceinline__ uint4 half_piece(uint4 x, int e) {  // 8 values of a 16-byte piece as bf16: the only, or half e
+  return !FP8 ? x : e ? cvt_fp8x8(x.z, x.w) : cvt_fp8x8(x.x, x.y);
 }
 __device__ __forceinline__ bool odd2(uint32_t x) {  // either bf16 of x is not finite
   return ((x & 0x7f80u) == 0x7f80u) | ((x & 0x7f800000u) == 0x7f800000u);
@@ -112,43 +118,74 @@ __device__ __forceinline__ void load_q(const TreeParams& p, const Row& w, int fi
   }
 }
 
-// One workgroup's part of the positions.
+// One workgroup's share: a row block of R packed rows of a sequence and a part of the sequence's units of 32 positions.
+// Work is shared out by the lengths as they are on the device: with nb row blocks of `total` units over all of them (of a
+// kv head), a part has L = total / max(p.target - nb, nb / 4) units at most, p.least at least, and a sequence of u units
+// ceil(u / L) parts of equal length. That makes max(p.target, nb + nb / 4 + 1) shares at most, which is the launch.
 struct Part {
-  int b, first, n, row0, rows, hk, split, u0, u1;
+  int b, first, n, row0, rows, hk, parts, u0, u1;
+  uint32_t slot;  // of the part's first row in the workspace; a row's parts lie HKV R slots apart
   int64_t ctx, total;
-  // false: nothing to do. Blocks and parts of a launch are numbered row block, part, kv head, the last fastest.
+  // false: nothing to do. Shares are numbered sequence, row block, part; the kv head is the fastest of a launch. Parts
+  // begin at multiples of step.
   __device__ __forceinline__ bool find(const TreeParams& p, int R, int D, int step) {
-    const int groups = p.HKV * p.splits;
-    const int rb = blockIdx.x / groups, at = blockIdx.x - rb * groups;
-    split = at / p.HKV;
-    hk = at - split * p.HKV;
-    if (rb == 0 && split == 0) zero_rows(p, hk, D);
-    const int G = p.HQ / p.HKV;
-    SeqPlace at_seq;
+    const int lane = threadIdx.x & 63, share = blockIdx.x / p.HKV, G = p.HQ / p.HKV;
+    hk = blockIdx.x - share * p.HKV;
+    if (share == 0) zero_rows(p, hk, D);
+    const int64_t most = p.pages > 0 ? p.max_pages * p.page : 0;
+    const auto units = [=](int i, int n) {
+      return n > 0 ? (int)((min(max((int64_t)p.ctx[i], (int64_t)0) + n, most) + 31) >> 5) : 0;
+    };
+    const auto blocks = [=](int n) { return (n * G + R - 1) / R; };
+    int L = 0x7fffffff;
+    if (p.target > 0) {
+      int64_t all = 0;
+      int nb = 0, carry = 0;
+      for (int64_t base = 0; base < p.B; base += 64) {
+        const int64_t i = base + lane;
+        const int x = max(carry, wave_scan_max(seq_bound(p.q_ptr, min(i, (int64_t)p.B), p.N)));
+        const int e = max(x, seq_bound(p.q_ptr, min(i + 1, (int64_t)p.B), p.N));
+        nb += blocks(e - x);
+        all += (int64_t)blocks(e - x) * units((int)min(i, (int64_t)p.B - 1), e - x);
+        carry = __builtin_amdgcn_readlane(e, 63);
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        nb += __shfl_xor(nb, o);
+        all += __shfl_xor(all, o);
+      }
+      const int64_t over = max(max(p.target - nb, nb / 4), 1);
+      L = (int)min((max((all + over - 1) / over, (int64_t)p.least) + step - 1) / step * step, (int64_t)L);
+    }
+    const auto cut = [=](int u) { return max(1, (int)(((uint32_t)u + (uint32_t)L - 1) / (uint32_t)L)); };
+    SeqPlace at;
     if (!seq_find(
-            p.q_ptr, p.B, p.N, [=](int m) { return (m * G + R - 1) / R; }, [=](int, int upto) { return upto > rb; }, at_seq))
+            p.q_ptr, p.B, p.N,
+            [=](int i, int m) { return blocks(m) * cut(units((int)min((int64_t)i, (int64_t)p.B - 1), m)); },
+            [=](int, int upto) { return upto > share; }, at))
       return false;
-    b = at_seq.seq;
-    first = at_seq.first;
-    n = at_seq.n;
-    row0 = (rb - at_seq.before) * R;
+    b = __builtin_amdgcn_readfirstlane(at.seq);
+    first = at.first;
+    n = at.n;
     rows = n * G;
     ctx = max(p.ctx[b], 0);
-    total = p.pages > 0 ? min(ctx + n, p.max_pages * p.page) : 0;
-    const int units = (int)((total + 31) >> 5);
-    const int part = max(step, ((units + p.splits - 1) / p.splits + step - 1) / step * step);
-    u0 = min(units, split * part);
-    u1 = min(units, u0 + part);
+    total = min(ctx + n, most);
+    const int u = units(b, n);
+    parts = __builtin_amdgcn_readfirstlane(cut(u));
+    const int k = share - at.before, rb = k / parts, part = k - rb * parts;
+    const int len = ((u + parts - 1) / parts + step - 1) / step * step;  // at most L: none is empty
+    row0 = rb * R;
+    u0 = min(u, part * len);
+    u1 = min(u, u0 + len);
+    slot = (uint32_t)blockIdx.x * R;
+    if (p.target > 0 && part == 0)  // what joins the rows' parts
+      for (int r = row0 + threadIdx.x; r < min(rows, row0 + R); r += blockDim.x)
+        p.joins[head_row(p, r)] = make_uint2(slot + r - row0, parts);
     return true;
   }
   __device__ __forceinline__ int64_t head_row(const TreeParams& p, int row) const {  // (row, head) of a packed row
     const int G = p.HQ / p.HKV, tk = row / G;
     return (int64_t)(first + tk) * p.HQ + hk * G + (row - tk * G);
-  }
-  // An empty part of a short sequence has no sums: its rows say so.
-  __device__ __forceinline__ void no_sums(const TreeParams& p, int R) const {
-    for (int r = row0 + threadIdx.x; r < min(rows, row0 + R); r += blockDim.x)
-      p.ml[head_row(p, r) * p.splits + split] = make_float2(-INFINITY, 0.f);
   }
 };
 
@@ -179,19 +216,16 @@ __device__ __forceinline__ float quarters_max(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Scores of 32 positions -> weights (the B operand of the outputs' product, and for the rare path as they are), with the
+// Scaled scores of 32 positions, base two, -> weights (the B operand of the outputs' product, and for the rare path as they are), with the
 // rows' reference maxima, sums and outputs brought up to date. edge: seen() says which of the positions the row sees.
-template <bool FP8, int DT, typename Seen>
-__device__ __forceinline__ void soft_weights(const f32x4 (&s)[2], float f2, const f32x4 (&kq)[2], const f32x4 (&vq)[2],
+template <bool FP8, int DT, typename Scale, typename Seen>
+__device__ __forceinline__ void soft_weights(const f32x4 (&s)[2], Scale vscale,
                                              bool edge, Seen seen, float& m, float& l, f32x4 (&acc)[DT], bf16x8& pf) {
   float w[8];
   const int g = (threadIdx.x & 63) >> 4;
   uint32_t see = ~0u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w[i] = s[i >> 2][i & 3] * f2;
-    if (FP8) w[i] *= kq[i >> 2][i & 3];
-  }
+  for (int i = 0; i < 8; ++i) w[i] = s[i >> 2][i & 3];
   if (edge) {
     see = seen() >> (g * 4);
 #pragma unroll
@@ -210,6 +244,11 @@ __device__ __forceinline__ void soft_weights(const f32x4 (&s)[2], float f2, cons
     for (int d = 0; d < DT; ++d) acc[d] *= a;
   }
   const float ref = m == -INFINITY ? 0.f : m;
+  f32x4 vq[2];
+  if (FP8) {
+    vq[0] = vscale(0);
+    vq[1] = vscale(1);
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     w[i] = __builtin_amdgcn_exp2f(w[i] - ref);
@@ -277,7 +316,6 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
 
   Part w;
   if (!w.find(p, R, D, 4)) return;
-  if (p.splits > 1 && w.u0 >= w.u1) return w.no_sums(p, R);
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Row rw(p, w.row0, w.rows, w.first, w.hk, c);
@@ -354,17 +392,19 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
           dst[i * STEP + h] = x;
         }
     }
-    f32x4 kq[2], vq[2];
-    if (FP8)
+    f32x4 vq[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        kq[t] = ks[t];
+    for (int t = 0; t < 2; ++t) {
+      s[t] *= f2;
+      if (FP8) {
+        s[t] *= ks[t];
         vq[t] = vs[t];
       }
+    }
     if (u + 4 < w.u1) load(u + 4);
     bf16x8 pf;
     soft_weights<FP8, DT>(
-        s, f2, kq, vq, edge, [&] { return rw.live ? there & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u; }, m, l, acc, pf);
+        s, [&](int t) { return vq[t]; }, edge, [&] { return rw.live ? there & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u; }, m, l, acc, pf);
     add_values<RS, DT>(vl, pf, edge && __any(odd), acc);
   }
 
@@ -390,7 +430,7 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)  // a wave without a reference has a sum only where every score was NaN
     sum += sm[k][r] == -INFINITY ? sl[k][r] : sl[k][r] * __builtin_amdgcn_exp2f(sm[k][r] - top);
-  const int64_t nh = w.head_row(p, row), i = nh * p.splits + w.split;
+  const int64_t nh = w.head_row(p, row), i = w.slot + r;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int q = 0; q < D / 64; ++q) {
@@ -398,13 +438,13 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
     f32x4 o{};
 #pragma unroll
     for (int k = 0; k < 4; ++k) o += *reinterpret_cast<const f32x4*>(swap + (k * R + r) * XS + d);
-    if (p.splits > 1)
+    if (w.parts > 1)
       *reinterpret_cast<f32x4*>(p.part + i * D + d) = o;
     else
       *reinterpret_cast<uint2*>(p.out + nh * D + d) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
   }
   if ((threadIdx.x & 15) != 0) return;
-  if (p.splits > 1)
+  if (w.parts > 1)
     p.ml[i] = make_float2(top, sum);
   else if (p.lse != nullptr)
     p.lse[nh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
@@ -452,7 +492,6 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
 
   Part w;
   if (!w.find(p, R, D, 1)) return;
-  if (p.splits > 1 && w.u0 >= w.u1) return w.no_sums(p, R);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wrow = w.row0 + wave * 16 * CT;
   const Table table(p, w);
@@ -463,8 +502,8 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     load_q<D>(p, Row(p, wrow + ct * 16, w.rows, w.first, w.hk, threadIdx.x & 15), w.first, false, qf[ct]);
 
   struct Pieces {
-    uint4 k[PL], v[PL];
-    float ks, vs;
+    uint4 at[PL];
+    float scale;
   };
   // the unit's rows of the cache and whether they are: of its first 16 positions, of the others
   int64_t r0, r1;
@@ -485,50 +524,49 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
       dma16(vr, &buf[h][1][(wave * 8 + i * RL) * RB], at + (pc ^ r * 2) * 16);
     }
   };
-  const auto fetch = [&](Pieces& x) {  // or to registers
+  // rows_of()'s rows of keys or of values to registers
+  const auto fetch = [&](const void* cache, const float* scales, Pieces& x) {
     const int lane = lane_anew(), sub = lane / PR, pc = lane % PR;
     const int64_t row = max(wave >> 1 ? r1 : r0, (int64_t)0);  // any row of the cache: it is not used
-    const auto kr = make_rsrc(static_cast<const uint8_t*>(p.kc) + row * SB, 16 * SB);
-    const auto vr = make_rsrc(static_cast<const uint8_t*>(p.vc) + row * SB, 16 * SB);
+    const auto rs = make_rsrc(static_cast<const uint8_t*>(cache) + row * SB, 16 * SB);
+#pragma unroll
+    for (int i = 0; i < PL; ++i) x.at[i] = bload(rs, ((wave & 1) * 8 + i * RL + sub) * SB + pc * 16);
+    if (FP8) x.scale = scales[row + (wave & 1) * 8 + (lane & 7)];
+  };
+  const auto store_keys = [&](const Pieces& x, int h) {  // and from there to half h
+    const int lane = lane_anew(), sub = lane / PR, pc = lane % PR;
 #pragma unroll
     for (int i = 0; i < PL; ++i) {
-      const int at = ((wave & 1) * 8 + i * RL + sub) * SB + pc * 16;
-      x.k[i] = bload(kr, at);
-      x.v[i] = bload(vr, at);
+      const int r = i * RL + sub;
+      uint8_t* const to = &buf[h][0][(wave * 8 + r) * RB];
+#pragma unroll
+      for (int e = 0; e < (FP8 ? 2 : 1); ++e)
+        *reinterpret_cast<uint4*>(to + ((FP8 ? pc * 2 + e : pc) ^ r) * 16) = half_piece<FP8>(x.at[i], e);
     }
-    if (FP8) {
-      x.ks = p.ks[row + (wave & 1) * 8 + (lane & 7)];
-      x.vs = p.vs[row + (wave & 1) * 8 + (lane & 7)];
-    }
+    if (FP8) sc[h][0][wave * 8 + (lane & 7)] = x.scale;  // the same from eight lanes
   };
-  const auto store = [&](Pieces& x, int u, int h, bool ok0, bool ok1) {  // the fetched unit u to LDS half h
+  // zeros for values that are not there or not finite
+  const auto store_values = [&](const Pieces& x, int u, int h, bool ok0, bool ok1) {
     const int lane = lane_anew(), sub = lane / PR, pc = lane % PR;
     const bool edge = is_edge(u, ok0 && ok1);
-    const uint32_t there = existing(w.total - (int64_t)u * 32, ok0, ok1);
+    const uint32_t there = existing(w.total - (int64_t)u * 32, ok0, ok1) >> wave * 8;
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < PL; ++i) {
       const int r = i * RL + sub;
-      uint8_t* const kd = &buf[h][0][(wave * 8 + r) * RB];
-      uint8_t* const vd = &buf[h][1][(wave * 8 + r) * RB];
-      if (edge && !(there >> (wave * 8 + r) & 1)) x.v[i] = make_uint4(0u, 0u, 0u, 0u);
+      uint8_t* const to = &buf[h][1][(wave * 8 + r) * RB];
 #pragma unroll
       for (int e = 0; e < (FP8 ? 2 : 1); ++e) {
-        const uint4 y = !FP8 ? x.k[i] : e ? cvt_fp8x8(x.k[i].z, x.k[i].w) : cvt_fp8x8(x.k[i].x, x.k[i].y);
-        uint4 z = !FP8 ? x.v[i] : e ? cvt_fp8x8(x.v[i].z, x.v[i].w) : cvt_fp8x8(x.v[i].x, x.v[i].y);
+        uint4 y = half_piece<FP8>(x.at[i], e);
         if (edge) {
-          odd |= odd2(z.x) | odd2(z.y) | odd2(z.z) | odd2(z.w);
-          z = make_uint4(even2(z.x), even2(z.y), even2(z.z), even2(z.w));
+          if (!(there >> r & 1)) y = make_uint4(0u, 0u, 0u, 0u);
+          odd |= odd2(y.x) | odd2(y.y) | odd2(y.z) | odd2(y.w);
+          y = make_uint4(even2(y.x), even2(y.y), even2(y.z), even2(y.w));
         }
-        const int j = FP8 ? pc * 2 + e : pc;
-        *reinterpret_cast<uint4*>(kd + (j ^ r) * 16) = y;
-        *reinterpret_cast<uint4*>(vd + (j ^ r * 2) * 16) = z;
+        *reinterpret_cast<uint4*>(to + ((FP8 ? pc * 2 + e : pc) ^ r * 2) * 16) = y;
       }
     }
-    if (FP8) {  // the same from eight lanes
-      sc[h][0][wave * 8 + (lane & 7)] = x.ks;
-      sc[h][1][wave * 8 + (lane & 7)] = x.vs;
-    }
+    if (FP8) sc[h][1][wave * 8 + (lane & 7)] = x.scale;
     if (edge && __any(odd)) odd_any = 1;
   };
 
@@ -550,9 +588,11 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     ok0 = r0 >= 0;
     ok1 = r1 >= 0;
     if (FP8 || is_edge(w.u0, ok0 && ok1)) {
-      Pieces x;
-      fetch(x);
-      store(x, w.u0, 0, ok0, ok1);
+      Pieces x, y;
+      fetch(p.kc, p.ks, x);
+      fetch(p.vc, p.vs, y);
+      store_keys(x, 0);
+      store_values(y, w.u0, 0, ok0, ok1);
     } else {
       dma(0);
     }
@@ -566,22 +606,25 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     const bool more = u + 1 < w.u1, ok2 = r0 >= 0, ok3 = r1 >= 0;
     Pieces next;
     if (FP8) {
-      if (more) fetch(next);
+      if (more) fetch(p.kc, p.ks, next);
     } else if (more) {
       if (is_edge(u + 1, ok2 && ok3)) {
-        Pieces x;
-        fetch(x);
-        store(x, u + 1, h ^ 1, ok2, ok3);
+        Pieces x, y;
+        fetch(p.kc, p.ks, x);
+        fetch(p.vc, p.vs, y);
+        store_keys(x, h ^ 1);
+        store_values(y, u + 1, h ^ 1, ok2, ok3);
       } else {
         dma(h ^ 1);
       }
+      rows_of(u + 2);
     }
-    if (more) rows_of(u + 2);
-    if (wrow < w.rows) {
-      const int lane = lane_anew(), g = lane >> 4, c = lane & 15, vrow = g * 4 + (c >> 2);
+    const bool live = wrow < w.rows;
+    f32x4 s[CT][2];
+    if (live) {
+      const int lane = lane_anew(), g = lane >> 4, c = lane & 15;
       const uint8_t* const kl = &buf[h][0][c * RB + (g ^ (c & 7)) * 16];
       const uint8_t* const kl4 = &buf[h][0][c * RB + (g ^ 4 ^ (c & 7)) * 16];
-      f32x4 s[CT][2];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) s[ct][0] = s[ct][1] = f32x4{};
       bf16x8 a[2][2];
@@ -602,20 +645,27 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const f32x4 kq = FP8 ? *reinterpret_cast<const f32x4*>(&sc[h][0][t * 16 + g * 4]) * f2 : f32x4{} + f2;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[ct][t] *= kq;
+      }
+    }
+    if (FP8 && more) {  // the next unit's values take the registers that its keys leave
+      store_keys(next, h ^ 1);
+      fetch(p.vc, p.vs, next);
+      rows_of(u + 2);
+    }
+    if (live) {
+      const int lane = lane_anew(), g = lane >> 4, c = lane & 15, vrow = g * 4 + (c >> 2);
       const int64_t p0 = (int64_t)u * 32;
       const bool edge = is_edge(u, ok0 && ok1);
-      f32x4 kq[2], vq[2];
-      if (FP8)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          kq[t] = *reinterpret_cast<const f32x4*>(&sc[h][0][t * 16 + g * 4]);
-          vq[t] = *reinterpret_cast<const f32x4*>(&sc[h][1][t * 16 + g * 4]);
-        }
       bf16x8 pf[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
         soft_weights<FP8, DT>(
-            s[ct], f2, kq, vq, edge,
+            s[ct], [&](int t) { return *reinterpret_cast<const f32x4*>(&sc[h][1][t * 16 + g * 4]); }, edge,
             [&] {
               const Row rw(p, wrow + ct * 16, w.rows, w.first, w.hk, lane_anew() & 15);
               return rw.live ? existing(w.total - p0, ok0, ok1) & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u;
@@ -640,7 +690,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (FP8 && more) store(next, u + 1, h ^ 1, ok2, ok3);
+    if (FP8 && more) store_values(next, u + 1, h ^ 1, ok2, ok3);
     ok0 = ok2;
     ok1 = ok3;
   }
@@ -652,18 +702,18 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     l[ct] += __shfl_xor(l[ct], 32);
     const Row rw(p, wrow + ct * 16, w.rows, w.first, w.hk, c);
     if (!rw.live) continue;
-    const int64_t nh = (int64_t)(w.first + rw.tok) * p.HQ + rw.head, i = nh * p.splits + w.split;
+    const int64_t nh = (int64_t)(w.first + rw.tok) * p.HQ + rw.head, i = w.slot + (wave * CT + ct) * 16 + c;
     const float inv = l[ct] == 0.f ? 0.f : 1.f / l[ct];
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const f32x4 o = acc[ct][d];
-      if (p.splits > 1)
+      if (w.parts > 1)
         *reinterpret_cast<f32x4*>(p.part + i * D + d * 16 + g * 4) = o;
       else
         *reinterpret_cast<uint2*>(p.out + nh * D + d * 16 + g * 4) = make_uint2(cvt_pk2(o[0] * inv, o[1] * inv), cvt_pk2(o[2] * inv, o[3] * inv));
     }
     if (g != 0) continue;
-    if (p.splits > 1)
+    if (w.parts > 1)
       p.ml[i] = make_float2(m[ct], l[ct]);
     else if (p.lse != nullptr)
       p.lse[nh] = l[ct] == 0.f ? -INFINITY : (m[ct] + log2f(l[ct])) * kLn2;
@@ -691,8 +741,8 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
           const float x = FP8 ? bf2f(cvt_fp8x2(static_cast<const uint8_t*>(p.vc)[v + d], false) & 0xffffu)
                               : bf2f(static_cast<const uint16_t*>(p.vc)[v + d]);
           if (fabsf(x) < INFINITY) continue;
-          if (p.splits > 1)
-            p.part[(nh * p.splits + w.split) * D + d] += x;
+          if (w.parts > 1)
+            p.part[(int64_t)(w.slot + (wave * CT + ct) * 16 + c) * D + d] += x;
           else
             p.out[nh * D + d] = (uint16_t)f2bf(bf2f(p.out[nh * D + d]) + x);
         }
@@ -703,26 +753,26 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
 
 // Joins the parts of a row: one wave per (row, head), 4 D / 256 dims a lane.
 template <int D>
-__global__ void __launch_bounds__(256) tree_join_k(TreeParams p) {
+__global__ void __launch_bounds__(256) tree_join_k(TreeParams p, int R) {
   constexpr int E = D / 64;
   const int64_t nh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (nh >= p.N * p.HQ) return;
-  const int64_t row = nh / p.HQ;
-  int lo, hi;
-  seq_span(p.q_ptr, p.B, p.N, lo, hi);
-  if (row < lo || row >= hi) return;  // of no sequence: it has its zeros
-  const float2* const ml = p.ml + nh * p.splits;
+  const uint2 at = p.joins[nh];
+  const int parts = (int)at.y;
+  if (parts < 2) return;  // done, or of no sequence
+  const int64_t step = (int64_t)p.HKV * R;
+  const float2* const ml = p.ml + at.x;
+  const float* const src = p.part + (int64_t)at.x * D + lane * E;
   float top = -INFINITY, sum = 0.f, o[E] = {};
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[s].x);
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 x = ml[s];
-    if (x.x == -INFINITY && x.y == 0.f) continue;  // nothing seen there; an empty part has no sums either
+  for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[s * step].x);
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float2 x = ml[s * step];  // a part without a maximum has zeros, or NaN where every score was
     const float f = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - top);
     sum += f * x.y;
-    const float* const src = p.part + (nh * p.splits + s) * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += f * src[e];
+    for (int e = 0; e < E; ++e) o[e] += f * src[s * step * D + e];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint32_t* const dst = reinterpret_cast<uint32_t*>(p.out + nh * D + lane * E);
@@ -738,9 +788,14 @@ TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, 
   const int64_t G = HQ / HKV, seqs = std::max<int64_t>(1, std::min<int64_t>(B, N)), mean = (N * G + seqs - 1) / seqs;
   t.rows = mean <= 16 ? 16 : mean <= 64 ? 64 : 128;
   // an upper bound of sum ceil(n_b G / rows) over the sequences with rows, which are `seqs` at most
-  t.blocks = (N * G + seqs * (t.rows - 1)) / t.rows;
-  const int64_t units = (max_pages * page + 31) / 32, base = t.blocks * HKV;
-  t.splits = std::max<int64_t>(1, std::min<int64_t>((512 + base - 1) / base, std::min<int64_t>(units / 8, 64)));
+  const int64_t blocks = (N * G + seqs * (t.rows - 1)) / t.rows, units = (max_pages * page + 31) / 32;
+  t.least = t.rows == 16 ? 4 : 8;
+  const int64_t at_once = (t.rows == 16 ? 256 : 512) * 256 / D;  // workgroups that the GPU holds
+  t.target = units > t.least ? std::max<int64_t>(1, at_once / HKV) : 0;
+  t.shares = t.target == 0 ? blocks
+                           : std::min<int64_t>(std::max<int64_t>(t.target, blocks + blocks / 4 + 1),
+                                               blocks * ((units + t.least - 1) / t.least));
+  t.slots = t.target == 0 ? 0 : t.shares * HKV * t.rows;
   return t;
 }
 
@@ -752,11 +807,11 @@ static void (*tree_kernel(int rows))(TreeParams) {
 hipError_t launch_tree_attn(const TreeParams& p, const TreePlan& t, int D, bool fp8, hipStream_t st) {
   const auto kernel = D == 256 ? (fp8 ? tree_kernel<256, true>(t.rows) : tree_kernel<256, false>(t.rows))
                                : (fp8 ? tree_kernel<128, true>(t.rows) : tree_kernel<128, false>(t.rows));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(t.blocks * p.HKV * t.splits)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(t.shares * p.HKV)), dim3(256), 0, st, p);
   hipError_t err = hipGetLastError();
-  if (err != hipSuccess || t.splits == 1) return err;
+  if (err != hipSuccess || t.target == 0) return err;
   hipLaunchKernelGGL(D == 256 ? tree_join_k<256> : tree_join_k<128>, dim3((unsigned)((p.N * p.HQ + 3) / 4)), dim3(256),
-                     0, st, p);
+                     0, st, p, t.rows);
   return hipGetLastError();
 }
 
