@@ -970,7 +970,7 @@ int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const
   float2* const ml = reinterpret_cast<float2*>(part + t.slots * D);
   const ojx::TreeParams p{static_cast<const uint16_t*>(q), q_ptr, ctx, bits, bits != nullptr ? words : 0, kc, vc, ks, vs,
                           table, max_pages, N, pages, B, HQ, HKV, page, scale, static_cast<uint16_t*>(out), lse,
-                          t.target, t.least, (uint32_t)(((1ULL << 32) + page / 16 - 1) / (page / 16)), part, ml,
+                          t.target, t.least, 0xffffffffu / (uint32_t)(page / 16), part, ml,
                           reinterpret_cast<uint2*>(ml + t.slots)};
   return hip_check(ojx::launch_tree_attn(p, t, D, fmt == OJX_KV_E4M3, static_cast<hipStream_t>(stream)),
                    "tree attention launch");

@@ -287,7 +287,7 @@ struct TreeParams {
   float scale;
   uint16_t* out; float* lse;              // [N, HQ, D]; [N, HQ] or null
   int target, least;                      // of tree_plan
-  uint32_t tiles_inv;                     // 2^32 / (page / 16), rounded up; not used for pages of 16
+  uint32_t tiles_inv;                     // (2^32 - 1) / (page / 16)
   float* part; float2* ml;                // [slots, D] sums, [slots] (maximum, base two; sum)
   uint2* joins;                           // [N, HQ] slot of a row's first part, parts
 };

@@ -197,14 +197,20 @@ struct Table {
   __device__ __forceinline__ Table(const TreeParams& p, const Part& w)
       : at((const_ints)(uintptr_t)(p.table + (int64_t)w.b * p.max_pages)), max_pages((int)p.max_pages), tiles(p.page >> 4),
         page(p.page), HKV(p.HKV), hk(w.hk), inv(p.tiles_inv), pages((uint32_t)p.pages) {}
-  // without a branch: a tile behind the table reads its last entry, and counts as none
-  __device__ __forceinline__ int64_t row(int t) const {
-    int i = (int)(((uint64_t)(uint32_t)t * inv) >> 32);  // t / tiles, or one more
-    i = tiles > 1 ? i - (i * tiles > t) : t;
-    const int pg = at[min(i, max_pages - 1)];
-    const int64_t r = ((int64_t)pg * HKV + hk) * page + (t - i * tiles) * 16;
-    return (i < max_pages) & ((uint32_t)pg < pages) ? r : -1;
+  __device__ __forceinline__ int index(int t) const {  // t / tiles
+    const int i = (int)(((uint64_t)(uint32_t)t * inv) >> 32);  // or one less
+    return i + ((i + 1) * tiles <= t);
   }
+  // the page of tile t, without a branch: a tile behind the table reads its last entry
+  __device__ __forceinline__ int entry(int t) const { return at[min(index(t), max_pages - 1)]; }
+  // the row, given that entry
+  __device__ __forceinline__ int64_t row(int t, int pg) const {
+    const int i = index(t);
+    const int64_t r = ((int64_t)pg * HKV + hk) * page + (t - i * tiles) * 16;
+    const bool ok = (i < max_pages) & ((uint32_t)pg < pages);
+    return ok ? r : -1;
+  }
+  __device__ __forceinline__ int64_t row(int t) const { return row(t, entry(t)); }
 };
 
 // The largest of lanes l, l ^ 16, l ^ 32, l ^ 48, by swaps of rows of 16 and halves of 32: no trip through LDS.
@@ -507,9 +513,14 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   };
   // the unit's rows of the cache and whether they are: of its first 16 positions, of the others
   int64_t r0, r1;
-  const auto rows_of = [&](int u) {
-    r0 = table.row(2 * u);
-    r1 = table.row(2 * u + 1);
+  const auto rows_of = [&](int u, int page0, int page1) {
+    r0 = table.row(2 * u, page0);
+    r1 = table.row(2 * u + 1, page1);
+  };
+  int e0 = 0, e1 = 0;  // the next unit's table entries, fetched an iteration before they are looked at
+  const auto entries_of = [&](int u) {
+    e0 = table.entry(2 * u);
+    e1 = table.entry(2 * u + 1);
   };
   const auto is_edge = [&](int u, bool ok) { return !ok || (int64_t)u * 32 + 32 > plain; };
   const auto dma = [&](int h) {  // rows_of()'s rows to half h
@@ -584,7 +595,9 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   __syncthreads();
   bool ok0 = false, ok1 = false;  // of the unit at hand
   if (w.u0 < w.u1) {
-    rows_of(w.u0);
+    entries_of(w.u0);
+    rows_of(w.u0, e0, e1);
+    entries_of(w.u0 + 1);
     ok0 = r0 >= 0;
     ok1 = r1 >= 0;
     if (FP8 || is_edge(w.u0, ok0 && ok1)) {
@@ -596,14 +609,16 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     } else {
       dma(0);
     }
-    rows_of(w.u0 + 1);
   }
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&buf[0][0][0];
   for (int u = w.u0; u < w.u1; ++u) {
     const int h = (u - w.u0) & 1;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows are there
     lds_barrier();
-    const bool more = u + 1 < w.u1, ok2 = r0 >= 0, ok3 = r1 >= 0;
+    const bool more = u + 1 < w.u1;
+    rows_of(u + 1, e0, e1);
+    entries_of(u + 2);
+    const bool ok2 = r0 >= 0, ok3 = r1 >= 0;
     Pieces next;
     if (FP8) {
       if (more) fetch(p.kc, p.ks, next);
@@ -617,7 +632,6 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
       } else {
         dma(h ^ 1);
       }
-      rows_of(u + 2);
     }
     const bool live = wrow < w.rows;
     f32x4 s[CT][2];
@@ -655,7 +669,6 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     if (FP8 && more) {  // the next unit's values take the registers that its keys leave
       store_keys(next, h ^ 1);
       fetch(p.vc, p.vs, next);
-      rows_of(u + 2);
     }
     if (live) {
       const int lane = lane_anew(), g = lane >> 4, c = lane & 15, vrow = g * 4 + (c >> 2);
@@ -727,7 +740,8 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     const int64_t nh = (int64_t)(w.first + rw.tok) * p.HQ + rw.head;
 #pragma unroll 1
     for (int u = w.u0; u < w.u1; ++u) {
-      rows_of(u);
+      entries_of(u);
+      rows_of(u, e0, e1);
       if (!is_edge(u, r0 >= 0 && r1 >= 0)) continue;
       const int64_t p0 = (int64_t)u * 32;
       const uint32_t see = existing(w.total - p0, r0 >= 0, r1 >= 0) & seen32(p, rw.words, rw.tok, p0 - w.ctx);
@@ -765,15 +779,22 @@ __global__ void __launch_bounds__(256) tree_join_k(TreeParams p, int R) {
   const float2* const ml = p.ml + at.x;
   const float* const src = p.part + (int64_t)at.x * D + lane * E;
   float top = -INFINITY, sum = 0.f, o[E] = {};
-  for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[s * step].x);
-#pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const float2 x = ml[s * step];  // a part without a maximum has zeros, or NaN where every score was
+  for (int s = lane; s < parts; s += 64) top = fmaxf(top, ml[s * step].x);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+  for (int s0 = 0; s0 < parts; s0 += 64) {
+    const float2 x = s0 + lane < parts ? ml[(s0 + lane) * step] : make_float2(top, 0.f);
+    // a part without a maximum has zeros, or NaN where every score was
     const float f = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - top);
     sum += f * x.y;
+#pragma unroll 4
+    for (int s = 0; s < min(parts - s0, 64); ++s) {
+      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += f * src[s * step * D + e];
+      for (int e = 0; e < E; ++e) o[e] += w * src[(s0 + s) * step * D + e];
+    }
   }
+  sum = wave_sum64(sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint32_t* const dst = reinterpret_cast<uint32_t*>(p.out + nh * D + lane * E);
 #pragma unroll
