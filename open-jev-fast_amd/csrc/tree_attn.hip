@@ -479,7 +479,7 @@ __device__ __forceinline__ void values4(uint32_t a0, uint32_t a1, uint32_t a2, u
 __device__ __forceinline__ int lane_anew() {
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));
-  return lane;
+  return lane & 63;  // known not to be negative: shifts, not divisions
 }
 
 // Many rows: 64 CT packed rows a workgroup, 16 CT of them a wave; all take the part's units of 32 positions in order, from
@@ -629,6 +629,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
         fetch(p.vc, p.vs, y);
         store_keys(x, h ^ 1);
         store_values(y, u + 1, h ^ 1, ok2, ok3);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // said here: else the compiler waits behind the DMAs of the other path, too
       } else {
         dma(h ^ 1);
       }
