@@ -77,15 +77,14 @@ __device__ __forceinline__ uint32_t even2(uint32_t x) {  // with zeros for those
 }
 
 // Positions p0 .. p0 + 31 of those that a row of drafted index i sees, as bits; w: its words.
-__device__ __forceinline__ uint32_t seen32(const TreeParams& p, const int64_t* w, int i, int64_t j0) {
+__device__ __forceinline__ uint32_t seen32(const TreeParams& p, const int64_t* w, int i, int j0) {
   if (j0 <= -32) return ~0u;
   if (w == nullptr) {
-    const int64_t c = i - j0 + 1;
+    const int c = i - j0 + 1;
     return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1;
   }
   if (j0 < 0) return ((uint32_t)w[0] << -j0) | ((1u << -j0) - 1);
-  const int64_t at = j0 >> 6;
-  const int sh = (int)(j0 & 63);
+  const int at = j0 >> 6, sh = j0 & 63;
   if (at >= p.words) return 0u;
   uint64_t x = (uint64_t)w[at] >> sh;
   if (sh > 32 && at + 1 < p.words) x |= (uint64_t)w[at + 1] << (64 - sh);
@@ -125,7 +124,7 @@ __device__ __forceinline__ void load_q(const TreeParams& p, const Row& w, int fi
 struct Part {
   int b, first, n, row0, rows, hk, parts, u0, u1;
   uint32_t slot;  // of the part's first row in the workspace; a row's parts lie HKV R slots apart
-  int64_t ctx, total;
+  int ctx, total;  // positions before the drafted ones; all of them that the table can hold
   // false: nothing to do. Shares are numbered sequence, row block, part; the kv head is the fastest of a launch. Parts
   // begin at multiples of step.
   __device__ __forceinline__ bool find(const TreeParams& p, int R, int D, int step) {
@@ -169,7 +168,7 @@ struct Part {
     n = at.n;
     rows = n * G;
     ctx = max(p.ctx[b], 0);
-    total = min(ctx + n, most);
+    total = (int)min((int64_t)ctx + n, most);
     const int u = units(b, n);
     parts = __builtin_amdgcn_readfirstlane(cut(u));
     const int k = share - at.before, rb = k / parts, part = k - rb * parts;
@@ -189,7 +188,7 @@ struct Part {
   }
 };
 
-// Row of the cache where the 16 positions of tile t begin, or -1 where there is none (a sequence with positions has pages).
+// Where in the cache the 16 positions of a tile are (a sequence with positions has pages).
 struct Table {
   const_ints at;
   int max_pages, tiles, page, HKV, hk;
@@ -203,14 +202,11 @@ struct Table {
   }
   // the page of tile t, without a branch: a tile behind the table reads its last entry
   __device__ __forceinline__ int entry(int t) const { return at[min(index(t), max_pages - 1)]; }
-  // the row, given that entry
+  __device__ __forceinline__ bool ok(int t, int pg) const { return (index(t) < max_pages) & ((uint32_t)pg < pages); }
+  // the row, given that entry; where there is none, any row of the cache (it is not used)
   __device__ __forceinline__ int64_t row(int t, int pg) const {
-    const int i = index(t);
-    const int64_t r = ((int64_t)pg * HKV + hk) * page + (t - i * tiles) * 16;
-    const bool ok = (i < max_pages) & ((uint32_t)pg < pages);
-    return ok ? r : -1;
+    return ((int64_t)(ok(t, pg) ? pg : 0) * HKV + hk) * page + (t - index(t) * tiles) * 16;
   }
-  __device__ __forceinline__ int64_t row(int t) const { return row(t, entry(t)); }
 };
 
 // The largest of lanes l, l ^ 16, l ^ 32, l ^ 48, by swaps of rows of 16 and halves of 32: no trip through LDS.
@@ -303,7 +299,7 @@ __device__ __forceinline__ void add_values(const uint16_t* vl, bf16x8 pf, bool o
 }
 
 // Which of the 32 positions from p0 exist: below the sequence's end, in pages of the cache.
-__device__ __forceinline__ uint32_t existing(int64_t left, bool ok0, bool ok1) {
+__device__ __forceinline__ uint32_t existing(int left, bool ok0, bool ok1) {
   return (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1) & ((ok0 ? 0xffffu : 0u) | (ok1 ? 0xffff0000u : 0u));
 }
 
@@ -336,9 +332,9 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
     int64_t row[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      row[t] = table.row(2 * u + t);
-      ok[t] = row[t] >= 0;
-      row[t] = max(row[t], (int64_t)0);  // any row of the cache: its values are not used
+      const int pg = table.entry(2 * u + t);
+      ok[t] = table.ok(2 * u + t, pg);
+      row[t] = table.row(2 * u + t, pg);
       const uint8_t* kb = static_cast<const uint8_t*>(p.kc) + row[t] * RB;
 #pragma unroll
       for (int f = 0; f < KL; ++f) kx[t][f] = *reinterpret_cast<const uint4*>(kb + c * RB + f * 64 + g * 16);
@@ -354,6 +350,7 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
   };
 
   const float f2 = p.scale * kLog2e;
+  const int full = min(w.ctx, w.total) >> 5;  // units below are seen by every row, if they are in the cache
   f32x4 acc[DT];
   float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -374,8 +371,8 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
         s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[f], s[t], 0, 0, 0);
       }
     }
-    const int64_t p0 = (int64_t)u * 32;
-    const bool edge = !(ok[0] && ok[1]) || p0 + 32 > min(w.ctx, w.total);
+    const int p0 = u * 32;
+    const bool edge = !(ok[0] && ok[1]) || u >= full;
     const uint32_t there = existing(w.total - p0, ok[0], ok[1]);
     bool odd = false;
     const auto piece = [&](int i, int h) {
@@ -501,7 +498,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wrow = w.row0 + wave * 16 * CT;
   const Table table(p, w);
-  const int64_t plain = min(w.ctx, w.total);  // positions below are seen by every row, if they are in the cache
+  const int full = min(w.ctx, w.total) >> 5;  // units below are seen by every row, if they are in the cache
   bf16x8 qf[CT][KF];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct)
@@ -511,21 +508,22 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     uint4 at[PL];
     float scale;
   };
-  // the unit's rows of the cache and whether they are: of its first 16 positions, of the others
-  int64_t r0, r1;
+  // this wave's row of a unit, and whether the unit's first 16 positions, and the others, are in the cache
+  int64_t row = 0;
+  bool in0 = false, in1 = false;
   const auto rows_of = [&](int u, int page0, int page1) {
-    r0 = table.row(2 * u, page0);
-    r1 = table.row(2 * u + 1, page1);
+    in0 = table.ok(2 * u, page0);
+    in1 = table.ok(2 * u + 1, page1);
+    row = table.row(2 * u + (wave >> 1), wave >> 1 ? page1 : page0);
   };
   int e0 = 0, e1 = 0;  // the next unit's table entries, fetched an iteration before they are looked at
   const auto entries_of = [&](int u) {
     e0 = table.entry(2 * u);
     e1 = table.entry(2 * u + 1);
   };
-  const auto is_edge = [&](int u, bool ok) { return !ok || (int64_t)u * 32 + 32 > plain; };
+  const auto is_edge = [&](int u, bool ok) { return !ok || u >= full; };
   const auto dma = [&](int h) {  // rows_of()'s rows to half h
     const int lane = lane_anew(), sub = lane / PR, pc = lane % PR;  // row and piece of a lane in a load
-    const int64_t row = wave >> 1 ? r1 : r0;
     const auto kr = make_rsrc(static_cast<const uint8_t*>(p.kc) + row * SB, 16 * SB);
     const auto vr = make_rsrc(static_cast<const uint8_t*>(p.vc) + row * SB, 16 * SB);
 #pragma unroll
@@ -538,7 +536,6 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   // rows_of()'s rows of keys or of values to registers
   const auto fetch = [&](const void* cache, const float* scales, Pieces& x) {
     const int lane = lane_anew(), sub = lane / PR, pc = lane % PR;
-    const int64_t row = max(wave >> 1 ? r1 : r0, (int64_t)0);  // any row of the cache: it is not used
     const auto rs = make_rsrc(static_cast<const uint8_t*>(cache) + row * SB, 16 * SB);
 #pragma unroll
     for (int i = 0; i < PL; ++i) x.at[i] = bload(rs, ((wave & 1) * 8 + i * RL + sub) * SB + pc * 16);
@@ -560,7 +557,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   const auto store_values = [&](const Pieces& x, int u, int h, bool ok0, bool ok1) {
     const int lane = lane_anew(), sub = lane / PR, pc = lane % PR;
     const bool edge = is_edge(u, ok0 && ok1);
-    const uint32_t there = existing(w.total - (int64_t)u * 32, ok0, ok1) >> wave * 8;
+    const uint32_t there = existing(w.total - u * 32, ok0, ok1) >> wave * 8;
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < PL; ++i) {
@@ -598,8 +595,8 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     entries_of(w.u0);
     rows_of(w.u0, e0, e1);
     entries_of(w.u0 + 1);
-    ok0 = r0 >= 0;
-    ok1 = r1 >= 0;
+    ok0 = in0;
+    ok1 = in1;
     if (FP8 || is_edge(w.u0, ok0 && ok1)) {
       Pieces x, y;
       fetch(p.kc, p.ks, x);
@@ -618,7 +615,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     const bool more = u + 1 < w.u1;
     rows_of(u + 1, e0, e1);
     entries_of(u + 2);
-    const bool ok2 = r0 >= 0, ok3 = r1 >= 0;
+    const bool ok2 = in0, ok3 = in1;
     Pieces next;
     if (FP8) {
       if (more) fetch(p.kc, p.ks, next);
@@ -673,7 +670,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     }
     if (live) {
       const int lane = lane_anew(), g = lane >> 4, c = lane & 15, vrow = g * 4 + (c >> 2);
-      const int64_t p0 = (int64_t)u * 32;
+      const int p0 = u * 32;
       const bool edge = is_edge(u, ok0 && ok1);
       bf16x8 pf[CT];
 #pragma unroll
@@ -743,13 +740,13 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
     for (int u = w.u0; u < w.u1; ++u) {
       entries_of(u);
       rows_of(u, e0, e1);
-      if (!is_edge(u, r0 >= 0 && r1 >= 0)) continue;
-      const int64_t p0 = (int64_t)u * 32;
-      const uint32_t see = existing(w.total - p0, r0 >= 0, r1 >= 0) & seen32(p, rw.words, rw.tok, p0 - w.ctx);
+      if (!is_edge(u, in0 && in1)) continue;
+      const int p0 = u * 32;
+      const uint32_t see = existing(w.total - p0, in0, in1) & seen32(p, rw.words, rw.tok, p0 - w.ctx);
 #pragma unroll 1
       for (int key = 0; key < 32; ++key) {
         if (!(see >> key & 1)) continue;
-        const int64_t v = ((key >> 4 ? r1 : r0) + (key & 15)) * D;
+        const int64_t v = (table.row(2 * u + (key >> 4), key >> 4 ? e1 : e0) + (key & 15)) * D;
 #pragma unroll 1
         for (int i = 0; i < D / 4; ++i) {
           const int d = (i >> 2) * 16 + g * 4 + (i & 3);  // what this lane has written
