@@ -118,9 +118,11 @@ __device__ __forceinline__ void load_q(const TreeParams& p, const Row& w, int fi
 }
 
 // One workgroup's share: a row block of R packed rows of a sequence and a part of the sequence's units of 32 positions.
-// Work is shared out by the lengths as they are on the device: with nb row blocks of `total` units over all of them (of a
-// kv head), a part has L = total / max(p.target - nb, nb / 4) units at most, p.least at least, and a sequence of u units
-// ceil(u / L) parts of equal length. That makes max(p.target, nb + nb / 4 + 1) shares at most, which is the launch.
+// Work is shared out by the lengths as they are on the device: a sequence of u units has ceil(u / L) parts of equal length
+// for each of its row blocks. With no more row blocks, nb, than workgroups run at once (p.target, of a kv head), L is the
+// least that makes p.target parts at most, found in steps of a sixteenth from the mean on: one round of workgroups, all
+// about as long. With more, L is four times the mean, so that the longest sequences do not come last and alone: nb + nb / 4
+// parts at most. No part has fewer than p.least units unless its sequence has.
 struct Part {
   int b, first, n, row0, rows, hk, parts, u0, u1;
   uint32_t slot;  // of the part's first row in the workspace; a row's parts lie HKV R slots apart
@@ -137,26 +139,46 @@ struct Part {
     };
     const auto blocks = [=](int n) { return (n * G + R - 1) / R; };
     int L = 0x7fffffff;
+    const auto cut = [&](int u) { return max(1, (int)(((uint32_t)u + (uint32_t)L - 1) / (uint32_t)L)); };
     if (p.target > 0) {
+      int bl = 0, un = 0;  // row blocks and units of a lane's sequence
+      const auto pass = [&](auto f) {
+        int carry = 0;
+        for (int64_t base = 0; base < p.B; base += 64) {
+          const int64_t i = base + lane;
+          const int x = max(carry, wave_scan_max(seq_bound(p.q_ptr, min(i, (int64_t)p.B), p.N)));
+          const int e = max(x, seq_bound(p.q_ptr, min(i + 1, (int64_t)p.B), p.N));
+          bl = blocks(e - x);
+          un = units((int)min(i, (int64_t)p.B - 1), e - x);
+          carry = __builtin_amdgcn_readlane(e, 63);
+          f();
+        }
+      };
       int64_t all = 0;
-      int nb = 0, carry = 0;
-      for (int64_t base = 0; base < p.B; base += 64) {
-        const int64_t i = base + lane;
-        const int x = max(carry, wave_scan_max(seq_bound(p.q_ptr, min(i, (int64_t)p.B), p.N)));
-        const int e = max(x, seq_bound(p.q_ptr, min(i + 1, (int64_t)p.B), p.N));
-        nb += blocks(e - x);
-        all += (int64_t)blocks(e - x) * units((int)min(i, (int64_t)p.B - 1), e - x);
-        carry = __builtin_amdgcn_readlane(e, 63);
-      }
+      int nb = 0;
+      pass([&] {
+        all += (int64_t)bl * un;
+        nb += bl;
+      });
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
-        nb += __shfl_xor(nb, o);
         all += __shfl_xor(all, o);
+        nb += __shfl_xor(nb, o);
       }
-      const int64_t over = max(max(p.target - nb, nb / 4), 1);
-      L = (int)min((max((all + over - 1) / over, (int64_t)p.least) + step - 1) / step * step, (int64_t)L);
+      const int by = nb <= p.target ? p.target : (nb + 3) / 4;
+      L = (int)min((max((all + by - 1) / by, (int64_t)p.least) + step - 1) / step * step, (int64_t)(1 << 27));
+      const auto shares = [&] {
+        int sum = 0;
+        const auto add = [&] { sum += __builtin_amdgcn_readlane(wave_scan_sum(bl * cut(un)), 63); };
+        if (p.B <= 64)
+          add();  // as the pass left them
+        else
+          pass(add);
+        return sum;
+      };
+      if (nb <= p.target)  // ends: with L as long as the longest sequence there are nb parts
+        while (L < (1 << 27) && shares() > p.target) L += ((L >> 4) / step + 1) * step;
     }
-    const auto cut = [=](int u) { return max(1, (int)(((uint32_t)u + (uint32_t)L - 1) / (uint32_t)L)); };
     SeqPlace at;
     if (!seq_find(
             p.q_ptr, p.B, p.N,
