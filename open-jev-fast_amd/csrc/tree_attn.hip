@@ -119,10 +119,13 @@ __device__ __forceinline__ void load_q(const TreeParams& p, const Row& w, int fi
 
 // One workgroup's share: a row block of R packed rows of a sequence and a part of the sequence's units of 32 positions.
 // Work is shared out by the lengths as they are on the device: a sequence of u units has ceil(u / L) parts of equal length
-// for each of its row blocks. With no more row blocks, nb, than workgroups run at once (p.target, of a kv head), L is the
-// least that makes p.target parts at most, found in steps of a sixteenth from the mean on: one round of workgroups, all
-// about as long. With more, L is four times the mean, so that the longest sequences do not come last and alone: nb + nb / 4
-// parts at most. No part has fewer than p.least units unless its sequence has.
+// for each of its row blocks. With up to 64 sequences and no more row blocks, nb, than workgroups run at once (p.target, of
+// a kv head), L is the least that makes p.target parts at most, found in steps of a sixteenth from the mean on: one round
+// of workgroups, all about as long (16 x 12 over up to 8192, e4m3: 111 us with as many parts for a short sequence as for a
+// long one, 72 this way; 64 x 4 over 4096: 237 us with the L below, which no row block of equal ones divides, 162). With
+// more, L is `total` units over all row blocks by max(p.target - nb, nb / 4), so that there are max(p.target, nb + nb / 4)
+// parts at most and the longest sequences do not come last and alone. No part has fewer than p.least units unless its
+// sequence has.
 struct Part {
   int b, first, n, row0, rows, hk, parts, u0, u1;
   uint32_t slot;  // of the part's first row in the workspace; a row's parts lie HKV R slots apart
@@ -141,43 +144,29 @@ struct Part {
     int L = 0x7fffffff;
     const auto cut = [&](int u) { return max(1, (int)(((uint32_t)u + (uint32_t)L - 1) / (uint32_t)L)); };
     if (p.target > 0) {
-      int bl = 0, un = 0;  // row blocks and units of a lane's sequence
-      const auto pass = [&](auto f) {
-        int carry = 0;
-        for (int64_t base = 0; base < p.B; base += 64) {
-          const int64_t i = base + lane;
-          const int x = max(carry, wave_scan_max(seq_bound(p.q_ptr, min(i, (int64_t)p.B), p.N)));
-          const int e = max(x, seq_bound(p.q_ptr, min(i + 1, (int64_t)p.B), p.N));
-          bl = blocks(e - x);
-          un = units((int)min(i, (int64_t)p.B - 1), e - x);
-          carry = __builtin_amdgcn_readlane(e, 63);
-          f();
-        }
-      };
       int64_t all = 0;
-      int nb = 0;
-      pass([&] {
+      int nb = 0, carry = 0, bl = 0, un = 0;  // bl, un: row blocks and units of a lane's sequence
+      for (int64_t base = 0; base < p.B; base += 64) {
+        const int64_t i = base + lane;
+        const int x = max(carry, wave_scan_max(seq_bound(p.q_ptr, min(i, (int64_t)p.B), p.N)));
+        const int e = max(x, seq_bound(p.q_ptr, min(i + 1, (int64_t)p.B), p.N));
+        bl = blocks(e - x);
+        un = units((int)min(i, (int64_t)p.B - 1), e - x);
         all += (int64_t)bl * un;
         nb += bl;
-      });
+        carry = __builtin_amdgcn_readlane(e, 63);
+      }
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         all += __shfl_xor(all, o);
         nb += __shfl_xor(nb, o);
       }
-      const int by = nb <= p.target ? p.target : (nb + 3) / 4;
+      const bool search = p.B <= 64 && nb <= p.target;
+      const int by = search ? p.target : max(max(p.target - nb, nb / 4), 1);
       L = (int)min((max((all + by - 1) / by, (int64_t)p.least) + step - 1) / step * step, (int64_t)(1 << 27));
-      const auto shares = [&] {
-        int sum = 0;
-        const auto add = [&] { sum += __builtin_amdgcn_readlane(wave_scan_sum(bl * cut(un)), 63); };
-        if (p.B <= 64)
-          add();  // as the pass left them
-        else
-          pass(add);
-        return sum;
-      };
-      if (nb <= p.target)  // ends: with L as long as the longest sequence there are nb parts
-        while (L < (1 << 27) && shares() > p.target) L += ((L >> 4) / step + 1) * step;
+      if (search)  // ends: with L as long as the longest sequence there are nb parts
+        while (L < (1 << 27) && __builtin_amdgcn_readlane(wave_scan_sum(bl * cut(un)), 63) > p.target)
+          L += ((L >> 4) / step + 1) * step;
     }
     SeqPlace at;
     if (!seq_find(

@@ -284,6 +284,67 @@ def test_tree_attn_odd_pointers(ext, dev):
     assert bool((out[3:7] != 0).any(1).all())
 
 
+SHARES = [
+    # drafted, cached, HKV, G, D, page: how row blocks and positions are shared out
+    ([1 + i % 3 for i in range(70)], [(i * 37) % 200 for i in range(69)] + [3001], 16, 2, 128, 64),   # more blocks than a round
+    ([8 + i % 13 for i in range(20)], [(i * 53) % 700 for i in range(20)], 16, 4, 128, 64),           # 64 rows, one round
+    ([10] * 66, [100] * 65 + [1500], 16, 4, 128, 64),                                                 # 64 rows, more blocks
+    ([0] * 30 + [12, 3] + [0] * 60 + [20, 9], [5] * 30 + [900, 70] + [40] * 60 + [0, 333], 4, 6, 128, 32),  # empty ones
+    ([40, 70, 33], [650, 31, 1200], 2, 4, 256, 64),                                                   # 128 rows
+    ([1] * 64, [640] * 64, 4, 6, 256, 64),                                                            # equal, decoding
+]
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("case", range(len(SHARES)))
+def test_tree_attn_shares(ext, C, dev, case, fmt):
+    n, ctx, HKV, G, D, page = SHARES[case]
+    _say(f"case shares {case} {fmt}")
+    c = _tree_case(n, ctx, HKV, G, D, page, fmt, dev, seed=100 + case, ext=ext)
+    out, lse = _run_tree(ext, c, dev)
+    _check_tree(C, c, out, lse, D ** -0.5)
+
+
+def test_tree_attn_more_parts_than_lanes(ext, dev):
+    """A context of more parts than a wave has lanes; with no scale, every weight is the same: the values' mean."""
+    ctx, D = 20011, 128
+    c = _tree_case([1], [ctx], 1, 2, D, 64, "bf16", dev, seed=8, chain=True, ext=ext)
+    out, lse = _run_tree(ext, c, dev, 0.0)
+    t = torch.arange(ctx + 1)
+    v = c["vc"][c["table"][0].long()[t // 64], 0, t % 64].double()
+    # fp32 sums of 20012 values in some order, then a division and a rounding to bf16 (half a step is 2^-8)
+    bound = (v.abs().mean(0) * (ctx + 3) * 2.0 ** -24 + v.mean(0).abs() * 2.0 ** -8) * 1.01
+    for h in range(2):
+        assert bool(((out[0, h * D:(h + 1) * D].cpu().double() - v.mean(0)).abs() <= bound).all())
+    assert abs(lse[0, 0].item() - math.log(ctx + 1)) <= math.log(ctx + 1) * 2.0 ** -21
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,G", [(5, 2), (14, 4), (40, 5)])
+def test_tree_attn_values_not_finite(ext, dev, n, G, fmt):
+    """With no scale every weight is one: an infinity (a NaN in e4m3) in the context reaches every row, one in a drafted
+    token the rows that see it; in their own dim only, and nothing else changes. Row blocks of 16, 64 and 128."""
+    _say(f"case values {n} {G} {fmt}")
+    ctx, page, D = 700, 64, 256
+    c = _tree_case([n], [ctx], 2, G, D, page, fmt, dev, seed=n, ext=ext)
+    clean, clean_lse = _run_tree(ext, c, dev, 0.0)
+    see = [bool(int(c["bits"][i, 0]) >> 2 & 1) for i in range(n)]  # who sees drafted token 2
+    assert any(see) and not all(see)
+    raw, hi, lo = (torch.uint8, 0x7f, 0xff) if fmt == "e4m3" else (torch.int16, 0x7f80, 0xff80 - 65536)
+    for pos, d, x in ((5, 3, hi), (ctx + 2, 7, lo)):
+        c["vc"].view(raw)[int(c["table"][0, pos // page]), :, pos % page, d] = x
+    out, lse = _run_tree(ext, c, dev, 0.0)
+    got, want = out.view(n, 2 * G, D).float().cpu(), clean.view(n, 2 * G, D).float().cpu()
+    bad = torch.zeros(n, 2 * G, D, dtype=torch.bool)
+    bad[..., 3] = True
+    bad[torch.tensor(see), :, 7] = True
+    if fmt == "bf16":
+        assert bool((got[..., 3] == math.inf).all()) and bool((got[torch.tensor(see), :, 7] == -math.inf).all())
+    else:
+        assert bool(torch.isnan(got[bad]).all())
+    assert torch.equal(got[~bad], want[~bad]) and torch.equal(lse, clean_lse)
+
+
 def test_tree_attn_empty(ext, dev):
     c = _tree_case([2], [20], 1, 2, 128, 16, "bf16", dev, seed=7, ext=ext)
     c["q"], c["bits"] = c["q"][:, :0].contiguous(), c["bits"][:0].contiguous()
