@@ -500,6 +500,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   constexpr int R = 64 * CT, KF = D / 32, DT = D / 16, SB = D * (FP8 ? 1 : 2), RB = D * 2;  // bytes of a row: cache, LDS
   constexpr int PR = SB / 16, RL = 64 / PR, PL = 8 / RL;  // 16-byte pieces of a row, rows a wave's load takes, loads of 8 rows
   constexpr int TILE = 32 * RB;
+  constexpr bool EARLY = FP8 && CT * D < 512;
   __shared__ __attribute__((aligned(1024))) uint8_t buf[2][2][TILE];  // keys, values
   __shared__ __attribute__((aligned(16))) float sc[2][2][32];
   __shared__ int odd_any;
@@ -618,17 +619,35 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
       dma(0);
     }
   }
+  Pieces nk, nv;  // EARLY: the next unit's, fetched an iteration before they are stored
+  const auto fetch_early = [&](int u) {
+    if (!EARLY || u >= w.u1) return;
+    rows_of(u, e0, e1);
+    entries_of(u + 1);
+    fetch(p.kc, p.ks, nk);
+    fetch(p.vc, p.vs, nv);
+  };
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // Q is there: else the loop waits for it, and so for the loads behind it, each time
+  fetch_early(w.u0 + 1);
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&buf[0][0][0];
   for (int u = w.u0; u < w.u1; ++u) {
     const int h = (u - w.u0) & 1;
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows are there
+    if (!FP8) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows are there
     lds_barrier();
     const bool more = u + 1 < w.u1;
-    rows_of(u + 1, e0, e1);
-    entries_of(u + 2);
+    if (!EARLY) {
+      rows_of(u + 1, e0, e1);
+      entries_of(u + 2);
+    }
     const bool ok2 = in0, ok3 = in1;
     Pieces next;
-    if (FP8) {
+    if (EARLY) {
+      if (more) {
+        store_keys(nk, h ^ 1);
+        store_values(nv, u + 1, h ^ 1, ok2, ok3);
+      }
+      fetch_early(u + 2);
+    } else if (FP8) {
       if (more) fetch(p.kc, p.ks, next);
     } else if (more) {
       if (is_edge(u + 1, ok2 && ok3)) {
@@ -675,7 +694,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
         for (int ct = 0; ct < CT; ++ct) s[ct][t] *= kq;
       }
     }
-    if (FP8 && more) {  // the next unit's values take the registers that its keys leave
+    if (FP8 && !EARLY && more) {  // the next unit's values take the registers that its keys leave
       store_keys(next, h ^ 1);
       fetch(p.vc, p.vs, next);
     }
@@ -712,7 +731,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (FP8 && more) store_values(next, u + 1, h ^ 1, ok2, ok3);
+    if (FP8 && !EARLY && more) store_values(next, u + 1, h ^ 1, ok2, ok3);
     ok0 = ok2;
     ok1 = ok3;
   }
