@@ -501,8 +501,10 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   constexpr int PR = SB / 16, RL = 64 / PR, PL = 8 / RL;  // 16-byte pieces of a row, rows a wave's load takes, loads of 8 rows
   constexpr int TILE = 32 * RB;
   constexpr bool EARLY = FP8 && CT * D < 512;
+  constexpr int QL = FP8 && !EARLY ? 3 : 0;  // steps of the last 16 rows' Q that stay in LDS: as many as two workgroups have room for
   __shared__ __attribute__((aligned(1024))) uint8_t buf[2][2][TILE];  // keys, values
   __shared__ __attribute__((aligned(16))) float sc[2][2][32];
+  __shared__ __attribute__((aligned(16))) uint4 qbuf[QL > 0 ? QL : 1][QL > 0 ? 256 : 1];
   __shared__ int odd_any;
 
   Part w;
@@ -516,6 +518,8 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   for (int ct = 0; ct < CT; ++ct)
     load_q<D>(p, Row(p, wrow + ct * 16, w.rows, w.first, w.hk, threadIdx.x & 15), w.first, false, qf[ct]);
 
+#pragma unroll
+  for (int f = 0; f < QL; ++f) qbuf[f][threadIdx.x] = __builtin_bit_cast(uint4, qf[CT - 1][KF - QL + f]);
   struct Pieces {
     uint4 at[PL];
     float scale;
@@ -679,11 +683,14 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
 #pragma unroll
       for (int f = 0; f < KF; ++f) {
         if (f + 1 < KF) keys(f + 1);
+        bf16x8 ql;
+        if (f >= KF - QL) ql = __builtin_bit_cast(bf16x8, qbuf[QL > 0 ? f - (KF - QL) : 0][wave * 64 + lane]);
         __builtin_amdgcn_sched_barrier(0);  // one step ahead: more would take the outputs' registers
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          s[ct][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[f & 1][0], qf[ct][f], s[ct][0], 0, 0, 0);
-          s[ct][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[f & 1][1], qf[ct][f], s[ct][1], 0, 0, 0);
+          const bf16x8 b = ct == CT - 1 && f >= KF - QL ? ql : qf[ct][f];
+          s[ct][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[f & 1][0], b, s[ct][0], 0, 0, 0);
+          s[ct][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[f & 1][1], b, s[ct][1], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
