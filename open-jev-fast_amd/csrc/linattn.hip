@@ -111,7 +111,8 @@ __device__ __forceinline__ void one_token(const LinParams& p, int64_t row, int h
                    pack2(p.scale * (t.sq.z + t.qk * u.z), p.scale * (t.sq.w + t.qk * u.w)));
 }
 
-// One workgroup per (row, value head).
+// One workgroup per (row, value head). What bounds it: the states, read and written once (64 rows of 48 heads, 403 MB:
+// 82.7 us, 4.9 TB/s, where a large copy reaches 5.2); for one row the chain of a state's load, three sums and its store, 5 us.
 template <bool DELTA>
 __global__ void __launch_bounds__(256) linattn_step_k(LinParams p, float* state, const int32_t* __restrict__ slot) {
   __shared__ float red[4 * 32 * 12];
@@ -245,7 +246,8 @@ __device__ __forceinline__ bool odd_top(uint32_t top) { return (top & 0xffffu) >
 //     when the contraction runs in its order; P T likewise.
 // LDS holds the ten lower blocks of each matrix, rows of 20 floats (so that 16 rows' 16-byte reads meet every bank once).
 // What bounds it: the chain of one chunk (loads, scan, substitution, up to 19 block products on one wave), so what counts
-// is how many workgroups a CU holds: four, by LDS and registers.
+// is how many workgroups a CU holds: four, by LDS and registers (16384 tokens of 48 heads: 155 us; 206 with two; MFMAs busy
+// 17% of the time, waves waiting half of theirs). A single round of them takes 11 us: 288 tokens.
 template <bool DELTA>
 __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
   constexpr int LD = 20, BLK = 16 * LD;
@@ -583,6 +585,11 @@ __device__ __forceinline__ bool odd_values(const bf16x4 (&v)[4]) {  // one of th
 // and DMAs stay in flight.
 __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Few sequences: four workgroups a sequence and value head, each of two slices of 16 value dims, and for each slice a wave
+// with the state in its accumulators and a wave for the outputs and the DMAs, which works a chunk behind: the chain of a
+// chunk's products that need the state is all that the chunks wait for.
+// What bounds it: that chain, 2.1 us a chunk (16384 tokens of 48 heads: 550 us; 1090 with all of a slice in one wave), half
+// of it K, Q and the chunk's matrices out of LDS, half the new state's products; MFMAs are busy 17% of the time.
 template <bool DELTA>
 __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   constexpr int SL = 4;                  // workgroups of a head
@@ -837,7 +844,9 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 }
 
 // Many sequences: a workgroup of eight waves per sequence and value head, each with one slice and all of its work, so that
-// two waves a SIMD fill each other's gaps and what they share is loaded once a head. (Here the waves that read K^T and V
+// two waves a SIMD fill each other's gaps and what they share is loaded once a head: 16 sequences of up to 539 tokens, 48
+// heads, 120 us (163 with slices as above), MFMAs busy 29%, 284 MB of memory, the chunks' matrices (25 KB each) more than
+// half of them. (Here the waves that read K^T and V
 // transposed have DMAs in flight, and the builtin makes the compiler wait for those: the reads are written out, with the
 // wait for themselves in the same block, so that the registers are filled when it ends.)
 template <int X0, int X1, int X2, int X3>

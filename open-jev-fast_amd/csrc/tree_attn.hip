@@ -6,25 +6,34 @@
 //   s_p = scale q . k_p,  m = max s_p,  out = sum exp(s_p - m) v_p / sum exp(s_p - m),  lse = m + log sum exp(s_p - m)
 // over the positions seen; a row that sees nothing gives zeros and lse = -inf.
 //
-// Work layout. The G = HQ / HKV query heads of a kv head read the same keys, so their rows (token, head) are packed: a
-// workgroup takes a block of 16 CT packed rows of one sequence and kv head and a part of the positions. Its four waves
-// take the part's units of 32 positions in turn and are independent until the end:
-//   * S^T = K Q^T on 16x16x32 MFMA: the K rows are the A operand, straight from the cache into registers (a lane's 16
-//     bytes are 8 bf16 or 16 e4m3 values of one key; the e4m3 form orders the contraction accordingly, for Q too), Q stays
-//     in registers. A lane then holds one row's scores of 4 positions of each 16.
-//   * the softmax runs per lane: the maximum needs two shuffles, the sum none until the end, and the reference maximum
+// Work layout. The G = HQ / HKV query heads of a kv head read the same keys, so their rows (token, head) are packed, and a
+// workgroup takes a block of packed rows of one sequence and kv head and a part of the positions, in units of 32:
+//   * S^T = K Q^T on 16x16x32 MFMA, K rows as the A operand, Q in registers as B. A lane then holds one row's scores of 4
+//     positions of each 16.
+//   * the softmax runs per lane: the maximum needs two lane swaps, the sum none until the end, and the reference maximum
 //     only moves when it has grown by 2^8 (the weights stay below 2^8, well inside fp32 and bf16), so that the outputs are
 //     rarely rescaled;
 //   * O^T += V^T P^T: P^T is the B operand as the lane holds it, with the contraction in the order 4 of the first 16
-//     positions, 4 of the second; V^T comes from the wave's own LDS rows by transposing reads (ds_read_b64_tr_b16: 16
-//     lanes get 4 x 16 elements column by column), rows padded by 32 bytes so that the reads spread over the banks.
-// The loads of the next unit, keys and values, go into the registers that the present unit has just left and arrive
-// behind its products. P is rounded to bf16 as every operand of these products is (half a step, 2^-8 of each weight); the
-// sum of the weights and the outputs are fp32.
+//     positions, 4 of the second; V^T comes from LDS rows by transposing reads (ds_read_b64_tr_b16: 16 lanes get 4 x 16
+//     elements column by column).
+// P is rounded to bf16 as every operand of these products is (half a step, 2^-8 of each weight); the sum of the weights and
+// the outputs are fp32. e4m3 keys and values become bf16, which is exact; a position's scales go into its score and weight.
 // Units in which a row may not see every position (drafted ones, the sequence's end, pages outside the cache) also mask,
-// take the values of places that nobody sees as zeros and, where a value is not finite, add position by position, so that
-// a NaN reaches the rows that see it and no other.
-// Where sequences and row blocks are few, the positions are split over more workgroups, whose sums a second launch joins.
+// take the values of places that nobody sees as zeros and keep values that are not finite apart, so that a NaN reaches the
+// rows that see it and no other.
+// The positions are split over workgroups so that one round of them fills the GPU; a second launch joins the parts.
+//
+// Three kernels of rows, by the mean packed rows of a sequence (tree_plan). Times of tree_attn, D = 256, four kv heads of
+// six query heads, bf16 / e4m3, in blocks of 16, 64 and 128 rows:
+//   16 sequences of  1 over 4096 ( 6 rows):  49 / 33,   51 /  48,   52 /  70 us -> 16 (bf16: 5.3 TB/s of the cache)
+//                    4           (24 rows):  92 / 64,   54 /  49,   55 /  71    -> 64
+//                   12           (72 rows): 168 / 122,  92 / 105,   68 /  71    -> 128
+//   4 sequences of  64 over 8192 (384 rows): 302 / 216, 99 / 128,   84 / 104    -> 128
+// What bounds them now: a single row block, the stream of the cache (64 x 4 over 4096, bf16: 203 us, 5.3 TB/s); several
+// row blocks, the steps of a wave between barriers: in the 16 x 12 case of up to 8192 (e4m3, 67 us) MFMAs are busy 11% of
+// the time, waves wait for memory and barriers 38% and to issue 21% of theirs; in the 4 x 64 case of up to 16384 (bf16, 78
+// us) 23, 28 and 33%. Of the 76 us of that kernel 20 are there without a unit (the workgroups' start, Q, the parts' sums
+// to memory: 56 MB), 10 go without the DMAs, 8 without three quarters of the outputs' products, 3 without the exponentials.
 #include "gemm_common.h"
 
 #include <algorithm>
@@ -229,11 +238,11 @@ __device__ __forceinline__ float quarters_max(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Scaled scores of 32 positions, base two, -> weights (the B operand of the outputs' product, and for the rare path as they are), with the
-// rows' reference maxima, sums and outputs brought up to date. edge: seen() says which of the positions the row sees.
+// Scaled scores of 32 positions, base two, -> weights (the B operand of the outputs' product), with the rows' reference
+// maxima, sums and outputs brought up to date. edge: seen() says which of the positions the row sees.
 template <bool FP8, int DT, typename Scale, typename Seen>
-__device__ __forceinline__ void soft_weights(const f32x4 (&s)[2], Scale vscale,
-                                             bool edge, Seen seen, float& m, float& l, f32x4 (&acc)[DT], bf16x8& pf) {
+__device__ __forceinline__ void soft_weights(const f32x4 (&s)[2], Scale vscale, bool edge, Seen seen, float& m, float& l,
+                                             f32x4 (&acc)[DT], bf16x8& pf) {
   float w[8];
   const int g = (threadIdx.x & 63) >> 4;
   uint32_t see = ~0u;
@@ -418,7 +427,8 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
     if (u + 4 < w.u1) load(u + 4);
     bf16x8 pf;
     soft_weights<FP8, DT>(
-        s, [&](int t) { return vq[t]; }, edge, [&] { return rw.live ? there & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u; }, m, l, acc, pf);
+        s, [&](int t) { return vq[t]; }, edge,
+        [&] { return rw.live ? there & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u; }, m, l, acc, pf);
     add_values<RS, DT>(vl, pf, edge && __any(odd), acc);
   }
 
@@ -491,17 +501,25 @@ __device__ __forceinline__ int lane_anew() {
 }
 
 // Many rows: 64 CT packed rows a workgroup, 16 CT of them a wave; all take the part's units of 32 positions in order, from
-// LDS, where a wave brings 8 of a unit's rows of keys and of values. Rows are not padded: the 16-byte chunk j of key r lies
-// at place j ^ r % 8 of its row, the pair of chunks j of value r at j ^ r % 8, which spreads both kinds of reads over the
-// banks. A bf16 cache's unit is fetched by LDS DMA (each lane fetches the chunk that belongs where the DMA puts it) an
-// iteration ahead, an e4m3 cache's through registers, where it becomes bf16.
+// LDS, where a wave brings 8 of a unit's rows of keys and of values. Two workgroups a CU: one's products go on in the
+// other's waits. Rows are not padded: the 16-byte chunk j of key r lies at place j ^ r % 8 of its row, the pair of chunks j
+// of value r at j ^ r % 8, which spreads both kinds of reads over the banks. A bf16 cache's unit is fetched by LDS DMA
+// (each lane fetches the chunk that belongs where the DMA puts it) an iteration ahead; an e4m3 cache's goes through
+// registers, where it becomes bf16: fetched an iteration before it is stored where there are registers for it (EARLY),
+// else keys and values in turn through the same ones. A unit that is an edge goes through registers, too, with zeros for
+// values that are not finite; what those add to the rows that see them is an infinity or a NaN whatever the weight, and is
+// added at the end.
+// The main loop has no register to spare at D = 256, CT = 2 (128 for the outputs, 64 for Q), and a wait for a reload from
+// scratch memory waits for the DMAs before it (4 x 64 over 16384, with 45 registers in scratch: 262 us). Hence lane_anew,
+// the scores' operands one step ahead and no more, and QL.
 template <int D, bool FP8, int CT>
 __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   constexpr int R = 64 * CT, KF = D / 32, DT = D / 16, SB = D * (FP8 ? 1 : 2), RB = D * 2;  // bytes of a row: cache, LDS
   constexpr int PR = SB / 16, RL = 64 / PR, PL = 8 / RL;  // 16-byte pieces of a row, rows a wave's load takes, loads of 8 rows
   constexpr int TILE = 32 * RB;
   constexpr bool EARLY = FP8 && CT * D < 512;
-  constexpr int QL = FP8 && !EARLY ? 3 : 0;  // steps of the last 16 rows' Q that stay in LDS: as many as two workgroups have room for
+  // steps of the last 16 rows' Q that stay in LDS, as many as two workgroups have room for (16 x 12 over 4096: 81 -> 71 us)
+  constexpr int QL = FP8 && !EARLY ? 3 : 0;
   __shared__ __attribute__((aligned(1024))) uint8_t buf[2][2][TILE];  // keys, values
   __shared__ __attribute__((aligned(16))) float sc[2][2][32];
   __shared__ __attribute__((aligned(16))) uint4 qbuf[QL > 0 ? QL : 1][QL > 0 ? 256 : 1];
@@ -842,10 +860,10 @@ __global__ void __launch_bounds__(256) tree_join_k(TreeParams p, int R) {
 TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, int page) {
   TreePlan t{};
   const int64_t G = HQ / HKV, seqs = std::max<int64_t>(1, std::min<int64_t>(B, N)), mean = (N * G + seqs - 1) / seqs;
-  t.rows = mean <= 16 ? 16 : mean <= 64 ? 64 : 128;
+  t.rows = mean <= 16 ? 16 : mean <= 64 ? 64 : 128;  // times on both sides: at the top of this file
   // an upper bound of sum ceil(n_b G / rows) over the sequences with rows, which are `seqs` at most
   const int64_t blocks = (N * G + seqs * (t.rows - 1)) / t.rows, units = (max_pages * page + 31) / 32;
-  t.least = t.rows == 16 ? 4 : 8;
+  t.least = t.rows == 16 ? 4 : 8;  // a unit for each wave; as much work as the start of a part
   const int64_t at_once = (t.rows == 16 ? 256 : 512) * 256 / D;  // workgroups that the GPU holds
   t.target = units > t.least ? std::max<int64_t>(1, at_once / HKV) : 0;
   t.shares = t.target == 0 ? blocks
