@@ -4,7 +4,8 @@ out/down + residual + RMSNorm) as hand-written gfx950 HIP kernels behind a C-ABI
 Modules:
     _lib      ctypes binding of libojx.so (C-ABI)
     ext       the reference extension's projection-path functions (add_rmsnorm*, silu_mul*, act_tables) and the
-              fused projections (mm, mm_silu_mul, mm_residual_rmsnorm, mm_splitk_f32, pack_gate_up)
+              fused projections (mm, mm_silu_mul, mm_residual_rmsnorm, mm_splitk_f32, pack_gate_up), and the attention
+              cores (kv_cache_write / read, tree_attn, linattn_prompt / step)
     lt_ext    the reference's cuBLASLt extension surface (lt_setup / lt_matmul / lt2_*)
     fastproj  FastQwen35's projection dispatch (_mm, _res, _silu_mul, _skmm, _split, _tune)
     build     in-tree hipcc build of libojx.so
