@@ -895,8 +895,8 @@ int check_tree(int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t
     return fail(OJX_ERR_SHAPE, "bad max_pages=%lld (at most 2^31 positions)", (long long)max_pages);
   if (N * HQ >= (1LL << 24))
     return fail(OJX_ERR_SHAPE, "N=%lld rows of %d heads: too many for one call", (long long)N, HQ);
-  // workgroups of 256 threads; a launch has fewer than 2^32 threads
-  if (N > 0 && ojx::tree_plan(N, B, HQ, HKV, D, max_pages, page).shares * HKV >= (1LL << 24))
+  // workgroups of up to 512 threads; a launch has fewer than 2^32 threads
+  if (N > 0 && ojx::tree_plan(N, B, HQ, HKV, D, max_pages, page).shares * HKV >= (1LL << 23))
     return fail(OJX_ERR_SHAPE, "N=%lld rows of B=%d sequences: too many for one call", (long long)N, B);
   return OJX_OK;
 }

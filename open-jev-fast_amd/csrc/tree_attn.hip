@@ -513,21 +513,24 @@ __device__ __forceinline__ int lane_anew() {
 // scratch memory waits for the DMAs before it (4 x 64 over 16384, with 45 registers in scratch: 262 us). Hence lane_anew,
 // the scores' operands one step ahead and no more, and QL.
 template <int D, bool FP8, int CT>
-__global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
+__global__ void __launch_bounds__(512, 2) tree_wide_k(TreeParams p) {
   constexpr int R = 64 * CT, KF = D / 32, DT = D / 16, SB = D * (FP8 ? 1 : 2), RB = D * 2;  // bytes of a row: cache, LDS
   constexpr int PR = SB / 16, RL = 64 / PR, PL = 8 / RL;  // 16-byte pieces of a row, rows a wave's load takes, loads of 8 rows
   constexpr int TILE = 32 * RB;
   constexpr bool EARLY = FP8 && CT * D < 512;
   // steps of the last 16 rows' Q that stay in LDS, as many as two workgroups have room for (16 x 12 over 4096: 81 -> 71 us)
   constexpr int QL = FP8 && !EARLY ? 3 : 0;
-  __shared__ __attribute__((aligned(1024))) uint8_t buf[2][2][TILE];  // keys, values
-  __shared__ __attribute__((aligned(16))) float sc[2][2][32];
-  __shared__ __attribute__((aligned(16))) uint4 qbuf[QL > 0 ? QL : 1][QL > 0 ? 256 : 1];
+  __shared__ __attribute__((aligned(1024))) uint8_t bufs[2][2][2][TILE];  // of each four waves, two of keys and values
+  __shared__ __attribute__((aligned(16))) float scs[2][2][2][32];
+  __shared__ float2 sums[2][R];
+  __shared__ __attribute__((aligned(16))) uint4 qbuf[QL > 0 ? QL : 1][QL > 0 ? 512 : 1];
   __shared__ int odd_any;
 
   Part w;
   if (!w.find(p, R, D, 1)) return;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3, four = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  auto& buf = bufs[four];
+  auto& sc = scs[four];
   const int wrow = w.row0 + wave * 16 * CT;
   const Table table(p, w);
   const int full = min(w.ctx, w.total) >> 5;  // units below are seen by every row, if they are in the cache
@@ -624,19 +627,20 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   }
   if (threadIdx.x == 0) odd_any = 0;
   __syncthreads();
+  const int ua = w.u0 + four;  // the four waves' units: every other one
   bool ok0 = false, ok1 = false;  // of the unit at hand
-  if (w.u0 < w.u1) {
-    entries_of(w.u0);
-    rows_of(w.u0, e0, e1);
-    entries_of(w.u0 + 1);
+  if (ua < w.u1) {
+    entries_of(ua);
+    rows_of(ua, e0, e1);
+    entries_of(ua + 2);
     ok0 = in0;
     ok1 = in1;
-    if (FP8 || is_edge(w.u0, ok0 && ok1)) {
+    if (FP8 || is_edge(ua, ok0 && ok1)) {
       Pieces x, y;
       fetch(p.kc, p.ks, x);
       fetch(p.vc, p.vs, y);
       store_keys(x, 0);
-      store_values(y, w.u0, 0, ok0, ok1);
+      store_values(y, ua, 0, ok0, ok1);
     } else {
       dma(0);
     }
@@ -645,45 +649,46 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
   const auto fetch_early = [&](int u) {
     if (!EARLY || u >= w.u1) return;
     rows_of(u, e0, e1);
-    entries_of(u + 1);
+    entries_of(u + 2);
     fetch(p.kc, p.ks, nk);
     fetch(p.vc, p.vs, nv);
   };
   __builtin_amdgcn_s_waitcnt(0x0f70);  // Q is there: else the loop waits for it, and so for the loads behind it, each time
-  fetch_early(w.u0 + 1);
-  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&buf[0][0][0];
-  for (int u = w.u0; u < w.u1; ++u) {
-    const int h = (u - w.u0) & 1;
+  fetch_early(ua + 2);
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&bufs[0][0][0][0];
+  const int rounds = (w.u1 - w.u0 + 1) >> 1;  // of all eight waves
+  for (int i = 0; i < rounds; ++i) {
+    const int u = ua + 2 * i, h = i & 1;
     if (!FP8) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows are there
     lds_barrier();
-    const bool more = u + 1 < w.u1;
+    const bool more = u + 2 < w.u1;
     if (!EARLY) {
-      rows_of(u + 1, e0, e1);
-      entries_of(u + 2);
+      rows_of(u + 2, e0, e1);
+      entries_of(u + 4);
     }
     const bool ok2 = in0, ok3 = in1;
     Pieces next;
     if (EARLY) {
       if (more) {
         store_keys(nk, h ^ 1);
-        store_values(nv, u + 1, h ^ 1, ok2, ok3);
+        store_values(nv, u + 2, h ^ 1, ok2, ok3);
       }
-      fetch_early(u + 2);
+      fetch_early(u + 4);
     } else if (FP8) {
       if (more) fetch(p.kc, p.ks, next);
     } else if (more) {
-      if (is_edge(u + 1, ok2 && ok3)) {
+      if (is_edge(u + 2, ok2 && ok3)) {
         Pieces x, y;
         fetch(p.kc, p.ks, x);
         fetch(p.vc, p.vs, y);
         store_keys(x, h ^ 1);
-        store_values(y, u + 1, h ^ 1, ok2, ok3);
+        store_values(y, u + 2, h ^ 1, ok2, ok3);
         __builtin_amdgcn_s_waitcnt(0x0f70);  // said here: else the compiler waits behind the DMAs of the other path, too
       } else {
         dma(h ^ 1);
       }
     }
-    const bool live = wrow < w.rows;
+    const bool live = wrow < w.rows && u < w.u1;
     f32x4 s[CT][2];
     if (live) {
       const int lane = lane_anew(), g = lane >> 4, c = lane & 15;
@@ -702,7 +707,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
       for (int f = 0; f < KF; ++f) {
         if (f + 1 < KF) keys(f + 1);
         bf16x8 ql;
-        if (f >= KF - QL) ql = __builtin_bit_cast(bf16x8, qbuf[QL > 0 ? f - (KF - QL) : 0][wave * 64 + lane]);
+        if (f >= KF - QL) ql = __builtin_bit_cast(bf16x8, qbuf[QL > 0 ? f - (KF - QL) : 0][four * 256 + wave * 64 + lane]);
         __builtin_amdgcn_sched_barrier(0);  // one step ahead: more would take the outputs' registers
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
@@ -737,7 +742,7 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
               return rw.live ? existing(w.total - p0, ok0, ok1) & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u;
             },
             m[ct], l[ct], acc[ct], pf[ct]);
-      const uint32_t at = lds + (h * 2 + 1) * TILE + vrow * RB + (vrow & 7) * 32 + (c & 3) * 8;
+      const uint32_t at = lds + (four * 4 + h * 2 + 1) * TILE + vrow * RB + (vrow & 7) * 32 + (c & 3) * 8;
 #pragma unroll
       for (int d0 = 0; d0 < DT; d0 += 4) {
         bf16x4 lo[4], hi[4];
@@ -756,33 +761,53 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (FP8 && !EARLY && more) store_values(next, u + 1, h ^ 1, ok2, ok3);
+    if (FP8 && !EARLY && more) store_values(next, u + 2, h ^ 1, ok2, ok3);
     ok0 = ok2;
     ok1 = ok3;
   }
 
+  // each four waves leave half of the dims to the others and join the other half of both sums
+  constexpr int HT = DT / 2;
   const int lane = lane_anew(), g = lane >> 4, c = lane & 15;
+  lds_barrier();
+  f32x4* const give = reinterpret_cast<f32x4*>(&bufs[0][0][0][0]) + (four * 4 + wave) * CT * HT * 64 + lane;
+  const f32x4* const take = reinterpret_cast<const f32x4*>(&bufs[0][0][0][0]) + ((four ^ 1) * 4 + wave) * CT * HT * 64 + lane;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     l[ct] += __shfl_xor(l[ct], 16);
     l[ct] += __shfl_xor(l[ct], 32);
+    if (g == 0) sums[four][(wave * CT + ct) * 16 + c] = make_float2(m[ct], l[ct]);
+#pragma unroll
+    for (int d = 0; d < HT; ++d) give[(ct * HT + d) * 64] = four ? acc[ct][d] : acc[ct][d + HT];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
     const Row rw(p, wrow + ct * 16, w.rows, w.first, w.hk, c);
     if (!rw.live) continue;
+    const float2 other = sums[four ^ 1][(wave * CT + ct) * 16 + c];
+    const float top = fmaxf(m[ct], other.x);
+    // four waves without a reference have a sum only where every score was NaN
+    const float fa = m[ct] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[ct] - top);
+    const float fb = other.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(other.x - top);
+    const float sum = four ? other.y * fb + l[ct] * fa : l[ct] * fa + other.y * fb;  // the same on both sides
     const int64_t nh = (int64_t)(w.first + rw.tok) * p.HQ + rw.head, i = w.slot + (wave * CT + ct) * 16 + c;
-    const float inv = l[ct] == 0.f ? 0.f : 1.f / l[ct];
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const f32x4 o = acc[ct][d];
+    for (int d = 0; d < HT; ++d) {
+      const f32x4 mine = four ? acc[ct][d + HT] : acc[ct][d];
+      const f32x4 o = mine * fa + take[(ct * HT + d) * 64] * fb;
+      const int at = (four * HT + d) * 16 + g * 4;
       if (w.parts > 1)
-        *reinterpret_cast<f32x4*>(p.part + i * D + d * 16 + g * 4) = o;
+        *reinterpret_cast<f32x4*>(p.part + i * D + at) = o;
       else
-        *reinterpret_cast<uint2*>(p.out + nh * D + d * 16 + g * 4) = make_uint2(cvt_pk2(o[0] * inv, o[1] * inv), cvt_pk2(o[2] * inv, o[3] * inv));
+        *reinterpret_cast<uint2*>(p.out + nh * D + at) = make_uint2(cvt_pk2(o[0] * inv, o[1] * inv), cvt_pk2(o[2] * inv, o[3] * inv));
     }
-    if (g != 0) continue;
+    if (g != 0 || four != 0) continue;
     if (w.parts > 1)
-      p.ml[i] = make_float2(m[ct], l[ct]);
+      p.ml[i] = make_float2(top, sum);
     else if (p.lse != nullptr)
-      p.lse[nh] = l[ct] == 0.f ? -INFINITY : (m[ct] + log2f(l[ct])) * kLn2;
+      p.lse[nh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
   }
 
   if (odd_any == 0) return;
@@ -803,8 +828,8 @@ __global__ void __launch_bounds__(256, 2) tree_wide_k(TreeParams p) {
         if (!(see >> key & 1)) continue;
         const int64_t v = (table.row(2 * u + (key >> 4), key >> 4 ? e1 : e0) + (key & 15)) * D;
 #pragma unroll 1
-        for (int i = 0; i < D / 4; ++i) {
-          const int d = (i >> 2) * 16 + g * 4 + (i & 3);  // what this lane has written
+        for (int i = 0; i < D / 8; ++i) {
+          const int d = (four * HT + (i >> 2)) * 16 + g * 4 + (i & 3);  // what this lane has written
           const float x = FP8 ? bf2f(cvt_fp8x2(static_cast<const uint8_t*>(p.vc)[v + d], false) & 0xffffu)
                               : bf2f(static_cast<const uint16_t*>(p.vc)[v + d]);
           if (fabsf(x) < INFINITY) continue;
@@ -864,7 +889,7 @@ TreePlan tree_plan(int64_t N, int B, int HQ, int HKV, int D, int64_t max_pages, 
   // an upper bound of sum ceil(n_b G / rows) over the sequences with rows, which are `seqs` at most
   const int64_t blocks = (N * G + seqs * (t.rows - 1)) / t.rows, units = (max_pages * page + 31) / 32;
   t.least = t.rows == 16 ? 4 : 8;  // a unit for each wave; as much work as the start of a part
-  const int64_t at_once = (t.rows == 16 ? 256 : 512) * 256 / D;  // workgroups that the GPU holds
+  const int64_t at_once = t.rows == 128 ? 256 : 256 * 256 / D;  // workgroups that the GPU holds
   t.target = units > t.least ? std::max<int64_t>(1, at_once / HKV) : 0;
   t.shares = t.target == 0 ? blocks
                            : std::min<int64_t>(std::max<int64_t>(t.target, blocks + blocks / 4 + 1),
@@ -881,7 +906,7 @@ static void (*tree_kernel(int rows))(TreeParams) {
 hipError_t launch_tree_attn(const TreeParams& p, const TreePlan& t, int D, bool fp8, hipStream_t st) {
   const auto kernel = D == 256 ? (fp8 ? tree_kernel<256, true>(t.rows) : tree_kernel<256, false>(t.rows))
                                : (fp8 ? tree_kernel<128, true>(t.rows) : tree_kernel<128, false>(t.rows));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(t.shares * p.HKV)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(t.shares * p.HKV)), dim3(t.rows == 16 ? 256 : 512), 0, st, p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || t.target == 0) return err;
   hipLaunchKernelGGL(D == 256 ? tree_join_k<256> : tree_join_k<128>, dim3((unsigned)((p.N * p.HQ + 3) / 4)), dim3(256),
