@@ -588,8 +588,8 @@ __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcn
 // Few sequences: four workgroups a sequence and value head, each of two slices of 16 value dims, and for each slice a wave
 // with the state in its accumulators and a wave for the outputs and the DMAs, which works a chunk behind: the chain of a
 // chunk's products that need the state is all that the chunks wait for.
-// What bounds it: that chain, 2.1 us a chunk (16384 tokens of 48 heads: 550 us; 1090 with all of a slice in one wave), half
-// of it K, Q and the chunk's matrices out of LDS, half the new state's products; MFMAs are busy 17% of the time.
+// What bounds it: that chain, 2 us a chunk (16384 tokens of 48 heads: 509 us; over 800 with all of a slice in one wave),
+// half of it K, Q and the chunk's matrices out of LDS, half the new state's products; MFMAs are busy 18% of the time.
 template <bool DELTA>
 __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   constexpr int SL = 4;                  // workgroups of a head

@@ -23,17 +23,17 @@
 // rows that see it and no other.
 // The positions are split over workgroups so that one round of them fills the GPU; a second launch joins the parts.
 //
-// Three kernels of rows, by the mean packed rows of a sequence (tree_plan). Times of tree_attn, D = 256, four kv heads of
-// six query heads, bf16 / e4m3, in blocks of 16, 64 and 128 rows:
-//   16 sequences of  1 over 4096 ( 6 rows):  49 / 33,   51 /  48,   52 /  70 us -> 16 (bf16: 5.3 TB/s of the cache)
-//                    4           (24 rows):  92 / 64,   54 /  49,   55 /  71    -> 64
-//                   12           (72 rows): 168 / 122,  92 / 105,   68 /  71    -> 128
-//   4 sequences of  64 over 8192 (384 rows): 302 / 216, 99 / 128,   84 / 104    -> 128
-// What bounds them now: a single row block, the stream of the cache (64 x 4 over 4096, bf16: 203 us, 5.3 TB/s); several
-// row blocks, the steps of a wave between barriers: in the 16 x 12 case of up to 8192 (e4m3, 67 us) MFMAs are busy 11% of
-// the time, waves wait for memory and barriers 38% and to issue 21% of theirs; in the 4 x 64 case of up to 16384 (bf16, 78
-// us) 23, 28 and 33%. Of the 76 us of that kernel 20 are there without a unit (the workgroups' start, Q, the parts' sums
-// to memory: 56 MB), 10 go without the DMAs, 8 without three quarters of the outputs' products, 3 without the exponentials.
+// Three sizes of row blocks, by the mean packed rows of a sequence (tree_plan). Times of tree_attn, D = 256, four kv heads
+// of six query heads, bf16 / e4m3, in blocks of 16, 64 and 128 rows:
+//   16 sequences of  1 over 4096 ( 6 rows):  49 /  33,   50 /  46,  53 /  66 us -> 16
+//                    4           (24 rows):  92 /  64,   52 /  47,  55 /  66    -> 64
+//                    8           (48 rows):  91 /  67,   54 /  50,  59 /  71    -> 64
+//                   12           (72 rows): 168 / 122,   71 /  81,  64 /  74    -> 128
+//   4 sequences of  64 over 8192 (384 rows): 302 / 216, 116 / 146,  82 / 107    -> 128
+// What bounds them now: a single row block of a bf16 cache, its stream (64 x 4 over 4096: 194 us, 5.5 TB/s); else the steps
+// of a wave between barriers: in the 16 x 12 case of up to 8192 (e4m3, 69 us) MFMAs are busy 10% of the time, waves wait
+// for memory and barriers 40% and to issue 21% of theirs; in the 4 x 64 case of up to 16384 (bf16, 77 us) 22, 34 and 31%.
+// Reading operands further ahead than the loops do changes neither.
 #include "gemm_common.h"
 
 #include <algorithm>
@@ -131,7 +131,7 @@ __device__ __forceinline__ void load_q(const TreeParams& p, const Row& w, int fi
 // for each of its row blocks. With up to 64 sequences and no more row blocks, nb, than workgroups run at once (p.target, of
 // a kv head), L is the least that makes p.target parts at most, found in steps of a sixteenth from the mean on: one round
 // of workgroups, all about as long (16 x 12 over up to 8192, e4m3: 111 us with as many parts for a short sequence as for a
-// long one, 72 this way; 64 x 4 over 4096: 237 us with the L below, which no row block of equal ones divides, 162). With
+// long one, 72 this way; 64 x 4 over 4096: 237 us with the L below, which equal row blocks fill badly, 162). With
 // more, L is `total` units over all row blocks by max(p.target - nb, nb / 4), so that there are max(p.target, nb + nb / 4)
 // parts at most and the longest sequences do not come last and alone. No part has fewer than p.least units unless its
 // sequence has.
@@ -500,10 +500,12 @@ __device__ __forceinline__ int lane_anew() {
   return lane & 63;  // known not to be negative: shifts, not divisions
 }
 
-// Many rows: 64 CT packed rows a workgroup, 16 CT of them a wave; all take the part's units of 32 positions in order, from
-// LDS, where a wave brings 8 of a unit's rows of keys and of values. Two workgroups a CU: one's products go on in the
-// other's waits. Rows are not padded: the 16-byte chunk j of key r lies at place j ^ r % 8 of its row, the pair of chunks j
-// of value r at j ^ r % 8, which spreads both kinds of reads over the banks. A bf16 cache's unit is fetched by LDS DMA
+// Many rows: 64 CT packed rows a workgroup of eight waves. Four of them take every other unit of 32 positions of the part,
+// the other four the units between; a wave has 16 CT of the rows, and brings 8 of its unit's rows of keys and of values to
+// LDS for its four. At the end the two sums of each row are joined through LDS, so that one part goes to memory (with four
+// waves a workgroup and two workgroups a CU: 16 x 16 over 4096 75 us where this takes 67, 4 x 64 of up to 16384 78 and 77).
+// Rows are not padded: the 16-byte chunk j of key r lies at place j ^ r % 8 of its row, the pair of chunks j of value r at
+// j ^ r % 8, which spreads both kinds of reads over the banks. A bf16 cache's unit is fetched by LDS DMA
 // (each lane fetches the chunk that belongs where the DMA puts it) an iteration ahead; an e4m3 cache's goes through
 // registers, where it becomes bf16: fetched an iteration before it is stored where there are registers for it (EARLY),
 // else keys and values in turn through the same ones. A unit that is an edge goes through registers, too, with zeros for

@@ -345,6 +345,26 @@ def test_tree_attn_values_not_finite(ext, dev, n, G, fmt):
     assert torch.equal(got[~bad], want[~bad]) and torch.equal(lse, clean_lse)
 
 
+@pytest.mark.parametrize("n,D", [(1, 256), (6, 128), (30, 256)])
+def test_tree_attn_graph_of_growing_contexts(ext, dev, n, D):
+    """One captured call, replayed while the contexts on the device grow and shrink: lengths are looked at on the device,
+    so every replay is the eager call's result for the lengths of the moment."""
+    c = _tree_case([n, n], [900, 1500], 2, 4, D, 64, "bf16", dev, seed=n, ext=ext)
+    d = {x: None if t is None else t.to(dev) for x, t in c.items()}
+    call = lambda: ext.tree_attn(d["q"], d["kc"], d["vc"], d["table"], d["ctx"], d["q_ptr"], d["bits"], want_lse=True)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = call()
+    for ctx in ([900, 1500], [0, 31], [17, 1500], [899, 2], [900, 1499]):
+        d["ctx"].copy_(torch.tensor(ctx, dtype=torch.int32))
+        want, want_lse = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
 def test_tree_attn_empty(ext, dev):
     c = _tree_case([2], [20], 1, 2, 128, 16, "bf16", dev, seed=7, ext=ext)
     c["q"], c["bits"] = c["q"][:, :0].contiguous(), c["bits"][:0].contiguous()
