@@ -27,7 +27,7 @@ __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t
 // Where row `slot` of head h lies in the cache, in rows; slots outside the cache give -1.
 __device__ __forceinline__ int64_t cache_row(int64_t slot, int h, int HKV, int64_t rows, int page) {
   if (slot < 0 || slot >= rows) return -1;
-  const int64_t p = slot / page;
+  const int64_t p = rows >> 32 == 0 ? (int64_t)((uint32_t)slot / (uint32_t)page) : slot / page;
   return (p * HKV + h) * page + (slot - p * page);
 }
 
@@ -37,15 +37,13 @@ __global__ void __launch_bounds__(256) kv_write_k(const uint16_t* __restrict__ k
                                                   void* vc, float* ks, float* vs, int64_t rows, int page) {
   constexpr int L = kRowLanes<D>, R = 256 / L;
   const int l = threadIdx.x % L;
-  const int64_t tasks = 2 * HKV * N;
-  for (int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / L; t < tasks; t += (int64_t)gridDim.x * R) {
-    const bool isv = t >= HKV * N;
-    const int64_t u = isv ? t - HKV * N : t;  // (head, token) in the order of the input
-    const int h = (int)(u / N);
-    const int64_t n = u - h * N;
+  const bool isv = blockIdx.y >= HKV;
+  const int h = isv ? blockIdx.y - HKV : blockIdx.y;
+  const uint16_t* const from = (isv ? v : k) + (int64_t)h * N * D + l * 8;
+  for (int64_t n = (int64_t)blockIdx.x * R + threadIdx.x / L; n < N; n += (int64_t)gridDim.x * R) {
+    const uint4 x = *reinterpret_cast<const uint4*>(from + n * D);  // not behind the slot's load
     const int64_t row = cache_row(slots[n], h, HKV, rows, page);
     if (row < 0) continue;  // the whole row's lanes
-    const uint4 x = *reinterpret_cast<const uint4*>((isv ? v : k) + u * D + l * 8);
     if (!FP8) {
       *reinterpret_cast<uint4*>(static_cast<uint16_t*>(isv ? vc : kc) + row * D + l * 8) = x;
       continue;
@@ -89,12 +87,10 @@ __global__ void __launch_bounds__(256) kv_read_k(const void* __restrict__ kc, co
                                                  int page) {
   constexpr int L = kRowLanes<D>, R = 256 / L;
   const int l = threadIdx.x % L;
-  const int64_t tasks = 2 * HKV * N;
-  for (int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / L; t < tasks; t += (int64_t)gridDim.x * R) {
-    const bool isv = t >= HKV * N;
-    const int64_t u = isv ? t - HKV * N : t;
-    const int h = (int)(u / N);
-    const int64_t n = u - h * N;
+  const bool isv = blockIdx.y >= HKV;
+  const int h = isv ? blockIdx.y - HKV : blockIdx.y;
+  uint16_t* const to = (isv ? v : k) + (int64_t)h * N * D + l * 8;
+  for (int64_t n = (int64_t)blockIdx.x * R + threadIdx.x / L; n < N; n += (int64_t)gridDim.x * R) {
     const int64_t row = cache_row(slots[n], h, HKV, rows, page);
     uint4 o = make_uint4(0u, 0u, 0u, 0u);
     if (row >= 0) {
@@ -109,13 +105,14 @@ __global__ void __launch_bounds__(256) kv_read_k(const void* __restrict__ kc, co
                        pack2(__builtin_amdgcn_cvt_f32_fp8(x.y, 2) * s, __builtin_amdgcn_cvt_f32_fp8(x.y, 3) * s));
       }
     }
-    *reinterpret_cast<uint4*>((isv ? v : k) + u * D + l * 8) = o;
+    *reinterpret_cast<uint4*>(to + n * D) = o;
   }
 }
 
-unsigned kv_grid(int64_t N, int HKV, int D) {
+// Token blocks, and a kv head's keys or values; at most about 16384 workgroups.
+dim3 kv_grid(int64_t N, int HKV, int D) {
   const int64_t per = 256 / (D / 8);
-  return (unsigned)std::min<int64_t>((2 * N * HKV + per - 1) / per, 8192);
+  return dim3((unsigned)std::min<int64_t>((N + per - 1) / per, std::max(1, 8192 / HKV)), (unsigned)(2 * HKV));
 }
 
 }  // namespace
@@ -125,7 +122,7 @@ hipError_t launch_kv_write(const uint16_t* k, const uint16_t* v, const int64_t* 
                            hipStream_t st) {
   const auto kernel = D == 256 ? (fp8 ? kv_write_k<256, true> : kv_write_k<256, false>)
                                : (fp8 ? kv_write_k<128, true> : kv_write_k<128, false>);
-  hipLaunchKernelGGL(kernel, dim3(kv_grid(N, HKV, D)), dim3(256), 0, st, k, v, slots, N, HKV, kc, vc, ks, vs, rows,
+  hipLaunchKernelGGL(kernel, kv_grid(N, HKV, D), dim3(256), 0, st, k, v, slots, N, HKV, kc, vc, ks, vs, rows,
                      page);
   return hipGetLastError();
 }
@@ -135,7 +132,7 @@ hipError_t launch_kv_read(const void* kc, const void* vc, const float* ks, const
                           hipStream_t st) {
   const auto kernel = D == 256 ? (fp8 ? kv_read_k<256, true> : kv_read_k<256, false>)
                                : (fp8 ? kv_read_k<128, true> : kv_read_k<128, false>);
-  hipLaunchKernelGGL(kernel, dim3(kv_grid(N, HKV, D)), dim3(256), 0, st, kc, vc, ks, vs, slots, N, HKV, k, v, rows,
+  hipLaunchKernelGGL(kernel, kv_grid(N, HKV, D), dim3(256), 0, st, kc, vc, ks, vs, slots, N, HKV, k, v, rows,
                      page);
   return hipGetLastError();
 }
