@@ -6,10 +6,10 @@
 // the rounding to four significant bits; with a scale that is no power of two the quotient would be rounded twice, and
 // e4m3 is a floating format: a larger share of its range used does not make its values more exact.
 //
-// Both directions move each row once. 16384 tokens of four heads of 256, 101 MB: read back in 18.7 us, 5.4 TB/s, as fast
-// as a large copy. Written in 27.3 us, 3.7 TB/s: the scale needs the whole row before the first value can be stored, so a
-// wave's chain is a load, the row's maximum over its lanes and a store; waves wait 47% of their time. A few rows cost the
-// launch: 3.2 us for 64 tokens.
+// Both directions move each row once. 16384 tokens of four heads of 256, 101 MB: read back in 17.4 us, 5.8 TB/s, as fast
+// as a large copy. Written in 22.5 us, 4.5 TB/s: the scale needs the whole row before the first value can be stored, so a
+// wave's chain is a load, the row's maximum over its lanes and a store (24.0 us with the maximum through LDS, 27.3 with the
+// values loaded behind the slots and 64-bit divisions for both). A few rows cost the launch: 2.8 us for 64 tokens.
 #include "ojx_internal.h"
 
 #include <algorithm>
@@ -29,6 +29,20 @@ __device__ __forceinline__ int64_t cache_row(int64_t slot, int h, int HKV, int64
   if (slot < 0 || slot >= rows) return -1;
   const int64_t p = rows >> 32 == 0 ? (int64_t)((uint32_t)slot / (uint32_t)page) : slot / page;
   return (p * HKV + h) * page + (slot - p * page);
+}
+
+// The largest value of a row's lanes, in each: rotations within 16 lanes, then a swap of the two halves of 32.
+template <int L>
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+#define OJX_ROR(n) x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x120 + (n), 0xf, 0xf, true))
+  OJX_ROR(8);
+  OJX_ROR(4);
+  OJX_ROR(2);
+  OJX_ROR(1);
+#undef OJX_ROR
+  if (L == 16) return x;
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return max(a[0], a[1]);
 }
 
 template <int D, bool FP8>
@@ -55,8 +69,7 @@ __global__ void __launch_bounds__(256) kv_write_k(const uint16_t* __restrict__ k
       const uint32_t a = w[i] & 0x7fffu, b = (w[i] >> 16) & 0x7fffu;
       top = max(top, max(a < 0x7f80u ? a : 0u, b < 0x7f80u ? b : 0u));
     }
-#pragma unroll
-    for (int off = L / 2; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+    top = row_max<L>(top);
     // top = 2^(E - 127) (1 + m / 128) and 448 = 2^8 * 1.75: one exponent more where 1 + m / 128 > 1.75
     int e = (int)(top >> 7) - 127 - 8 + ((top & 0x7f) > 96 ? 1 : 0);
     e = top == 0 ? 0 : max(e, -126);
