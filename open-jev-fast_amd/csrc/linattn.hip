@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 
 // Many sequences: a workgroup of eight waves per sequence and value head, each with one slice and all of its work, so that
 // two waves a SIMD fill each other's gaps and what they share is loaded once a head: 16 sequences of up to 539 tokens, 48
-// heads, 120 us (163 with slices as above), MFMAs busy 29%, 284 MB of memory, the chunks' matrices (25 KB each) more than
+// heads, 120 us (163 with slices as above), MFMAs busy 29%, 246 MB of memory, the chunks' matrices (25 KB each) nearly
 // half of them. (Here the waves that read K^T and V
 // transposed have DMAs in flight, and the builtin makes the compiler wait for those: the reads are written out, with the
 // wait for themselves in the same block, so that the registers are filled when it ends.)
@@ -892,8 +892,11 @@ __global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t sq = blockIdx.x / p.HV;
-  const int h = blockIdx.x - (int)(sq * p.HV), hk = h / (p.HV / p.HK);
+  // the value heads of a key head on one XCD, as above (163 -> 161 us, 176 -> 128 MB read)
+  const uint32_t b = blockIdx.x, per = p.HV / p.HK, whole = (uint32_t)p.S * p.HK / 8 * (8 * per);
+  const uint32_t wg = b < whole ? (b / (8 * per) * 8 + b % 8) * per + b / 8 % per : b;
+  const int64_t sq = wg / p.HV;
+  const int h = wg - (int)(sq * p.HV), hk = h / per;
   if (sq == p.S) return zero_rows(p, h);
   SeqPlace place;
   if (!seq_find(p.seq_ptr, p.S, p.R, seq_chunks, [=](int i, int) { return i == (int)sq; }, place)) return;
