@@ -291,19 +291,25 @@ __device__ __forceinline__ float weight_of(bf16x8 pf, int key) {
   return bf2f((uint32_t)__shfl((int)(slot & 1 ? z >> 16 : z & 0xffffu), from));
 }
 
-// O^T += V^T P^T over 32 positions from LDS rows of RS values; one by one where a value is not finite, so that a weight of
-// zero takes nothing.
-template <int RS, int DT>
-__device__ __forceinline__ void add_values(const uint16_t* vl, bf16x8 pf, bool odd, f32x4 (&acc)[DT]) {
+// O^T += V^T P^T over 32 positions from LDS rows of RS values; one by one where a value is not finite, so that a row takes
+// nothing from a position that it does not see (seen() gives those that it does). From one that it sees, a value that is not
+// finite goes in whatever the weight, also where that is too small for fp32: an infinity keeps its sign.
+template <int RS, int DT, typename Seen>
+__device__ __forceinline__ void add_values(const uint16_t* vl, bf16x8 pf, bool odd, Seen seen, f32x4 (&acc)[DT]) {
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   if (odd) {
+    const uint32_t see = seen();
 #pragma unroll 1
     for (int key = 0; key < 32; ++key) {
       const float wk = weight_of(pf, key);
+      const bool on = see >> key & 1;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[d][r] += wk == 0.f ? 0.f : wk * bf2f(vl[key * RS + d * 16 + g * 4 + r]);
+        for (int r = 0; r < 4; ++r) {
+          const float x = bf2f(vl[key * RS + d * 16 + g * 4 + r]);
+          acc[d][r] += !on ? 0.f : wk == 0.f && !(fabsf(x) < INFINITY) ? x : wk * x;
+        }
     }
     return;
   }
@@ -426,10 +432,9 @@ __global__ void __launch_bounds__(256, 1) tree_narrow_k(TreeParams p) {
     }
     if (u + 4 < w.u1) load(u + 4);
     bf16x8 pf;
-    soft_weights<FP8, DT>(
-        s, [&](int t) { return vq[t]; }, edge,
-        [&] { return rw.live ? there & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u; }, m, l, acc, pf);
-    add_values<RS, DT>(vl, pf, edge && __any(odd), acc);
+    const auto seen = [&] { return rw.live ? there & seen32(p, rw.words, rw.tok, p0 - w.ctx) : 0u; };
+    soft_weights<FP8, DT>(s, [&](int t) { return vq[t]; }, edge, seen, m, l, acc, pf);
+    add_values<RS, DT>(vl, pf, edge && __any(odd), seen, acc);
   }
 
   // the four waves' sums, each brought to the largest reference

@@ -345,6 +345,35 @@ def test_tree_attn_values_not_finite(ext, dev, n, G, fmt):
     assert torch.equal(got[~bad], want[~bad]) and torch.equal(lse, clean_lse)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,G", [(5, 2), (14, 4), (40, 5)])
+def test_tree_attn_values_not_finite_of_no_weight(ext, dev, n, G, fmt):
+    """A value that is not finite reaches every row that sees it, also where its weight is too small for fp32: scores of
+    -256 beside scores around zero. Of a drafted token and of the context's last one; row blocks of 16, 64 and 128."""
+    _say(f"case no weight {n} {G} {fmt}")
+    ctx, page, D = 700, 64, 256
+    c = _tree_case([n], [ctx], 2, G, D, page, fmt, dev, seed=n, ext=ext)
+    c["q"].fill_(1)
+    at = [(int(c["table"][0, pos // page]), pos % page) for pos in (ctx + 2, ctx - 1)]
+    for t, o in at:
+        c["kc"].view(torch.uint8 if fmt == "e4m3" else torch.int16)[t, :, o] = 0xd8 if fmt == "e4m3" else 0xc180 - 65536  # -16
+        if fmt == "e4m3":
+            c["ks"][t, :, o] = 1.0
+    clean, clean_lse = _run_tree(ext, c, dev)
+    see = torch.tensor([bool(int(c["bits"][i, 0]) >> 2 & 1) for i in range(n)])
+    assert bool(see.any()) and not bool(see.all())
+    raw, inf = (torch.uint8, 0x7f) if fmt == "e4m3" else (torch.int16, 0x7f80)
+    for (t, o), d in zip(at, (7, 3)):
+        c["vc"].view(raw)[t, :, o, d] = inf
+    out, lse = _run_tree(ext, c, dev)
+    got, want = out.view(n, 2 * G, D).float().cpu(), clean.view(n, 2 * G, D).float().cpu()
+    bad = torch.zeros(n, 2 * G, D, dtype=torch.bool)
+    bad[see, :, 7] = True
+    bad[..., 3] = True
+    assert bool(torch.isfinite(want).all()) and not bool(torch.isfinite(got[bad]).any())
+    assert torch.equal(got[~bad], want[~bad]) and torch.equal(lse, clean_lse)
+
+
 @pytest.mark.parametrize("n,D", [(1, 256), (6, 128), (30, 256)])
 def test_tree_attn_graph_of_growing_contexts(ext, dev, n, D):
     """One captured call, replayed while the contexts on the device grow and shrink: lengths are looked at on the device,
