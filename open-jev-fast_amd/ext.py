@@ -663,7 +663,9 @@ def linattn_prompt(q, k, v, g, beta, seq_ptr, state=None, src=None, scale=None):
     if n < 0:
         check(2)
     ws = _scratch(n, q)
-    check(lib().ojx_linattn_prompt(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(seq_ptr), _ptr(state), _ptr(src),
+    # a pool of no states has no address, and none stands for zeros: any other, which 0 slots keep from being read
+    at = _ptr(last if state is not None and slots == 0 else state)
+    check(lib().ojx_linattn_prompt(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(seq_ptr), at, _ptr(src),
                                    slots, R, S, HV, HK, float(128 ** -0.5 if scale is None else scale), _ptr(o),
                                    _ptr(last), _ptr(ws), n, _stream()))
     return o, last

@@ -618,6 +618,16 @@ def test_linattn_prompt_without_rows(ext, dev):
     assert tuple(o.shape) == (0, 256) and torch.equal(last[0], pool[2]) and bool((last[1] == 0).all())
 
 
+def test_linattn_prompt_of_an_empty_pool(ext, C, dev):
+    """A pool of no states has none to start from: sequences that name one are NaN, as with every source outside the
+    states, and the others start from zeros."""
+    args = _lin_case(30, 1, 2, True, seed=4)
+    ptr, src = torch.tensor([0, 10, 30], dtype=torch.int32), torch.tensor([-1, 0], dtype=torch.int32)
+    o, last = ext.linattn_prompt(*_put(dev, *args, ptr, torch.zeros(0, 2, 128, 128), src))
+    assert bool(torch.isnan(last[1]).all()) and bool(torch.isnan(o[10:].float()).all())
+    _check_lin(C, [t[:10].contiguous() for t in args], [10], None, o[:10], last[:1], 128 ** -0.5)
+
+
 def test_linattn_is_causal_in_what_is_not_finite(ext, dev):
     """NaN and infinities reach no token before theirs, in their own chunk as little as in others."""
     args = _lin_case(150, 1, 2, True, seed=33)
