@@ -628,6 +628,169 @@ def test_linattn_prompt_of_an_empty_pool(ext, C, dev):
     _check_lin(C, [t[:10].contiguous() for t in args], [10], None, o[:10], last[:1], 128 ** -0.5)
 
 
+# ------------------------------------------------------------- many heads: a workgroup of eight waves a sequence and head
+_SHORT = [0, 1, 64, 3, 65, 17, 130, 63, 2, 33]
+MANY = [
+    # lengths, HK, G: sequences times value heads on both sides of 96, where the form for many heads begins
+    (_SHORT * 9 + _SHORT[4:], 1, 1),                 # 96: the last of the form for few
+    (_SHORT * 9 + _SHORT[3:], 1, 1),                 # 97, a head each: no multiple of the eight XCDs
+    ((_SHORT * 4)[:33], 1, 3),                       # 99
+    ([65, 0, 200, 64, 1, 63, 129], 5, 3),            # 105, of 35 key heads
+    ([70, 0, 65], 16, 3),                            # 144: the model's heads
+    ([0] * 100 + [5], 1, 2),                         # all but one empty
+]
+
+
+def _many_case(case, delta, lead=5, tail=9):
+    """Rows of no sequence before and behind the sequences, NaN in them; every third sequence from zeros, one from a state
+    that is not there, the others from a pool's."""
+    lengths, HK, G = MANY[case]
+    R, S, HV = sum(lengths), len(lengths), HK * G
+    args = _lin_case(lead + R + tail, HK, G, delta, seed=50 + case, sharp=case % 2 == 1)
+    for t in args:
+        if t is not None:
+            t[:lead], t[lead + R:] = math.nan, math.nan
+    ptr = torch.tensor([lead] + list(lead + torch.tensor(lengths).cumsum(0)), dtype=torch.int32)
+    pool = torch.randn(S + 2, HV, 128, 128, generator=torch.Generator().manual_seed(case)) * 0.1
+    src = torch.tensor([(3 * s) % (S + 2) if s % 3 else -1 for s in range(S)], dtype=torch.int32)
+    src[S // 2] = S + 2
+    return args, ptr, pool, src
+
+
+def _check_many(C, args, ptr, pool, src, o, last):
+    """Against the oracle; sequences from states that are not there are NaN, and the rows of no sequence zeros."""
+    lead, S = int(ptr[0]), ptr.numel() - 1
+    lengths = (ptr[1:] - ptr[:-1]).tolist()
+    end = lead + sum(lengths)
+    o, last = o.cpu(), last.cpu()
+    assert bool((o[:lead] == 0).all()) and bool((o[end:] == 0).all())
+    state = None
+    if pool is not None:
+        state = torch.where((src >= 0)[:, None, None, None], pool[src.clamp(0, pool.shape[0] - 1).long()], torch.zeros(()))
+        for s in range(S):
+            if int(src[s]) >= pool.shape[0]:
+                at = slice(int(ptr[s]), int(ptr[s + 1]))
+                assert bool(torch.isnan(last[s]).all()) and bool(torch.isnan(o[at].float()).all())
+                # for the comparison below, as if it had started from zeros
+                state[s] = last[s] = 0
+                if lengths[s] == 0:
+                    continue
+                sub = [None if t is None else t[at].contiguous() for t in args]
+                ro, rs, _, _ = C.linattn(*sub, [lengths[s]], None, 128 ** -0.5)
+                o[at], last[s] = ro.reshape(ro.shape[0], -1).bfloat16(), rs[0].float()
+    inner = [None if t is None else t[lead:end].contiguous() for t in args]
+    _check_lin(C, inner, lengths, state, o[lead:end], last, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_linattn_prompt_many(ext, C, dev, case, delta):
+    _say(f"case many {case} delta={delta}")
+    args, ptr, pool, src = _many_case(case, delta)
+    o, last = ext.linattn_prompt(*_put(dev, *args, ptr, pool, src))
+    _check_many(C, args, ptr, pool, src, o, last)
+    o, last = ext.linattn_prompt(*_put(dev, *args, ptr))
+    _check_many(C, args, ptr, None, None, o, last)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_linattn_prompt_many_falling_pointers(ext, C, dev, delta):
+    """Pointers in no order, some outside the rows: sequences begin where those before them ended."""
+    R, S = 400, 120
+    g = torch.Generator().manual_seed(61)
+    args = _lin_case(R, 1, 2, delta, seed=61)
+    raw = (torch.arange(S + 1) * 4 + torch.randint(-60, 60, (S + 1,), generator=g)).int()
+    raw[0], raw[50], raw[-1] = 3, 1 << 30, -7
+    raw[51:] = torch.randint(-500, 500, (S - 50,), generator=g).int()
+    raw[49] = 250
+    at = raw.clamp(0, R).cummax(0).values
+    o, last = ext.linattn_prompt(*_put(dev, *args, raw))
+    _check_many(C, args, at, None, None, o, last)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_linattn_prompt_many_not_finite(ext, C, dev, delta):
+    """A value that is not finite in the middle chunk of one of many sequences: what it reaches by the formula is not
+    finite, and everything else is the oracle's, in the chunks behind it, too."""
+    lengths, HK, G = [30] * 16 + [200] + [30] * 17, 1, 3
+    R, HV = sum(lengths), 3
+    args = _lin_case(R, HK, G, delta, seed=71)
+    ptr = torch.tensor([0] + list(torch.tensor(lengths).cumsum(0)), dtype=torch.int32)
+    first, at = int(ptr[16]), int(ptr[16]) + 100
+    o, st, bo, bs = C.linattn(*args, lengths, None, 128 ** -0.5)
+    for which, value in (("q", math.inf), ("k", math.nan), ("v", math.nan), ("v", -math.inf), ("g", math.nan),
+                         ("g", math.inf), ("beta", math.inf)):
+        if which == "beta" and not delta:
+            continue
+        _say(f"case many not finite {which} {value} delta={delta}")
+        bad = [None if t is None else t.clone() for t in args]
+        hit = torch.zeros(R, HV, 128, dtype=torch.bool)        # outputs that are not finite
+        lost = torch.zeros(HV, 128, dtype=torch.bool)          # value dims of the sequence's state
+        if which == "q":
+            bad[0][at, 5] = value
+            hit[at] = True
+        elif which == "k":
+            bad[1][at, 5] = value
+            hit[at:first + 200], lost[:] = True, True
+        elif which == "v":
+            bad[2][at, 128 + 37] = value
+            hit[at:first + 200, 1, 37], lost[1, 37] = True, True
+        else:
+            bad[3 if which == "g" else 4][at, 2] = value
+            hit[at:first + 200, 2], lost[2] = True, True
+        out, last = (t.cpu() for t in ext.linattn_prompt(*_put(dev, *bad, ptr)))
+        out = out.double().reshape(R, HV, 128)
+        assert not bool(torch.isfinite(out[hit]).any()) and bool(torch.isfinite(out[~hit]).all())
+        assert bool(((out - o).abs()[~hit] <= bo[~hit]).all())
+        cols = last[16].transpose(1, 2)                        # [HV, value dims, key dims]
+        if which == "k" and not delta:
+            assert not bool(torch.isfinite(cols[..., 5]).any())
+            assert bool(torch.isfinite(cols[..., :5]).all()) and bool(torch.isfinite(cols[..., 6:]).all())
+        elif which == "v":
+            assert not bool(torch.isfinite(cols[lost]).all(1).any())
+        elif bool(lost.any()):
+            assert not bool(torch.isfinite(cols[lost]).any())
+        keep = torch.ones(34, HV, dtype=torch.bool)
+        keep[16] = ~lost.any(1)
+        err = (last.double() - st).norm(dim=(2, 3))
+        assert bool((err[keep] <= bs[keep]).all())
+        assert bool(torch.isfinite(cols[~lost]).all())
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_linattn_prompt_many_in_a_graph(ext, dev, delta):
+    """A captured call, replayed over other inputs and pointers, with eager calls between, equals the eager call; so do
+    calls on two streams at once, and the same call again."""
+    args, ptr, pool, src = _many_case(2, delta)
+    d = _put(dev, *args, ptr, pool, src)
+    call = lambda: ext.linattn_prompt(*d)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, last = call()
+    other = _put(dev, *_many_case(2, delta)[0])
+    for x in other[:3]:
+        x.mul_(0.5)
+    for i, lengths in enumerate(([3] * 33, [0] * 32 + [400], _SHORT * 3 + [40, 64, 1])):
+        d[5].copy_(torch.tensor([5] + list(5 + torch.tensor(lengths).cumsum(0)), dtype=torch.int32))
+        d[2].copy_(other[2] if i % 2 == 0 else args[2])
+        a, b = call(), call()
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y, z in ((out, a[0], b[0]), (last, a[1], b[1])):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and torch.equal(y.view(torch.uint8), z.view(torch.uint8))
+    want = call()
+    torch.cuda.synchronize()
+    got = []
+    for s in (torch.cuda.Stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(s):
+            got.append(call())
+    torch.cuda.synchronize()
+    for x in got:
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(x, want))
+
+
 def test_linattn_is_causal_in_what_is_not_finite(ext, dev):
     """NaN and infinities reach no token before theirs, in their own chunk as little as in others."""
     args = _lin_case(150, 1, 2, True, seed=33)
