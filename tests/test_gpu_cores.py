@@ -556,6 +556,35 @@ def test_linattn_step(ext, C, dev, R, HK, G, delta):
         assert bool((o[1] == 0).all()) and bool(torch.isnan(o[3].float()).all()) and bool(torch.isnan(o[4].float()).all())
 
 
+@pytest.mark.parametrize("delta", [True, False])
+def test_linattn_step_of_slots_named_again(ext, C, dev, delta):
+    """The first row that names a slot has it; every later one is NaN and leaves the states alone. Rows apart by less and
+    by more than a workgroup's 256 threads, a slot named three times, idle rows between."""
+    R = 600
+    args = _lin_case(R, 1, 1, delta, seed=81)
+    g = torch.Generator().manual_seed(81)
+    pool = torch.randn(R + 40, 1, 128, 128, generator=g) * 0.1
+    slot = torch.randperm(R + 40, generator=g)[:R].int()
+    again = {10: 3, 70: 3, 200: 100, 255: 0, 256: 1, 257: 2, 300: 5, 511: 255 + 45, 513: 254, 560: 520, 598: 256 + 7, 599: 597}
+    for r, of in again.items():
+        slot[r] = slot[of]                     # row 511 names what row 300 took from row 5
+    idle = [4, 63, 64, 258, 512]
+    slot[idle[:3]], slot[idle[3:]] = -1, -(1 << 31)
+    assert int(slot[511]) == int(slot[5])
+    d = _put(dev, *args, pool, slot)
+    o = ext.linattn_step(*d).cpu()
+    got = d[5].cpu()
+    runs = [r for r in range(R) if r not in again and r not in idle]
+    assert len({int(slot[r]) for r in runs}) == len(runs)
+    at = slot[runs].long()
+    _check_lin(C, [None if t is None else t[runs].contiguous() for t in args], [1] * len(runs), pool[at], o[runs], got[at],
+               128 ** -0.5)
+    rest = torch.ones(R + 40, dtype=torch.bool)
+    rest[at] = False
+    assert torch.equal(got[rest], pool[rest])
+    assert bool(torch.isnan(o[list(again)].float()).all()) and bool((o[idle] == 0).all())
+
+
 def test_linattn_steps_go_on_from_a_prompt(ext, C, dev):
     """A prompt, then single tokens on its states, against the oracle's whole sequences."""
     lengths, more, HK, G = [70, 3, 129], 5, 1, 3
