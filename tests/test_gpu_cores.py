@@ -257,6 +257,38 @@ def test_tree_attn_masks_and_bad_pages(ext, C, dev, D, fmt):
     assert bool((lse[2] == -math.inf).all()) and bool((lse[-3:] == -math.inf).all()) and len(keep) == N - 1
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,G", [(5, 2), (14, 4), (40, 5)])
+def test_tree_attn_unseen_places_change_nothing(ext, dev, n, G, fmt):
+    """The same bits whatever lies in places that no row sees: free pages, places behind the sequences' ends, pages that the
+    table names wrongly, drafted tokens that no row has a bit for. Row blocks of 16, 64 and 128."""
+    _say(f"case unseen {n} {G} {fmt}")
+    page, D = 32, 256
+    c = _tree_case([n, n], [300, 45], 2, G, D, page, fmt, dev, seed=n, ext=ext)
+    c["bits"][:, 0] &= ~(1 << 2)               # drafted token 2: nobody's, not even its own
+    lost = int(c["table"][0, 3])
+    c["table"][0, 3] = -1
+    seen = torch.zeros(c["kc"].shape[0], page, dtype=torch.bool)
+    for b, ctx in enumerate((300, 45)):
+        for p in range(ctx + n):
+            if int(c["table"][b, p // page]) >= 0 and p != ctx + 2:
+                seen[int(c["table"][b, p // page]), p % page] = True
+    assert not bool(seen[lost].any())
+    want = _run_tree(ext, c, dev)
+    raw, bad = (torch.uint8, 0x7f) if fmt == "e4m3" else (torch.int16, 0x7fc0)
+    for x in (c["kc"], c["vc"]):
+        x.view(raw).transpose(1, 2)[~seen] = bad
+    # the values of a drafted token that rows do see elsewhere stay numbers: those that are not go one by one, in another order
+    for b, ctx in enumerate((300, 45)):
+        t, o = int(c["table"][b, (ctx + 2) // page]), (ctx + 2) % page
+        c["vc"][t, :, o] = torch.full((), 7.0).to(c["vc"].dtype)
+    if fmt == "e4m3":
+        c["ks"].transpose(1, 2)[~seen], c["vs"].transpose(1, 2)[~seen] = math.nan, math.inf
+    got = _run_tree(ext, c, dev)
+    assert bool(torch.isfinite(want[0].float()).all())
+    assert torch.equal(got[0].view(torch.int16), want[0].view(torch.int16)) and torch.equal(got[1], want[1])
+
+
 def test_tree_attn_table_ends_early(ext, C, dev):
     """Positions past max_pages * page are not seen, drafted ones among them."""
     c = _tree_case([6], [60], 2, 3, 128, 16, "bf16", dev, seed=5, ext=ext)
