@@ -151,3 +151,91 @@ def linattn(q, k, v, g, beta, lengths, state, scale):
         st[s], E[s] = M, err
         at += lengths[s]
     return o, st, bo, E
+
+
+def linattn_chunk(q, k, v, g, beta, lengths, state, scale):
+    """linattn for sequences of at most 64 tokens from given states, with bounds entry by entry instead of by norms:
+    (o fp64 [R, HV, 128], states, bound of |o - kernel| [R, HV, 128], bound of |states - kernel| [S, HV, 128, 128]).
+
+    They hold for a kernel that takes the tokens of a sequence at once,
+      A_ij = beta_i e^(G_i - G_j) k_i . k_j (j < i),  P_ij = e^(G_i - G_j) q_i . k_j (j <= i),  T = (I + A)^-1 diag(beta),
+      X = V - diag(e^G) K S0,  U = T X,  O = scale (diag(e^G) Q S0 + P U),  S = e^(G_n) S0 + K^T diag(e^(G_n - G)) U
+    (T the identity and U = V without beta), sums in fp32, and lets S0, X, P T, diag(e^(G_n - G)) T and U into its
+    products as two bf16 pieces. Of x, hi = bf16(x) and lo = bf16(x - hi) leave out at most U^2 |x|; a product of two such
+    factors leaves out lo lo, U^2 of it at most, besides. A sum of n terms is off by at most 2 F n times the sum of their
+    magnitudes, in any order and also where additions are cut off instead of rounded; n doubles with the pieces. An
+    exponential is off by its argument's rounding and a step of its own. The errors go through the formulas in magnitudes."""
+    R, HV = g.shape
+    HK = k.shape[1] // 128
+    G = HV // HK
+    q, k, v = (x.double().reshape(R, -1, 128) for x in (q, k, v))
+    q, k = q.repeat_interleave(G, 1), k.repeat_interleave(G, 1)
+    g, beta = g.double(), None if beta is None else beta.double()
+    S = len(lengths)
+    st, o = torch.zeros(S, HV, 128, 128, dtype=torch.float64), torch.zeros(R, HV, 128, dtype=torch.float64)
+    bs, bo = torch.zeros_like(st), torch.zeros_like(o)
+    pieces, dot, tiny = U * U, 2 * F * 256, 1e-35     # tiny: factors below the smallest fp32 step
+
+    def expo(x):
+        """e^x and its relative error: the argument, to base two, in fp32, and a step of fp32 for the exponential."""
+        return x.exp(), 1.01 * F * x.abs() + 3 * F
+
+    at = 0
+    for s, n in enumerate(lengths):
+        assert n <= 64
+        for h in range(HV):
+            S0 = torch.zeros(128, 128, dtype=torch.float64) if state is None else state[s, h].double()
+            if n == 0:
+                st[s, h] = S0
+                continue
+            r = slice(at, at + n)
+            Q, K, V = q[r, h], k[r, h], v[r, h]
+            cum = g[r, h].cumsum(0)
+            low = torch.ones(n, n, dtype=torch.float64).tril()
+            fade, dfade = expo(torch.where(low > 0, cum[:, None] - cum[None], 0.0))
+            fade = fade * low
+            since, dsince = (x[:, None] for x in expo(cum))
+            to, dto = (x[:, None] for x in expo(cum[-1] - cum))
+            KS, QS, SA = K @ S0, Q @ S0, S0.abs()
+            dKS, dQS = ((pieces + 2 * dot) * (x.abs() @ SA) for x in (K, Q))
+            P = fade * (Q @ K.T)
+            dP = fade * (dot * (Q.abs() @ K.abs().T) + (dfade + 2 * F) * (Q @ K.T).abs())
+            if beta is None:
+                X, dX, T, dT = V, torch.zeros_like(V), None, None
+                W, dW = P, dP                                       # what X meets for the outputs
+                u, du = V, torch.zeros_like(V)
+                end, dend = to * V, (dto + F) * (to * V).abs()      # U, decayed to the end
+            else:
+                b = beta[r, h][:, None]
+                A = (b * fade * (K @ K.T)).tril(-1)
+                dA = (b.abs() * fade * (dot * (K.abs() @ K.abs().T) + (dfade + 3 * F) * (K @ K.T).abs())).tril(-1)
+                I = torch.eye(n, dtype=torch.float64)
+                inv = torch.linalg.solve_triangular(I + A, I, upper=False)
+                # forward substitution is off by |T| |L| |T| F n; put together from blocks of 16, each block row passes on
+                # what the ones above are off by, through |T| |L| again
+                E, own = inv.abs() @ (I + A).abs(), torch.zeros_like(A)
+                power = 2 * F * (n + 2) * inv.abs()
+                for _ in range(1 if n <= 16 else 4):
+                    power = E @ power
+                    own = own + power
+                T = inv * b.T
+                dT = (inv.abs() @ dA @ inv.abs() + own) * b.abs().T + F * T.abs()
+                X = V - since * KS
+                dX = since * dKS + (dsince + 2 * F) * (since * KS).abs() + F * X.abs()
+                W = P @ T
+                dW = P.abs() @ dT + dP @ T.abs() + 2 * F * n * (P.abs() @ T.abs())
+                W, dW = W.tril(), dW.tril()
+                u = T @ X
+                both = (3 * pieces + 2 * F * 3 * n) * (T.abs() @ X.abs())
+                end, dend = to * u, to * (T.abs() @ dX + dT @ X.abs() + both + (dto + 2 * F) * (T.abs() @ X.abs()))
+            S1, all_, dall = to * u, since[-1], dsince[-1]
+            st[s, h] = all_ * S0 + K.T @ S1
+            bs[s, h] = ((dall + 2 * F) * all_ * SA + K.abs().T @ (dend + pieces * end.abs())
+                        + 2 * F * (2 * n + 2) * (K.abs().T @ end.abs() + all_ * SA)) * 1.01 + tiny
+            o[r, h] = scale * (since * QS + P @ u)
+            left = (3 if beta is not None else 1) * pieces
+            err = since * dQS + (dsince + 3 * F) * (since * QS).abs() + W.abs() @ dX + dW @ X.abs()
+            err = err + (left + 2 * F * (3 * n + 4)) * (W.abs() @ X.abs()) + 2 * F * (since * QS).abs()
+            bo[r, h] = (abs(scale) * err * (1 + U) + U * o[r, h].abs()) * 1.01 + tiny
+        at += n
+    return o, st, bo, bs

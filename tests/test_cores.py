@@ -57,6 +57,74 @@ def test_linattn_oracle_closed_forms():
     assert torch.allclose(st[0, 0].T @ k[-1], v[-1], atol=1e-10)
 
 
+# ------------------------------------------------------------------------------------------------------------ precision
+def _pieces(x, lo=True):
+    """x as the bf16 pieces hi and lo: 16 bits (lo=False: hi alone)."""
+    x = x.float()
+    hi = x.bfloat16().float()
+    return (hi + (x - hi).bfloat16().float() if lo else hi).double()
+
+
+def _chunk_in_pieces(q, k, v, g, beta, lengths, state, scale, drop=None):
+    """The chunk's formulas in 64 bits with the factors named in linattn_chunk in two bf16 pieces, `drop` in one: what a
+    kernel with exact sums gives. One key head a value head."""
+    R, HV = g.shape
+    q, k, v = (x.double().reshape(R, HV, 128) for x in (q, k, v))
+    o, st = torch.zeros(R, HV, 128, dtype=torch.float64), torch.zeros(len(lengths), HV, 128, 128, dtype=torch.float64)
+    two = lambda x, name: _pieces(x, drop != name)  # noqa: E731
+    at = 0
+    for s, n in enumerate(lengths):
+        for h in range(HV):
+            r = slice(at, at + n)
+            Q, K, V, S0, cum = q[r, h], k[r, h], v[r, h], state[s, h].double(), g[r, h].double().cumsum(0)
+            fade = torch.where(torch.ones(n, n).tril() > 0, cum[:, None] - cum[None], -math.inf).exp()
+            since, to = cum.exp()[:, None], (cum[-1] - cum).exp()[:, None]
+            W = P = fade * (Q @ K.T)
+            X, T = V, torch.eye(n, dtype=torch.float64)
+            if beta is not None:
+                b = beta[r, h].double()
+                T = torch.linalg.inv(T + b[:, None] * (fade * (K @ K.T)).tril(-1)) * b[None]
+                X, W = two(V - since * (K @ two(S0, "state of X")), "X"), P @ T
+                end = two(two(to * T, "T") @ X, "U")
+            else:
+                end = two(to * V, "U")
+            st[s, h] = since[-1] * S0 + K.T @ end
+            o[r, h] = (scale * (since * (Q @ two(S0, "state of O")) + two(W, "P T") @ X)).bfloat16().double()
+        at += n
+    return o, st
+
+
+def _short(delta, seed=0):
+    """Sequences of 1 to 64 tokens, two heads, states of their own, decays around 1 and slow ones."""
+    g = torch.Generator().manual_seed(seed)
+    lengths = [1, 2, 3, 5, 8, 16, 24, 40, 64]
+    R = sum(lengths)
+    qk = torch.nn.functional.silu(torch.randn(2, R, 2, 128, generator=g) + 0.3)
+    qk = (qk / qk.norm(dim=-1, keepdim=True)).bfloat16().reshape(2, R, 256)
+    v = torch.randn(R, 256, generator=g).bfloat16()
+    gate = -torch.rand(R, 2, generator=g) * torch.tensor([1.0, 0.02])
+    beta = torch.sigmoid(torch.randn(R, 2, generator=g)).bfloat16() if delta else None
+    return (qk[0], qk[1], v, gate, beta), lengths, torch.randn(len(lengths), 2, 128, 128, generator=g)
+
+
+def test_linattn_chunk_is_linattn():
+    for delta in (True, False):
+        args, lengths, state = _short(delta)
+        a, b = C.linattn(*args, lengths, state, 0.1), C.linattn_chunk(*args, lengths, state, 0.1)
+        assert torch.allclose(a[0], b[0], atol=1e-11) and torch.allclose(a[1], b[1], atol=1e-11)
+
+
+@pytest.mark.parametrize("delta,drop", [(True, x) for x in (None, "state of X", "X", "T", "U", "state of O", "P T")]
+                         + [(False, x) for x in (None, "U", "state of O", "P T")])
+def test_linattn_chunk_bounds_see_a_missing_piece(delta, drop):
+    """Two pieces of every factor stay within the bounds; any one of them in a single piece does not."""
+    args, lengths, state = _short(delta, 1)
+    o, st, bo, bs = C.linattn_chunk(*args, lengths, state, 128 ** -0.5)
+    go, gs = _chunk_in_pieces(*args, lengths, state, 128 ** -0.5, drop)
+    worst = max(((go - o).abs() / bo).max().item(), ((gs - st).abs() / bs).max().item())
+    assert worst <= 1 if drop is None else worst > 2, worst
+
+
 # ----------------------------------------------------------------------------------------------------------------- bits
 def test_tree_bits(ext):
     b = ext.tree_bits([[-1, 0, 0, 2, -1], [], [-1]])

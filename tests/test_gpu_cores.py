@@ -852,6 +852,41 @@ def test_linattn_prompt_many_in_a_graph(ext, dev, delta):
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(x, want))
 
 
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("HK,G", [(2, 1), (1, 3), (4, 3), (16, 1)])
+def test_linattn_prompt_keeps_two_pieces(ext, C, dev, HK, G, delta):
+    """Entry by entry, sequences of up to 64 tokens from given states stay within what two bf16 pieces a factor and fp32
+    sums give (in bounds that a single piece of any factor breaks). Both forms: 18 and 27 heads, 108 and 144."""
+    _say(f"case pieces HK={HK} G={G} delta={delta}")
+    lengths = [1, 2, 3, 5, 8, 16, 24, 40, 64]
+    args = _lin_case(sum(lengths), HK, G, delta, seed=90 + HK)
+    ptr = torch.tensor([0] + list(torch.tensor(lengths).cumsum(0)), dtype=torch.int32)
+    state = torch.randn(9, HK * G, 128, 128, generator=torch.Generator().manual_seed(HK))
+    o, last = ext.linattn_prompt(*_put(dev, *args, ptr, state))
+    want, st, bo, bs = C.linattn_chunk(*args, lengths, state, 128 ** -0.5)
+    eo, es = (o.cpu().double().reshape(want.shape) - want).abs(), (last.cpu().double() - st).abs()
+    _say(f"  out {(eo / bo).max().item():.3f}, state {(es / bs).max().item():.3f} of the bounds")
+    assert bool((eo <= bo).all()) and bool((es <= bs).all())
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("HK,G", [(1, 3), (37, 3)])
+def test_linattn_prompt_hands_its_state_on_exactly(ext, dev, HK, G, delta):
+    """A long sequence is its chunks of 64 tokens in calls of their own, each from the state that the one before left, to
+    the bit: what holds for one chunk holds for all. Both forms."""
+    _say(f"case chunks HK={HK} G={G} delta={delta}")
+    R = 64 * 5 + 9
+    q, k, v, g, beta = _put(dev, *_lin_case(R, HK, G, delta, seed=95, sharp=True))
+    ptr = lambda n: torch.tensor([0, n], dtype=torch.int32, device=dev)  # noqa: E731
+    o, last = ext.linattn_prompt(q, k, v, g, beta, ptr(R))
+    state = None
+    for t in range(0, R, 64):
+        r = slice(t, min(R, t + 64))
+        part, state = ext.linattn_prompt(q[r], k[r], v[r], g[r], None if beta is None else beta[r], ptr(r.stop - t), state)
+        assert torch.equal(part, o[r]), t
+    assert torch.equal(state, last)
+
+
 def test_linattn_is_causal_in_what_is_not_finite(ext, dev):
     """NaN and infinities reach no token before theirs, in their own chunk as little as in others."""
     args = _lin_case(150, 1, 2, True, seed=33)
