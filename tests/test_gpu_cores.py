@@ -434,6 +434,28 @@ def test_tree_attn_empty(ext, dev):
     assert tuple(out.shape) == (0, 256) and tuple(lse.shape) == (0, 2)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("page", [16, 112, 240, 1008, 1024])
+def test_tree_attn_pages(ext, C, dev, page, fmt):
+    """The smallest and the largest page, and some that are no power of two: where a position lies is a division."""
+    _say(f"case page {page} {fmt}")
+    c = _tree_case([3, 1, 21], [0, 1030, 257], 1, 4, 128, page, fmt, dev, seed=page, ext=ext)
+    out, lse = _run_tree(ext, c, dev)
+    _check_tree(C, c, out, lse, 128 ** -0.5)
+
+
+def test_cores_without_sequences(ext, dev):
+    """Rows and no sequence at all: zeros (lse -inf), and no states."""
+    c = _tree_case([4], [20], 2, 3, 256, 16, "bf16", dev, seed=9, ext=ext)
+    for pages in (2, 400):
+        none = dict(c, ctx=c["ctx"][:0], q_ptr=c["q_ptr"][:1], table=torch.zeros(0, pages, dtype=torch.int32))
+        out, lse = _run_tree(ext, none, dev)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    for delta in (True, False):
+        o, last = ext.linattn_prompt(*_put(dev, *_lin_case(200, 1, 3, delta, seed=9), torch.zeros(1, dtype=torch.int32)))
+        assert bool((o == 0).all()) and tuple(last.shape) == (0, 3, 128, 128)
+
+
 def test_tree_attn_long(ext, C, dev):
     """A long context, checked on a few rows: every split of it and their join."""
     for fmt, n, ctx in (("e4m3", 1, 20011), ("bf16", 13, 9001)):
