@@ -891,7 +891,7 @@ int check_tree(int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t
     return fail(OJX_ERR_SHAPE, "HQ=%d must be a multiple of HKV=%d, at most 64 times it", HQ, HKV);
   if (page < 16 || page % 16 != 0 || page > 1024)
     return fail(OJX_ERR_SHAPE, "page=%d must be a multiple of 16, at most 1024", page);
-  if (max_pages < 0 || max_pages * page >= (1LL << 31))
+  if (max_pages < 0 || max_pages >= (1LL << 31) || max_pages * page >= (1LL << 31))  // each, so that no product wraps
     return fail(OJX_ERR_SHAPE, "bad max_pages=%lld (at most 2^31 positions)", (long long)max_pages);
   if (N * HQ >= (1LL << 24))
     return fail(OJX_ERR_SHAPE, "N=%lld rows of %d heads: too many for one call", (long long)N, HQ);
@@ -979,7 +979,7 @@ int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const
 int64_t ojx_linattn_prompt_workspace(int64_t R, int64_t S, int32_t HV, int32_t HK, int32_t delta) {
   // a workgroup of 256 threads per sequence and head at most; a launch has fewer than 2^32 threads
   if (HK < 1 || HV < HK || HV % HK != 0 || HV > 1024 || R < 0 || R >= (1LL << 31) || S < 0 ||
-      4 * (S + 1) * HV >= (1LL << 24) || ojx::linattn_chunks(R, S) * HV >= (1LL << 24)) {
+      S >= (1LL << 31) || 4 * (S + 1) * HV >= (1LL << 24) || ojx::linattn_chunks(R, S) * HV >= (1LL << 24)) {
     fail(OJX_ERR_SHAPE, "bad sizes R=%lld S=%lld HV=%d HK=%d", (long long)R, (long long)S, HV, HK);
     return -1;
   }

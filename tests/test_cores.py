@@ -220,6 +220,19 @@ def test_linattn_refusals(pkg, p):
         assert prompt(ws=p, nws=need - 1) == 3 and prompt(ws=None, nws=need) == 3
 
 
+def test_refusals_of_sizes_whose_products_wrap(pkg, p):
+    """Page and sequence counts whose products with the other sizes come back to something small in 64 bits."""
+    L = pkg._lib.lib()
+    for MP, page in ((1 << 60, 16), (1 << 58, 64), ((1 << 60) + 1, 16), (1 << 62, 1024)):
+        assert L.ojx_tree_attn_workspace(4, 2, 6, 2, 256, MP, page) == -1
+        assert L.ojx_tree_attn(p, p, p, None, 0, p, p, None, None, 0, p, MP, 4, 2, 6, 2, 256, 8, page, 0.1, p, None, None, 0,
+                               None) == 2
+    for S in (1 << 61, (1 << 61) - 1, (1 << 62) - 1, (1 << 63) - 1, 1 << 31):
+        for HV, HK in ((6, 2), (1, 1), (1024, 16)):
+            assert L.ojx_linattn_prompt_workspace(5, S, HV, HK, 1) == -1
+            assert L.ojx_linattn_prompt(p, p, p, p, p, p, None, None, 0, 5, S, HV, HK, 0.1, p, p, p, 1 << 40, None) == 2
+
+
 def test_python_refusals(ext):
     """CPU tensors are refused like everywhere in the package."""
     x = torch.zeros(2, 3, 256, dtype=torch.bfloat16)
