@@ -200,7 +200,7 @@ int ojx_linattn_prep(const void* proj, const int32_t* hist, const int32_t* rep_p
  * holds values: OJX_KV_BF16 (16-bit patterns, ks and vs NULL) or OJX_KV_E4M3 (OCP e4m3 bytes and one fp32 scale for each
  * token and head, ks, vs [pages, HKV, page]; a value is byte * scale). slots int64 [N]: token n's place, page index * page
  * + offset; a slot outside [0, pages * page) is skipped by the write and read back as zeros. D = 128 or 256, page a
- * multiple of 16, at most 1024.
+ * multiple of 16, at most 1024, HKV at most 1024.
  * The write quantises: scale = the smallest power of two 2^e, e >= -126, with max |x| / 2^e <= 448 over the row's finite
  * values (1 for a row of zeros); stored = e4m3(x / scale), nearest, ties to even; NaN for a value that is not finite. It
  * touches nothing but the slots named. Two tokens with the same slot leave either's values there, or a mix of both.
@@ -222,9 +222,13 @@ int ojx_kv_cache_read(const void* kc, const void* vc, const float* ks, const flo
  * Positions from ctx[b] + n_b or max_pages * page on, and pages whose table entry is outside [0, pages), are not seen,
  * whatever lies there. Query head h reads kv head h / (HQ / HKV).
  *   out[n][h] = sum_t p_t v_t / sum_t p_t, p_t = exp(scale q . k_t), bf16 [N, HQ, D]; lse (may be NULL) = log sum_t p_t,
- * fp32 [N, HQ]. A row that sees nothing, and a row of no sequence, gives zeros and -infinity.
- * q bf16 [HQ, N, D] (ojx_fullattn_prep's qt). D = 128 or 256, HQ a multiple of HKV. workspace: ojx_tree_attn_workspace
- * bytes of device memory, 16-byte aligned (0 = none needed); it depends on sizes only. */
+ * fp32 [N, HQ]. A row that sees nothing, and a row of no sequence, gives zeros and -infinity. A value that is not finite
+ * makes that dim of every row that sees it not finite, however small its weight. Weights are rounded to bf16; they and the
+ * values are summed in fp32 before the division, the weights up to 2^8: values past 2^119 over the positions overflow.
+ * q bf16 [HQ, N, D] (ojx_fullattn_prep's qt). D = 128 or 256, HQ a multiple of HKV and at most 64 times it. At most 65536
+ * sequences, N * HQ below 2^24, max_pages * page below 2^31 (OJX_ERR_SHAPE otherwise; -1 from the workspace's size).
+ * workspace: ojx_tree_attn_workspace bytes of device memory, 16-byte aligned (0 = none needed); it depends on sizes only
+ * and serves any lengths: a call that need not split its positions leaves it unused. */
 int64_t ojx_tree_attn_workspace(int64_t N, int32_t B, int32_t HQ, int32_t HKV, int32_t D, int64_t max_pages,
                                 int32_t page);
 int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const int64_t* bits, int32_t words,
@@ -237,16 +241,17 @@ int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const
  * A value head carries a state S [128 key dims][128 value dims], fp32; a token does
  *   S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q
  * (the gated delta rule), or with beta NULL u = v (plain decayed sums). q, k bf16 [R, HK, 128], v bf16 [R, HV, 128],
- * g fp32 [R, HV] (-infinity clears the state), beta bf16 [R, HV], o bf16 [R, HV, 128]; value head h reads key head
+ * g fp32 [R, HV] (-infinity clears a state of finite values), beta bf16 [R, HV], o bf16 [R, HV, 128]; value head h reads key head
  * h / (HV / HK).
  * ojx_linattn_prompt runs whole sequences: sequence s has rows seq_ptr[s] .. seq_ptr[s+1] - 1 (int32 [S + 1],
  * non-decreasing; none allowed). It starts from state[src[s]] (state fp32 [slots, HV, 128, 128], src int32 [S]; src[s] < 0
  * = zeros, src[s] >= slots = NaN; src NULL = s itself; state NULL = zeros for all) and leaves its last state in
  * state_out[s] (fp32 [S, HV, 128, 128], not overlapping state). Rows of no sequence get zeros. workspace:
  * ojx_linattn_prompt_workspace bytes of device memory, 16-byte aligned (0 = none needed); it depends on sizes only.
+ * HV at most 1024; 4 (S + 1) HV, and the chunks of 64 tokens (R / 64 + S at most) times HV, below 2^24.
  * ojx_linattn_step runs one token for each of R rows on state[slot[r]], updated in place (slot int32 [R]). A row whose
  * slot is negative is idle: it gets zeros. A slot of state_slots or more, or one that an earlier row names too, gives NaN
- * for that row and leaves the states alone. */
+ * for that row and leaves the states alone. R * HV below 2^24. */
 int64_t ojx_linattn_prompt_workspace(int64_t R, int64_t S, int32_t HV, int32_t HK, int32_t delta);
 int ojx_linattn_prompt(const void* q, const void* k, const void* v, const float* g, const void* beta,
                        const int32_t* seq_ptr, const float* state, const int32_t* src, int64_t state_slots, int64_t R,

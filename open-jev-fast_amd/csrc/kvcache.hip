@@ -9,7 +9,8 @@
 // Both directions move each row once. 16384 tokens of four heads of 256, 101 MB: read back in 17.4 us, 5.8 TB/s, as fast
 // as a large copy. Written in 22.5 us, 4.5 TB/s: the scale needs the whole row before the first value can be stored, so a
 // wave's chain is a load, the row's maximum over its lanes and a store (24.0 us with the maximum through LDS, 27.3 with the
-// values loaded behind the slots and 64-bit divisions for both). A few rows cost the launch: 2.8 us for 64 tokens.
+// values loaded behind the slots and 64-bit divisions for both). In bf16, 134 MB, 26.0 us written and 21.8 read (5.2 and 6.2
+// TB/s). A few rows cost the launch: 2.8 us for 64 tokens.
 #include "ojx_internal.h"
 
 #include <algorithm>

@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = wave & 1;
   // Workgroups go to the eight XCDs in turn. Of 32, the four of a head are eight apart: one L2 serves them (16384 tokens: 682
-  // -> 638 us, 1369 -> 449 MB read), and the heads still take the XCDs in turn, so that sequences of unlike lengths share them
+  // -> 638 us, 1369 -> 459 MB read), and the heads still take the XCDs in turn, so that sequences of unlike lengths share them
   const uint32_t b = blockIdx.x, whole = (uint32_t)p.S * p.HV / 8 * (8 * SL);
   const uint32_t wg = b < whole ? (b / (8 * SL) * 8 + b % 8) * SL + b / 8 % SL : b;
   const int64_t sq = wg / (p.HV * SL);
@@ -849,8 +849,8 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 
 // Many sequences: a workgroup of eight waves per sequence and value head, each with one slice and all of its work, so that
 // two waves a SIMD fill each other's gaps and what they share is loaded once a head: 16 sequences of up to 539 tokens, 48
-// heads, 120 us (163 with slices as above), MFMAs busy 29%, 246 MB of memory, the chunks' matrices (25 KB each) nearly
-// half of them. (Here the waves that read K^T and V
+// heads, 118 us in this kernel (184 with slices as above), MFMAs busy 29%, 246 MB of memory, the chunks' matrices (25 KB
+// each) nearly half of them. (Here the waves that read K^T and V
 // transposed have DMAs in flight, and the builtin makes the compiler wait for those: the reads are written out, with the
 // wait for themselves in the same block, so that the registers are filled when it ends.)
 template <int X0, int X1, int X2, int X3>
@@ -892,7 +892,7 @@ __global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // the value heads of a key head on one XCD, as above (163 -> 161 us, 176 -> 128 MB read)
+  // the value heads of a key head on one XCD, as above (the call 163 -> 161 us, this kernel 176 -> 128 MB read)
   const uint32_t b = blockIdx.x, per = p.HV / p.HK, whole = (uint32_t)p.S * p.HK / 8 * (8 * per);
   const uint32_t wg = b < whole ? (b / (8 * per) * 8 + b % 8) * per + b / 8 % per : b;
   const int64_t sq = wg / p.HV;
@@ -1021,8 +1021,10 @@ __global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
 }
 
 constexpr int many_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * 768); }
-// Sequences times value heads up to which the workgroups of two slices run (four of them a head). Both kernels, 500 tokens
-// a sequence: 48 heads 33 us with slices, 47 with eight waves a head; 96 43-49 and 49-51; 144 59 and 54; 288 87 and 63.
+// Sequences times value heads up to which the workgroups of two slices run (four of them a head). Calls of 48-head sequences,
+// with slices and with eight waves a head: 500 tokens each, one sequence 32 and 49 us, two 50 and 51, three 71 and 56, six
+// 116 and 107; 4096 tokens each, one 159 and 297, two 312 and 340, three 461 and 383, six 811 and 772. (Three of unlike
+// lengths, 4096 and less: 322 and 352.)
 constexpr int64_t kFew = 96;
 constexpr int prompt_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * (512 + 64)) + 2 * (8192 + 4096) + 16; }
 

@@ -24,16 +24,19 @@
 // The positions are split over workgroups so that one round of them fills the GPU; a second launch joins the parts.
 //
 // Three sizes of row blocks, by the mean packed rows of a sequence (tree_plan). Times of tree_attn, D = 256, four kv heads
-// of six query heads, bf16 / e4m3, in blocks of 16, 64 and 128 rows:
-//   16 sequences of  1 over 4096 ( 6 rows):  49 /  33,   50 /  46,  53 /  66 us -> 16
-//                    4           (24 rows):  92 /  64,   52 /  47,  55 /  66    -> 64
-//                    8           (48 rows):  91 /  67,   54 /  50,  59 /  71    -> 64
-//                   12           (72 rows): 168 / 122,   71 /  81,  64 /  74    -> 128
-//   4 sequences of  64 over 8192 (384 rows): 302 / 216, 116 / 146,  82 / 107    -> 128
-// What bounds them now: a single row block of a bf16 cache, its stream (64 x 4 over 4096: 194 us, 5.5 TB/s); else the steps
+// of six query heads, three caches in turn, bf16 / e4m3, in blocks of 16, 64 and 128 rows:
+//   16 sequences of  1 over 4096 ( 6 rows):  57 /  36,   58 /  45,  60 /  70 us -> 16
+//                    4           (24 rows):  65 /  43,   60 /  47,  62 /  72    -> 64
+//                    8           (48 rows): 101 /  67,   62 /  49,  65 /  75    -> 64
+//                   12           (72 rows): 180 / 124,   78 /  81,  67 /  78    -> 128
+//   4 sequences of  64 over 8192 (384 rows): 310 / 214, 134 / 145,  85 / 107    -> 128
+// An e4m3 cache is half the bytes, but its values become bf16 on their way to LDS: faster than bf16 up to 48 rows or so a
+// sequence (64 x 1 over 4096: 104 and 188 us, 64 x 4: 139 and 187), slower from 72 on.
+// What bounds them now: a single row block of a bf16 cache, its stream (64 x 4 over 4096: 187 us, 5.8 TB/s); else the steps
 // of a wave between barriers: in the 16 x 12 case of up to 8192 (e4m3, 69 us) MFMAs are busy 10% of the time, waves wait
-// for memory and barriers 40% and to issue 21% of theirs; in the 4 x 64 case of up to 16384 (bf16, 77 us) 22, 34 and 31%.
-// Reading operands further ahead than the loops do changes neither.
+// for memory and barriers 40% and to issue 21% of theirs; in the 4 x 64 case of up to 16384 (bf16, 78 us) 21, 35 and 31%.
+// Reading operands further ahead than the loops do changes neither. A chain of 2048 rows over nothing takes 258 / 305 us:
+// each of its row blocks runs the whole sequence's units, and all of them as edges.
 #include "gemm_common.h"
 
 #include <algorithm>
@@ -130,11 +133,10 @@ __device__ __forceinline__ void load_q(const TreeParams& p, const Row& w, int fi
 // Work is shared out by the lengths as they are on the device: a sequence of u units has ceil(u / L) parts of equal length
 // for each of its row blocks. With up to 64 sequences and no more row blocks, nb, than workgroups run at once (p.target, of
 // a kv head), L is the least that makes p.target parts at most, found in steps of a sixteenth from the mean on: one round
-// of workgroups, all about as long (16 x 12 over up to 8192, e4m3: 111 us with as many parts for a short sequence as for a
-// long one, 72 this way; 64 x 4 over 4096: 237 us with the L below, which equal row blocks fill badly, 162). With
-// more, L is `total` units over all row blocks by max(p.target - nb, nb / 4), so that there are max(p.target, nb + nb / 4)
-// parts at most and the longest sequences do not come last and alone. No part has fewer than p.least units unless its
-// sequence has.
+// of workgroups, all about as long (16 x 12 over up to 8192, e4m3: 77 us with the L below, 69 this way; equal lengths
+// are level). With more, L is `total` units over all row blocks by max(p.target - nb, nb / 4), so that there are
+// max(p.target, nb + nb / 4) parts at most and the longest sequences do not come last and alone. No part has fewer than
+// p.least units unless its sequence has.
 struct Part {
   int b, first, n, row0, rows, hk, parts, u0, u1;
   uint32_t slot;  // of the part's first row in the workspace; a row's parts lie HKV R slots apart
@@ -525,7 +527,8 @@ __global__ void __launch_bounds__(512, 2) tree_wide_k(TreeParams p) {
   constexpr int PR = SB / 16, RL = 64 / PR, PL = 8 / RL;  // 16-byte pieces of a row, rows a wave's load takes, loads of 8 rows
   constexpr int TILE = 32 * RB;
   constexpr bool EARLY = FP8 && CT * D < 512;
-  // steps of the last 16 rows' Q that stay in LDS, as many as two workgroups have room for (16 x 12 over 4096: 81 -> 71 us)
+  // steps of the last 16 rows' Q that stay in LDS, as many as a workgroup has room for: with them 155 KB of the CU's 160
+  // (16 x 12 over 4096, 72 rows each: 87 us with none, 85 with two, 79 with three; 4 x 64 over 8192: 114, 110, 106)
   constexpr int QL = FP8 && !EARLY ? 3 : 0;
   __shared__ __attribute__((aligned(1024))) uint8_t bufs[2][2][2][TILE];  // of each four waves, two of keys and values
   __shared__ __attribute__((aligned(16))) float scs[2][2][2][32];
