@@ -241,8 +241,8 @@ int ojx_tree_attn(const void* q, const int32_t* q_ptr, const int32_t* ctx, const
  * A value head carries a state S [128 key dims][128 value dims], fp32; a token does
  *   S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q
  * (the gated delta rule), or with beta NULL u = v (plain decayed sums). q, k bf16 [R, HK, 128], v bf16 [R, HV, 128],
- * g fp32 [R, HV] (-infinity clears a state of finite values), beta bf16 [R, HV], o bf16 [R, HV, 128]; value head h reads key head
- * h / (HV / HK).
+ * g fp32 [R, HV] (-infinity clears a state of finite values), beta bf16 [R, HV], o bf16 [R, HV, 128]; value head h reads
+ * key head h / (HV / HK).
  * ojx_linattn_prompt runs whole sequences: sequence s has rows seq_ptr[s] .. seq_ptr[s+1] - 1 (int32 [S + 1],
  * non-decreasing; none allowed). It starts from state[src[s]] (state fp32 [slots, HV, 128, 128], src int32 [S]; src[s] < 0
  * = zeros, src[s] >= slots = NaN; src NULL = s itself; state NULL = zeros for all) and leaves its last state in

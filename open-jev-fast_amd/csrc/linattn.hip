@@ -149,7 +149,10 @@ __global__ void __launch_bounds__(256) linattn_step_k(LinParams p, float* state,
 // diag(e^(G_C - G)) T, the two products in which T is used. linattn_prompt_k then goes through a sequence's chunks in order.
 //
 // Precision. The states are fp32, and so is what makes them: a factor that is not a bf16 input (S0, X, U, the products with
-// T) enters its products as two bf16 pieces, hi + lo, which keep 16 bits and more (K, Q and V are bf16 already).
+// T) enters its products as two bf16 pieces, hi + lo, which keep 16 bits and more (K, Q and V are bf16 already). The states
+// come out 5e-6 off 64 bits, relative to their norm, after 288 tokens as after 16384 (1.4e-6 without the delta rule; fp32
+// products would be 1.2e-7 off). A third piece is half as many products again on the chain that bounds the prompts, for
+// states that meet bf16 on every other side: the outputs are as far off either way, by their own rounding.
 // Differences of G are taken in 64 bits before they are rounded: after a long decay G is large, and its fp32 steps would
 // show in e^(G_i - G_j).
 // A chunk with a value that is not finite, or a decay above 1, goes token by token (the same recurrence), so that nothing

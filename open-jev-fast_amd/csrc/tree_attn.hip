@@ -16,8 +16,8 @@
 //   * O^T += V^T P^T: P^T is the B operand as the lane holds it, with the contraction in the order 4 of the first 16
 //     positions, 4 of the second; V^T comes from LDS rows by transposing reads (ds_read_b64_tr_b16: 16 lanes get 4 x 16
 //     elements column by column).
-// P is rounded to bf16 as every operand of these products is (half a step, 2^-8 of each weight); the sum of the weights and
-// the outputs are fp32. e4m3 keys and values become bf16, which is exact; a position's scales go into its score and weight.
+// P is rounded to bf16 as every operand of these products is (half a step, 2^-8 of each weight): outputs are up to a fourth
+// further off than their own rounding alone; the sum of the weights and the outputs are fp32. e4m3 keys and values become bf16, which is exact; a position's scales go into its score and weight.
 // Units in which a row may not see every position (drafted ones, the sequence's end, pages outside the cache) also mask,
 // take the values of places that nobody sees as zeros and keep values that are not finite apart, so that a NaN reaches the
 // rows that see it and no other.

@@ -517,7 +517,8 @@ def kv_cache_write(k, v, slots, kc, vc, ks=None, vs=None):
     """Writes N tokens' keys and values into a paged cache, in place. k, v bf16 [HKV, N, D] (fullattn_prep2's kt and vt,
     with or without their batch axis); slots int64 [N], page index * page + place (outside the cache: not written); kc, vc
     [pages, HKV, page, D], bf16, or float8_e4m3fn with the rows' scales ks, vs fp32 [pages, HKV, page]. The e4m3 form
-    stores x / scale with scale the smallest power of two that brings the row within +-448."""
+    stores x / scale with scale the smallest power of two that brings the row within +-448. Two tokens with one slot leave a
+    mixture of both there."""
     HKV, N, D = _heads_rows(k, "k")
     if tuple(_heads_rows(v, "v")) != (HKV, N, D):
         raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
