@@ -406,6 +406,24 @@ def test_tree_attn_values_not_finite_of_no_weight(ext, dev, n, G, fmt):
     assert torch.equal(got[~bad], want[~bad]) and torch.equal(lse, clean_lse)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,G", [(5, 2), (14, 4), (40, 5)])
+def test_tree_attn_keys_not_finite(ext, dev, n, G, fmt):
+    """A NaN in a drafted token's key makes the rows that see it NaN, lse included, and changes no bit of the others."""
+    _say(f"case keys {n} {G} {fmt}")
+    ctx, page, D = 700, 64, 128
+    c = _tree_case([n, 3], [ctx, 40], 2, G, D, page, fmt, dev, seed=n, ext=ext)
+    want, want_lse = _run_tree(ext, c, dev)
+    see = torch.tensor([bool(int(c["bits"][i, 0]) >> 2 & 1) for i in range(n)] + [False] * 3)
+    assert bool(see.any()) and not bool(see[:n].all())
+    raw, bad = (torch.uint8, 0x7f) if fmt == "e4m3" else (torch.int16, 0x7fc0)
+    c["kc"].view(raw)[int(c["table"][0, (ctx + 2) // page]), :, (ctx + 2) % page, 9] = bad
+    out, lse = _run_tree(ext, c, dev)
+    see = see.to(dev)
+    assert bool(torch.isnan(out[see].float()).all()) and bool(torch.isnan(lse[see]).all())
+    assert torch.equal(out[~see], want[~see]) and torch.equal(lse[~see], want_lse[~see])
+
+
 @pytest.mark.parametrize("n,D", [(1, 256), (6, 128), (30, 256)])
 def test_tree_attn_graph_of_growing_contexts(ext, dev, n, D):
     """One captured call, replayed while the contexts on the device grow and shrink: lengths are looked at on the device,
@@ -907,6 +925,47 @@ def test_linattn_prompt_hands_its_state_on_exactly(ext, dev, HK, G, delta):
         part, state = ext.linattn_prompt(q[r], k[r], v[r], g[r], None if beta is None else beta[r], ptr(r.stop - t), state)
         assert torch.equal(part, o[r]), t
     assert torch.equal(state, last)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("HK,G,more", [(1, 2, 0), (2, 1, 60)])
+def test_linattn_prompt_decays_above_one(ext, C, dev, HK, G, more, delta):
+    """A decay above 1 is no decay of these layers, but a number: chunks with one go token by token, others do not. Both
+    forms."""
+    _say(f"case above one HK={HK} G={G} more={more} delta={delta}")
+    lengths = [200, 1, 70] + [5] * more
+    args = _lin_case(sum(lengths), HK, G, delta, seed=77)
+    for t, x in ((70, 0.3), (100, 1e-3), (200, 2.0), (sum(lengths) - 1, 0.05)):
+        args[3][t, -1] = x
+    ptr = torch.tensor([0] + list(torch.tensor(lengths).cumsum(0)), dtype=torch.int32)
+    o, last = ext.linattn_prompt(*_put(dev, *args, ptr))
+    _check_lin(C, args, lengths, None, o, last, 128 ** -0.5)
+
+
+def test_linattn_past_32_bits(ext, dev):
+    """States, rows and scratch whose offsets pass 2^32: the same bits as in a call on a few."""
+    HK, HV, slots = 16, 48, 5600
+    pool = torch.empty(slots, HV, 128, 128, device=dev)        # 4.4e9 values
+    g = torch.Generator(device=dev).manual_seed(3)
+    some = torch.randn(2, HV, 128, 128, device=dev, generator=g)
+    at = torch.tensor([slots - 1, 0], dtype=torch.int32, device=dev)
+    pool[at.long()] = some
+    args = _put(dev, *_lin_case(140, HK, 3, True, seed=3))
+    ptr = torch.tensor([0, 70, 140], dtype=torch.int32, device=dev)
+    few = torch.arange(2, dtype=torch.int32, device=dev)
+    a, b = ext.linattn_prompt(*args, ptr, pool, at), ext.linattn_prompt(*args, ptr, some, few)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    one = [t[:2].contiguous() for t in args]
+    a, b = ext.linattn_step(*one, pool, at), ext.linattn_step(*one, some, few)
+    assert torch.equal(a, b) and torch.equal(pool[at.long()], some)
+    del pool
+    R, tail = 360000, 300                                      # 4.4e9 bytes of v, 6.8e9 of scratch
+    big = [(torch.randn(R, n, device=dev, generator=g) * 0.1).bfloat16() for n in (HK * 128, HK * 128, HV * 128)]
+    big += [-torch.rand(R, HV, device=dev, generator=g), torch.rand(R, HV, device=dev, generator=g).bfloat16()]
+    ends = torch.tensor([0, R - tail, R], dtype=torch.int32, device=dev)
+    a = ext.linattn_prompt(*big, ends)
+    b = ext.linattn_prompt(*[t[R - tail:].contiguous() for t in big], torch.tensor([0, tail], dtype=torch.int32, device=dev))
+    assert torch.equal(a[0][R - tail:], b[0]) and torch.equal(a[1][1:], b[1]) and bool(torch.isfinite(a[1]).all())
 
 
 def test_linattn_is_causal_in_what_is_not_finite(ext, dev):
