@@ -149,10 +149,10 @@ __global__ void __launch_bounds__(256) linattn_step_k(LinParams p, float* state,
 // diag(e^(G_C - G)) T, the two products in which T is used. linattn_prompt_k then goes through a sequence's chunks in order.
 //
 // Precision. The states are fp32, and so is what makes them: a factor that is not a bf16 input (S0, X, U, the products with
-// T) enters its products as two bf16 pieces, hi + lo, which keep 16 bits and more (K, Q and V are bf16 already). The states
-// come out 5e-6 off 64 bits, relative to their norm, after 288 tokens as after 16384 (1.4e-6 without the delta rule; fp32
-// products would be 1.2e-7 off). A third piece is half as many products again on the chain that bounds the prompts, for
-// states that meet bf16 on every other side: the outputs are as far off either way, by their own rounding.
+// T) enters the products that make states as three bf16 pieces, which hold all of an fp32, and leave out what is 2^-24 of
+// the result. The states come out 1e-7 off 64 bits, relative to their norm, after 288 tokens as after 16384 (torch's fp32
+// products: 1.2e-7; with two pieces: 5e-6, and 637 us for 16384 tokens in place of 758, 163 for 16 x 539 in place of 190).
+// Outputs are rounded to bf16, half a step of 2^-8: what only they meet (S0 with Q, P T, X with P T) enters in two pieces.
 // Differences of G are taken in 64 bits before they are rounded: after a long decay G is large, and its fp32 steps would
 // show in e^(G_i - G_j).
 // A chunk with a value that is not finite, or a decay above 1, goes token by token (the same recurrence), so that nothing
@@ -171,7 +171,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t head_rows(const void* x, int64
 }
 
 // What a chunk of a head leaves for linattn_prompt_k, in the order in which it goes to LDS. The matrices are A operands of
-// 16 x 32 products, one lane's 8 values after the other, hi and lo: operand (it, ks) covers tokens 16 it .. + 15 against
+// 16 x 32 products, one lane's 8 values after the other, piece by piece: operand (it, ks) covers tokens 16 it .. + 15 against
 // tokens 32 ks .. + 31, the latter in the order in which a lane holds the other factor: 4 of the first 16, 4 of the
 // second. Those above the diagonal are left out: (0, 0), (1, 0), (2, 0), (2, 1), (3, 0), (3, 1) are here.
 struct ChunkWork {
@@ -180,7 +180,7 @@ struct ChunkWork {
   int32_t odd;                                  // token by token
   int32_t pad[62];
   uint16_t P[2][6][64][8];                      // scale P T (without the delta rule scale P)
-  uint16_t T[2][6][64][8];                      // diag(to) T; the delta rule's last part
+  uint16_t T[3][6][64][8];                      // diag(to) T; the delta rule's last part
 };
 static_assert(offsetof(ChunkWork, P) == 1024, "whole 1-KB pieces");
 constexpr int chunk_bytes(bool delta) { return delta ? (int)sizeof(ChunkWork) : (int)offsetof(ChunkWork, T); }
@@ -188,17 +188,30 @@ __device__ __forceinline__ constexpr int frag(int it, int ks) { return it < 2 ? 
 
 __device__ __forceinline__ int seq_chunks(int, int n) { return (n + kChunk - 1) / kChunk; }
 
-// Two bf16 pieces of 8 values: x = hi + lo to 16 bits.
-__device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8& hi, bf16x8& lo) {
-  uint32_t h[4], l[4];
+// x and y less a pair of bf16.
+__device__ __forceinline__ void less_pair(float& x, float& y, uint32_t pair) {
+  x -= __uint_as_float(pair << 16);
+  y -= __uint_as_float(pair & 0xffff0000u);
+}
+// bf16 pieces of 8 values: hi + lo is x to 16 bits, with low all of an fp32's 24.
+__device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8& hi, bf16x8& lo, bf16x8& low) {
+  uint32_t h[4], l[4], m[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float x = i < 2 ? a[2 * i] : b[2 * i - 4], y = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+    float x = i < 2 ? a[2 * i] : b[2 * i - 4], y = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
     h[i] = cvt_pk2(x, y);
-    l[i] = cvt_pk2(x - __uint_as_float(h[i] << 16), y - __uint_as_float(h[i] & 0xffff0000u));
+    less_pair(x, y, h[i]);
+    l[i] = cvt_pk2(x, y);
+    less_pair(x, y, l[i]);
+    m[i] = cvt_pk2(x, y);
   }
   hi = __builtin_bit_cast(bf16x8, make_uint4(h[0], h[1], h[2], h[3]));
   lo = __builtin_bit_cast(bf16x8, make_uint4(l[0], l[1], l[2], l[3]));
+  low = __builtin_bit_cast(bf16x8, make_uint4(m[0], m[1], m[2], m[3]));
+}
+__device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8& hi, bf16x8& lo) {
+  bf16x8 low;  // not asked for, not computed
+  split8(a, b, hi, lo, low);
 }
 __device__ __forceinline__ f32x4 widen(bf16x4 x) {
   const uint2 v = __builtin_bit_cast(uint2, x);
@@ -425,9 +438,11 @@ __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
     *reinterpret_cast<bf16x8*>(out->P[0][frag(w, ks)][lane]) = hi;
     *reinterpret_cast<bf16x8*>(out->P[1][frag(w, ks)][lane]) = lo;
     if (DELTA) {
-      split8(*reinterpret_cast<const f32x4*>(Ab + x), *reinterpret_cast<const f32x4*>(Ab + y) * (both ? 1.f : 0.f), hi, lo);
+      bf16x8 low;
+      split8(*reinterpret_cast<const f32x4*>(Ab + x), *reinterpret_cast<const f32x4*>(Ab + y) * (both ? 1.f : 0.f), hi, lo, low);
       *reinterpret_cast<bf16x8*>(out->T[0][frag(w, ks)][lane]) = hi;
       *reinterpret_cast<bf16x8*>(out->T[1][frag(w, ks)][lane]) = lo;
+      *reinterpret_cast<bf16x8*>(out->T[2][frag(w, ks)][lane]) = low;
     }
   }
   if (w != 0) return;
@@ -462,29 +477,38 @@ __device__ __forceinline__ void zero_rows(const LinParams& p, int h) {
 // the stage are there; X's pieces are there.
 __device__ __forceinline__ constexpr int key_dim(int d, int g) { return (d >> 1) * 32 + g * 8 + (d & 1) * 4; }
 
-// x = the 64 rows at `rows` (aoff: a lane's place in a row of 16 for key dims 32 s ..) times the state's two pieces.
-// Products on one accumulator follow each other with others between them: one waits for the one before on its accumulator
-// twice as long as it occupies the unit.
-__device__ __forceinline__ void rows_times(const uint8_t* rows, const int (&aoff)[4], const bf16x8 (&sh)[4],
-                                           const bf16x8 (&sl)[4], f32x4 (&x)[4]) {
+// x = the 64 rows at `rows` (aoff: a lane's place in a row of 16 for key dims 32 s ..) times the state's pieces, sp[0] the
+// largest; the others are summed apart, so that only sp[0]'s sums round at the size of the result. Products on one
+// accumulator follow each other with others between them: one waits for the one before on its accumulator twice as long as
+// it occupies the unit.
+template <int PIECES>
+__device__ __forceinline__ void rows_times(const uint8_t* rows, const int (&aoff)[4], const bf16x8 (&sp)[PIECES][4],
+                                           f32x4 (&x)[4]) {
+  f32x4 rest[4];
 #pragma unroll
-  for (int it = 0; it < 4; ++it) x[it] = f32x4{};
+  for (int it = 0; it < 4; ++it) x[it] = rest[it] = f32x4{};
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     bf16x8 a[4];
 #pragma unroll
     for (int it = 0; it < 4; ++it) a[it] = *reinterpret_cast<const bf16x8*>(rows + it * 4096 + aoff[s]);
 #pragma unroll
-    for (int part = 0; part < 2; ++part)
+    for (int part = 0; part < PIECES; ++part)
 #pragma unroll
-      for (int it = 0; it < 4; ++it) x[it] = mfma(a[it], part == 0 ? sh[s] : sl[s], x[it]);
+      for (int it = 0; it < 4; ++it) {
+        f32x4& to = PIECES > 2 && part > 0 ? rest[it] : x[it];
+        to = mfma(a[it], sp[part][s], to);
+      }
   }
+#pragma unroll
+  for (int it = 0; it < 4; ++it)
+    if (PIECES > 2) x[it] += rest[it];
 }
 
-// x += m b, m a chunk's lower triangular matrix in two pieces, b in two (lo lo is left out) or, exact, in one.
-template <bool TWO>
-__device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], int lane, const bf16x8 (&bh)[2],
-                                            const bf16x8 (&bl)[2], f32x4 (&x)[4]) {
+// x += P b for the outputs, P a chunk's lower triangular matrix in two pieces, b in two (lo lo is left out) or, exact, in one.
+template <bool TWO, int PIECES>
+__device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], int lane, const bf16x8 (&b)[PIECES][2],
+                                            f32x4 (&x)[4]) {
 #pragma unroll
   for (int part = 0; part < 2; ++part)
 #pragma unroll
@@ -495,8 +519,33 @@ __device__ __forceinline__ void lower_times(const uint16_t (&m)[2][6][64][8], in
 #pragma unroll
       for (int piece = 0; piece < (TWO && part == 0 ? 2 : 1); ++piece)
 #pragma unroll
-        for (int it = 2 * k; it < 4; ++it) x[it] = mfma(a[it], piece == 0 ? bh[k] : bl[k], x[it]);
+        for (int it = 2 * k; it < 4; ++it) x[it] = mfma(a[it], b[piece][k], x[it]);
     }
+}
+
+// u = T X, both in three pieces: the products of pieces down to 2^-16 of the largest, that one summed apart from the others.
+__device__ __forceinline__ void strengths_times(const uint16_t (&T)[3][6][64][8], int lane, const bf16x8 (&xp)[3][2],
+                                                f32x4 (&u)[4]) {
+  f32x4 rest[4];
+#pragma unroll
+  for (int it = 0; it < 4; ++it) u[it] = rest[it] = f32x4{};
+#pragma unroll
+  for (int part = 0; part < 3; ++part)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      bf16x8 a[4];
+#pragma unroll
+      for (int it = 2 * k; it < 4; ++it) a[it] = *reinterpret_cast<const bf16x8*>(T[part][frag(it, k)][lane]);
+#pragma unroll
+      for (int piece = 0; piece < 3 - part; ++piece)
+#pragma unroll
+        for (int it = 2 * k; it < 4; ++it) {
+          f32x4& to = part + piece > 0 ? rest[it] : u[it];
+          to = mfma(a[it], xp[piece][k], to);
+        }
+    }
+#pragma unroll
+  for (int it = 0; it < 4; ++it) u[it] += rest[it];
 }
 
 // The state that sequence sq starts from: value dim dv, this lane's key dims.
@@ -669,11 +718,11 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
       stage_barrier();
       const bool more = ch + 1 < chunks;
       uint8_t* const other = smem + ((ch + 1) & 1) * STAGE;
-      bf16x8 sh[4], sl[4];
+      bf16x8 sp[2][4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        sh[s] = s0[(2 * s) * 64];
-        sl[s] = s0[(2 * s + 1) * 64];
+        sp[0][s] = s0[(2 * s) * 64];
+        sp[1][s] = s0[(2 * s + 1) * 64];
       }
       // the next chunk's DMAs, in two lots: all at once they would hold up the wave
       if (more) {
@@ -681,7 +730,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         fetch(1, t0 + kChunk, other);
       }
       f32x4 x[4];
-      rows_times(stage + QO, aoff, sh, sl, x);
+      rows_times(stage + QO, aoff, sp, x);
 #pragma unroll
       for (int it = 0; it < 4; ++it) x[it] *= *reinterpret_cast<const f32x4*>(cw.out + it * 16 + g * 4);
       if (more) {
@@ -693,13 +742,13 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         wait_vmcnt<0>();
         continue;
       }
-      bf16x8 xh[2], xl[2];
+      bf16x8 xp[2][2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        xh[k] = x0[(2 * k) * 64];
-        if (DELTA) xl[k] = x0[(2 * k + 1) * 64];
+        xp[0][k] = x0[(2 * k) * 64];
+        if (DELTA) xp[1][k] = x0[(2 * k + 1) * 64];
       }
-      lower_times<DELTA>(cw.P, lane, xh, xl, x);
+      lower_times<DELTA>(cw.P, lane, xp, x);
       store_out(p, head_rows(p.o, first + t0, cnt, p.HV, h), g, dv, x);
     }
     return;
@@ -716,17 +765,18 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   // Every step is taken in halves, so that one half's conversions run behind the other's products; products on one
   // accumulator are two apart (one waits for the one before it twice as long as it occupies the unit); what the second part
   // of a chunk reads from LDS is read in the first.
-  bf16x8 sh[4], sl[4];
+  bf16x8 sp[3][4];
+  const auto split_state = [&](int s) { split8(st[2 * s], st[2 * s + 1], sp[0][s], sp[1][s], sp[2][s]); };
 #pragma unroll
-  for (int s = 0; s < 4; ++s) split8(st[2 * s], st[2 * s + 1], sh[s], sl[s]);
+  for (int s = 0; s < 4; ++s) split_state(s);
   for (int ch = 0; ch < chunks; ++ch) {
     const int t0 = ch * kChunk, cnt = min(kChunk, n - t0);
     const uint8_t* const stage = smem + (ch & 1) * STAGE;
     const ChunkWork& cw = *reinterpret_cast<const ChunkWork*>(stage);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      s0[(2 * s) * 64] = sh[s];
-      s0[(2 * s + 1) * 64] = sl[s];
+      s0[(2 * s) * 64] = sp[0][s];
+      s0[(2 * s + 1) * 64] = sp[1][s];
     }
     stage_barrier();
     const auto tr = [](const uint8_t* a) {
@@ -734,7 +784,7 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
     };
     // The order of the reads from LDS is fixed (sched_barrier): each goes out while the products before its use run.
     f32x4 x[4], from[4], to[4];
-    bf16x8 ka[2][4][2], T[2][6];
+    bf16x8 ka[2][4][2], T[3][6];
     bf16x4 vt[4], kt[8][4];  // V's columns (X's accumulators' places); K^T: accumulator d's key dims, tokens 16 t + 4 g ..
     if (DELTA) {
 #pragma unroll
@@ -746,13 +796,15 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
             ka[half][s][e] = *reinterpret_cast<const bf16x8*>(stage + KO + half * 8192 + e * 4096 + aoff[s]);
     }
     const auto keys_times_state = [&](int half) {
-      x[2 * half] = x[2 * half + 1] = f32x4{};
+      f32x4 sum[2][2]{};  // the largest piece's products, the others'
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+        for (int part = 0; part < 3; ++part)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) x[2 * half + e] = mfma(ka[half][s][e], part == 0 ? sh[s] : sl[s], x[2 * half + e]);
+          for (int e = 0; e < 2; ++e) sum[part > 0][e] = mfma(ka[half][s][e], sp[part][s], sum[part > 0][e]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) x[2 * half + e] = sum[0][e] + sum[1][e];
     };
     __builtin_amdgcn_sched_barrier(0);
     if (DELTA) keys_times_state(0);
@@ -770,11 +822,11 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
     __builtin_amdgcn_sched_barrier(0);
     if (DELTA) keys_times_state(1);
     __builtin_amdgcn_sched_barrier(0);
-    if (DELTA)
+    if (DELTA) {
 #pragma unroll
-      for (int f = 0; f < 6; ++f) {
-        T[0][f] = *reinterpret_cast<const bf16x8*>(cw.T[0][f][lane]);
-        T[1][f] = *reinterpret_cast<const bf16x8*>(cw.T[1][f][lane]);
+      for (int f = 0; f < 6; ++f)
+#pragma unroll
+        for (int part = 0; part < 3; ++part) T[part][f] = *reinterpret_cast<const bf16x8*>(cw.T[part][f][lane]);
       }
     __builtin_amdgcn_sched_barrier(0);
     const bool slow = __any(odd != 0 || odd_values(vt));
@@ -783,11 +835,11 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
       stage_barrier();
       by_tokens<DELTA>(p, stage + KO, stage + QO, first + t0, cnt, h, g, dv, st);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) split8(st[2 * s], st[2 * s + 1], sh[s], sl[s]);
+      for (int s = 0; s < 4; ++s) split_state(s);
       continue;
     }
 
-    bf16x8 xh[2], xl[2];  // X, or V itself
+    bf16x8 xp[3][2];  // X, or V itself
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (DELTA) {
@@ -795,12 +847,12 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
         for (int it = 2 * k; it < 2 * k + 2; ++it) {
           x[it] = widen(vt[it]) - from[it] * x[it];
         }
-        split8(x[2 * k], x[2 * k + 1], xh[k], xl[k]);
-        x0[(2 * k + 1) * 64] = xl[k];
+        split8(x[2 * k], x[2 * k + 1], xp[0][k], xp[1][k], xp[2][k]);
+        x0[(2 * k + 1) * 64] = xp[1][k];
       } else {
-        xh[k] = join(vt[2 * k], vt[2 * k + 1]);
+        xp[0][k] = join(vt[2 * k], vt[2 * k + 1]);
       }
-      x0[(2 * k) * 64] = xh[k];
+      x0[(2 * k) * 64] = xp[0][k];
     }
 #pragma unroll
     for (int s = 0; s < 4; ++s)
@@ -816,36 +868,44 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 #pragma unroll
     for (int half = 0; half < 2; ++half)
       if (DELTA) {
-        u[2 * half] = u[2 * half + 1] = f32x4{};
+        f32x4 sum[2][2]{};  // the product of the largest pieces, those down to 2^-16 of it
 #pragma unroll
         for (int k = 0; k <= half; ++k)
 #pragma unroll
-          for (int part = 0; part < 3; ++part)  // hi hi, hi lo, lo hi
+          for (int part = 0; part < 3; ++part)
 #pragma unroll
-            for (int it = 2 * half; it < 2 * half + 2; ++it)
-              u[it] = mfma(T[part >> 1][frag(it, k)], part & 1 ? xl[k] : xh[k], u[it]);
+            for (int piece = 0; piece < 3 - part; ++piece)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                sum[part + piece > 0][e] = mfma(T[part][frag(2 * half + e, k)], xp[piece][k], sum[part + piece > 0][e]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) u[2 * half + e] = sum[0][e] + sum[1][e];
       } else {
         u[2 * half] = to[2 * half] * widen(vt[2 * half]);
         u[2 * half + 1] = to[2 * half + 1] * widen(vt[2 * half + 1]);
       }
-    // the state
-#pragma unroll
-    for (int d = 0; d < 8; ++d) st[d] *= all;
+    // the state: what the chunk adds is summed by itself, so that the state rounds once a chunk
+    f32x4 add[8];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      bf16x8 uh, ul;
-      split8(u[2 * k], u[2 * k + 1], uh, ul);
+      bf16x8 up[3];
+      split8(u[2 * k], u[2 * k + 1], up[0], up[1], up[2]);
 #pragma unroll
       for (int d = 0; d < 8; d += 2) {
         const bf16x8 a = join(kt[d][2 * k], kt[d][2 * k + 1]), b = join(kt[d + 1][2 * k], kt[d + 1][2 * k + 1]);
-        st[d] = mfma(a, uh, st[d]);
-        st[d + 1] = mfma(b, uh, st[d + 1]);
-        st[d] = mfma(a, ul, st[d]);
-        st[d + 1] = mfma(b, ul, st[d + 1]);
-        if (k == 1 && d >= 2) split8(st[d - 2], st[d - 1], sh[d / 2 - 1], sl[d / 2 - 1]);
+        if (k == 0) add[d] = add[d + 1] = f32x4{};
+#pragma unroll
+        for (int part = 2; part >= 0; --part) {
+          add[d] = mfma(a, up[part], add[d]);
+          add[d + 1] = mfma(b, up[part], add[d + 1]);
+        }
+        if (k == 0) continue;
+        st[d] = st[d] * all + add[d];
+        st[d + 1] = st[d + 1] * all + add[d + 1];
+        if (d >= 2) split_state(d / 2 - 1);
       }
     }
-    split8(st[6], st[7], sh[3], sl[3]);
+    split_state(3);
   }
   store_state(p, sq, h, g, dv, st);
 }
@@ -969,33 +1029,41 @@ __global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
       wait_vmcnt<0>();
       continue;
     }
-    bf16x8 sh[4], sl[4];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) split8(st[2 * s], st[2 * s + 1], sh[s], sl[s]);
+    bf16x8 sp[2][4];  // the state before the chunk, for the outputs
     if (more) fetch(1, t0 + kChunk, other);
-    bf16x8 xh[2], xl[2];  // X, or V itself
+    bf16x8 xp[3][2];  // X, or V itself
     if (DELTA) {
       f32x4 x[4];
-      rows_times(stage + KO, aoff, sh, sl, x);
+      bf16x8 all3[3][4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        split8(st[2 * s], st[2 * s + 1], all3[0][s], all3[1][s], all3[2][s]);
+        sp[0][s] = all3[0][s];
+        sp[1][s] = all3[1][s];
+      }
+      rows_times(stage + KO, aoff, all3, x);
 #pragma unroll
       for (int it = 0; it < 4; ++it)
         x[it] = widen(vt[it]) - *reinterpret_cast<const f32x4*>(cw.from + it * 16 + g * 4) * x[it];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) split8(x[2 * k], x[2 * k + 1], xh[k], xl[k]);
+      for (int k = 0; k < 2; ++k) split8(x[2 * k], x[2 * k + 1], xp[0][k], xp[1][k], xp[2][k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) xh[k] = join(vt[2 * k], vt[2 * k + 1]);
+      for (int s = 0; s < 4; ++s) split8(st[2 * s], st[2 * s + 1], sp[0][s], sp[1][s]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) xp[0][k] = join(vt[2 * k], vt[2 * k + 1]);
     }
     // U, decayed to the chunk's end, and the state
-    bf16x8 uh[2], ul[2];
+    bf16x8 up[3][2];
     {
       f32x4 u[4];
+      if (DELTA)
+        strengths_times(cw.T, lane, xp, u);
+      else
 #pragma unroll
-      for (int it = 0; it < 4; ++it)
-        u[it] = DELTA ? f32x4{} : *reinterpret_cast<const f32x4*>(cw.to + it * 16 + g * 4) * widen(vt[it]);
-      if (DELTA) lower_times<true>(cw.T, lane, xh, xl, u);
+        for (int it = 0; it < 4; ++it) u[it] = *reinterpret_cast<const f32x4*>(cw.to + it * 16 + g * 4) * widen(vt[it]);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) split8(u[2 * k], u[2 * k + 1], uh[k], ul[k]);
+      for (int k = 0; k < 2; ++k) split8(u[2 * k], u[2 * k + 1], up[0][k], up[1][k], up[2][k]);
     }
     const float all = cw.all;
 #pragma unroll
@@ -1003,21 +1071,21 @@ __global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
       bf16x4 kt[4][4];  // key dims of d .. d + 3, tokens 16 t + 4 g ..
       tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2], stage + toff[d / 2] + 8, kt[0], kt[1]);
       tr_read8<0, 4096, 8192, 12288>(stage + toff[d / 2 + 1], stage + toff[d / 2 + 1] + 8, kt[2], kt[3]);
+      f32x4 add[4]{};  // by itself, so that the state rounds once a chunk
 #pragma unroll
-      for (int e = 0; e < 4; ++e) st[d + e] *= all;
+      for (int part = 2; part >= 0; --part)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+          for (int e = 0; e < 4; ++e) add[e] = mfma(join(kt[e][2 * k], kt[e][2 * k + 1]), up[part][k], add[e]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            st[d + e] = mfma(join(kt[e][2 * k], kt[e][2 * k + 1]), part == 0 ? uh[k] : ul[k], st[d + e]);
+      for (int e = 0; e < 4; ++e) st[d + e] = st[d + e] * all + add[e];
     }
     f32x4 x[4];
-    rows_times(stage + QO, aoff, sh, sl, x);
+    rows_times(stage + QO, aoff, sp, x);
 #pragma unroll
     for (int it = 0; it < 4; ++it) x[it] *= *reinterpret_cast<const f32x4*>(cw.out + it * 16 + g * 4);
-    lower_times<DELTA>(cw.P, lane, xh, xl, x);
+    lower_times<DELTA>(cw.P, lane, xp, x);
     store_out(p, head_rows(p.o, first + t0, cnt, p.HV, h), g, dv, x);
   }
   store_state(p, sq, h, g, dv, st);

@@ -109,7 +109,7 @@ def linattn(q, k, v, g, beta, lengths, state, scale):
     """Sequences one after the other in the rows, state fp64 [S, HV, 128, 128] or None. (o fp64 [R, HV, 128], states,
     bound of |o - kernel| [R, HV, 128], bound of the states' error in the 2-norm of each head [S, HV]).
 
-    A kernel that keeps the state's products to two bf16 pieces commits at each token errors of at most e = 2 u^2 times
+    A kernel with two bf16 pieces or more in the state's products commits at each token errors of at most e = 2 u^2 times
     what it adds up: S^T k, the u of the tokens before in its chunk of 64, and the new state. An error in S is carried on
     by e^g (I - beta k k^T), which is no larger than e^g while beta |k|^2 <= 2: the bound E of the state's error follows
     the recurrence E <- e^g E + committed, and |o| is off by scale |q| E, by u on each factor that it takes in bf16 and
@@ -160,11 +160,12 @@ def linattn_chunk(q, k, v, g, beta, lengths, state, scale):
     They hold for a kernel that takes the tokens of a sequence at once,
       A_ij = beta_i e^(G_i - G_j) k_i . k_j (j < i),  P_ij = e^(G_i - G_j) q_i . k_j (j <= i),  T = (I + A)^-1 diag(beta),
       X = V - diag(e^G) K S0,  U = T X,  O = scale (diag(e^G) Q S0 + P U),  S = e^(G_n) S0 + K^T diag(e^(G_n - G)) U
-    (T the identity and U = V without beta), sums in fp32, and lets S0, X, P T, diag(e^(G_n - G)) T and U into its
-    products as two bf16 pieces. Of x, hi = bf16(x) and lo = bf16(x - hi) leave out at most U^2 |x|; a product of two such
-    factors leaves out lo lo, U^2 of it at most, besides. A sum of n terms is off by at most 2 F n times the sum of their
-    magnitudes, in any order and also where additions are cut off instead of rounded; n doubles with the pieces. An
-    exponential is off by its argument's rounding and a step of its own. The errors go through the formulas in magnitudes."""
+    (T the identity and U = V without beta), sums in fp32, and lets S0, X, diag(e^(G_n - G)) T and U into the products that
+    make states as three bf16 pieces, S0, P T and X into those that make outputs as two. Of x, hi = bf16(x) and lo =
+    bf16(x - hi) leave out at most U^2 |x|, a third piece U^3 |x|; a product of two such factors leaves out its smallest, lo
+    lo or three of U^3, besides. A sum of n terms is off by at most 2 F n times the sum of their magnitudes, in any order and
+    also where additions are cut off instead of rounded; n grows with the pieces. An exponential is off by its argument's
+    rounding and a step of its own. The errors go through the formulas in magnitudes."""
     R, HV = g.shape
     HK = k.shape[1] // 128
     G = HV // HK
@@ -174,7 +175,8 @@ def linattn_chunk(q, k, v, g, beta, lengths, state, scale):
     S = len(lengths)
     st, o = torch.zeros(S, HV, 128, 128, dtype=torch.float64), torch.zeros(R, HV, 128, dtype=torch.float64)
     bs, bo = torch.zeros_like(st), torch.zeros_like(o)
-    pieces, dot, tiny = U * U, 2 * F * 256, 1e-35     # tiny: factors below the smallest fp32 step
+    two, three, dot = U * U, U ** 3, 2 * F * 256
+    tiny = 1e-35                                                # factors below the smallest fp32 step
 
     def expo(x):
         """e^x and its relative error: the argument, to base two, in fp32, and a step of fp32 for the exponential."""
@@ -197,7 +199,7 @@ def linattn_chunk(q, k, v, g, beta, lengths, state, scale):
             since, dsince = (x[:, None] for x in expo(cum))
             to, dto = (x[:, None] for x in expo(cum[-1] - cum))
             KS, QS, SA = K @ S0, Q @ S0, S0.abs()
-            dKS, dQS = ((pieces + 2 * dot) * (x.abs() @ SA) for x in (K, Q))
+            dKS, dQS = ((left + 2 * dot) * (x.abs() @ SA) for x, left in ((K, three), (Q, two)))
             P = fade * (Q @ K.T)
             dP = fade * (dot * (Q.abs() @ K.abs().T) + (dfade + 2 * F) * (Q @ K.T).abs())
             if beta is None:
@@ -226,14 +228,14 @@ def linattn_chunk(q, k, v, g, beta, lengths, state, scale):
                 dW = P.abs() @ dT + dP @ T.abs() + 2 * F * n * (P.abs() @ T.abs())
                 W, dW = W.tril(), dW.tril()
                 u = T @ X
-                both = (3 * pieces + 2 * F * 3 * n) * (T.abs() @ X.abs())
+                both = (6 * three + 2 * F * 6 * n) * (T.abs() @ X.abs())
                 end, dend = to * u, to * (T.abs() @ dX + dT @ X.abs() + both + (dto + 2 * F) * (T.abs() @ X.abs()))
             S1, all_, dall = to * u, since[-1], dsince[-1]
             st[s, h] = all_ * S0 + K.T @ S1
-            bs[s, h] = ((dall + 2 * F) * all_ * SA + K.abs().T @ (dend + pieces * end.abs())
-                        + 2 * F * (2 * n + 2) * (K.abs().T @ end.abs() + all_ * SA)) * 1.01 + tiny
+            bs[s, h] = ((dall + 4 * F) * all_ * SA + K.abs().T @ (dend + three * end.abs())
+                        + 2 * F * (3 * n + 2) * (K.abs().T @ end.abs())) * 1.01 + tiny
             o[r, h] = scale * (since * QS + P @ u)
-            left = (3 if beta is not None else 1) * pieces
+            left = (3 if beta is not None else 1) * two
             err = since * dQS + (dsince + 3 * F) * (since * QS).abs() + W.abs() @ dX + dW @ X.abs()
             err = err + (left + 2 * F * (3 * n + 4)) * (W.abs() @ X.abs()) + 2 * F * (since * QS).abs()
             bo[r, h] = (abs(scale) * err * (1 + U) + U * o[r, h].abs()) * 1.01 + tiny

@@ -894,8 +894,8 @@ def test_linattn_prompt_many_in_a_graph(ext, dev, delta):
 
 @pytest.mark.parametrize("delta", [True, False])
 @pytest.mark.parametrize("HK,G", [(2, 1), (1, 3), (4, 3), (16, 1)])
-def test_linattn_prompt_keeps_two_pieces(ext, C, dev, HK, G, delta):
-    """Entry by entry, sequences of up to 64 tokens from given states stay within what two bf16 pieces a factor and fp32
+def test_linattn_prompt_keeps_its_pieces(ext, C, dev, HK, G, delta):
+    """Entry by entry, sequences of up to 64 tokens from given states stay within what the pieces of the factors and fp32
     sums give (in bounds that a single piece of any factor breaks). Both forms: 18 and 27 heads, 108 and 144."""
     _say(f"case pieces HK={HK} G={G} delta={delta}")
     lengths = [1, 2, 3, 5, 8, 16, 24, 40, 64]
@@ -907,6 +907,24 @@ def test_linattn_prompt_keeps_two_pieces(ext, C, dev, HK, G, delta):
     eo, es = (o.cpu().double().reshape(want.shape) - want).abs(), (last.cpu().double() - st).abs()
     _say(f"  out {(eo / bo).max().item():.3f}, state {(es / bs).max().item():.3f} of the bounds")
     assert bool((eo <= bo).all()) and bool((es <= bs).all())
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("S,HV", [(3, 2), (40, 3)])
+def test_linattn_prompt_states_are_fp32(ext, C, dev, S, HV, delta):
+    """States within a few steps of fp32 of 64 bits, relative to their norm, where a factor short of its third piece would
+    be 13 off and more. What a chunk leaves is down to e^-0.6 after the next, so that a long sequence is off by at most
+    1 / (1 - e^-0.6) = 2.2 times as much. Both forms."""
+    from tests.test_cores import STATE_STEPS, slow_chunks
+    _say(f"case fp32 S={S} HV={HV} delta={delta}")
+    args, lengths, state = slow_chunks(S, HV, delta, 5)
+    for each in ([64] * S, [64 * S] + [0] * (S - 1) if S < 10 else [64] * (S - 4) + [256, 0, 0, 0]):
+        ptr = torch.tensor([0] + list(torch.tensor(each).cumsum(0)), dtype=torch.int32)
+        last = ext.linattn_prompt(*_put(dev, *args, ptr, state))[1].cpu().double()
+        st = C.linattn(*args, each, state, 1.0)[1]
+        steps = (last - st).norm(dim=(2, 3)) / st.norm(dim=(2, 3)) / C.F
+        _say(f"  {steps.max().item():.2f} steps")
+        assert bool((steps <= STATE_STEPS * (1.0 if max(each) <= 64 else 2.2)).all())
 
 
 @pytest.mark.parametrize("delta", [True, False])
