@@ -262,8 +262,8 @@ __device__ __forceinline__ bool odd_top(uint32_t top) { return (top & 0xffffu) >
 //     when the contraction runs in its order; P T likewise.
 // LDS holds the ten lower blocks of each matrix, rows of 20 floats (so that 16 rows' 16-byte reads meet every bank once).
 // What bounds it: the chain of one chunk (loads, scan, substitution, up to 19 block products on one wave), so what counts
-// is how many workgroups a CU holds: four, by LDS and registers (16384 tokens of 48 heads: 155 us; 206 with two; MFMAs busy
-// 17% of the time, waves waiting half of theirs). A single round of them takes 11 us: 288 tokens.
+// is how many workgroups a CU holds: four, by LDS and registers (16384 tokens of 48 heads: 160 us; with two 206 against 155
+// before; MFMAs busy 16-19% of the time, waves waiting half of theirs). A single round of them takes 11 us: 288 tokens.
 template <bool DELTA>
 __global__ void __launch_bounds__(256, 4) linattn_chunk_k(LinParams p) {
   constexpr int LD = 20, BLK = 16 * LD;
@@ -640,8 +640,9 @@ __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcn
 // Few sequences: four workgroups a sequence and value head, each of two slices of 16 value dims, and for each slice a wave
 // with the state in its accumulators and a wave for the outputs and the DMAs, which works a chunk behind: the chain of a
 // chunk's products that need the state is all that the chunks wait for.
-// What bounds it: that chain, 2 us a chunk (16384 tokens of 48 heads: 509 us; over 800 with all of a slice in one wave),
-// half of it K, Q and the chunk's matrices out of LDS, half the new state's products; MFMAs are busy 18% of the time.
+// What bounds it: that chain, 2.4 us a chunk (16384 tokens of 48 heads: 600 us; with two pieces a factor 509, and over 800
+// with all of a slice in one wave): products that wait for each other, and the splits between them; MFMAs are busy 19% of the
+// time.
 template <bool DELTA>
 __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   constexpr int SL = 4;                  // workgroups of a head
@@ -652,8 +653,9 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = wave & 1;
-  // Workgroups go to the eight XCDs in turn. Of 32, the four of a head are eight apart: one L2 serves them (16384 tokens: 682
-  // -> 638 us, 1369 -> 459 MB read), and the heads still take the XCDs in turn, so that sequences of unlike lengths share them
+  // Workgroups go to the eight XCDs in turn. Of 32, the four of a head are eight apart: one L2 serves them (16384 tokens, with
+  // two pieces a factor: 682 -> 638 us, 1369 -> 459 MB read; with three 516 MB), and the heads still take the XCDs in turn,
+  // so that sequences of unlike lengths share them
   const uint32_t b = blockIdx.x, whole = (uint32_t)p.S * p.HV / 8 * (8 * SL);
   const uint32_t wg = b < whole ? (b / (8 * SL) * 8 + b % 8) * SL + b / 8 % SL : b;
   const int64_t sq = wg / (p.HV * SL);
@@ -912,10 +914,10 @@ __global__ void __launch_bounds__(256, 1) linattn_prompt_k(LinParams p) {
 
 // Many sequences: a workgroup of eight waves per sequence and value head, each with one slice and all of its work, so that
 // two waves a SIMD fill each other's gaps and what they share is loaded once a head: 16 sequences of up to 539 tokens, 48
-// heads, 118 us in this kernel (184 with slices as above), MFMAs busy 29%, 246 MB of memory, the chunks' matrices (25 KB
-// each) nearly half of them. (Here the waves that read K^T and V
-// transposed have DMAs in flight, and the builtin makes the compiler wait for those: the reads are written out, with the
-// wait for themselves in the same block, so that the registers are filled when it ends.)
+// heads, 151 us in this kernel (237 with slices as above), MFMAs busy 33%, 260 MB of memory, the chunks' matrices (31 KB
+// each) about half of them. (Here the waves that read K^T and V transposed have DMAs in flight, and the builtin makes the
+// compiler wait for those: the reads are written out, with the wait for themselves in the same block, so that the registers
+// are filled when it ends.)
 template <int X0, int X1, int X2, int X3>
 __device__ __forceinline__ void tr_read4(const uint8_t* pa, bf16x4 (&a)[4]) {
   const uint32_t x = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)pa;
@@ -955,7 +957,8 @@ __global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // the value heads of a key head on one XCD, as above (the call 163 -> 161 us, this kernel 176 -> 128 MB read)
+  // the value heads of a key head on one XCD, as above (with two pieces a factor: the call 163 -> 161 us, this kernel 176 ->
+  // 128 MB read; with three 142 MB)
   const uint32_t b = blockIdx.x, per = p.HV / p.HK, whole = (uint32_t)p.S * p.HK / 8 * (8 * per);
   const uint32_t wg = b < whole ? (b / (8 * per) * 8 + b % 8) * per + b / 8 % per : b;
   const int64_t sq = wg / p.HV;
@@ -1093,9 +1096,9 @@ __global__ void __launch_bounds__(512, 1) linattn_many_k(LinParams p) {
 
 constexpr int many_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * 768); }
 // Sequences times value heads up to which the workgroups of two slices run (four of them a head). Calls of 48-head sequences,
-// with slices and with eight waves a head: 500 tokens each, one sequence 32 and 49 us, two 50 and 51, three 71 and 56, six
-// 116 and 107; 4096 tokens each, one 159 and 297, two 312 and 340, three 461 and 383, six 811 and 772. (Three of unlike
-// lengths, 4096 and less: 322 and 352.)
+// with slices and with eight waves a head: 500 tokens each, one sequence 37 and 58 us, two 59 and 59, three 84 and 66, six
+// 143 and 127; 4096 tokens each, one 203 and 367, two 386 and 416, three 570 and 459, six 985 and 932. (Three of unlike
+// lengths, 4096 and less: 396 and 427.)
 constexpr int64_t kFew = 96;
 constexpr int prompt_lds(bool delta) { return 2 * (chunk_bytes(delta) + kChunk * (512 + 64)) + 2 * (8192 + 4096) + 16; }
 

@@ -10,7 +10,8 @@ Written from the definitions, one row or token at a time, apart from any kernel:
   linattn        linear attention token by token, with a bound of the kernel's error beside it
 
 The bounds follow the roundings a kernel is entitled to: half a step of bf16, u = 2^-8, on its output and on the weights
-that a matrix product takes in bf16; fp32 sums; and, for the states, factors of two bf16 pieces (u^2 = 2^-16 together).
+that a matrix product takes in bf16; fp32 sums; and, for linear attention, factors of two or three bf16 pieces (u^2 = 2^-16
+and u^3 = 2^-24 together).
 """
 import math
 
