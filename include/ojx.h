@@ -261,6 +261,87 @@ int ojx_linattn_step(const void* q, const void* k, const void* v, const float* g
                      const int32_t* slot, int64_t state_slots, int64_t R, int32_t HV, int32_t HK, float scale, void* o,
                      ojx_stream_t stream);
 
+/* Linear attention of drafted tokens: ojx_linattn_step for a tree of them, on states that stay as they are. Sequence b has
+ * the rows q_ptr[b] .. q_ptr[b+1] - 1 (int32 [B + 1], non-decreasing) and the state state[slot[b]] (slot int32 [B]). Row j of
+ * a sequence follows its row parents[j] (int32 [N], indexes within the sequence), or the state itself where parents[j] is
+ * not in [0, j); parents NULL: the row before it. Its output is that of ojx_linattn_prompt on the tokens of its path from
+ * the state: o bf16 [N, HV, 128]. A negative slot gives zeros, a slot of state_slots or more NaN; sequences may share a
+ * slot. Rows of no sequence get zeros. Operands as there. workspace: ojx_linattn_tree_workspace bytes of device memory,
+ * 16-byte aligned (0 = none needed). HV at most 1024, (B + 1) HV and N HV below 2^24.
+ * ojx_linattn_keep takes the states forward over the tokens that were kept: sequence b's rows path[q_ptr[b] + i], i = 0 ..
+ * count[b] - 1 (int32 [N] and [B], as ojx_verify_drafts leaves them; no more than the sequence has rows), one after the
+ * other, into state[slot[b]], in place. Entries outside the sequence are left out. States of no slot (negative, or
+ * state_slots and more), of a slot that an earlier sequence names too, and of no kept token stay as they are. */
+int64_t ojx_linattn_tree_workspace(int64_t N, int32_t B, int32_t HV, int32_t HK);
+int ojx_linattn_tree(const void* q, const void* k, const void* v, const float* g, const void* beta, const float* state,
+                     const int32_t* slot, int64_t state_slots, const int32_t* q_ptr, const int32_t* parents, int64_t N,
+                     int32_t B, int32_t HV, int32_t HK, float scale, void* o, void* workspace, int64_t workspace_bytes,
+                     ojx_stream_t stream);
+int ojx_linattn_keep(const void* k, const void* v, const float* g, const void* beta, float* state, const int32_t* slot,
+                     int64_t state_slots, const int32_t* q_ptr, const int32_t* path, const int32_t* count, int64_t N,
+                     int32_t B, int32_t HV, int32_t HK, ojx_stream_t stream);
+
+/* Verification of drafted tokens against the target's distributions. Sequence b has the rows q_ptr[b] .. q_ptr[b+1] - 1 of
+ * N; its row 0 is its last token, which stands, row j >= 1 the drafted token tokens[j] (int64 [N]) behind row parents[j]
+ * (int32 [N], indexes within the sequence; a row whose parents[j] is not in [0, j) is never accepted; NULL: the row before
+ * it). logits [N, V] (OJX_F32 or OJX_BF16, row stride ldl >= V, no alignment needed): row j's are the target's behind token
+ * j; with T = temperature[b] (fp32 [B]; NULL: 1) p = softmax(logits / T), or, where T is not above 0, all on the first
+ * largest logit. probs [N, V] (row stride ldp) or NULL: row j's is the distribution that the tokens behind row j were drawn
+ * from, each by itself (values that are not above 0 count as 0; not read where T is not above 0); NULL: they were certain.
+ * u fp32 [N], uniform in [0, 1).
+ * From row 0 on, the tokens behind the current row are tried in order: token x with the number u_j is accepted if
+ * u_j q(x) t < w(x), where w is what is left of p and t its sum (p and 1 at first). A token rejected leaves max(w / t - q,
+ * 0), without probs w less that token. An accepted row becomes the current one. When none is left, the next token is the
+ * first i with w_0 + .. + w_i > u_(row 0) t: the tokens come out distributed as the target's own. Where nothing is left of
+ * p, it is drawn from p. All in 64 bits.
+ * path int32 [N]: of each sequence the accepted rows in order, row 0 first, then -1; count int32 [B]: how many; next int64
+ * [B]. A sequence without rows gives count 0 and next -1. A row with a NaN or +infinity among its logits, or none above
+ * -infinity, accepts nothing and gives next -1. path is -1 in rows of no sequence.
+ * workspace: ojx_verify_drafts_workspace bytes of device memory, 16-byte aligned. V at most 2^22; (V / 8192 + 1) times N and
+ * B below 2^24, B at most 65536 (OJX_ERR_SHAPE otherwise; -1 from the workspace's size). */
+enum { OJX_F32 = 0, OJX_BF16 = 1 };
+int64_t ojx_verify_drafts_workspace(int64_t N, int32_t B, int64_t V, int32_t has_probs);
+int ojx_verify_drafts(const void* logits, int32_t logits_type, int64_t ldl, const int64_t* tokens, const int32_t* q_ptr,
+                      const float* u, const int32_t* parents, const void* probs, int32_t probs_type, int64_t ldp,
+                      const float* temperature, int64_t N, int32_t B, int64_t V, int32_t* path, int32_t* count,
+                      int64_t* next, void* workspace, int64_t workspace_bytes, ojx_stream_t stream);
+
+/* The kept tokens' keys and values moved together in a paged cache, in place: of sequence b the row at position ctx[b] +
+ * path[q_ptr[b] + i] goes to position ctx[b] + i, i = 0 .. count[b] - 1, all as if read before any is written. path, count
+ * and q_ptr as in ojx_verify_drafts (path rises; an entry below i or outside the sequence is left out), ctx and table as
+ * in ojx_tree_attn: a position without a page is neither read nor written. The cache is ojx_kv_cache_write's, `layers` of
+ * them one after the other ([layers, pages, HKV, page, D], scales [layers, pages, HKV, page]) that share one table; 2
+ * layers HKV at most 65535, and times B below 2^24. */
+int ojx_kv_cache_keep(void* kc, void* vc, float* ks, float* vs, int32_t fmt, int64_t layers, int64_t pages, int32_t HKV,
+                      int32_t page, int32_t D, const int32_t* table, int64_t max_pages, const int32_t* ctx,
+                      const int32_t* q_ptr, const int32_t* path, const int32_t* count, int64_t N, int32_t B,
+                      ojx_stream_t stream);
+
+/* Pages of a paged cache, managed where the tables are. table int32 [B, max_pages] names each sequence's pages (an entry
+ * outside [0, pages): none), refs int32 [pages] counts the entries that name each page, in all tables; a page whose count
+ * is not above 0 is free. Pages are taken from the lowest free one on, sequence by sequence; every call is deterministic.
+ * ojx_kv_pages_resize: sequence b gets pages for tokens[b] tokens (int32 [B]; negative: stays as it is): entries behind
+ * them are given back (counted down, -1), entries that name no page get one. missing int32 [B]: entries that got none, as
+ * the pool or the table had no room (they are -1).
+ * ojx_kv_pages_fork: slot b's sequence becomes a copy of slot src[b]'s (int32 [B]; b itself: stays as it is; outside [0, B):
+ * empty), all at once: tables and ctx (int32 [B]) are those before the call. Its own pages are given back, the pages that
+ * are full with the other's ctx tokens are shared, and a last page that is not full is taken anew: pairs int32 [B, 2] =
+ * (the other's last page, the new one), to be copied by ojx_kv_pages_copy in every layer before anything else is written
+ * to the cache or taken from the pool; (-1, -1) where there is none. A slot for which the pool has no page gets (page, -1)
+ * and ends with its last full page: ctx says so.
+ * ojx_kv_pages_copy: page pairs[i][0] -> page pairs[i][1] of a cache of `layers` layers (see ojx_kv_cache_keep), i < n; pairs
+ * with a page outside [0, pages) are left out. Pages written must not be among those read.
+ * workspace: ojx_kv_pages_workspace bytes of device memory, 16-byte aligned (fork: 1 for ojx_kv_pages_fork). B at most
+ * 65536, B max_pages below 2^31, a copy at most 2^24 pieces of 16 KB, n at most 65535. */
+int64_t ojx_kv_pages_workspace(int64_t B, int64_t max_pages, int64_t pages, int32_t fork);
+int ojx_kv_pages_resize(int32_t* table, int64_t max_pages, int32_t* refs, int64_t pages, const int32_t* tokens, int64_t B,
+                        int32_t page, int32_t* missing, void* workspace, int64_t workspace_bytes, ojx_stream_t stream);
+int ojx_kv_pages_fork(int32_t* table, int64_t max_pages, int32_t* ctx, int32_t* refs, int64_t pages, const int32_t* src,
+                      int64_t B, int32_t page, int32_t* pairs, void* workspace, int64_t workspace_bytes,
+                      ojx_stream_t stream);
+int ojx_kv_pages_copy(void* kc, void* vc, float* ks, float* vs, int32_t fmt, int64_t layers, int64_t pages, int32_t HKV,
+                      int32_t page, int32_t D, const int32_t* pairs, int64_t n, ojx_stream_t stream);
+
 /* Bytes of the static device scratch behind ojx_gemm_residual_rmsnorm_noalloc (one array per GPU). */
 #define OJX_NOALLOC_SCRATCH_BYTES (32LL << 20)
 

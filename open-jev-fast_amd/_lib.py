@@ -67,6 +67,19 @@ EXPORTS = {
     "ojx_linattn_prompt": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _f32, _p, _p, _p,
                                           _i64, _p]),
     "ojx_linattn_step": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _f32, _p, _p]),
+    "ojx_linattn_tree_workspace": (ctypes.c_int64, [_i64, _i32, _i32, _i32]),
+    "ojx_linattn_tree": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _p, _p, _i64, _i32, _i32, _i32, _f32, _p, _p, _i64,
+                                        _p]),
+    "ojx_linattn_keep": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i32, _i32, _p]),
+    "ojx_verify_drafts_workspace": (ctypes.c_int64, [_i64, _i32, _i64, _i32]),
+    "ojx_verify_drafts": (ctypes.c_int, [_p, _i32, _i64, _p, _p, _p, _p, _p, _i32, _i64, _p, _i64, _i32, _i64, _p, _p, _p,
+                                         _p, _i64, _p]),
+    "ojx_kv_cache_keep": (ctypes.c_int, [_p, _p, _p, _p, _i32, _i64, _i64, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _p, _i64,
+                                         _i32, _p]),
+    "ojx_kv_pages_workspace": (ctypes.c_int64, [_i64, _i64, _i64, _i32]),
+    "ojx_kv_pages_resize": (ctypes.c_int, [_p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _i64, _p]),
+    "ojx_kv_pages_fork": (ctypes.c_int, [_p, _i64, _p, _p, _i64, _p, _i64, _i32, _p, _p, _i64, _p]),
+    "ojx_kv_pages_copy": (ctypes.c_int, [_p, _p, _p, _p, _i32, _i64, _i64, _i32, _i32, _i32, _p, _i64, _p]),
     "ojx_add_rmsnorm": (ctypes.c_int, [_p, _p, _p, _p, _f32, _p, _p, _i64, _i64, _p]),
     "ojx_add_rmsnorm_sk": (ctypes.c_int, [_p, _p, _i32, _p, _p, _f32, _p, _p, _i64, _i64, _p]),
     "ojx_silu_mul": (ctypes.c_int, [_p, _p, _i64, _i64, _p]),
@@ -77,6 +90,7 @@ EXPORTS = {
 }
 
 KV_BF16, KV_E4M3 = 0, 1
+F32, BF16 = 0, 1
 KIND_PLAIN, KIND_SILU_MUL, KIND_RESIDUAL, KIND_PACKED = 0, 1, 2, 4
 
 _lib = None

@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(HERE, "libojx.so")
 SOURCES = ["gemm.hip", "gemm_sk.hip", "gemm_kx_a.hip", "gemm_kx_b.hip", "gemm_kx_c.hip", "epilogue.hip", "prep.hip", "kvcache.hip",
-           "tree_attn.hip", "linattn.hip", "api.hip"]
+           "tree_attn.hip", "linattn.hip", "lintree.hip", "kvpages.hip", "drafts.hip", "api.hip"]
 OBJDIR = os.path.join(HERE, "_build")
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -30,7 +30,7 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
 
 # The attention cores keep sums that both MFMA and VALU code update: with the products' results in ordinary registers (not
 # the accumulation ones) nothing is copied between the two files on every update, and nothing spills.
-FILE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in ("tree_attn.hip", "linattn.hip")}
+FILE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in ("tree_attn.hip", "linattn.hip", "lintree.hip")}
 
 
 def source_files():

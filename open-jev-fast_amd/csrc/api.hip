@@ -914,7 +914,199 @@ int check_linattn(const void* q, const void* k, const void* v, const float* g, c
   return OJX_OK;
 }
 
+int check_lintree_sizes(int64_t N, int32_t B, int32_t HV, int32_t HK) {
+  if (HK < 1 || HV < HK || HV % HK != 0 || HV > 1024)
+    return fail(OJX_ERR_SHAPE, "HV=%d must be a multiple of HK=%d, at most 1024", HV, HK);
+  if (N < 0 || N >= (1LL << 31) || B < 0 || (B + 1LL) * HV >= (1LL << 24) || N * HV >= (1LL << 24))
+    return fail(OJX_ERR_SHAPE, "N=%lld rows of B=%d sequences of %d heads: too many for one call", (long long)N, B, HV);
+  return OJX_OK;
+}
+
+int check_lintree(const void* k, const void* v, const float* g, const void* beta, const float* state, const int32_t* slot,
+                  int64_t state_slots, const int32_t* q_ptr, int64_t N, int32_t B, int32_t HV, int32_t HK) {
+  OJX_TRY(check_lintree_sizes(N, B, HV, HK));
+  if (state_slots < 0 || state_slots >= (1LL << 31))
+    return fail(OJX_ERR_SHAPE, "bad state_slots=%lld", (long long)state_slots);
+  if (N == 0) return OJX_OK;
+  if (k == nullptr || v == nullptr || g == nullptr || q_ptr == nullptr) return fail(OJX_ERR_ARG, "null k, v, g or q_ptr");
+  if (B > 0 && (slot == nullptr || (state == nullptr && state_slots > 0)))
+    return fail(OJX_ERR_ARG, "null state or slot");
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(g, 4) || !aligned(beta, 2) || !aligned(state, 16) ||
+      !aligned(slot, 4) || !aligned(q_ptr, 4))
+    return fail(OJX_ERR_ARG, "k, v and the states must be 16-byte aligned");
+  return OJX_OK;
+}
+
+int check_layers(int64_t layers, int32_t HKV, int32_t D, int32_t fmt, int64_t pages, int32_t page, const void* kc,
+                 const void* vc, const float* ks, const float* vs) {
+  if (layers < 0 || layers > 65535 || 2 * layers * HKV > 65535)
+    return fail(OJX_ERR_SHAPE, "%lld layers of %d heads: too many for one call", (long long)layers, HKV);
+  if (layers == 0) return check_cache(HKV, D, fmt, 0, page, nullptr, nullptr, nullptr, nullptr);
+  return check_cache(HKV, D, fmt, pages, page, kc, vc, ks, vs);
+}
+
+int check_pages(const int32_t* table, int64_t max_pages, const int32_t* refs, int64_t pages, int64_t B, int32_t page) {
+  if (B < 0 || B > 65536 || max_pages < 0 || max_pages >= (1LL << 31) || B * max_pages >= (1LL << 31))
+    return fail(OJX_ERR_SHAPE, "bad table of %lld sequences and %lld pages", (long long)B, (long long)max_pages);
+  if (pages < 0 || pages >= (1LL << 31)) return fail(OJX_ERR_SHAPE, "bad page count %lld", (long long)pages);
+  if (page < 16 || page % 16 != 0 || page > 1024)
+    return fail(OJX_ERR_SHAPE, "page=%d must be a multiple of 16, at most 1024", page);
+  if ((B * max_pages > 0 && table == nullptr) || (pages > 0 && refs == nullptr))
+    return fail(OJX_ERR_ARG, "null table or refs");
+  if (!aligned(table, 4) || !aligned(refs, 4)) return fail(OJX_ERR_ARG, "table and refs must be 4-byte aligned");
+  return OJX_OK;
+}
+
+int check_work(const char* what, const void* workspace, int64_t have, int64_t need) {
+  if (need > 0 && (workspace == nullptr || have < need || !aligned(workspace, 16)))
+    return fail(OJX_ERR_WORKSPACE, "%s needs %lld bytes of 16-byte aligned workspace, got %lld", what, (long long)need,
+                (long long)have);
+  return OJX_OK;
+}
+
 }  // namespace
+
+int64_t ojx_linattn_tree_workspace(int64_t N, int32_t B, int32_t HV, int32_t HK) {
+  if (check_lintree_sizes(N, B, HV, HK) != OJX_OK) return -1;
+  return N * HV * 128 * 4;
+}
+
+int ojx_linattn_tree(const void* q, const void* k, const void* v, const float* g, const void* beta, const float* state,
+                     const int32_t* slot, int64_t state_slots, const int32_t* q_ptr, const int32_t* parents, int64_t N,
+                     int32_t B, int32_t HV, int32_t HK, float scale, void* o, void* workspace, int64_t workspace_bytes,
+                     ojx_stream_t stream) {
+  OJX_TRY(check_lintree(k, v, g, beta, state, slot, state_slots, q_ptr, N, B, HV, HK));
+  if (N == 0) return OJX_OK;
+  if (q == nullptr || o == nullptr) return fail(OJX_ERR_ARG, "null q or o");
+  if (!aligned(q, 16) || !aligned(o, 16) || !aligned(parents, 4)) return fail(OJX_ERR_ARG, "q and o must be 16-byte aligned");
+  OJX_TRY(check_work("linear attention of drafts", workspace, workspace_bytes, ojx_linattn_tree_workspace(N, B, HV, HK)));
+  const ojx::LinTreeParams p{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
+                             static_cast<const uint16_t*>(v), g, static_cast<const uint16_t*>(beta),
+                             const_cast<float*>(state), slot, q_ptr, parents, nullptr, nullptr, static_cast<uint16_t*>(o),
+                             static_cast<float*>(workspace), N, state_slots, B, HV, HK, scale};
+  return hip_check(ojx::launch_linattn_tree(p, static_cast<hipStream_t>(stream)), "linear attention of drafts launch");
+}
+
+int ojx_linattn_keep(const void* k, const void* v, const float* g, const void* beta, float* state, const int32_t* slot,
+                     int64_t state_slots, const int32_t* q_ptr, const int32_t* path, const int32_t* count, int64_t N,
+                     int32_t B, int32_t HV, int32_t HK, ojx_stream_t stream) {
+  OJX_TRY(check_lintree(k, v, g, beta, state, slot, state_slots, q_ptr, N, B, HV, HK));
+  if (N == 0 || B == 0 || state_slots == 0) return OJX_OK;
+  if (path == nullptr || count == nullptr) return fail(OJX_ERR_ARG, "null path or count");
+  if (!aligned(path, 4) || !aligned(count, 4)) return fail(OJX_ERR_ARG, "path and count must be 4-byte aligned");
+  const ojx::LinTreeParams p{nullptr, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), g,
+                             static_cast<const uint16_t*>(beta), state, slot, q_ptr, nullptr, path, count, nullptr, nullptr,
+                             N, state_slots, B, HV, HK, 1.f};
+  return hip_check(ojx::launch_linattn_keep(p, static_cast<hipStream_t>(stream)), "linear attention keep launch");
+}
+
+int64_t ojx_verify_drafts_workspace(int64_t N, int32_t B, int64_t V, int32_t has_probs) {
+  if (N < 0 || N >= (1LL << 24) || B < 0 || B > 65536 || V < 1 || V > (1LL << 22) ||
+      N * ojx::draft_chunks(V) >= (1LL << 24) || B * ojx::draft_chunks(V) >= (1LL << 24)) {
+    fail(OJX_ERR_SHAPE, "bad sizes N=%lld B=%d V=%lld", (long long)N, B, (long long)V);
+    return -1;
+  }
+  return ojx::draft_work_bytes(N, B, V, has_probs != 0);
+}
+
+int ojx_verify_drafts(const void* logits, int32_t logits_type, int64_t ldl, const int64_t* tokens, const int32_t* q_ptr,
+                      const float* u, const int32_t* parents, const void* probs, int32_t probs_type, int64_t ldp,
+                      const float* temperature, int64_t N, int32_t B, int64_t V, int32_t* path, int32_t* count,
+                      int64_t* next, void* workspace, int64_t workspace_bytes, ojx_stream_t stream) {
+  const int64_t need = ojx_verify_drafts_workspace(N, B, V, probs != nullptr);
+  if (need < 0) return OJX_ERR_SHAPE;
+  if ((logits_type != OJX_F32 && logits_type != OJX_BF16) ||
+      (probs != nullptr && probs_type != OJX_F32 && probs_type != OJX_BF16))
+    return fail(OJX_ERR_ARG, "unknown type of logits (%d) or probs (%d)", logits_type, probs_type);
+  if (ldl < V || ldl >= (1LL << 31) || (probs != nullptr && (ldp < V || ldp >= (1LL << 31))))
+    return fail(OJX_ERR_ARG, "bad row strides ldl=%lld ldp=%lld for V=%lld", (long long)ldl, (long long)ldp, (long long)V);
+  if (N == 0 && B == 0) return OJX_OK;
+  if (q_ptr == nullptr || (B > 0 && (count == nullptr || next == nullptr)) ||
+      (N > 0 && (logits == nullptr || tokens == nullptr || u == nullptr || path == nullptr)))
+    return fail(OJX_ERR_ARG, "null logits, tokens, q_ptr, u or output");
+  if (!aligned(logits, logits_type == OJX_F32 ? 4 : 2) || !aligned(probs, probs_type == OJX_F32 ? 4 : 2) ||
+      !aligned(tokens, 8) || !aligned(next, 8) || !aligned(q_ptr, 4) || !aligned(u, 4) || !aligned(parents, 4) ||
+      !aligned(temperature, 4) || !aligned(path, 4) || !aligned(count, 4))
+    return fail(OJX_ERR_ARG, "misaligned pointer");
+  OJX_TRY(check_work("verification", workspace, workspace_bytes, need));
+  ojx::DraftParams p{};
+  p.logits = logits, p.ldl = ldl, p.probs = probs, p.ldp = ldp, p.tokens = tokens, p.q_ptr = q_ptr, p.parents = parents;
+  p.u = u, p.temp = temperature, p.path = path, p.count = count, p.next = next, p.N = N, p.V = V, p.B = B;
+  return hip_check(ojx::launch_verify(p, logits_type == OJX_F32, probs_type == OJX_F32, static_cast<uint8_t*>(workspace),
+                                      static_cast<hipStream_t>(stream)), "verification launch");
+}
+
+int ojx_kv_cache_keep(void* kc, void* vc, float* ks, float* vs, int32_t fmt, int64_t layers, int64_t pages, int32_t HKV,
+                      int32_t page, int32_t D, const int32_t* table, int64_t max_pages, const int32_t* ctx,
+                      const int32_t* q_ptr, const int32_t* path, const int32_t* count, int64_t N, int32_t B,
+                      ojx_stream_t stream) {
+  OJX_TRY(check_layers(layers, HKV, D, fmt, pages, page, kc, vc, ks, vs));
+  if (N < 0 || N >= (1LL << 31) || B < 0 || B > 65536 || 2 * layers * HKV * B >= (1LL << 24))
+    return fail(OJX_ERR_SHAPE, "bad sizes N=%lld B=%d for %lld layers", (long long)N, B, (long long)layers);
+  if (max_pages < 0 || max_pages >= (1LL << 31)) return fail(OJX_ERR_SHAPE, "bad max_pages=%lld", (long long)max_pages);
+  if (N == 0 || B == 0 || layers == 0 || pages == 0 || max_pages == 0) return OJX_OK;
+  if (table == nullptr || ctx == nullptr || q_ptr == nullptr || path == nullptr || count == nullptr)
+    return fail(OJX_ERR_ARG, "null table, ctx, q_ptr, path or count");
+  if (!aligned(table, 4) || !aligned(ctx, 4) || !aligned(q_ptr, 4) || !aligned(path, 4) || !aligned(count, 4))
+    return fail(OJX_ERR_ARG, "misaligned pointer");
+  const bool fp8 = fmt == OJX_KV_E4M3;
+  const ojx::KeepParams p{kc, vc, fp8 ? ks : nullptr, fp8 ? vs : nullptr, table, max_pages, ctx, q_ptr, path, count, N,
+                          pages, B, HKV, page};
+  return hip_check(ojx::launch_kv_keep(p, (int)layers, D * (fp8 ? 1 : 2), static_cast<hipStream_t>(stream)),
+                   "cache keep launch");
+}
+
+int64_t ojx_kv_pages_workspace(int64_t B, int64_t max_pages, int64_t pages, int32_t fork) {
+  if (B < 0 || B > 65536 || max_pages < 0 || max_pages >= (1LL << 31) || B * max_pages >= (1LL << 31) || pages < 0 ||
+      pages >= (1LL << 31)) {
+    fail(OJX_ERR_SHAPE, "bad table of %lld sequences and %lld pages", (long long)B, (long long)max_pages);
+    return -1;
+  }
+  return ojx::pages_work_ints(B, max_pages, pages, fork != 0) * 4;
+}
+
+int ojx_kv_pages_resize(int32_t* table, int64_t max_pages, int32_t* refs, int64_t pages, const int32_t* tokens, int64_t B,
+                        int32_t page, int32_t* missing, void* workspace, int64_t workspace_bytes, ojx_stream_t stream) {
+  OJX_TRY(check_pages(table, max_pages, refs, pages, B, page));
+  if (B == 0) return OJX_OK;
+  if (tokens == nullptr || missing == nullptr) return fail(OJX_ERR_ARG, "null tokens or missing");
+  if (!aligned(tokens, 4) || !aligned(missing, 4)) return fail(OJX_ERR_ARG, "misaligned pointer");
+  OJX_TRY(check_work("a resize", workspace, workspace_bytes, ojx_kv_pages_workspace(B, max_pages, pages, 0)));
+  ojx::PagesParams p{};
+  p.table = table, p.max_pages = max_pages, p.refs = refs, p.pages = pages, p.tokens = tokens, p.out = missing, p.B = B;
+  p.page = page;
+  return hip_check(ojx::launch_pages(p, false, static_cast<int32_t*>(workspace), static_cast<hipStream_t>(stream)),
+                   "page resize launch");
+}
+
+int ojx_kv_pages_fork(int32_t* table, int64_t max_pages, int32_t* ctx, int32_t* refs, int64_t pages, const int32_t* src,
+                      int64_t B, int32_t page, int32_t* pairs, void* workspace, int64_t workspace_bytes,
+                      ojx_stream_t stream) {
+  OJX_TRY(check_pages(table, max_pages, refs, pages, B, page));
+  if (B == 0) return OJX_OK;
+  if (ctx == nullptr || src == nullptr || pairs == nullptr) return fail(OJX_ERR_ARG, "null ctx, src or pairs");
+  if (!aligned(ctx, 4) || !aligned(src, 4) || !aligned(pairs, 4)) return fail(OJX_ERR_ARG, "misaligned pointer");
+  OJX_TRY(check_work("a fork", workspace, workspace_bytes, ojx_kv_pages_workspace(B, max_pages, pages, 1)));
+  ojx::PagesParams p{};
+  p.table = table, p.max_pages = max_pages, p.refs = refs, p.pages = pages, p.src = src, p.ctx = ctx, p.out = pairs, p.B = B;
+  p.page = page;
+  return hip_check(ojx::launch_pages(p, true, static_cast<int32_t*>(workspace), static_cast<hipStream_t>(stream)),
+                   "page fork launch");
+}
+
+int ojx_kv_pages_copy(void* kc, void* vc, float* ks, float* vs, int32_t fmt, int64_t layers, int64_t pages, int32_t HKV,
+                      int32_t page, int32_t D, const int32_t* pairs, int64_t n, ojx_stream_t stream) {
+  OJX_TRY(check_layers(layers, HKV, D, fmt, pages, page, kc, vc, ks, vs));
+  const bool fp8 = fmt == OJX_KV_E4M3;
+  const int64_t bytes = (int64_t)HKV * page * D * (fp8 ? 1 : 2);
+  if (n < 0 || n > 65535 || (bytes + 16383) / 16384 * n * 2 * layers >= (1LL << 24))
+    return fail(OJX_ERR_SHAPE, "%lld pages of %lld layers: too many for one call", (long long)n, (long long)layers);
+  if (n == 0 || layers == 0 || pages == 0) return OJX_OK;
+  if (pairs == nullptr) return fail(OJX_ERR_ARG, "null pairs");
+  if (!aligned(pairs, 4)) return fail(OJX_ERR_ARG, "misaligned pointer");
+  const ojx::CopyParams p{kc, vc, fp8 ? ks : nullptr, fp8 ? vs : nullptr, pairs, pages, bytes, (int64_t)HKV * page};
+  return hip_check(ojx::launch_pages_copy(p, n, (int)layers, static_cast<hipStream_t>(stream)), "page copy launch");
+}
 
 int ojx_kv_cache_write(const void* k, const void* v, const int64_t* slots, int64_t N, int32_t HKV, int32_t D,
                        int32_t fmt, void* kc, void* vc, float* ks, float* vs, int64_t pages, int32_t page,

@@ -321,4 +321,69 @@ int64_t linattn_work_bytes(int64_t R, int64_t S, int HV, bool delta);
 hipError_t launch_linattn_step(const LinParams& p, float* state, const int32_t* slot, hipStream_t st);
 hipError_t launch_linattn_prompt(const LinParams& p, hipStream_t st);
 
+// Linear attention of drafted tokens and of the kept ones (lintree.hip); heads of 128.
+struct LinTreeParams {
+  const uint16_t* q; const uint16_t* k;   // [N, HK, 128] (q: trees)
+  const uint16_t* v;                      // [N, HV, 128]
+  const float* g; const uint16_t* beta;   // [N, HV]; beta null: no delta rule
+  float* state; const int32_t* slot;      // [slots, HV, 128, 128], [B]
+  const int32_t* q_ptr;                   // [B + 1]
+  const int32_t* parents;                 // [N], or null: each row follows the one before it (trees)
+  const int32_t* path; const int32_t* count;  // [N], [B] (kept tokens)
+  uint16_t* o;                            // [N, HV, 128] (trees)
+  float* u;                               // [N, HV, 128] workspace (trees)
+  int64_t N, slots;
+  int B, HV, HK;
+  float scale;
+};
+hipError_t launch_linattn_tree(const LinTreeParams& p, hipStream_t st);
+hipError_t launch_linattn_keep(const LinTreeParams& p, hipStream_t st);
+
+// Accepted rows and pages of a paged cache (kvpages.hip).
+struct KeepParams {
+  void* kc; void* vc; float* ks; float* vs;  // [layers, pages, HKV, page, D] and [layers, pages, HKV, page] or null
+  const int32_t* table; int64_t max_pages;   // [B, max_pages]
+  const int32_t* ctx; const int32_t* q_ptr; const int32_t* path; const int32_t* count;
+  int64_t N, pages;
+  int B, HKV, page;
+};
+hipError_t launch_kv_keep(const KeepParams& p, int layers, int row_bytes, hipStream_t st);
+struct PagesParams {
+  int32_t* table; int64_t max_pages;      // [B, max_pages]
+  int32_t* refs; int64_t pages;           // [pages] table entries that name each page
+  const int32_t* tokens;                  // [B] (resize)
+  const int32_t* src; int32_t* ctx;       // [B], [B] (fork)
+  int32_t* out;                           // [B] pages missing; [B, 2] pages to copy (fork)
+  int64_t B;
+  int page;
+  int32_t *have, *need, *first, *last, *len, *taken, *rows;  // workspace, by launch_pages
+};
+int64_t pages_work_ints(int64_t B, int64_t max_pages, int64_t pages, bool fork);
+hipError_t launch_pages(PagesParams p, bool fork, int32_t* work, hipStream_t st);
+struct CopyParams {
+  void* kc; void* vc; float* ks; float* vs;
+  const int32_t* pairs;                   // [n, 2] from, to
+  int64_t pages, bytes, scales;           // of a page in a layer: bytes of keys, scales of keys
+};
+hipError_t launch_pages_copy(const CopyParams& p, int64_t n, int layers, hipStream_t st);
+
+// Verification of drafted tokens (drafts.hip).
+constexpr int kDraftRounds = 3;           // rejections of a sequence whose sums are made by the whole chip
+struct DraftParams {
+  const void* logits; int64_t ldl;        // [N, V], row stride
+  const void* probs; int64_t ldp;         // [N, V], or null
+  const int64_t* tokens; const int32_t* q_ptr;
+  const int32_t* parents;                 // [N], or null: each row follows the one before it
+  const float* u; const float* temp;      // [N]; [B] or null (1)
+  int32_t* path; int32_t* count; int64_t* next;
+  int64_t N, V;
+  int B, chunks, rounds;
+  struct DraftChunk* parts;               // [N, chunks] workspace
+  struct DraftRow* rows;                  // [N]
+  double* sums;                           // [rounds, B, chunks]
+};
+int64_t draft_chunks(int64_t V);
+int64_t draft_work_bytes(int64_t N, int64_t B, int64_t V, bool probs);
+hipError_t launch_verify(DraftParams p, bool f32, bool probs_f32, uint8_t* work, hipStream_t st);
+
 }  // namespace ojx

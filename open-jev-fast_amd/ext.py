@@ -686,3 +686,219 @@ def linattn_step(q, k, v, g, beta, state, slot, scale=None):
     check(lib().ojx_linattn_step(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(slot), state.shape[0],
                                  R, HV, HK, float(128 ** -0.5 if scale is None else scale), _ptr(o), _stream()))
     return o
+
+
+# ------------------------------------------------------------------------------------------------ drafted tokens
+def _chk_rows(q_ptr, N, parents=None, path=None, count=None):
+    """B of the sequences that q_ptr int32 [B + 1] makes of N rows."""
+    _chk(q_ptr, "q_ptr", torch.int32)
+    B = q_ptr.numel() - 1
+    if B < 0:
+        raise RuntimeError("q_ptr must be [B + 1]")
+    for t, nm, n in ((parents, "parents", N), (path, "path", N), (count, "count", B)):
+        if t is not None:
+            _chk(t, nm, torch.int32)
+            if t.numel() != n:
+                raise RuntimeError(f"{nm} must have {n} elements, got {t.numel()}")
+    return B
+
+
+def _chk_slots(state, slot, HV, B):
+    _chk_states(state, HV)
+    _chk(slot, "slot", torch.int32)
+    if slot.numel() != B:
+        raise RuntimeError(f"slot must have B={B} elements, got {slot.numel()}")
+
+
+def linattn_tree(q, k, v, g, beta, state, slot, q_ptr, parents=None, scale=None):
+    """linattn_step for drafted tokens, a tree of them or a line: o bf16 [N, HV 128], on states that stay as they are.
+    Sequence b's rows are q_ptr[b] .. q_ptr[b+1] - 1 (int32 [B + 1]), its state is state[slot[b]] (fp32 [slots, HV, 128,
+    128], int32 [B]). Row j of a sequence follows its row parents[j] (int32 [N], indexes within the sequence), or the state
+    itself where parents[j] is not one of 0 .. j - 1; parents=None: each row follows the one before it. A row's output is that
+    of its path's tokens, from the state on. A negative slot gives zeros, a slot that is not in state NaN; a row of no sequence gives
+    zeros. Operands as in linattn_prompt. linattn_keep then takes the states over the tokens that are kept."""
+    N, HV, HK = _chk_linattn(q, k, v, g, beta)
+    B = _chk_rows(q_ptr, N, parents)
+    _chk_slots(state, slot, HV, B)
+    _one_device(q, k, v, g, beta, state, slot, q_ptr, parents)
+    o = torch.empty_like(v)
+    n = lib().ojx_linattn_tree_workspace(N, B, HV, HK)
+    if n < 0:
+        check(2)
+    ws = _scratch(n, q)
+    check(lib().ojx_linattn_tree(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(slot), state.shape[0],
+                                 _ptr(q_ptr), _ptr(parents), N, B, HV, HK, float(128 ** -0.5 if scale is None else scale),
+                                 _ptr(o), _ptr(ws), n, _stream()))
+    return o
+
+
+def linattn_keep(k, v, g, beta, state, slot, q_ptr, path, count):
+    """Takes states forward over the tokens that were kept, in place: state[slot[b]] over sequence b's rows path[q_ptr[b] +
+    i], i < count[b], one after the other (path int32 [N] and count int32 [B] as verify_drafts gives them; the other
+    operands as linattn_tree took them). A slot that is not in state, or that an earlier sequence has too, is left alone."""
+    N, HV, HK = _chk_linattn(k, k, v, g, beta)
+    B = _chk_rows(q_ptr, N, None, path, count)
+    if path is None or count is None:
+        raise RuntimeError("path and count must be tensors")
+    _chk_slots(state, slot, HV, B)
+    _one_device(k, v, g, beta, state, slot, q_ptr, path, count)
+    check(lib().ojx_linattn_keep(_ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(slot), state.shape[0], _ptr(q_ptr),
+                                 _ptr(path), _ptr(count), N, B, HV, HK, _stream()))
+
+
+def _chk_vocab(t, name, N=None, V=None):
+    """(type, N, V, row stride) of logits or probabilities: rows may be further apart than they are long."""
+    kind = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}.get(t.dtype)
+    if kind is None:
+        raise RuntimeError(f"{name} must be torch.float32 or torch.bfloat16, got {t.dtype}")
+    if not t.is_cuda or t.dim() != 2 or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise RuntimeError(f"{name} must be CUDA [N, V] with contiguous rows, got {tuple(t.shape)}")
+    if N is not None and tuple(t.shape) != (N, V):
+        raise RuntimeError(f"{name} must be [N={N}, V={V}], got {tuple(t.shape)}")
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ld < t.shape[1]:
+        raise RuntimeError(f"{name} has rows that overlap")
+    return kind, t.shape[0], t.shape[1], ld
+
+
+def verify_drafts(logits, tokens, q_ptr, u, parents=None, probs=None, temperature=None):
+    """Drafted tokens accepted or not, from given random numbers, so that what comes out is distributed as the target's own
+    tokens: (path int32 [N], count int32 [B], next int64 [B]).
+
+    Sequence b's rows are q_ptr[b] .. q_ptr[b+1] - 1 (int32 [B + 1]): row 0 is its last token, row j >= 1 the drafted token
+    tokens[j] (int64 [N]) behind row parents[j] (int32 [N], within the sequence; None: the row before it). logits [N, V],
+    fp32 or bf16 (rows may have a stride): row j's are the target's behind token j. temperature fp32 [B], or None for 1; 0
+    takes the first largest logit. probs [N, V], fp32 or bf16: row j's is the distribution that the tokens behind row j were
+    drawn from, each by itself; None: they were certain (looked up). u fp32 [N] in [0, 1): row j's number tests its token,
+    row 0's draws the next one.
+
+    path has each sequence's accepted rows in order, row 0 first, and -1 behind them; count says how many, next is the token
+    behind the last of them (-1: its logits are no distribution, or the sequence has no rows). kv_cache_keep and
+    linattn_keep take path and count as they are."""
+    kind, N, V, ldl = _chk_vocab(logits, "logits")
+    _chk(tokens, "tokens", torch.int64)
+    _chk(u, "u", torch.float32)
+    if tokens.numel() != N or u.numel() != N:
+        raise RuntimeError(f"tokens and u must have N={N} elements, got {tokens.numel()} and {u.numel()}")
+    B = _chk_rows(q_ptr, N, parents)
+    pkind, ldp = 0, 0
+    if probs is not None:
+        pkind, _, _, ldp = _chk_vocab(probs, "probs", N, V)
+    if temperature is not None:
+        _chk(temperature, "temperature", torch.float32)
+        if temperature.numel() != B:
+            raise RuntimeError(f"temperature must have B={B} elements, got {temperature.numel()}")
+    _one_device(logits, tokens, q_ptr, u, parents, probs, temperature)
+    path, count = q_ptr.new_empty(N), q_ptr.new_empty(B)
+    token = tokens.new_empty(B)
+    n = lib().ojx_verify_drafts_workspace(N, B, V, probs is not None)
+    if n < 0:
+        check(2)
+    ws = _scratch(n, logits)
+    check(lib().ojx_verify_drafts(_ptr(logits), kind, ldl, _ptr(tokens), _ptr(q_ptr), _ptr(u), _ptr(parents), _ptr(probs),
+                                  pkind, ldp, _ptr(temperature), N, B, V, _ptr(path), _ptr(count), _ptr(token), _ptr(ws), n,
+                                  _stream()))
+    return path, count, token
+
+
+def _chk_layers(kc, vc, ks, vs):
+    """(format, layers, pages, HKV, page, D) of a cache [pages, HKV, page, D], or of several layers' [layers, pages, ..]."""
+    if kc.dim() == 5:
+        if vc.dim() != 5 or kc.shape != vc.shape or (ks is not None and (ks.dim() != 4 or ks.shape[0] != kc.shape[0])) or (
+                vs is not None and (vs.dim() != 4 or vs.shape[0] != kc.shape[0])):
+            raise RuntimeError(f"kc {tuple(kc.shape)} and vc {tuple(vc.shape)} must be one shape, with scales of its first "
+                               "four sizes")
+        layers, pages = kc.shape[:2]
+        one = [None if t is None else t.flatten(0, 1) if t.is_contiguous() else t for t in (kc, vc, ks, vs)]
+    else:
+        if kc.dim() != 4:
+            raise RuntimeError(f"kc must be [pages, HKV, page, D] or [layers, pages, HKV, page, D], got {tuple(kc.shape)}")
+        layers, pages, one = 1, kc.shape[0], (kc, vc, ks, vs)
+    HKV, D = kc.shape[-3], kc.shape[-1]
+    fmt, _, page = _chk_cache(*one, HKV, D)
+    return fmt, layers, pages, HKV, page, D
+
+
+def _chk_table(table, B=None):
+    _chk(table, "table", torch.int32)
+    if table.dim() != 2 or (B is not None and table.shape[0] != B):
+        raise RuntimeError(f"table {tuple(table.shape)} must be [B{'' if B is None else '=' + str(B)}, max_pages]")
+    return table.shape
+
+
+def kv_cache_keep(kc, vc, table, ctx, q_ptr, path, count, ks=None, vs=None):
+    """Moves the kept tokens' keys and values together, in place: sequence b's row at position ctx[b] + path[q_ptr[b] + i]
+    goes to ctx[b] + i, i < count[b] (path and count as verify_drafts gives them, ctx, table and q_ptr as tree_attn takes
+    them). The cache as in kv_cache_write, or that of several layers with one table: [layers, pages, HKV, page, D], scales
+    [layers, pages, HKV, page]. Add count to ctx afterwards."""
+    fmt, layers, pages, HKV, page, D = _chk_layers(kc, vc, ks, vs)
+    if path is None or count is None:
+        raise RuntimeError("path and count must be tensors")
+    _chk(path, "path", torch.int32)
+    N = path.numel()
+    B = _chk_rows(q_ptr, N, None, path, count)
+    MP = _chk_table(table, B)[1]
+    _chk(ctx, "ctx", torch.int32)
+    if ctx.numel() != B:
+        raise RuntimeError(f"ctx must have B={B} elements, got {ctx.numel()}")
+    _one_device(kc, vc, ks, vs, table, ctx, q_ptr, path, count)
+    check(lib().ojx_kv_cache_keep(_ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), fmt, layers, pages, HKV, page, D, _ptr(table), MP,
+                                  _ptr(ctx), _ptr(q_ptr), _ptr(path), _ptr(count), N, B, _stream()))
+
+
+def _pages_call(table, refs, per_slot, name):
+    B, MP = _chk_table(table)
+    _chk(refs, "refs", torch.int32)
+    _chk(per_slot, name, torch.int32)
+    if per_slot.numel() != B:
+        raise RuntimeError(f"{name} must have B={B} elements, got {per_slot.numel()}")
+    return B, MP, refs.numel()
+
+
+def kv_pages_resize(table, refs, tokens, page):
+    """Gives every sequence the pages that tokens[b] tokens need (int32 [B]; negative: left as it is), in place: table int32
+    [B, max_pages], refs int32 [pages] = how many table entries name each page. Entries behind that are given back (-1),
+    entries that name no page get the lowest free ones, sequence by sequence. tokens[b] = 0 frees a sequence. Returns missing
+    int32 [B]: entries for which the pool or the table had no room."""
+    B, MP, pages = _pages_call(table, refs, tokens, "tokens")
+    _one_device(table, refs, tokens)
+    missing = table.new_empty(B)
+    n = lib().ojx_kv_pages_workspace(B, MP, pages, 0)
+    if n < 0:
+        check(2)
+    ws = _scratch(n, table)
+    check(lib().ojx_kv_pages_resize(_ptr(table), MP, _ptr(refs), pages, _ptr(tokens), B, page, _ptr(missing), _ptr(ws), n,
+                                    _stream()))
+    return missing
+
+
+def kv_pages_fork(table, ctx, refs, src, page):
+    """Slot b's sequence becomes a copy of slot src[b]'s (int32 [B]; b itself: left as it is; outside 0 .. B - 1: empty), in
+    place and all at once: full pages are shared, a last page that is not full is taken anew. Returns pairs int32 [B, 2], the
+    pages to copy: kv_pages_copy does that for a layer or several, and has to before anything else writes to the cache or
+    takes pages. A slot for which the pool has no page left ends with its last full page (its ctx says so)."""
+    B, MP, pages = _pages_call(table, refs, src, "src")
+    _chk(ctx, "ctx", torch.int32)
+    if ctx.numel() != B:
+        raise RuntimeError(f"ctx must have B={B} elements, got {ctx.numel()}")
+    _one_device(table, ctx, refs, src)
+    pairs = table.new_empty((B, 2))
+    n = lib().ojx_kv_pages_workspace(B, MP, pages, 1)
+    if n < 0:
+        check(2)
+    ws = _scratch(n, table)
+    check(lib().ojx_kv_pages_fork(_ptr(table), MP, _ptr(ctx), _ptr(refs), pages, _ptr(src), B, page, _ptr(pairs), _ptr(ws),
+                                  n, _stream()))
+    return pairs
+
+
+def kv_pages_copy(kc, vc, pairs, ks=None, vs=None):
+    """Copies page pairs[i][0] to page pairs[i][1] (int32 [n, 2], as kv_pages_fork gives them; a pair with a page outside the
+    cache is left out) in a cache of one layer or several (see kv_cache_keep). No page may be both read and written."""
+    fmt, layers, pages, HKV, page, D = _chk_layers(kc, vc, ks, vs)
+    _chk(pairs, "pairs", torch.int32)
+    if pairs.dim() != 2 or pairs.shape[1] != 2:
+        raise RuntimeError(f"pairs must be [n, 2], got {tuple(pairs.shape)}")
+    _one_device(kc, vc, ks, vs, pairs)
+    check(lib().ojx_kv_pages_copy(_ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), fmt, layers, pages, HKV, page, D, _ptr(pairs),
+                                  pairs.shape[0], _stream()))
