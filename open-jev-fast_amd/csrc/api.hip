@@ -1002,7 +1002,7 @@ int ojx_linattn_keep(const void* k, const void* v, const float* g, const void* b
 
 int64_t ojx_verify_drafts_workspace(int64_t N, int32_t B, int64_t V, int32_t has_probs) {
   if (N < 0 || N >= (1LL << 24) || B < 0 || B > 65536 || V < 1 || V > (1LL << 22) ||
-      N * ojx::draft_chunks(V) >= (1LL << 24) || B * ojx::draft_chunks(V) >= (1LL << 24)) {
+      N * ojx::draft_chunks(V) >= (1LL << 24) || B * ojx::draft_chunks(V) >= (1LL << 22)) {
     fail(OJX_ERR_SHAPE, "bad sizes N=%lld B=%d V=%lld", (long long)N, B, (long long)V);
     return -1;
   }

@@ -14,9 +14,10 @@
 //
 //   draft_chunks_k  a workgroup per chunk of a row: its largest logit, where it is, and the sum of the exponentials below it
 //   draft_rows_k    a wave per row: those put together; p and q of the row's token under the row that it follows
-//   draft_sums_k    (with q, once for each of the first rejections) a workgroup per chunk of a sequence: walks over the rows
-//                   up to that rejection, all it needs being in draft_rows_k's few numbers, and sums w over the chunk
+//   draft_sums_k    once for each of the first rejections: a workgroup per chunk of a sequence walks over the rows up to that
+//                   rejection, all it needs being in draft_rows_k's few numbers, and sums w over the chunk
 //   draft_next_k    a workgroup per sequence: the whole walk, the accepted rows, the next token
+// The two in the middle are launched with q and more than a few chunks; otherwise draft_next_k does their work.
 #include "ojx_internal.h"
 
 #include <algorithm>
@@ -35,6 +36,11 @@ struct DraftRow {
   double p, q;       // of the row's token, in the row above it; p < 0: no such row
   int32_t above, ok; // the row above in the sequence, or -1; ok: the row has a distribution
   int64_t token;
+};
+
+struct DraftWalk {
+  int j, cur, count, rejections;  // the next row to look at, the current one, accepted so far
+  double a, t;
 };
 
 namespace {
@@ -88,16 +94,82 @@ __device__ __forceinline__ float temperature(const DraftParams& p, int b) {
   const float t = p.temp == nullptr ? 1.f : p.temp[b];
   return t > 0.f ? t : 0.f;
 }
-// exp((x - top) / T), rt = 1 / T
-__device__ __forceinline__ double weight(float x, float top, double rt) {
-  return x == -INFINITY ? 0.0 : exp(((double)x - (double)top) * rt);
+// 2^f for |f| <= 1/2, 1.1e-12 off at most: a polynomial of degree 8, interpolated at Chebyshev's nodes, then its first
+// coefficient made 1 (a degree more: 2e-14). That error moves the borders between tokens by as much: one draw in some 10^7
+// may fall on the other side of one.
+__device__ __forceinline__ double exp2_part(double f) {
+  double x = 0x1.63d136366db24p-20;
+  x = fma(x, f, 0x1.00dc4a532fb8ep-16);
+  x = fma(x, f, 0x1.4308ac85aa947p-13);
+  x = fma(x, f, 0x1.5d8745a728441p-10);
+  x = fma(x, f, 0x1.3b2ab7181b755p-7);
+  x = fma(x, f, 0x1.c6b08dd6fd234p-5);
+  x = fma(x, f, 0x1.ebfbdff823cedp-3);
+  x = fma(x, f, 0x1.62e42fef84cf0p-1);
+  return fma(x, f, 1.0);
+}
+constexpr double kRound = 0x1.8p52;  // added and taken off again: rounds to a whole number, whose low bits it leaves in the sum
+__device__ __forceinline__ double times_exp2(double x, double rounded) {
+  return __hiloint2double(__double2hiint(x) + (int)((uint32_t)__double2loint(rounded) << 20), __double2loint(x));
+}
+// 2^y for y <= 1/2; 2^-1000 where y is below -1000 or NaN.
+__device__ __forceinline__ double exp2_down(double y) {
+  y = fmax(y, -1000.0);
+  const double t = y + kRound;
+  return times_exp2(exp2_part(y - (t - kRound)), t);
 }
 
-__device__ __forceinline__ double wave_add(double x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+// exp((x - top) / T) = 2^((x - top) c), c = 1 / (T log 2). In the loops over whole rows it is made as 2^(x c - k), k the
+// whole number next to top c, times `rest` = 2^(k - top c): 14 operations a logit instead of 17, where the library's
+// exponential would be 40 (the largest case makes 71 million of them, and is bound by them). `plain` says that the sizes do
+// not allow it. A logit of -infinity counts as 2^-990 there, next to nothing.
+struct Scale {
+  double c, top, bias, rest;
+  float least;  // logits below it count as this
+  bool plain;
+};
+__device__ __forceinline__ Scale scale_of(float temp, float top) {
+  Scale s;
+  s.c = 0x1.71547652b82fep+0 / (double)temp;
+  s.top = top;
+  const double y = s.top * s.c, k = (y + kRound) - kRound;
+  s.bias = kRound - k;
+  s.rest = exp2_part(-fma(s.top, s.c, -k));
+  s.least = (float)((k - 990.0) / s.c);
+  s.plain = !(fabs(y) < 0x1p23) || !(s.least > -INFINITY);
+  return s;
 }
+// Without `rest`; not where `plain`.
+__device__ __forceinline__ double weight_part(float x, const Scale& s) {
+  const double v = __builtin_elementwise_maximum(x, s.least), t = fma(v, s.c, s.bias);
+  return times_exp2(exp2_part(fma(v, s.c, -(t - s.bias))), t);
+}
+__device__ __forceinline__ double weight(float x, const Scale& s) { return exp2_down(((double)x - s.top) * s.c); }
+__device__ __forceinline__ double weight_or_none(float x, const Scale& s) {
+  const double y = ((double)x - s.top) * s.c;
+  return y > -1000.0 ? exp2_down(y) : 0.0;
+}
+
+// Sum of x over the lanes up to and including this one: by lane shifts within rows of 16, and the rows' last lanes handed on
+// (a lane outside reads as zero).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, ROWS, 0xf, false);
+  return x + __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ double wave_upto(double x) {
+  x = dpp_add<0x111, 0xf>(x);
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);
+  return dpp_add<0x143, 0xc>(x);
+}
+__device__ __forceinline__ double lane_of(double x, int l) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), l), __builtin_amdgcn_readlane(__double2loint(x), l));
+}
+__device__ __forceinline__ double wave_add(double x) { return lane_of(wave_upto(x), 63); }
 // Sum over the workgroup, in wave order; red: 16 doubles.
 __device__ __forceinline__ double block_add(double x, double* red) {
   x = wave_add(x);
@@ -133,20 +205,18 @@ __global__ void __launch_bounds__(256) draft_chunks_k(DraftParams p) {
   const int b = owner(p, r, place);
   if (b < 0) return;
   const float t = temperature(p, b);
-  float top = -INFINITY;
-  bool odd = false;
+  float top = -INFINITY;  // NaN where one is
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      top = fmaxf(top, x[i][j]);
-      odd |= !(x[i][j] < INFINITY);
-    }
+    for (int j = 0; j < 8; ++j) top = __builtin_elementwise_maximum(top, x[i][j]);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  for (int o = 32; o > 0; o >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, o));
   if ((threadIdx.x & 63) == 0) tops[wave] = top;
-  odd = __syncthreads_or(odd);
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = __builtin_elementwise_maximum(top, tops[i]);
+  const bool odd = !(top < INFINITY);
   DraftChunk out{odd ? __uint_as_float(0x7fc00000u) : top, 0, 0.0};
   if (t == 0.f) {  // the same for all threads
     int32_t at = 0x7fffffff;
@@ -162,13 +232,22 @@ __global__ void __launch_bounds__(256) draft_chunks_k(DraftParams p) {
     out.at = min(min(ats[0], ats[1]), min(ats[2], ats[3]));
     out.sum = 1.0;
   } else {
-    const double rt = 1.0 / (double)t;
+    const Scale sc = scale_of(t, top);
     double s = 0.0;
-    if (top > -INFINITY && !odd)
+    if (top > -INFINITY && !odd) {
+      if (!sc.plain) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += weight(x[i][j], top, rt);
+          for (int j = 0; j < 8; ++j) s += weight_part(x[i][j], sc);
+        s *= sc.rest;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s += weight(x[i][j], sc);
+      }
+    }
     out.sum = block_add(s, red);
   }
   if (threadIdx.x == 0) p.parts[r * p.chunks + chunk] = out;
@@ -189,10 +268,10 @@ __device__ __forceinline__ void row_total(const DraftParams& p, int64_t r, float
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   at = 0x7fffffff;
   sum = 0.0;
-  const double rt = t > 0.f ? 1.0 / (double)t : 0.0;
+  const Scale sc = scale_of(t > 0.f ? t : 1.f, top);
   for (int c = lane; c < p.chunks; c += 64) {
     if (t == 0.f && parts[c].top == top) at = min(at, parts[c].at);
-    if (t > 0.f && parts[c].top > -INFINITY) sum += parts[c].sum * exp(((double)parts[c].top - (double)top) * rt);
+    if (t > 0.f) sum += parts[c].sum * weight(parts[c].top, sc);  // the sum is 0 where the largest is -infinity
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
@@ -200,70 +279,67 @@ __device__ __forceinline__ void row_total(const DraftParams& p, int64_t r, float
   if (__any(odd)) top = __uint_as_float(0x7fc00000u);
 }
 
+// What the walk has to know of row j of a sequence; the whole wave calls.
 template <typename T, typename Q, bool PROBS>
-__global__ void __launch_bounds__(256) draft_rows_k(DraftParams p) {
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= p.N) return;
+__device__ __forceinline__ void row_info(const DraftParams& p, int64_t first, int j, float t) {
   const int lane = threadIdx.x & 63;
-  SeqPlace place;
-  const int b = owner(p, r, place);
-  if (b < 0) {
-    if (lane == 0) p.path[r] = -1;
-    return;
-  }
-  const float t = temperature(p, b);
-  const int j = (int)(r - place.first);
+  const int64_t r = first + j;
   DraftRow out{};
+  int above = p.parents == nullptr ? j - 1 : p.parents[r];
+  out.token = p.tokens[r];
+  if (above < 0 || above >= j) above = -1;
   row_total(p, r, t, out.top, out.at, out.sum);
   out.ok = out.top > -INFINITY;  // not NaN
-  out.token = p.tokens[r];
-  int above = p.parents == nullptr ? j - 1 : p.parents[r];
-  if (above < 0 || above >= j) above = -1;
   out.above = above;
   out.p = -1.0;
   out.q = 1.0;
   if (above >= 0) {
-    const int64_t a = place.first + above;
+    const int64_t a = first + above;
+    const bool in = out.token >= 0 && out.token < p.V;
+    const int64_t token = in ? out.token : 0;
+    const float x = value(static_cast<const T*>(p.logits) + a * p.ldl + token);
+    const float q = PROBS ? value(static_cast<const Q*>(p.probs) + a * p.ldp + token) : 0.f;
     float top;
     int32_t at;
     double sum;
     row_total(p, a, t, top, at, sum);
-    const bool in = out.token >= 0 && out.token < p.V;
     // without q a token that an earlier child has too is gone with that one
     bool gone = !in;
-    if (!PROBS || t == 0.f)
+    if (p.parents != nullptr && (!PROBS || t == 0.f)) {
       for (int i = above + 1 + lane; i < j; i += 64)
-        gone |= (p.parents == nullptr ? i - 1 : p.parents[place.first + i]) == above && p.tokens[place.first + i] == out.token;
-    gone = __any(gone);
+        gone |= p.parents[first + i] == above && p.tokens[first + i] == out.token;
+      gone = __any(gone);
+    }
     if (top > -INFINITY) {
       out.p = 0.0;
       if (!gone) {
         if (t == 0.f)
           out.p = out.token == at ? 1.0 : 0.0;
         else
-          out.p = weight(value(static_cast<const T*>(p.logits) + a * p.ldl + out.token), top, 1.0 / (double)t) / sum;
+          out.p = weight_or_none(x, scale_of(t, top)) / sum;
       }
-      if (PROBS && t > 0.f) {
-        out.q = in ? value(static_cast<const Q*>(p.probs) + a * p.ldp + out.token) : 0.f;
-        if (!(out.q > 0.0)) out.q = 0.0;
-      }
+      if (PROBS && t > 0.f) out.q = in && q > 0.f ? (double)q : 0.0;
     }
   }
   if (lane == 0) p.rows[r] = out;
 }
 
-// Where the walk over a sequence's rows stands.
-struct Walk {
-  int j, cur, count, rejections;
-  double a, t;
-};
+template <typename T, typename Q>
+__global__ void __launch_bounds__(256) draft_rows_k(DraftParams p) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= p.N) return;
+  SeqPlace place;
+  const int b = owner(p, r, place);
+  if (b >= 0) row_info<T, Q, true>(p, place.first, (int)(r - place.first), temperature(p, b));
+}
 
-// On to the next rejection whose sum of what is left is not known (true), or to the end (false); the whole wave calls, with
-// the walk the same in all lanes. sum(i) is the sum after rejection i; known says how many there are. write(i, j): row j is
-// the i-th accepted.
-template <bool PROBS, typename Sum, typename Write>
-__device__ __forceinline__ bool walk_on(const DraftParams& p, const SeqPlace& s, float temp, Walk& w, int known, Sum sum,
-                                        Write write) {
+// Where the walk over a sequence's rows stands.
+using Walk = DraftWalk;
+
+// On to the next rejection with q (true: what is left has to be summed before the walk can go on), or to the end; the whole
+// wave calls, with the walk the same in all lanes. write(i, j): row j is the i-th accepted.
+template <bool PROBS, typename Write>
+__device__ __forceinline__ bool walk_on(const DraftParams& p, const SeqPlace& s, float temp, Walk& w, Write write) {
   const int lane = threadIdx.x & 63;
   for (int base = w.j & ~63; base < s.n; base += 64) {
     const int mine = min(base + lane, s.n - 1);
@@ -273,7 +349,7 @@ __device__ __forceinline__ bool walk_on(const DraftParams& p, const SeqPlace& s,
     for (; w.j < min(base + 64, s.n); ++w.j) {
       const int l = w.j - base;
       if (__builtin_amdgcn_readlane(above, l) != w.cur) continue;
-      const double x = __shfl(rp, l), q = __shfl(rq, l), v = __shfl(u, l);
+      const double x = lane_of(rp, l), q = lane_of(rq, l), v = lane_of(u, l);
       if (x < 0.0) continue;
       const double left = PROBS && temp > 0.f ? (w.a > 0.0 ? fmax(x - w.a * q, 0.0) : x) : x;
       if (v * q * w.t < left) {
@@ -285,11 +361,8 @@ __device__ __forceinline__ bool walk_on(const DraftParams& p, const SeqPlace& s,
       } else if (PROBS && temp > 0.f) {
         w.a += w.t;
         ++w.rejections;
-        if (w.rejections > known) {
-          ++w.j;
-          return true;
-        }
-        w.t = sum(w.rejections - 1);
+        ++w.j;
+        return true;
       } else {
         ++w.rejections;
         if (temp > 0.f) w.t -= x;
@@ -299,72 +372,101 @@ __device__ __forceinline__ bool walk_on(const DraftParams& p, const SeqPlace& s,
   return false;
 }
 
-// What is left of a row's distribution at eight places: p in units of the largest logit's (scale 1), or with q as it is.
+// What is left of a row's distribution at eight places: p in units of the largest logit's (unit 1), or with q as it is.
 template <typename T, typename Q, bool PROBS>
-__device__ __forceinline__ void left_of(const DraftParams& p, int64_t r, int64_t e, float top, double rt, double scale,
-                                        double a, double (&w)[8]) {
-  float x[8];
+__device__ __forceinline__ void left_of(const DraftParams& p, int64_t r, int64_t e, Scale sc, double unit, double a,
+                                        double (&w)[8]) {
+  float x[8], q[8];
   eight(static_cast<const T*>(p.logits) + r * p.ldl, e, p.V, -INFINITY, x);
+  if (PROBS && a > 0.0) eight(static_cast<const Q*>(p.probs) + r * p.ldp, e, p.V, 0.f, q);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = weight(x[i], top, rt) * scale;
-  if (PROBS && a > 0.0) {
-    float q[8];
-    eight(static_cast<const Q*>(p.probs) + r * p.ldp, e, p.V, 0.f, q);
+  for (int i = 0; i < 8; ++i) w[i] = weight_or_none(x[i], sc) * unit;
+  if (PROBS && a > 0.0)
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = q[i] > 0.f ? fmax(w[i] - a * (double)q[i], 0.0) : w[i];
-  }
 }
 
+// The sum after rejection i of sequence b, from draft_sums_k; the whole wave calls.
+__device__ __forceinline__ double known_sum(const DraftParams& p, int b, int i) {
+  double x = 0.0;
+  for (int c = threadIdx.x & 63; c < p.chunks; c += 64) x += p.sums[((int64_t)i * p.B + b) * p.chunks + c];
+  return wave_add(x);
+}
+
+// Rejection number `round`. Chunk 0's workgroup leaves where the walk stands (rejections = round + 1: at this rejection;
+// fewer: it is over) and the rows accepted on the way.
 template <typename T, typename Q>
-__global__ void __launch_bounds__(256) draft_sums_k(DraftParams p, int round) {
+__global__ void __launch_bounds__(1024) draft_sums_k(DraftParams p, int round) {
   __shared__ double red[16];
   __shared__ Walk held;
-  __shared__ int stop;
-  const int b = blockIdx.x / (uint32_t)p.chunks, chunk = blockIdx.x - b * p.chunks;
+  const int b = blockIdx.x / (uint32_t)p.chunks, chunk = blockIdx.x - b * p.chunks, lane = threadIdx.x & 63;
+  DraftWalk* const walks = p.walks + (int64_t)round * p.B;
+  Walk w{1, 0, 1, 0, 0.0, 1.0};
+  if (round > 0) {
+    w = walks[b - p.B];
+    if (w.rejections < round) {
+      if (chunk == 0 && threadIdx.x == 0) walks[b] = w;
+      return;
+    }
+  }
+  const float t = temperature(p, b);
   SeqPlace s;
   if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == b; }, s)) return;
-  const float t = temperature(p, b);
-  if (s.n == 0 || t == 0.f) return;
   if (threadIdx.x < 64) {
-    Walk w{1, 0, 1, 0, 0.0, 1.0};
-    const auto sum = [&](int i) {
-      double x = 0.0;
-      for (int c = threadIdx.x; c < p.chunks; c += 64) x += p.sums[((int64_t)i * p.B + b) * p.chunks + c];
-      return wave_add(x);
-    };
-    const bool here = walk_on<true>(p, s, t, w, round, sum, [](int, int) {});
-    if (threadIdx.x == 0) {
+    if (round > 0) w.t = known_sum(p, b, round - 1);
+    walk_on<true>(p, s, t, w, [&](int i, int j) {
+      if (chunk == 0 && lane == 0) p.path[s.first + i] = j;
+    });
+    if (t == 0.f) w.rejections = 0;  // these need no sums
+    if (lane == 0) {
       held = w;
-      stop = !here;
+      if (chunk == 0) walks[b] = w;
     }
   }
   __syncthreads();
-  if (stop) return;
-  const int64_t r = s.first + held.cur;
-  const DraftRow row = p.rows[r];
-  const double rt = 1.0 / (double)t, scale = 1.0 / row.sum;
-  const int64_t e0 = (int64_t)chunk * kPiece - lead(static_cast<const T*>(p.logits) + r * p.ldl);
+  w = held;
+  if (w.rejections <= round) return;
+  const int64_t r = s.first + w.cur;
+  const Scale sc = scale_of(t, p.rows[r].top);
+  const double unit = 1.0 / p.rows[r].sum;
+  const T* const row = static_cast<const T*>(p.logits) + r * p.ldl;
+  const int64_t e = (int64_t)chunk * kPiece - lead(row) + threadIdx.x * 8;
   double x = 0.0;
-  for (int i = 0; i < 4; ++i) {
-    double w[8];
-    left_of<T, Q, true>(p, r, e0 + (i * 256 + threadIdx.x) * 8, row.top, rt, scale, held.a, w);
+  if (sc.plain) {
+    double left[8];
+    left_of<T, Q, true>(p, r, e, sc, unit, w.a, left);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x += w[k];
+    for (int k = 0; k < 8; ++k) x += left[k];
+  } else {
+    float l[8], q[8];
+    eight(row, e, p.V, -INFINITY, l);
+    eight(static_cast<const Q*>(p.probs) + r * p.ldp, e, p.V, 0.f, q);
+    const double part = unit * sc.rest;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x += fmax(weight_part(l[k], sc) * part - (q[k] > 0.f ? w.a * (double)q[k] : 0.0), 0.0);
   }
   x = block_add(x, red);
   if (threadIdx.x == 0) p.sums[((int64_t)round * p.B + b) * p.chunks + chunk] = x;
 }
 
-// Dynamic LDS: chunks doubles, what is left in each chunk.
+// Dynamic LDS: chunks doubles, what is left in each chunk. The workgroup after the last sequence's has the rows of none.
 template <typename T, typename Q, bool PROBS>
 __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
   extern __shared__ double chunk_left[];
-  __shared__ double red[16], tail[16];
+  __shared__ double red[4][16], tail[16];
   __shared__ Walk held;
   __shared__ int need, pick;
   __shared__ double level;
-  __shared__ int64_t found, last;
-  const int b = blockIdx.x;
+  __shared__ long long found, last;
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (b == p.B) {
+    int lo, hi;
+    seq_span(p.q_ptr, p.B, p.N, lo, hi);
+    for (int64_t r = threadIdx.x; r < p.N; r += 1024)
+      if (r < lo || r >= hi) p.path[r] = -1;
+    return;
+  }
+  const float t = temperature(p, b);
   SeqPlace s;
   if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == b; }, s)) return;
   if (s.n == 0) {
@@ -374,41 +476,61 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     }
     return;
   }
-  const float t = temperature(p, b);
-  const double rt = t > 0.f ? 1.0 / (double)t : 0.0;
-  // what is left in one chunk, to all threads; without q less the children's tokens, all of them rejected
-  const auto chunk_sum = [&](int64_t r, const DraftRow& row, double scale, double a, int chunk, bool less) {
-    const int64_t e = (int64_t)chunk * kPiece - lead(static_cast<const T*>(p.logits) + r * p.ldl) + threadIdx.x * 8;
-    double w[8];
-    left_of<T, Q, PROBS>(p, r, e, row.top, rt, scale, a, w);
-    if (less)
-      for (int j = (int)(r - s.first) + 1; j < s.n; ++j) {
-        const int64_t x = p.rows[s.first + j].token - e;
-        if (p.rows[s.first + j].above == (int)(r - s.first) && x >= 0 && x < 8)
+  if (!PROBS || p.rounds == 0) {
+    for (int j = wave; j < s.n; j += 16) row_info<T, Q, PROBS>(p, s.first, j, t);
+    __syncthreads();
+  }
+
+  // what is left in four chunks, to all threads; `less`: without the tokens of the row's children, all of them rejected
+  const auto chunk_sums = [&](int64_t r, Scale sc, double unit, double a, int c0, int many, bool less) {
+    const int64_t e0 = (int64_t)c0 * kPiece - lead(static_cast<const T*>(p.logits) + r * p.ldl) + threadIdx.x * 8;
+    double sum[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = i == (int)x ? 0.0 : w[i];
-      }
-    double x = 0.0;
+    for (int k = 0; k < 4; ++k) {
+      sum[k] = 0.0;
+      if (k >= many) continue;
+      const int64_t e = e0 + (int64_t)k * kPiece;
+      double w[8];
+      left_of<T, Q, PROBS>(p, r, e, sc, unit, a, w);
+      if (less)
+        for (int j = (int)(r - s.first) + 1; j < s.n; ++j) {
+          const int64_t x = p.rows[s.first + j].token - e;
+          if (p.rows[s.first + j].above == (int)(r - s.first) && x >= 0 && x < 8)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x += w[i];
-    return block_add(x, red);
+            for (int i = 0; i < 8; ++i) w[i] = i == (int)x ? 0.0 : w[i];
+        }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[k] += w[i];
+      sum[k] = wave_add(sum[k]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (lane == 0) red[k][wave] = sum[k];
+    __syncthreads();
+    double all = 0.0;
+    for (int k = 0; k < many; ++k) {
+      double x = 0.0;
+      for (int v = 0; v < 16; ++v) x += red[k][v];
+      if (threadIdx.x == 0) chunk_left[c0 + k] = x;
+      all += x;
+    }
+    return all;
   };
 
+  // from the start, or from the last rejection that draft_sums_k was launched for, if there were so many
   Walk w{1, 0, 1, 0, 0.0, 1.0};
-  const auto known_sum = [&](int i) {
-    double x = 0.0;
-    for (int c = threadIdx.x & 63; c < p.chunks; c += 64) x += p.sums[((int64_t)i * p.B + b) * p.chunks + c];
-    return wave_add(x);
-  };
-  int known = PROBS ? p.rounds : 0;
-  bool fresh = false;  // chunk_left holds the last rejection's sums
+  if (PROBS && p.rounds > 0) {
+    w = p.walks[(int64_t)(p.rounds - 1) * p.B + b];
+    if (t > 0.f && w.rejections == p.rounds && wave == 0) w.t = known_sum(p, b, p.rounds - 1);
+  }
   if (threadIdx.x == 0) p.path[s.first] = 0;
   while (true) {
-    if (threadIdx.x < 64) {
-      const bool more = walk_on<PROBS>(p, s, t, w, known, known_sum, [&](int i, int j) {
-        if (threadIdx.x == 0) p.path[s.first + i] = j;
+    if (wave == 0) {
+      const bool more = walk_on<PROBS>(p, s, t, w, [&](int i, int j) {
+        if (lane == 0) p.path[s.first + i] = j;
       });
-      if (threadIdx.x == 0) {
+      if (lane == 0) {
         held = w;
         need = more;
       }
@@ -418,19 +540,12 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     const bool more = need;
     __syncthreads();
     if (!more) break;
-    // a rejection beyond the ones summed by the whole chip
+    // a rejection beyond the ones that draft_sums_k was launched for
     const int64_t r = s.first + w.cur;
-    const DraftRow row = p.rows[r];
-    double all = 0.0;
-    for (int c = 0; c < p.chunks; ++c) {
-      const double x = chunk_sum(r, row, 1.0 / row.sum, w.a, c, false);
-      if (threadIdx.x == 0) chunk_left[c] = x;
-      all += x;
-    }
-    w.t = all;
-    known = w.rejections;
-    fresh = true;
-    __syncthreads();
+    const Scale sc = scale_of(t, p.rows[r].top);
+    const double unit = 1.0 / p.rows[r].sum;
+    w.t = 0.0;
+    for (int c = 0; c < p.chunks; c += 4) w.t += chunk_sums(r, sc, unit, w.a, c, min(4, p.chunks - c), false);
   }
   for (int i = w.count + threadIdx.x; i < s.n; i += 1024) p.path[s.first + i] = -1;
   const int64_t r = s.first + w.cur;
@@ -443,73 +558,89 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     return;
   }
   // what is left in each chunk, in probabilities with q, otherwise in units of the largest logit's
-  double scale = PROBS ? 1.0 / row.sum : 1.0, a = w.a;
-  const bool rejected = PROBS ? a > 0.0 : w.rejections > 0;
+  const Scale sc = scale_of(t, row.top);
+  const double unit = PROBS ? 1.0 / row.sum : 1.0;
+  double a = w.a;
   const auto whole = [&]() {
     for (int c = threadIdx.x; c < p.chunks; c += 1024) {
       const DraftChunk x = p.parts[r * p.chunks + c];
-      chunk_left[c] = x.top > -INFINITY ? x.sum * exp(((double)x.top - (double)row.top) * rt) * scale : 0.0;
+      chunk_left[c] = x.sum * weight(x.top, sc) * unit;
     }
     __syncthreads();
   };
   bool less = false;
-  if (PROBS && rejected) {
-    if (!fresh || w.rejections <= p.rounds)
+  if (PROBS && a > 0.0) {
+    if (w.rejections <= p.rounds)  // else they are there from the walk
       for (int c = threadIdx.x; c < p.chunks; c += 1024)
         chunk_left[c] = p.sums[((int64_t)(w.rejections - 1) * p.B + b) * p.chunks + c];
     __syncthreads();
   } else {
     whole();
     if (!PROBS) {
-      // the chunks of the children's tokens again without them; each once
-      const int first = lead(static_cast<const T*>(p.logits) + r * p.ldl);
-      for (int j = w.cur + 1; j < s.n; ++j) {
-        const DraftRow child = p.rows[s.first + j];
-        if (child.above != w.cur || child.token < 0 || child.token >= p.V) continue;
-        less = true;
-        const int c = (int)((child.token + first) / kPiece);
-        const double x = chunk_sum(r, row, scale, a, c, true);
-        if (threadIdx.x == 0) chunk_left[c] = x;
-        __syncthreads();
+      // less the children's tokens; a chunk of which little is left (cancelled digits) is summed again without them
+      if (wave == 0) {
+        const int first = lead(static_cast<const T*>(p.logits) + r * p.ldl);
+        bool some = false;
+        for (int j0 = w.cur + 1; j0 < s.n; j0 += 64) {
+          const DraftRow* const child = p.rows + s.first + min(j0 + lane, s.n - 1);
+          const double x = j0 + lane < s.n && child->above == w.cur ? child->p : 0.0;
+          const int c = x > 0.0 ? (int)((child->token + first) / kPiece) : 0;
+          for (unsigned long long m = __ballot(x > 0.0); m != 0; m &= m - 1) {
+            const int l = __builtin_ctzll(m), at = __builtin_amdgcn_readlane(c, l);
+            const double before = chunk_left[at], after = before - lane_of(x, l) * row.sum;
+            some = true;
+            if (lane == 0) chunk_left[at] = before < 0.0 || after < 1e-3 * before ? -1.0 : after;
+          }
+        }
+        if (lane == 0) need = some;
       }
+      __syncthreads();
+      less = need;
+      if (less)
+        for (int c = 0; c < p.chunks; ++c) {
+          if (chunk_left[c] >= 0.0) continue;  // the same for the whole workgroup: written before the barriers above
+          chunk_sums(r, sc, unit, a, c, 1, true);
+          __syncthreads();
+        }
     }
   }
   for (int again = 0; again < 2; ++again) {
     // the chunk in which the sum passes its share; the last one that has anything where none does
-    if (threadIdx.x == 0) {
+    if (wave == 0) {
       double all = 0.0;
-      for (int c = 0; c < p.chunks; ++c) all += chunk_left[c];
+      for (int c0 = 0; c0 < p.chunks; c0 += 64) all += wave_add(c0 + lane < p.chunks ? chunk_left[c0 + lane] : 0.0);
       const double share = (double)p.u[s.first] * all;
-      double before = 0.0;
-      int at = -1, any = -1;
-      double at_any = 0.0;
-      for (int c = 0; c < p.chunks; ++c) {
-        if (!(chunk_left[c] > 0.0)) continue;
-        any = c;
-        at_any = before;
-        if (before + chunk_left[c] > share) {
-          at = c;
-          break;
+      double before = 0.0, at_before = 0.0;
+      int at = -1;
+      for (int c0 = 0; c0 < p.chunks; c0 += 64) {
+        const double x = c0 + lane < p.chunks ? chunk_left[c0 + lane] : 0.0, upto = wave_upto(x);
+        const unsigned long long some = __ballot(x > 0.0), hit = __ballot(x > 0.0 && before + upto > share);
+        if (some != 0) {
+          const int l = hit != 0 ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
+          at = c0 + l;
+          at_before = before + (lane_of(upto, l) - lane_of(x, l));
         }
-        before += chunk_left[c];
+        if (hit != 0) break;
+        before += lane_of(upto, 63);
       }
-      pick = at >= 0 ? at : any;
-      level = share - (at >= 0 ? before : at_any);
-      found = 0x7fffffffffffffff;
-      last = -1;
+      if (lane == 0) {
+        pick = at;
+        level = share - at_before;
+        found = 0x7fffffffffffffffLL;
+        last = -1;
+      }
     }
     __syncthreads();
     if (pick >= 0) break;
     // nothing left: the row's own distribution
     a = 0.0;
     less = false;
-    __syncthreads();
     whole();
   }
   if (pick >= 0) {
     const int64_t e = (int64_t)pick * kPiece - lead(static_cast<const T*>(p.logits) + r * p.ldl) + threadIdx.x * 8;
     double x[8];
-    left_of<T, Q, PROBS>(p, r, e, row.top, rt, scale, a, x);
+    left_of<T, Q, PROBS>(p, r, e, sc, unit, a, x);
     if (less)
       for (int j = w.cur + 1; j < s.n; ++j) {
         const int64_t k = p.rows[s.first + j].token - e;
@@ -521,32 +652,27 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) mine += x[i];
     // the sum of the places before this thread's
-    double upto = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(upto, o);
-      if ((threadIdx.x & 63) >= o) upto += y;
-    }
-    if ((threadIdx.x & 63) == 63) tail[threadIdx.x >> 6] = upto;
+    const double upto = wave_upto(mine);
+    if (lane == 63) tail[wave] = upto;
     __syncthreads();
     double before = upto - mine;
-    for (int v = 0; v < (int)(threadIdx.x >> 6); ++v) before += tail[v];
-    int64_t hit = 0x7fffffffffffffff, some = -1;
+    for (int v = 0; v < wave; ++v) before += tail[v];
+    long long hit = 0x7fffffffffffffffLL, some = -1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       before += x[i];
       if (x[i] > 0.0) {
         some = e + i;
-        if (before > level && hit == 0x7fffffffffffffff) hit = e + i;
+        if (before > level && hit == 0x7fffffffffffffffLL) hit = e + i;
       }
     }
-    if (hit != 0x7fffffffffffffff) atomicMin(reinterpret_cast<long long*>(&found), (long long)hit);
-    if (some >= 0) atomicMax(reinterpret_cast<long long*>(&last), (long long)some);
+    if (hit != 0x7fffffffffffffffLL) atomicMin(&found, hit);
+    if (some >= 0) atomicMax(&last, some);
     __syncthreads();
   }
   if (threadIdx.x == 0) {
     p.count[b] = w.count;
-    p.next[b] = found != 0x7fffffffffffffff ? found : last;
+    p.next[b] = found != 0x7fffffffffffffffLL ? found : last;
   }
 }
 
@@ -556,33 +682,33 @@ int64_t draft_chunks(int64_t V) { return (V + 7 + kPiece - 1) / kPiece; }
 
 int64_t draft_work_bytes(int64_t N, int64_t B, int64_t V, bool probs) {
   const int64_t c = draft_chunks(V);
-  return N * c * (int64_t)sizeof(DraftChunk) + N * (int64_t)sizeof(DraftRow) + (probs ? kDraftRounds * B * c * 8 : 0);
+  return N * c * (int64_t)sizeof(DraftChunk) + N * (int64_t)sizeof(DraftRow) + (probs ? kDraftRounds * B * (c * 8 + (int64_t)sizeof(DraftWalk)) : 0);
 }
 
 hipError_t launch_verify(DraftParams p, bool f32, bool probs_f32, uint8_t* work, hipStream_t st) {
   p.chunks = (int)draft_chunks(p.V);
-  // in a line of tokens nothing follows a rejection but the next token
-  p.rounds = p.probs == nullptr ? 0 : p.parents != nullptr ? kDraftRounds : 1;
+  // In a line of tokens nothing follows a rejection but the next token. A few chunks are summed by one workgroup sooner than
+  // by another launch.
+  p.rounds = p.probs == nullptr || p.chunks <= 4 ? 0 : p.parents != nullptr ? kDraftRounds : 1;
   p.parts = reinterpret_cast<DraftChunk*>(work);
   p.rows = reinterpret_cast<DraftRow*>(p.parts + p.N * p.chunks);
-  p.sums = reinterpret_cast<double*>(p.rows + p.N);
+  p.walks = reinterpret_cast<DraftWalk*>(p.rows + p.N);
+  p.sums = reinterpret_cast<double*>(p.walks + kDraftRounds * p.B);
   const dim3 wide(256), parts((unsigned)(p.N * p.chunks)), rows((unsigned)((p.N + 3) / 4));
-  if (p.N > 0) {
-    hipLaunchKernelGGL(f32 ? draft_chunks_k<float> : draft_chunks_k<uint16_t>, parts, wide, 0, st, p);
-    const auto rows_k = p.probs == nullptr ? (f32 ? draft_rows_k<float, float, false> : draft_rows_k<uint16_t, float, false>)
-                        : probs_f32 ? (f32 ? draft_rows_k<float, float, true> : draft_rows_k<uint16_t, float, true>)
-                                    : (f32 ? draft_rows_k<float, uint16_t, true> : draft_rows_k<uint16_t, uint16_t, true>);
+  if (p.N > 0) hipLaunchKernelGGL(f32 ? draft_chunks_k<float> : draft_chunks_k<uint16_t>, parts, wide, 0, st, p);
+  if (p.rounds > 0 && p.N > 0 && p.B > 0) {
+    const auto rows_k = probs_f32 ? (f32 ? draft_rows_k<float, float> : draft_rows_k<uint16_t, float>)
+                                  : (f32 ? draft_rows_k<float, uint16_t> : draft_rows_k<uint16_t, uint16_t>);
+    const auto sums_k = probs_f32 ? (f32 ? draft_sums_k<float, float> : draft_sums_k<uint16_t, float>)
+                                  : (f32 ? draft_sums_k<float, uint16_t> : draft_sums_k<uint16_t, uint16_t>);
     hipLaunchKernelGGL(rows_k, rows, wide, 0, st, p);
+    for (int i = 0; i < p.rounds; ++i)
+      hipLaunchKernelGGL(sums_k, dim3((unsigned)(p.B * p.chunks)), dim3(1024), 0, st, p, i);
   }
-  if (p.B == 0) return hipGetLastError();
-  const auto sums_k = probs_f32 ? (f32 ? draft_sums_k<float, float> : draft_sums_k<uint16_t, float>)
-                                : (f32 ? draft_sums_k<float, uint16_t> : draft_sums_k<uint16_t, uint16_t>);
-  for (int i = 0; i < p.rounds; ++i)
-    hipLaunchKernelGGL(sums_k, dim3((unsigned)(p.B * p.chunks)), wide, 0, st, p, i);
   const auto next_k = p.probs == nullptr ? (f32 ? draft_next_k<float, float, false> : draft_next_k<uint16_t, float, false>)
                       : probs_f32 ? (f32 ? draft_next_k<float, float, true> : draft_next_k<uint16_t, float, true>)
                                   : (f32 ? draft_next_k<float, uint16_t, true> : draft_next_k<uint16_t, uint16_t, true>);
-  hipLaunchKernelGGL(next_k, dim3((unsigned)p.B), dim3(1024), p.chunks * 8, st, p);
+  hipLaunchKernelGGL(next_k, dim3((unsigned)(p.B + 1)), dim3(1024), p.chunks * 8, st, p);
   return hipGetLastError();
 }
 

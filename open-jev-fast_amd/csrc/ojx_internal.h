@@ -368,7 +368,7 @@ struct CopyParams {
 hipError_t launch_pages_copy(const CopyParams& p, int64_t n, int layers, hipStream_t st);
 
 // Verification of drafted tokens (drafts.hip).
-constexpr int kDraftRounds = 3;           // rejections of a sequence whose sums are made by the whole chip
+constexpr int kDraftRounds = 6;           // rejections of a sequence whose sums are made by the whole chip
 struct DraftParams {
   const void* logits; int64_t ldl;        // [N, V], row stride
   const void* probs; int64_t ldp;         // [N, V], or null
@@ -380,6 +380,7 @@ struct DraftParams {
   int B, chunks, rounds;
   struct DraftChunk* parts;               // [N, chunks] workspace
   struct DraftRow* rows;                  // [N]
+  struct DraftWalk* walks;                // [rounds, B]
   double* sums;                           // [rounds, B, chunks]
 };
 int64_t draft_chunks(int64_t V);
