@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
   __shared__ Walk held;
   __shared__ int need, pick;
   __shared__ double level;
-  __shared__ long long found, last;
+  __shared__ int first_hit[16], last_some[16];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (b == p.B) {
     int lo, hi;
@@ -626,8 +626,6 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
       if (lane == 0) {
         pick = at;
         level = share - at_before;
-        found = 0x7fffffffffffffffLL;
-        last = -1;
       }
     }
     __syncthreads();
@@ -657,22 +655,33 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     __syncthreads();
     double before = upto - mine;
     for (int v = 0; v < wave; ++v) before += tail[v];
-    long long hit = 0x7fffffffffffffffLL, some = -1;
+    int hit = -1, some = -1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       before += x[i];
       if (x[i] > 0.0) {
-        some = e + i;
-        if (before > level && hit == 0x7fffffffffffffffLL) hit = e + i;
+        some = (int)e + i;
+        if (before > level && hit < 0) hit = (int)e + i;
       }
     }
-    if (hit != 0x7fffffffffffffffLL) atomicMin(&found, hit);
-    if (some >= 0) atomicMax(&last, some);
+    // the first place of the first wave that has one, else the last place with anything
+    const unsigned long long hits = __ballot(hit >= 0), somes = __ballot(some >= 0);
+    if (lane == 0) {
+      first_hit[wave] = hits != 0 ? __builtin_amdgcn_readlane(hit, __builtin_ctzll(hits)) : -1;
+      last_some[wave] = somes != 0 ? __builtin_amdgcn_readlane(some, 63 - __builtin_clzll(somes)) : -1;
+    }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
+    int at = -1;
+    if (pick >= 0) {
+      for (int v = 15; v >= 0; --v)
+        if (at < 0) at = last_some[v];
+      for (int v = 15; v >= 0; --v)
+        if (first_hit[v] >= 0) at = first_hit[v];
+    }
     p.count[b] = w.count;
-    p.next[b] = found != 0x7fffffffffffffffLL ? found : last;
+    p.next[b] = at;
   }
 }
 
