@@ -130,7 +130,11 @@ __device__ __forceinline__ void by_rows(const LinTreeParams& p, const SeqPlace& 
   }
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int kTree = 64;  // rows that a sequence may have to be taken at once
+
+// 16-byte pieces of 16 rows that are read at once spread over the banks.
+__device__ __forceinline__ constexpr int swizzle(int r) { return (r & 7) << 1 | (r >> 3 & 1); }
 
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -143,25 +147,22 @@ __device__ __forceinline__ f32x4 times(const f32x4& at, const f32x4& b, f32x4 c)
   for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(at[r], b[r], c, 0, 0, 0);
   return c;
 }
-// Is (row, col) in the lower left part of a pair of blocks of `size`?
-__device__ __forceinline__ bool joins(int row, int col, int size) {
-  return (row / size & 1) == 1 && (col / size & 1) == 0 && row / (2 * size) == col / (2 * size);
-}
 // The transposed inverse of I + a, a strictly lower triangular, at = a transposed: inverses of blocks of 1, 2, 4, 8 joined
-// two by two, T <- T - T a T with a's part below the diagonal blocks, T kept both ways.
+// two by two, T <- T - T a T with the part of a that joins blocks of this size, T kept both ways. That part is where row and
+// column differ in the size's bit and in none above it.
 __device__ __forceinline__ f32x4 inverse(const f32x4& a, const f32x4& at, int g, int c) {
   f32x4 t, tt;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int i = 4 * g + r;
-    t[r] = (i == c ? 1.f : 0.f) - (joins(i, c, 1) ? a[r] : 0.f);
-    tt[r] = (i == c ? 1.f : 0.f) - (joins(c, i, 1) ? at[r] : 0.f);
+    const int differ = (4 * g + r) ^ c;
+    t[r] = differ == 0 ? 1.f : (differ & 15) == 1 ? -a[r] : 0.f;
+    tt[r] = differ == 0 ? 1.f : (differ & 15) == 1 ? -at[r] : 0.f;
   }
 #pragma unroll
   for (int size = 2; size <= 8; size *= 2) {
     f32x4 m;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) m[r] = joins(c, 4 * g + r, size) ? at[r] : 0.f;
+    for (int r = 0; r < 4; ++r) m[r] = (((4 * g + r) ^ c) & (16 - size)) == size ? at[r] : 0.f;
     const f32x4 w = times(m, t, f32x4{});
     const f32x4 down = size < 8 ? times(tt, w, f32x4{}) : f32x4{};
     tt -= times(w, tt, f32x4{});
@@ -176,6 +177,9 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = cvt_pk2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
 }
 
+// LDS reads and writes of all waves are done; global loads stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // A sequence's rows at once, in blocks of 16 (a block's rows are tokens, its columns value dims; with two value dims, 2 c and
 // 2 c + 1 of the wave's 32, for each lane): with
 //   A_ij = beta_i e^(G_i - G_j) k_i . k_j  and  P_ij = e^(G_i - G_j) q_i . k_j  for the ancestors j of i (in P also i itself),
@@ -183,12 +187,18 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 // block row after block row. S0 enters as two bf16 pieces (what it makes is rounded to bf16 in the end), everything else in
 // fp32. A product with a zero in place of a row that is no ancestor is only right for finite numbers: where a U is not finite
 // or a decay is above 1, the head goes row by row instead.
+// Loads come back in the order in which they were made, so the rows' go first: while the state is on its way the four waves
+// make the blocks of A, P and the inverses of A's diagonal ones, each once, and hand them to each other in LDS as the operands
+// that they are.
 template <bool DELTA>
-__global__ void __launch_bounds__(256, 2) lintree_k(LinTreeParams p) {
-  __shared__ float red[4 * 32 * 12];
-  __shared__ double sums[4][kTree];      // every wave's own
-  __shared__ uint64_t seen[4][kTree];
-  __shared__ float strength[4][kTree];
+__global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
+  __shared__ __attribute__((aligned(16))) f32x4 mats[19][64];
+  __shared__ __attribute__((aligned(16))) bf16x8 rows[2][kTree][16];  // K and Q, piece x of a row r at x ^ swizzle(r)
+  __shared__ double sums[kTree];  // every wave writes the same there
+  __shared__ uint64_t seen[kTree];
+  __shared__ float strength[kTree];
+  float* const red = reinterpret_cast<float*>(mats);  // row by row
+  static_assert(sizeof(mats) >= 4 * 32 * 12 * 4, "by_rows' sums");
   const int64_t b = blockIdx.x / p.HV;
   const int h = blockIdx.x - (int)(b * p.HV), hk = h / (p.HV / p.HK);
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -202,21 +212,11 @@ __global__ void __launch_bounds__(256, 2) lintree_k(LinTreeParams p) {
     return;
   }
   const int64_t slot = p.slot[b];
-  const bool there = slot >= 0 && slot < p.slots;
-  const int dv = w * 32 + c * 2;
-  float2 st[4][8];  // key dims 32 s + 8 g + j
-  if (there) {
-    const float* const from = p.state + (slot * p.HV + h) * (kHD * kHD) + g * 8 * kHD + dv;
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) st[s][j] = *reinterpret_cast<const float2*>(from + (s * 32 + j) * kHD);
-  }
   SeqPlace at;
   if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == (int)b; }, at)) return;
   const int n = at.n;
   if (n == 0) return;
-  if (!there) {
+  if (slot < 0 || slot >= p.slots) {
     const uint32_t x = slot < 0 ? 0u : 0x7fc07fc0u;
     for (int i = threadIdx.x >> 5; i < n; i += 8)
       *reinterpret_cast<uint2*>(p.o + ((int64_t)(at.first + i) * p.HV + h) * kHD + (threadIdx.x & 31) * 4) = make_uint2(x, x);
@@ -227,15 +227,49 @@ __global__ void __launch_bounds__(256, 2) lintree_k(LinTreeParams p) {
     return;
   }
 
-  // a row a lane: its ancestors and itself, and the sum of their decays (to base two, in 64 bits: differences of long sums
-  // are taken), by jumps of 1, 2, 4 .. rows up the tree
-  bool odd = false;
+  const int dv = w * 32 + c * 2, blocks = (n + 15) >> 4;
+  float gate, beta;
+  int up;
+  bf16x8 kf[4], qf[4];    // a piece a thread of each block's rows of K and Q
+  uint32_t vw[4][4];   // this lane's values of rows 16 I + 4 g + r
   {
     const int64_t row = at.first + min(lane, n - 1);
-    const float gate = p.g[row * p.HV + h], beta = DELTA ? bf2f(p.beta[row * p.HV + h]) : 1.f;
-    int up = p.parents == nullptr ? lane - 1 : p.parents[row];
+    gate = p.g[row * p.HV + h];
+    beta = DELTA ? bf2f(p.beta[row * p.HV + h]) : 1.f;
+    up = p.parents == nullptr ? lane - 1 : p.parents[row];
+  }
+#pragma unroll
+  for (int I = 0; I < 4; ++I)
+    if (I < blocks) {
+      const int64_t row = at.first + min(I * 16 + ((int)threadIdx.x >> 4), n - 1);
+      const int64_t from = (row * p.HK + hk) * kHD + (threadIdx.x & 15) * 8;
+      kf[I] = *reinterpret_cast<const bf16x8*>(p.k + from);
+      qf[I] = *reinterpret_cast<const bf16x8*>(p.q + from);
+    }
+#pragma unroll
+  for (int I = 0; I < 4; ++I)
+    if (I < blocks)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t row = at.first + min(I * 16 + g * 4 + r, n - 1);
+        vw[I][r] = *reinterpret_cast<const uint32_t*>(p.v + (row * p.HV + h) * kHD + dv);
+      }
+  asm volatile("" ::: "memory");  // the state's loads stay behind
+  f32x2 st[4][8];                 // key dims 32 s + 8 g + j
+  {
+    const float* const from = p.state + (slot * p.HV + h) * (kHD * kHD) + g * 8 * kHD + dv;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) st[s][j] = *reinterpret_cast<const f32x2*>(from + (s * 32 + j) * kHD);
+  }
+  asm volatile("" ::: "memory");
+
+  // a row a lane: its ancestors and itself, and the sum of their decays (to base two, in 64 bits: differences of long sums
+  // are taken), by jumps of 1, 2, 4 .. rows up the tree
+  bool odd = !(gate <= 0.f) || !(fabsf(beta) < INFINITY);
+  {
     if (up < 0 || up >= lane || lane >= n) up = -1;
-    odd = !(gate <= 0.f) || !(fabsf(beta) < INFINITY);
     // e^-200 is 0 in fp32: -infinity does no worse, and differences of sums stay numbers
     double G = lane < n ? (double)fmaxf(gate, -200.f) * 0x1.71547652b82fep+0 : 0.0;
     uint64_t path = lane < n ? 1ull << lane : 0ull;
@@ -250,129 +284,133 @@ __global__ void __launch_bounds__(256, 2) lintree_k(LinTreeParams p) {
         up = next;
       }
     }
-    sums[w][lane] = G;
-    seen[w][lane] = path;
-    strength[w][lane] = beta;
+    sums[lane] = G;
+    seen[lane] = path;
+    strength[lane] = beta;
   }
-  // the state's pieces
-  bf16x8 hi[4][2], lo[4][2];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    uint32_t ph[2][4], pl[2][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      split2(st[s][2 * j].x, st[s][2 * j + 1].x, ph[0][j], pl[0][j]);
-      split2(st[s][2 * j].y, st[s][2 * j + 1].y, ph[1][j], pl[1][j]);
+  for (int I = 0; I < 4; ++I)
+    if (I < blocks) {
+      const int r = (int)threadIdx.x >> 4, x = (threadIdx.x & 15) ^ swizzle(r);
+      rows[0][I * 16 + r][x] = kf[I];
+      rows[1][I * 16 + r][x] = qf[I];
     }
-#pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      hi[s][f] = __builtin_bit_cast(bf16x8, make_uint4(ph[f][0], ph[f][1], ph[f][2], ph[f][3]));
-      lo[s][f] = __builtin_bit_cast(bf16x8, make_uint4(pl[f][0], pl[f][1], pl[f][2], pl[f][3]));
-    }
-  }
-  const auto operand = [&](const uint16_t* x, int block, int s) {  // row 16 block + c, dims 32 s + 8 g .. + 7
-    const int64_t row = at.first + min(block * 16 + c, n - 1);
-    return *reinterpret_cast<const bf16x8*>(x + (row * p.HK + hk) * kHD + s * 32 + g * 8);
+  lds_barrier();
+  const auto operand = [&](int which, int block, int s) {  // row 16 block + c, dims 32 s + 8 g .. + 7
+    return rows[which][block * 16 + c][(s * 4 + g) ^ swizzle(c)];
   };
+  const auto fade = [&](double from, double to) { return __builtin_amdgcn_exp2f((float)(from - to)); };
 
-  f32x4 u[4][2];
+  // mats: the transposed inverses of the diagonal blocks 0 .. 2, the blocks' P transposed 3 .. 6; below the diagonal -A
+  // transposed 7 .. 12 and P transposed 13 .. 18. Wave w has diagonal block w and the pairs w and w + 4 of the six others.
+  // The fourth inverse stays with its wave until the rows' place is free: with 1 KB less, three workgroups fit a CU.
+  f32x4 fourth = {};
 #pragma unroll
-  for (int I = 0; I < 4; ++I) {
-    if (I * 16 >= n) break;
-    bf16x8 kf[4], qf[4];
+  for (int turn = 0; turn < 3; ++turn) {
+    // pairs (1, 0), (2, 0), (2, 1), (3, 0), (3, 1), (3, 2)
+    const int pair = turn == 2 ? w + 4 : w, I = turn == 0 ? w : pair == 0 ? 1 : pair <= 2 ? 2 : 3;
+    const int J = turn == 0 ? w : pair == 0 ? 0 : pair <= 2 ? pair - 1 : pair - 3;
+    if (I >= blocks || (turn > 0 && pair > 5)) continue;  // the same for the wave
+    const int i = I * 16 + c;
+    const uint64_t path = seen[i];
+    const double Gi = sums[i];
+    f32x4 kk = {}, qk = {};
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      kf[s] = operand(p.k, I, s);
-      qf[s] = operand(p.q, I, s);
+      const bf16x8 kj = operand(0, J, s);
+      if (DELTA) kk = mfma(kj, turn == 0 ? kj : operand(0, I, s), kk);
+      qk = mfma(kj, operand(1, I, s), qk);
     }
-    uint32_t vw[4];
+    f32x4 a, down;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int64_t row = at.first + min(I * 16 + g * 4 + r, n - 1);
-      vw[r] = *reinterpret_cast<const uint32_t*>(p.v + (row * p.HV + h) * kHD + dv);
+      const int j = J * 16 + g * 4 + r;
+      const bool in = path >> j & 1;
+      const float e = in ? fade(Gi, sums[j]) : 0.f;
+      qk[r] = in ? e * qk[r] : 0.f;
+      if (DELTA) {
+        a[r] = in && i != j ? strength[i] * e * kk[r] : 0.f;
+        // the block itself, from the other side (its products are symmetric)
+        if (turn == 0) down[r] = i != j && (seen[j] >> i & 1) ? strength[j] * fade(sums[j], Gi) * kk[r] : 0.f;
+      }
     }
-    f32x4 x[2] = {}, o[2] = {};
+    mats[turn == 0 ? 3 + w : 13 + pair][lane] = qk;
+    if (DELTA) {
+      const f32x4 x = turn == 0 ? inverse(down, a, g, c) : -a;
+      if (turn == 0 && w == 3)
+        fourth = x;
+      else
+        mats[turn == 0 ? w : 7 + pair][lane] = x;
+    }
+  }
+  lds_barrier();
+
+  // K S0 and Q S0
+  f32x4 u[4][2], o[4][2];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+  for (int I = 0; I < 4; ++I)
+#pragma unroll
+    for (int f = 0; f < 2; ++f) u[I][f] = o[I][f] = f32x4{};
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    uint32_t hi[2][4], lo[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      split2(st[s][2 * j].x, st[s][2 * j + 1].x, hi[0][j], lo[0][j]);
+      split2(st[s][2 * j].y, st[s][2 * j + 1].y, hi[1][j], lo[1][j]);
+    }
+#pragma unroll
+    for (int I = 0; I < 4; ++I) {
+      if (I >= blocks) break;
+      const bf16x8 kf = operand(0, I, s), qf = operand(1, I, s);
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        if (DELTA) {
-          x[f] = mfma(kf[s], hi[s][f], x[f]);
-          x[f] = mfma(kf[s], lo[s][f], x[f]);
-        }
-        o[f] = mfma(qf[s], hi[s][f], o[f]);
-        o[f] = mfma(qf[s], lo[s][f], o[f]);
+        const bf16x8 sh = __builtin_bit_cast(bf16x8, make_uint4(hi[f][0], hi[f][1], hi[f][2], hi[f][3]));
+        const bf16x8 sl = __builtin_bit_cast(bf16x8, make_uint4(lo[f][0], lo[f][1], lo[f][2], lo[f][3]));
+        if (DELTA) u[I][f] = mfma(kf, sl, mfma(kf, sh, u[I][f]));
+        o[I][f] = mfma(qf, sl, mfma(qf, sh, o[I][f]));
       }
-    // this lane's rows of the block as rows of X and O: 16 I + 4 g + r; as columns of the transposed matrices: 16 I + c
-    float since[4];
+    }
+  }
+
+  f32x4* const late = reinterpret_cast<f32x4*>(rows);
+  if (DELTA && blocks == 4) {
+    lds_barrier();
+    if (w == 3) late[lane] = fourth;
+    lds_barrier();
+  }
+
+#pragma unroll
+  for (int I = 0; I < 4; ++I) {
+    if (I >= blocks) break;
+    f32x4 x[2];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = I * 16 + g * 4 + r;
-      since[r] = __builtin_amdgcn_exp2f((float)sums[w][i]);
-      const float beta = strength[w][i];
+      const float since = __builtin_amdgcn_exp2f((float)sums[i]), by = strength[i];
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const float v = f == 0 ? __uint_as_float(vw[r] << 16) : __uint_as_float(vw[r] & 0xffff0000u);
-        x[f][r] = i < n ? (DELTA ? beta * (v - since[r] * x[f][r]) : v) : 0.f;
-        o[f][r] *= since[r];
+        const float v = __uint_as_float(f == 0 ? vw[I][r] << 16 : vw[I][r] & 0xffff0000u);
+        x[f][r] = i < n ? (DELTA ? by * (v - since * u[I][f][r]) : v) : 0.f;
+        o[I][f][r] *= since;
       }
     }
-    const double Gc = sums[w][I * 16 + c];
-    const uint64_t path = seen[w][I * 16 + c];
-    const float beta = strength[w][I * 16 + c];
 #pragma unroll
     for (int J = 0; J < I; ++J) {
-      f32x4 kk = {}, qk = {};
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const bf16x8 kj = operand(p.k, J, s);
-        if (DELTA) kk = mfma(kj, kf[s], kk);
-        qk = mfma(kj, qf[s], qk);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = J * 16 + g * 4 + r;
-        const bool in = path >> j & 1;
-        const float fade = in ? __builtin_amdgcn_exp2f((float)(Gc - sums[w][j])) : 0.f;
-        kk[r] = in ? -beta * fade * kk[r] : 0.f;
-        qk[r] = in ? fade * qk[r] : 0.f;
-      }
+      const int pair = I * (I - 1) / 2 + J;
+      const f32x4 a = mats[7 + pair][lane], pj = mats[13 + pair][lane];
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        if (DELTA) x[f] = times(kk, u[J][f], x[f]);
-        o[f] = times(qk, u[J][f], o[f]);
+        if (DELTA) x[f] = times(a, u[J][f], x[f]);
+        o[I][f] = times(pj, u[J][f], o[I][f]);
       }
     }
-    f32x4 kk = {}, qk = {}, a, at_;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (DELTA) kk = mfma(kf[s], kf[s], kk);
-      qk = mfma(kf[s], qf[s], qk);
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = I * 16 + g * 4 + r;  // row of the transposed, column c; and row of A, column c
-      const bool in = path >> j & 1;
-      const float fade = in ? __builtin_amdgcn_exp2f((float)(Gc - sums[w][j])) : 0.f;
-      qk[r] = in ? fade * qk[r] : 0.f;
-      if (DELTA) {
-        at_[r] = in && g * 4 + r != c ? beta * fade * kk[r] : 0.f;
-        const bool down = seen[w][j] >> (I * 16 + c) & 1;
-        a[r] = down && g * 4 + r != c
-                   ? strength[w][j] * __builtin_amdgcn_exp2f((float)(sums[w][j] - Gc)) * kk[r] : 0.f;
-      }
-    }
-    if (DELTA) {
-      const f32x4 tt = inverse(a, at_, g, c);
-#pragma unroll
-      for (int f = 0; f < 2; ++f) u[I][f] = times(tt, x[f], f32x4{});
-    } else {
-      u[I][0] = x[0];
-      u[I][1] = x[1];
-    }
+    const f32x4 pi = mats[3 + I][lane];
+    const f32x4 t = !DELTA ? f32x4{} : I < 3 ? mats[I][lane] : late[lane];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
-      o[f] = times(qk, u[I][f], o[f]);
+      u[I][f] = DELTA ? times(t, x[f], f32x4{}) : x[f];
+      o[I][f] = times(pi, u[I][f], o[I][f]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) odd |= !(fabsf(u[I][f][r]) < INFINITY);
     }
@@ -381,71 +419,102 @@ __global__ void __launch_bounds__(256, 2) lintree_k(LinTreeParams p) {
       const int i = I * 16 + g * 4 + r;
       if (i < n)
         *reinterpret_cast<uint32_t*>(p.o + ((int64_t)(at.first + i) * p.HV + h) * kHD + dv) =
-            cvt_pk2(p.scale * o[0][r], p.scale * o[1][r]);
+            cvt_pk2(p.scale * o[I][0][r], p.scale * o[I][1][r]);
     }
   }
   if (__syncthreads_or(odd)) by_rows<DELTA>(p, at, slot, h, hk, red);
 }
 
-// The kept tokens of sequence b, rows path[0 .. count - 1] of its own, through its state one after the other.
+// x summed over the four groups of 16 lanes, in all of them.
+__device__ __forceinline__ float add_rows(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The kept tokens of sequence b, rows path[0 .. count - 1] of its own, through its state one after the other. A wave has 32
+// value dims of a head's state, lane (g, c) the key dims 32 g .. + 31 of value dims 2 c and 2 c + 1 of those: no wave waits
+// for another. Rows of 16 tokens at a time go through LDS, read while the state is on its way.
 template <bool DELTA>
-__global__ void __launch_bounds__(256) linattn_keep_k(LinTreeParams p) {
-  __shared__ float red[2][4 * 32 * 7];
-  const int64_t b = blockIdx.x / p.HV;
-  const int h = blockIdx.x - (int)(b * p.HV), hk = h / (p.HV / p.HK);
-  const int c = threadIdx.x & 31, rg = threadIdx.x >> 5;
+__global__ void __launch_bounds__(64) linattn_keep_k(LinTreeParams p) {
+  constexpr int kTokens = 16;
+  __shared__ __attribute__((aligned(16))) uint16_t keys[kTokens][kHD];
+  __shared__ __attribute__((aligned(16))) uint16_t values[kTokens][32];
+  const int lane = threadIdx.x, g = lane >> 4, c = lane & 15;
+  const int64_t wg = blockIdx.x >> 2, b = wg / p.HV;
+  const int h = (int)(wg - b * p.HV), hk = h / (p.HV / p.HK), dv = (blockIdx.x & 3) * 32;
+  const int64_t slot = p.slot[b];
+  const int count = p.count[b];
   SeqPlace at;
   if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == (int)b; }, at)) return;
-  const int n = min(at.n, p.count[b]);
-  const int64_t slot = p.slot[b];
+  const int n = min(at.n, count);
   // A slot belongs to the first sequence that names it: two workgroups that update one state would race.
-  bool twice = slot < 0 || slot >= p.slots;
-  for (int64_t i = threadIdx.x; i < b; i += 256) twice |= p.slot[i] == slot;
-  if (__syncthreads_or(twice) || n <= 0) return;
-  float* const st = p.state + (slot * p.HV + h) * (kHD * kHD) + rg * 16 * kHD + c * 4;
-  float4 s[16];
+  bool twice = slot < 0 || slot >= p.slots || n <= 0;
+  for (int64_t i = lane; i < b; i += 64) twice |= p.slot[i] == slot;
+  if (__any(twice)) return;
+  int mine = lane < min(n, kTokens) ? p.path[at.first + lane] : -1;
+  float* const st = p.state + (slot * p.HV + h) * (kHD * kHD) + g * 32 * kHD + dv + c * 2;
+  f32x2 s[32];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = *reinterpret_cast<const float4*>(st + i * kHD);
-  for (int i = 0, turn = 0; i < n; ++i) {
-    const int r = p.path[at.first + i];
-    if (r < 0 || r >= at.n) continue;  // the same for the whole workgroup
-    const int64_t row = at.first + r;
-    float k[16], f[4] = {};
-    load16(p.k + (row * p.HK + hk) * kHD + rg * 16, k);
-    const uint2 vw = *reinterpret_cast<const uint2*>(p.v + (row * p.HV + h) * kHD + c * 4);
-    const float a = expf(p.g[row * p.HV + h]);
+  for (int i = 0; i < 32; ++i) s[i] = *reinterpret_cast<const f32x2*>(st + i * kHD);
+  for (int i0 = 0; i0 < n; i0 += kTokens) {
+    if (i0 > 0) mine = lane < min(n - i0, kTokens) ? p.path[at.first + i0 + lane] : -1;
+    const bool valid = mine >= 0 && mine < at.n;
+    const int64_t row = at.first + (valid ? mine : 0);
+    unsigned long long todo = __ballot(valid);
+    const float gate = p.g[row * p.HV + h], beta = DELTA ? bf2f(p.beta[row * p.HV + h]) : 1.f;
+    uint4 piece[4], value;
 #pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      s[x].x *= a;
-      s[x].y *= a;
-      s[x].z *= a;
-      s[x].w *= a;
-    }
-    float u[4] = {bf2f(vw.x & 0xffffu), bf2f(vw.x >> 16), bf2f(vw.y & 0xffffu), bf2f(vw.y >> 16)};
-    if (DELTA) {
+    for (int j = 0; j < 4; ++j)  // tokens 4 j + g, 16 bytes a lane
+      piece[j] = *reinterpret_cast<const uint4*>(p.k + ((int64_t)__shfl((int)row, j * 4 + g) * p.HK + hk) * kHD + c * 8);
+    value = *reinterpret_cast<const uint4*>(p.v + ((int64_t)__shfl((int)row, lane >> 2) * p.HV + h) * kHD + dv +
+                                            (lane & 3) * 8);
 #pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        f[0] += s[x].x * k[x];
-        f[1] += s[x].y * k[x];
-        f[2] += s[x].z * k[x];
-        f[3] += s[x].w * k[x];
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(&keys[j * 4 + g][c * 8]) = piece[j];
+    *reinterpret_cast<uint4*>(&values[lane >> 2][(lane & 3) * 8]) = value;
+    const float decay = expf(gate);
+    for (; todo != 0; todo &= todo - 1) {
+      const int i = __builtin_ctzll(todo);
+      const float a = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(decay), i));
+      const uint32_t vw = *reinterpret_cast<const uint32_t*>(&values[i][c * 2]);
+      f32x2 u = {__uint_as_float(vw << 16), __uint_as_float(vw & 0xffff0000u)};
+      float k[32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 x = *reinterpret_cast<const uint4*>(&keys[i][g * 32 + j * 8]);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          k[j * 8 + 2 * m] = __uint_as_float(w[m] << 16);
+          k[j * 8 + 2 * m + 1] = __uint_as_float(w[m] & 0xffff0000u);
+        }
       }
-      add_groups(f, red[turn]);
-      turn ^= 1;
-      const float beta = bf2f(p.beta[row * p.HV + h]);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) u[x] = beta * (u[x] - f[x]);
-    }
+      for (int j = 0; j < 32; ++j) {
+        s[j].x *= a;
+        s[j].y *= a;
+      }
+      if (DELTA) {
+        float x[2][2] = {};
 #pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      s[x].x += k[x] * u[0];
-      s[x].y += k[x] * u[1];
-      s[x].z += k[x] * u[2];
-      s[x].w += k[x] * u[3];
+        for (int j = 0; j < 32; ++j) {
+          x[j & 1][0] += s[j].x * k[j];
+          x[j & 1][1] += s[j].y * k[j];
+        }
+        const float by = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(beta), i));
+        u.x = by * (u.x - add_rows(x[0][0] + x[1][0]));
+        u.y = by * (u.y - add_rows(x[0][1] + x[1][1]));
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        s[j].x += k[j] * u.x;
+        s[j].y += k[j] * u.y;
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) *reinterpret_cast<float4*>(st + i * kHD) = s[i];
+  for (int i = 0; i < 32; ++i) *reinterpret_cast<f32x2*>(st + i * kHD) = s[i];
 }
 
 }  // namespace
@@ -457,8 +526,8 @@ hipError_t launch_linattn_tree(const LinTreeParams& p, hipStream_t st) {
 }
 
 hipError_t launch_linattn_keep(const LinTreeParams& p, hipStream_t st) {
-  hipLaunchKernelGGL(p.beta != nullptr ? linattn_keep_k<true> : linattn_keep_k<false>, dim3((unsigned)((int64_t)p.B * p.HV)),
-                     dim3(256), 0, st, p);
+  hipLaunchKernelGGL(p.beta != nullptr ? linattn_keep_k<true> : linattn_keep_k<false>, dim3((unsigned)((int64_t)p.B * p.HV * 4)),
+                     dim3(64), 0, st, p);
   return hipGetLastError();
 }
 
