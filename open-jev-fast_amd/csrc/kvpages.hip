@@ -141,7 +141,7 @@ __device__ __forceinline__ int take(const PagesParams& p, int wanted, int32_t* t
     int32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      r[i] = t + i < p.pages ? p.refs[t + i] : 1;
+      r[i] = t + i < p.pages ? __hip_atomic_load(p.refs + t + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 1;
       mine += r[i] <= 0;
     }
     int at = found + block_before(mine, red, all);
@@ -280,8 +280,7 @@ __global__ void __launch_bounds__(1024) resize_small_k(PagesParams p) {
     const int64_t tokens = p.tokens[b], want = (tokens + p.page - 1) / p.page;
     p.out[b] = tokens < 0 ? 0 : (int32_t)max(want - p.max_pages, (int64_t)0);
   }
-  __threadfence();  // counts and outputs, before other threads go on with them
-  __syncthreads();
+  __syncthreads();  // counts (atomic, and read so) and outputs, before other threads go on with them
   const int have = take(p, wanted, taken, red);
   __syncthreads();
 #pragma unroll
@@ -340,15 +339,13 @@ __global__ void __launch_bounds__(1024) fork_small_k(PagesParams p) {
     rank[k] = wanted + before;
     wanted += all;
   }
-  __threadfence();  // counts, and reads of the tables before they change
-  __syncthreads();
+  __syncthreads();  // counts (atomic, and read so), and reads of the tables before they change
   const int have = take(p, wanted, taken, red);
 #pragma unroll
   for (int k = 0; k < kSmall / 1024; ++k) {
     const int f = k * 1024 + threadIdx.x;
     if (f < many && p.src[f / MP] != f / MP) p.table[f] = now[k];
   }
-  __threadfence();
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kSmall / 1024; ++k) {

@@ -437,13 +437,17 @@ __device__ __forceinline__ float add_rows(float x) {
 // value dims of a head's state, lane (g, c) the key dims 32 g .. + 31 of value dims 2 c and 2 c + 1 of those: no wave waits
 // for another. Rows of 16 tokens at a time go through LDS, read while the state is on its way.
 template <bool DELTA>
-__global__ void __launch_bounds__(64) linattn_keep_k(LinTreeParams p) {
+__global__ void __launch_bounds__(128) linattn_keep_k(LinTreeParams p) {
   constexpr int kTokens = 16;
-  __shared__ __attribute__((aligned(16))) uint16_t keys[kTokens][kHD];
-  __shared__ __attribute__((aligned(16))) uint16_t values[kTokens][32];
-  const int lane = threadIdx.x, g = lane >> 4, c = lane & 15;
-  const int64_t wg = blockIdx.x >> 2, b = wg / p.HV;
-  const int h = (int)(wg - b * p.HV), hk = h / (p.HV / p.HK), dv = (blockIdx.x & 3) * 32;
+  __shared__ __attribute__((aligned(16))) uint16_t all_keys[2][kTokens][kHD];
+  __shared__ __attribute__((aligned(16))) uint16_t all_values[2][kTokens][32];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  auto& keys = all_keys[w];
+  auto& values = all_values[w];
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const uint32_t wave = blockIdx.x * (blockDim.x >> 6) + w;
+  const int64_t b = (wave >> 2) / p.HV;
+  const int h = (int)((wave >> 2) - b * p.HV), hk = h / (p.HV / p.HK), dv = (wave & 3) * 32;
   const int64_t slot = p.slot[b];
   const int count = p.count[b];
   SeqPlace at;
@@ -526,8 +530,11 @@ hipError_t launch_linattn_tree(const LinTreeParams& p, hipStream_t st) {
 }
 
 hipError_t launch_linattn_keep(const LinTreeParams& p, hipStream_t st) {
-  hipLaunchKernelGGL(p.beta != nullptr ? linattn_keep_k<true> : linattn_keep_k<false>, dim3((unsigned)((int64_t)p.B * p.HV * 4)),
-                     dim3(64), 0, st, p);
+  // Few heads: every wave a workgroup of its own, so that they take all CUs (4 sequences of 48 heads 8.6 us, 9.1 with two waves
+  // a workgroup, 9.4 with four); many: two (16 sequences 18.3 us, 21.4 with one, 17.7 with four).
+  const int threads = (int64_t)p.B * p.HV <= 384 ? 64 : 128;
+  hipLaunchKernelGGL(p.beta != nullptr ? linattn_keep_k<true> : linattn_keep_k<false>, dim3((unsigned)((int64_t)p.B * p.HV * 256 / threads)),
+                     dim3(threads), 0, st, p);
   return hipGetLastError();
 }
 
