@@ -41,11 +41,14 @@ struct DraftRow {
 struct DraftWalk {
   int j, cur, count, rejections;  // the next row to look at, the current one, accepted so far
   double a, t;
+  int first, n;                   // the sequence's rows, its temperature
+  float temp, pad;
 };
 
 namespace {
 
 constexpr int kPiece = 8192;  // logits of a chunk
+constexpr int kSumThreads = 512;  // of a chunk of draft_sums_k (the largest case 109 us, 112 with 256, 114 with 1024)
 
 __device__ __forceinline__ float value(const uint16_t* p) { return bf2f(*p); }
 __device__ __forceinline__ float value(const float* p) { return *p; }
@@ -81,6 +84,45 @@ __device__ __forceinline__ void eight(const T* row, int64_t e, int64_t V, float 
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = e + i >= 0 && e + i < V ? value(p + i) : none;
+  }
+}
+// The same, still packed.
+template <typename T>
+struct Raw {
+  uint4 x[sizeof(T) / 2];
+};
+__device__ __forceinline__ void pack(const float (&f)[8], Raw<uint16_t>& r) {  // exact: they come from bf16
+  r.x[0] = make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+}
+__device__ __forceinline__ void pack(const float (&f)[8], Raw<float>& r) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    r.x[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
+                        __float_as_uint(f[4 * i + 3]));
+}
+template <typename T>
+__device__ __forceinline__ Raw<T> eight_raw(const T* row, int64_t e, int64_t V) {
+  Raw<T> r;
+  const T* const p = row + e;
+  if (e >= 0 && e + 8 <= V && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.x[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = e + i >= 0 && e + i < V ? value(p + i) : -INFINITY;
+    pack(f, r);
+  }
+  return r;
+}
+__device__ __forceinline__ void open(const Raw<uint16_t>& r, float (&f)[8]) { unpack(r.x[0], f); }
+__device__ __forceinline__ void open(const Raw<float>& r, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float x[4];
+    unpack(r.x[i], x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[i * 4 + j] = x[j];
   }
 }
 // Places of a row are taken from its first 16-byte border on: this many before the row's own first place.
@@ -189,68 +231,86 @@ __device__ __forceinline__ int owner(const DraftParams& p, int64_t r, SeqPlace& 
                                                                                                               : -1;
 }
 
+// `each` chunks of a row for a workgroup, the next one's logits on their way while one is summed.
 template <typename T>
-__global__ void __launch_bounds__(256) draft_chunks_k(DraftParams p) {
-  __shared__ float tops[4];
+__global__ void __launch_bounds__(256) draft_chunks_k(DraftParams p, int each, int groups) {
+  __shared__ float tops[4], temp;
   __shared__ int32_t ats[4];
+  __shared__ int some;
   __shared__ double red[16];
-  const int64_t r = blockIdx.x / (uint32_t)p.chunks;
-  const int chunk = blockIdx.x - (int)(r * p.chunks), wave = threadIdx.x >> 6;
+  const int64_t r = blockIdx.x / (uint32_t)groups;
+  const int first = (blockIdx.x - (int)(r * groups)) * each, last = min(first + each, p.chunks), wave = threadIdx.x >> 6;
   const T* const row = static_cast<const T*>(p.logits) + r * p.ldl;
-  const int64_t e0 = (int64_t)chunk * kPiece - lead(row);
-  float x[4][8];
+  const int64_t e = (int64_t)threadIdx.x * 8 - lead(row);
+  Raw<T> raw[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) eight(row, e0 + (i * 256 + threadIdx.x) * 8, p.V, -INFINITY, x[i]);
-  SeqPlace place;
-  const int b = owner(p, r, place);
-  if (b < 0) return;
-  const float t = temperature(p, b);
-  float top = -INFINITY;  // NaN where one is
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = __builtin_elementwise_maximum(top, x[i][j]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, o));
-  if ((threadIdx.x & 63) == 0) tops[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = __builtin_elementwise_maximum(top, tops[i]);
-  const bool odd = !(top < INFINITY);
-  DraftChunk out{odd ? __uint_as_float(0x7fc00000u) : top, 0, 0.0};
-  if (t == 0.f) {  // the same for all threads
-    int32_t at = 0x7fffffff;
-#pragma unroll
-    for (int i = 3; i >= 0; --i)
-#pragma unroll
-      for (int j = 7; j >= 0; --j)
-        if (x[i][j] == top) at = (int32_t)(e0 + (i * 256 + threadIdx.x) * 8 + j);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
-    if ((threadIdx.x & 63) == 0) ats[wave] = at;
-    __syncthreads();
-    out.at = min(min(ats[0], ats[1]), min(ats[2], ats[3]));
-    out.sum = 1.0;
-  } else {
-    const Scale sc = scale_of(t, top);
-    double s = 0.0;
-    if (top > -INFINITY && !odd) {
-      if (!sc.plain) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) s += weight_part(x[i][j], sc);
-        s *= sc.rest;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) s += weight(x[i][j], sc);
-      }
+  for (int i = 0; i < 4; ++i) raw[i] = eight_raw(row, e + (int64_t)first * kPiece + i * 2048, p.V);
+  if (wave == 0) {
+    SeqPlace place;
+    const int b = owner(p, r, place);
+    if (threadIdx.x == 0) {
+      some = b >= 0;
+      temp = b >= 0 ? temperature(p, b) : 0.f;
     }
-    out.sum = block_add(s, red);
   }
-  if (threadIdx.x == 0) p.parts[r * p.chunks + chunk] = out;
+  __syncthreads();
+  if (!some) return;
+  const float t = temp;
+  for (int chunk = first; chunk < last; ++chunk) {
+    float x[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) open(raw[i], x[i]);
+    if (chunk + 1 < last)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = eight_raw(row, e + (int64_t)(chunk + 1) * kPiece + i * 2048, p.V);
+    float top = -INFINITY;  // NaN where one is
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = __builtin_elementwise_maximum(top, x[i][j]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, o));
+    if ((threadIdx.x & 63) == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __builtin_elementwise_maximum(top, tops[i]);
+    const bool odd = !(top < INFINITY);
+    DraftChunk out{odd ? __uint_as_float(0x7fc00000u) : top, 0, 0.0};
+    if (t == 0.f) {  // the same for all threads
+      int32_t at = 0x7fffffff;
+#pragma unroll
+      for (int i = 3; i >= 0; --i)
+#pragma unroll
+        for (int j = 7; j >= 0; --j)
+          if (x[i][j] == top) at = (int32_t)(e + (int64_t)chunk * kPiece + i * 2048 + j);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
+      if ((threadIdx.x & 63) == 0) ats[wave] = at;
+      __syncthreads();
+      out.at = min(min(ats[0], ats[1]), min(ats[2], ats[3]));
+      out.sum = 1.0;
+      __syncthreads();  // before the next chunk's
+    } else {
+      const Scale sc = scale_of(t, top);
+      double s = 0.0;
+      if (top > -INFINITY && !odd) {
+        if (!sc.plain) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += weight_part(x[i][j], sc);
+          s *= sc.rest;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += weight(x[i][j], sc);
+        }
+      }
+      out.sum = block_add(s, red);
+    }
+    if (threadIdx.x == 0) p.parts[r * p.chunks + chunk] = out;
+  }
 }
 
 // A row's chunks put together; the whole wave calls.
@@ -339,33 +399,33 @@ using Walk = DraftWalk;
 // On to the next rejection with q (true: what is left has to be summed before the walk can go on), or to the end; the whole
 // wave calls, with the walk the same in all lanes. write(i, j): row j is the i-th accepted.
 template <bool PROBS, typename Write>
-__device__ __forceinline__ bool walk_on(const DraftParams& p, const SeqPlace& s, float temp, Walk& w, Write write) {
+__device__ __forceinline__ bool walk_on(const DraftParams& p, Walk& w, Write write) {
   const int lane = threadIdx.x & 63;
-  for (int base = w.j & ~63; base < s.n; base += 64) {
-    const int mine = min(base + lane, s.n - 1);
-    const DraftRow* const row = p.rows + s.first + mine;
+  for (int base = w.j & ~63; base < w.n; base += 64) {
+    const int mine = min(base + lane, w.n - 1);
+    const DraftRow* const row = p.rows + w.first + mine;
     const int above = row->above;
-    const double rp = row->p, rq = row->q, u = p.u[s.first + mine];
-    for (; w.j < min(base + 64, s.n); ++w.j) {
+    const double rp = row->p, rq = row->q, u = p.u[w.first + mine];
+    for (; w.j < min(base + 64, w.n); ++w.j) {
       const int l = w.j - base;
       if (__builtin_amdgcn_readlane(above, l) != w.cur) continue;
       const double x = lane_of(rp, l), q = lane_of(rq, l), v = lane_of(u, l);
       if (x < 0.0) continue;
-      const double left = PROBS && temp > 0.f ? (w.a > 0.0 ? fmax(x - w.a * q, 0.0) : x) : x;
+      const double left = PROBS && w.temp > 0.f && w.a > 0.0 ? fmax(x - w.a * q, 0.0) : x;
       if (v * q * w.t < left) {
         write(w.count, w.j);
         ++w.count;
         w.cur = w.j;
         w.a = 0.0;
         w.t = 1.0;
-      } else if (PROBS && temp > 0.f) {
+      } else if (PROBS && w.temp > 0.f) {
         w.a += w.t;
         ++w.rejections;
         ++w.j;
         return true;
       } else {
         ++w.rejections;
-        if (temp > 0.f) w.t -= x;
+        if (w.temp > 0.f) w.t -= x;
       }
     }
   }
@@ -393,57 +453,76 @@ __device__ __forceinline__ double known_sum(const DraftParams& p, int b, int i) 
   return wave_add(x);
 }
 
+// The sum of what is left with q at 8 E places, `step` apart by eights; not where sc is plain.
+template <typename T, typename Q, int E>
+__device__ __forceinline__ double left_sum(const DraftParams& p, int64_t r, int64_t e, int64_t step, const Scale& sc,
+                                           double unit, double a) {
+  float l[E][8], q[E][8];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    eight(static_cast<const T*>(p.logits) + r * p.ldl, e + i * step, p.V, -INFINITY, l[i]);
+    eight(static_cast<const Q*>(p.probs) + r * p.ldp, e + i * step, p.V, 0.f, q[i]);
+  }
+  // a logit of -infinity counts for 2^-990 in weight_part: nothing may be left of it
+  const double part = unit * sc.rest, none = 0x1p-980 * part;
+  double x = 0.0;
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      x += fmax(weight_part(l[i][k], sc) * part - (q[i][k] > 0.f ? a * (double)q[i][k] : none), 0.0);
+  return x;
+}
+
 // Rejection number `round`. Chunk 0's workgroup leaves where the walk stands (rejections = round + 1: at this rejection;
 // fewer: it is over) and the rows accepted on the way.
-template <typename T, typename Q>
-__global__ void __launch_bounds__(1024) draft_sums_k(DraftParams p, int round) {
+template <typename T, typename Q, int THREADS>
+__global__ void __launch_bounds__(THREADS) draft_sums_k(DraftParams p, int round) {
   __shared__ double red[16];
   __shared__ Walk held;
   const int b = blockIdx.x / (uint32_t)p.chunks, chunk = blockIdx.x - b * p.chunks, lane = threadIdx.x & 63;
   DraftWalk* const walks = p.walks + (int64_t)round * p.B;
-  Walk w{1, 0, 1, 0, 0.0, 1.0};
-  if (round > 0) {
-    w = walks[b - p.B];
-    if (w.rejections < round) {
-      if (chunk == 0 && threadIdx.x == 0) walks[b] = w;
-      return;
-    }
-  }
-  const float t = temperature(p, b);
-  SeqPlace s;
-  if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == b; }, s)) return;
   if (threadIdx.x < 64) {
-    if (round > 0) w.t = known_sum(p, b, round - 1);
-    walk_on<true>(p, s, t, w, [&](int i, int j) {
-      if (chunk == 0 && lane == 0) p.path[s.first + i] = j;
-    });
-    if (t == 0.f) w.rejections = 0;  // these need no sums
+    Walk w{1, 0, 1, 0, 0.0, 1.0};
+    if (round == 0) {
+      SeqPlace s;
+      w.temp = temperature(p, b);
+      if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == b; }, s)) s.n = 0;
+      w.first = s.first;
+      w.n = s.n;
+    } else {
+      w = walks[b - p.B];
+    }
+    if (w.rejections == round) {
+      if (round > 0) w.t = known_sum(p, b, round - 1);
+      walk_on<true>(p, w, [&](int i, int j) {
+        if (chunk == 0 && lane == 0) p.path[w.first + i] = j;
+      });
+      if (w.temp == 0.f) w.rejections = 0;  // these need no sums
+    }
     if (lane == 0) {
       held = w;
       if (chunk == 0) walks[b] = w;
     }
   }
   __syncthreads();
-  w = held;
+  const Walk w = held;
   if (w.rejections <= round) return;
-  const int64_t r = s.first + w.cur;
-  const Scale sc = scale_of(t, p.rows[r].top);
+  const int64_t r = w.first + w.cur;
+  const Scale sc = scale_of(w.temp, p.rows[r].top);
   const double unit = 1.0 / p.rows[r].sum;
   const T* const row = static_cast<const T*>(p.logits) + r * p.ldl;
   const int64_t e = (int64_t)chunk * kPiece - lead(row) + threadIdx.x * 8;
   double x = 0.0;
   if (sc.plain) {
-    double left[8];
-    left_of<T, Q, true>(p, r, e, sc, unit, w.a, left);
+    for (int i = 0; i < kPiece; i += THREADS * 8) {
+      double left[8];
+      left_of<T, Q, true>(p, r, e + i, sc, unit, w.a, left);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x += left[k];
+      for (int k = 0; k < 8; ++k) x += left[k];
+    }
   } else {
-    float l[8], q[8];
-    eight(row, e, p.V, -INFINITY, l);
-    eight(static_cast<const Q*>(p.probs) + r * p.ldp, e, p.V, 0.f, q);
-    const double part = unit * sc.rest;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x += fmax(weight_part(l[k], sc) * part - (q[k] > 0.f ? w.a * (double)q[k] : 0.0), 0.0);
+    x = left_sum<T, Q, kPiece / THREADS / 8>(p, r, e, THREADS * 8, sc, unit, w.a);
   }
   x = block_add(x, red);
   if (threadIdx.x == 0) p.sums[((int64_t)round * p.B + b) * p.chunks + chunk] = x;
@@ -466,10 +545,21 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
       if (r < lo || r >= hi) p.path[r] = -1;
     return;
   }
-  const float t = temperature(p, b);
-  SeqPlace s;
-  if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == b; }, s)) return;
-  if (s.n == 0) {
+  // from the start, or from the last rejection that draft_sums_k was launched for, if there were so many
+  Walk w{1, 0, 1, 0, 0.0, 1.0};
+  if (PROBS && p.rounds > 0) {
+    w = p.walks[(int64_t)(p.rounds - 1) * p.B + b];
+  } else {
+    SeqPlace s;
+    w.temp = temperature(p, b);
+    if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == b; }, s)) return;
+    w.first = s.first;
+    w.n = s.n;
+  }
+  const int64_t first = w.first;
+  const int n = w.n;
+  const float t = w.temp;
+  if (n == 0) {
     if (threadIdx.x == 0) {
       p.count[b] = 0;
       p.next[b] = -1;
@@ -477,12 +567,12 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     return;
   }
   if (!PROBS || p.rounds == 0) {
-    for (int j = wave; j < s.n; j += 16) row_info<T, Q, PROBS>(p, s.first, j, t);
+    for (int j = wave; j < n; j += 16) row_info<T, Q, PROBS>(p, first, j, t);
     __syncthreads();
   }
 
   // what is left in four chunks, to all threads; `less`: without the tokens of the row's children, all of them rejected
-  const auto chunk_sums = [&](int64_t r, Scale sc, double unit, double a, int c0, int many, bool less) {
+  const auto chunk_sums = [&](int64_t r, const Scale& sc, double unit, double a, int c0, int many, bool less) {
     const int64_t e0 = (int64_t)c0 * kPiece - lead(static_cast<const T*>(p.logits) + r * p.ldl) + threadIdx.x * 8;
     double sum[4];
 #pragma unroll
@@ -490,12 +580,16 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
       sum[k] = 0.0;
       if (k >= many) continue;
       const int64_t e = e0 + (int64_t)k * kPiece;
+      if (PROBS && !sc.plain) {
+        sum[k] = wave_add(left_sum<T, Q, 1>(p, r, e, 0, sc, unit, a));
+        continue;
+      }
       double w[8];
       left_of<T, Q, PROBS>(p, r, e, sc, unit, a, w);
       if (less)
-        for (int j = (int)(r - s.first) + 1; j < s.n; ++j) {
-          const int64_t x = p.rows[s.first + j].token - e;
-          if (p.rows[s.first + j].above == (int)(r - s.first) && x >= 0 && x < 8)
+        for (int j = (int)(r - first) + 1; j < n; ++j) {
+          const int64_t x = p.rows[first + j].token - e;
+          if (p.rows[first + j].above == (int)(r - first) && x >= 0 && x < 8)
 #pragma unroll
             for (int i = 0; i < 8; ++i) w[i] = i == (int)x ? 0.0 : w[i];
         }
@@ -518,17 +612,12 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     return all;
   };
 
-  // from the start, or from the last rejection that draft_sums_k was launched for, if there were so many
-  Walk w{1, 0, 1, 0, 0.0, 1.0};
-  if (PROBS && p.rounds > 0) {
-    w = p.walks[(int64_t)(p.rounds - 1) * p.B + b];
-    if (t > 0.f && w.rejections == p.rounds && wave == 0) w.t = known_sum(p, b, p.rounds - 1);
-  }
-  if (threadIdx.x == 0) p.path[s.first] = 0;
+  if (PROBS && w.rejections == p.rounds && p.rounds > 0 && wave == 0) w.t = known_sum(p, b, p.rounds - 1);
+  if (threadIdx.x == 0) p.path[first] = 0;
   while (true) {
     if (wave == 0) {
-      const bool more = walk_on<PROBS>(p, s, t, w, [&](int i, int j) {
-        if (lane == 0) p.path[s.first + i] = j;
+      const bool more = walk_on<PROBS>(p, w, [&](int i, int j) {
+        if (lane == 0) p.path[first + i] = j;
       });
       if (lane == 0) {
         held = w;
@@ -541,14 +630,14 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     __syncthreads();
     if (!more) break;
     // a rejection beyond the ones that draft_sums_k was launched for
-    const int64_t r = s.first + w.cur;
+    const int64_t r = first + w.cur;
     const Scale sc = scale_of(t, p.rows[r].top);
     const double unit = 1.0 / p.rows[r].sum;
     w.t = 0.0;
     for (int c = 0; c < p.chunks; c += 4) w.t += chunk_sums(r, sc, unit, w.a, c, min(4, p.chunks - c), false);
   }
-  for (int i = w.count + threadIdx.x; i < s.n; i += 1024) p.path[s.first + i] = -1;
-  const int64_t r = s.first + w.cur;
+  for (int i = w.count + threadIdx.x; i < n; i += 1024) p.path[first + i] = -1;
+  const int64_t r = first + w.cur;
   const DraftRow row = p.rows[r];
   if (!row.ok || t == 0.f) {
     if (threadIdx.x == 0) {
@@ -564,7 +653,7 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
   const auto whole = [&]() {
     for (int c = threadIdx.x; c < p.chunks; c += 1024) {
       const DraftChunk x = p.parts[r * p.chunks + c];
-      chunk_left[c] = x.sum * weight(x.top, sc) * unit;
+      chunk_left[c] = x.sum * weight_or_none(x.top, sc) * unit;
     }
     __syncthreads();
   };
@@ -579,12 +668,12 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     if (!PROBS) {
       // less the children's tokens; a chunk of which little is left (cancelled digits) is summed again without them
       if (wave == 0) {
-        const int first = lead(static_cast<const T*>(p.logits) + r * p.ldl);
+        const int ahead = lead(static_cast<const T*>(p.logits) + r * p.ldl);
         bool some = false;
-        for (int j0 = w.cur + 1; j0 < s.n; j0 += 64) {
-          const DraftRow* const child = p.rows + s.first + min(j0 + lane, s.n - 1);
-          const double x = j0 + lane < s.n && child->above == w.cur ? child->p : 0.0;
-          const int c = x > 0.0 ? (int)((child->token + first) / kPiece) : 0;
+        for (int j0 = w.cur + 1; j0 < n; j0 += 64) {
+          const DraftRow* const child = p.rows + first + min(j0 + lane, n - 1);
+          const double x = j0 + lane < n && child->above == w.cur ? child->p : 0.0;
+          const int c = x > 0.0 ? (int)((child->token + ahead) / kPiece) : 0;
           for (unsigned long long m = __ballot(x > 0.0); m != 0; m &= m - 1) {
             const int l = __builtin_ctzll(m), at = __builtin_amdgcn_readlane(c, l);
             const double before = chunk_left[at], after = before - lane_of(x, l) * row.sum;
@@ -604,82 +693,84 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
         }
     }
   }
+  int at = -1;
   for (int again = 0; again < 2; ++again) {
     // the chunk in which the sum passes its share; the last one that has anything where none does
     if (wave == 0) {
       double all = 0.0;
       for (int c0 = 0; c0 < p.chunks; c0 += 64) all += wave_add(c0 + lane < p.chunks ? chunk_left[c0 + lane] : 0.0);
-      const double share = (double)p.u[s.first] * all;
-      double before = 0.0, at_before = 0.0;
-      int at = -1;
+      const double share = (double)p.u[first] * all;
+      double before = 0.0, pick_before = 0.0;
+      int c = -1;
       for (int c0 = 0; c0 < p.chunks; c0 += 64) {
         const double x = c0 + lane < p.chunks ? chunk_left[c0 + lane] : 0.0, upto = wave_upto(x);
         const unsigned long long some = __ballot(x > 0.0), hit = __ballot(x > 0.0 && before + upto > share);
         if (some != 0) {
           const int l = hit != 0 ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
-          at = c0 + l;
-          at_before = before + (lane_of(upto, l) - lane_of(x, l));
+          c = c0 + l;
+          pick_before = before + (lane_of(upto, l) - lane_of(x, l));
         }
         if (hit != 0) break;
         before += lane_of(upto, 63);
       }
       if (lane == 0) {
-        pick = at;
-        level = share - at_before;
+        pick = c;
+        level = share - pick_before;
       }
     }
     __syncthreads();
-    if (pick >= 0) break;
-    // nothing left: the row's own distribution
-    a = 0.0;
-    less = false;
-    whole();
-  }
-  if (pick >= 0) {
-    const int64_t e = (int64_t)pick * kPiece - lead(static_cast<const T*>(p.logits) + r * p.ldl) + threadIdx.x * 8;
-    double x[8];
-    left_of<T, Q, PROBS>(p, r, e, sc, unit, a, x);
-    if (less)
-      for (int j = w.cur + 1; j < s.n; ++j) {
-        const int64_t k = p.rows[s.first + j].token - e;
-        if (p.rows[s.first + j].above == w.cur && k >= 0 && k < 8)
+    const int c = pick;
+    if (c >= 0) {
+      const int64_t e = (int64_t)c * kPiece - lead(static_cast<const T*>(p.logits) + r * p.ldl) + threadIdx.x * 8;
+      double x[8];
+      left_of<T, Q, PROBS>(p, r, e, sc, unit, a, x);
+      if (less)
+        for (int j = w.cur + 1; j < n; ++j) {
+          const int64_t k = p.rows[first + j].token - e;
+          if (p.rows[first + j].above == w.cur && k >= 0 && k < 8)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = i == (int)k ? 0.0 : x[i];
+            for (int i = 0; i < 8; ++i) x[i] = i == (int)k ? 0.0 : x[i];
+        }
+      double mine = 0.0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine += x[i];
+      // the sum of the places before this thread's
+      const double upto = wave_upto(mine);
+      if (lane == 63) tail[wave] = upto;
+      __syncthreads();
+      double before = upto - mine;
+      for (int v = 0; v < wave; ++v) before += tail[v];
+      int hit = -1, some = -1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        before += x[i];
+        if (x[i] > 0.0) {
+          some = (int)e + i;
+          if (before > level && hit < 0) hit = (int)e + i;
+        }
       }
-    double mine = 0.0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mine += x[i];
-    // the sum of the places before this thread's
-    const double upto = wave_upto(mine);
-    if (lane == 63) tail[wave] = upto;
-    __syncthreads();
-    double before = upto - mine;
-    for (int v = 0; v < wave; ++v) before += tail[v];
-    int hit = -1, some = -1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      before += x[i];
-      if (x[i] > 0.0) {
-        some = (int)e + i;
-        if (before > level && hit < 0) hit = (int)e + i;
+      // the first place of the first wave that has one, else the last place with anything
+      const unsigned long long hits = __ballot(hit >= 0), somes = __ballot(some >= 0);
+      hit = __builtin_amdgcn_readlane(hit, hits != 0 ? __builtin_ctzll(hits) : 0);
+      some = __builtin_amdgcn_readlane(some, somes != 0 ? 63 - __builtin_clzll(somes) : 0);
+      if (lane == 0) {
+        first_hit[wave] = hit;
+        last_some[wave] = some;
       }
-    }
-    // the first place of the first wave that has one, else the last place with anything
-    const unsigned long long hits = __ballot(hit >= 0), somes = __ballot(some >= 0);
-    if (lane == 0) {
-      first_hit[wave] = hits != 0 ? __builtin_amdgcn_readlane(hit, __builtin_ctzll(hits)) : -1;
-      last_some[wave] = somes != 0 ? __builtin_amdgcn_readlane(some, 63 - __builtin_clzll(somes)) : -1;
-    }
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    int at = -1;
-    if (pick >= 0) {
-      for (int v = 15; v >= 0; --v)
-        if (at < 0) at = last_some[v];
+      __syncthreads();
+      for (int v = 0; v < 16; ++v)
+        if (last_some[v] >= 0) at = last_some[v];
       for (int v = 15; v >= 0; --v)
         if (first_hit[v] >= 0) at = first_hit[v];
     }
+    if (at >= 0) break;  // the same for all threads
+    // nothing left: the row's own distribution
+    a = 0.0;
+    less = false;
+    __syncthreads();
+    whole();
+  }
+  if (threadIdx.x == 0) {
     p.count[b] = w.count;
     p.next[b] = at;
   }
@@ -703,16 +794,21 @@ hipError_t launch_verify(DraftParams p, bool f32, bool probs_f32, uint8_t* work,
   p.rows = reinterpret_cast<DraftRow*>(p.parts + p.N * p.chunks);
   p.walks = reinterpret_cast<DraftWalk*>(p.rows + p.N);
   p.sums = reinterpret_cast<double*>(p.walks + kDraftRounds * p.B);
-  const dim3 wide(256), parts((unsigned)(p.N * p.chunks)), rows((unsigned)((p.N + 3) / 4));
-  if (p.N > 0) hipLaunchKernelGGL(f32 ? draft_chunks_k<float> : draft_chunks_k<uint16_t>, parts, wide, 0, st, p);
+  const dim3 wide(256), rows((unsigned)((p.N + 3) / 4));
+  if (p.N > 0) {
+    // two chunks a workgroup where there are enough of them for the chip twice over: 50 us in place of 53 in the largest case
+    const int each = p.N * p.chunks >= 8192 ? 2 : 1, groups = (p.chunks + each - 1) / each;
+    hipLaunchKernelGGL(f32 ? draft_chunks_k<float> : draft_chunks_k<uint16_t>, dim3((unsigned)(p.N * groups)), wide, 0, st, p,
+                       each, groups);
+  }
   if (p.rounds > 0 && p.N > 0 && p.B > 0) {
     const auto rows_k = probs_f32 ? (f32 ? draft_rows_k<float, float> : draft_rows_k<uint16_t, float>)
                                   : (f32 ? draft_rows_k<float, uint16_t> : draft_rows_k<uint16_t, uint16_t>);
-    const auto sums_k = probs_f32 ? (f32 ? draft_sums_k<float, float> : draft_sums_k<uint16_t, float>)
-                                  : (f32 ? draft_sums_k<float, uint16_t> : draft_sums_k<uint16_t, uint16_t>);
+    const auto sums_k = probs_f32 ? (f32 ? draft_sums_k<float, float, kSumThreads> : draft_sums_k<uint16_t, float, kSumThreads>)
+                                  : (f32 ? draft_sums_k<float, uint16_t, kSumThreads> : draft_sums_k<uint16_t, uint16_t, kSumThreads>);
     hipLaunchKernelGGL(rows_k, rows, wide, 0, st, p);
     for (int i = 0; i < p.rounds; ++i)
-      hipLaunchKernelGGL(sums_k, dim3((unsigned)(p.B * p.chunks)), dim3(1024), 0, st, p, i);
+      hipLaunchKernelGGL(sums_k, dim3((unsigned)(p.B * p.chunks)), dim3(kSumThreads), 0, st, p, i);
   }
   const auto next_k = p.probs == nullptr ? (f32 ? draft_next_k<float, float, false> : draft_next_k<uint16_t, float, false>)
                       : probs_f32 ? (f32 ? draft_next_k<float, float, true> : draft_next_k<uint16_t, float, true>)

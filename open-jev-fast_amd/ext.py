@@ -19,6 +19,7 @@ allocator on their inputs' device and every launch goes on torch's current strea
 CUDA/HIP graph.
 """
 import ctypes
+import functools
 import weakref
 
 import torch
@@ -689,25 +690,41 @@ def linattn_step(q, k, v, g, beta, state, slot, scale=None):
 
 
 # ------------------------------------------------------------------------------------------------ drafted tokens
-def _chk_rows(q_ptr, N, parents=None, path=None, count=None):
-    """B of the sequences that q_ptr int32 [B + 1] makes of N rows."""
-    _chk(q_ptr, "q_ptr", torch.int32)
+def _chk_each(*named):
+    """_chk of (tensor, name, dtype) one after the other, without a call for each that is as it should be."""
+    for t, name, dtype in named:
+        if t is None or not t.is_cuda or t.dtype is not dtype or not t.is_contiguous():
+            _chk(t, name, dtype)
+
+
+@functools.lru_cache(1024)
+def _work_bytes(name, *sizes):
+    """The library's answer to how much workspace calls of these sizes need."""
+    n = getattr(lib(), name)(*sizes)
+    if n < 0:
+        check(2)
+    return n
+
+
+def _chk_count(t, name, n):
+    if t.numel() != n:
+        raise RuntimeError(f"{name} must have {n} elements, got {t.numel()}")
+
+
+def _chk_rows(q_ptr, N, *counted):
+    """B of the sequences that q_ptr int32 [B + 1] makes of N rows; counted: (tensor, name, one each of N rows?)."""
     B = q_ptr.numel() - 1
     if B < 0:
         raise RuntimeError("q_ptr must be [B + 1]")
-    for t, nm, n in ((parents, "parents", N), (path, "path", N), (count, "count", B)):
-        if t is not None:
-            _chk(t, nm, torch.int32)
-            if t.numel() != n:
-                raise RuntimeError(f"{nm} must have {n} elements, got {t.numel()}")
+    for t, name, rows in counted:
+        _chk_count(t, name, N if rows else B)
     return B
 
 
 def _chk_slots(state, slot, HV, B):
     _chk_states(state, HV)
-    _chk(slot, "slot", torch.int32)
-    if slot.numel() != B:
-        raise RuntimeError(f"slot must have B={B} elements, got {slot.numel()}")
+    _chk_each((slot, "slot", torch.int32))
+    _chk_count(slot, "slot", B)
 
 
 def linattn_tree(q, k, v, g, beta, state, slot, q_ptr, parents=None, scale=None):
@@ -718,13 +735,15 @@ def linattn_tree(q, k, v, g, beta, state, slot, q_ptr, parents=None, scale=None)
     of its path's tokens, from the state on. A negative slot gives zeros, a slot that is not in state NaN; a row of no sequence gives
     zeros. Operands as in linattn_prompt. linattn_keep then takes the states over the tokens that are kept."""
     N, HV, HK = _chk_linattn(q, k, v, g, beta)
-    B = _chk_rows(q_ptr, N, parents)
+    _chk_each((q_ptr, "q_ptr", torch.int32))
+    B = _chk_rows(q_ptr, N)
+    if parents is not None:
+        _chk_each((parents, "parents", torch.int32))
+        _chk_count(parents, "parents", N)
     _chk_slots(state, slot, HV, B)
     _one_device(q, k, v, g, beta, state, slot, q_ptr, parents)
     o = torch.empty_like(v)
-    n = lib().ojx_linattn_tree_workspace(N, B, HV, HK)
-    if n < 0:
-        check(2)
+    n = _work_bytes("ojx_linattn_tree_workspace", N, B, HV, HK)
     ws = _scratch(n, q)
     check(lib().ojx_linattn_tree(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(slot), state.shape[0],
                                  _ptr(q_ptr), _ptr(parents), N, B, HV, HK, float(128 ** -0.5 if scale is None else scale),
@@ -737,9 +756,8 @@ def linattn_keep(k, v, g, beta, state, slot, q_ptr, path, count):
     i], i < count[b], one after the other (path int32 [N] and count int32 [B] as verify_drafts gives them; the other
     operands as linattn_tree took them). A slot that is not in state, or that an earlier sequence has too, is left alone."""
     N, HV, HK = _chk_linattn(k, k, v, g, beta)
-    B = _chk_rows(q_ptr, N, None, path, count)
-    if path is None or count is None:
-        raise RuntimeError("path and count must be tensors")
+    _chk_each((q_ptr, "q_ptr", torch.int32), (path, "path", torch.int32), (count, "count", torch.int32))
+    B = _chk_rows(q_ptr, N, (path, "path", True), (count, "count", False))
     _chk_slots(state, slot, HV, B)
     _one_device(k, v, g, beta, state, slot, q_ptr, path, count)
     check(lib().ojx_linattn_keep(_ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(slot), state.shape[0], _ptr(q_ptr),
@@ -776,24 +794,21 @@ def verify_drafts(logits, tokens, q_ptr, u, parents=None, probs=None, temperatur
     behind the last of them (-1: its logits are no distribution, or the sequence has no rows). kv_cache_keep and
     linattn_keep take path and count as they are."""
     kind, N, V, ldl = _chk_vocab(logits, "logits")
-    _chk(tokens, "tokens", torch.int64)
-    _chk(u, "u", torch.float32)
-    if tokens.numel() != N or u.numel() != N:
-        raise RuntimeError(f"tokens and u must have N={N} elements, got {tokens.numel()} and {u.numel()}")
-    B = _chk_rows(q_ptr, N, parents)
+    _chk_each((tokens, "tokens", torch.int64), (u, "u", torch.float32), (q_ptr, "q_ptr", torch.int32))
+    B = _chk_rows(q_ptr, N, (tokens, "tokens", True), (u, "u", True))
+    if parents is not None:
+        _chk_each((parents, "parents", torch.int32))
+        _chk_count(parents, "parents", N)
     pkind, ldp = 0, 0
     if probs is not None:
         pkind, _, _, ldp = _chk_vocab(probs, "probs", N, V)
     if temperature is not None:
-        _chk(temperature, "temperature", torch.float32)
-        if temperature.numel() != B:
-            raise RuntimeError(f"temperature must have B={B} elements, got {temperature.numel()}")
+        _chk_each((temperature, "temperature", torch.float32))
+        _chk_count(temperature, "temperature", B)
     _one_device(logits, tokens, q_ptr, u, parents, probs, temperature)
     path, count = q_ptr.new_empty(N), q_ptr.new_empty(B)
     token = tokens.new_empty(B)
-    n = lib().ojx_verify_drafts_workspace(N, B, V, probs is not None)
-    if n < 0:
-        check(2)
+    n = _work_bytes("ojx_verify_drafts_workspace", N, B, V, probs is not None)
     ws = _scratch(n, logits)
     check(lib().ojx_verify_drafts(_ptr(logits), kind, ldl, _ptr(tokens), _ptr(q_ptr), _ptr(u), _ptr(parents), _ptr(probs),
                                   pkind, ldp, _ptr(temperature), N, B, V, _ptr(path), _ptr(count), _ptr(token), _ptr(ws), n,
@@ -801,29 +816,33 @@ def verify_drafts(logits, tokens, q_ptr, u, parents=None, probs=None, temperatur
     return path, count, token
 
 
+_CACHE = {torch.bfloat16: _lib.KV_BF16, torch.float8_e4m3fn: _lib.KV_E4M3}
+
+
 def _chk_layers(kc, vc, ks, vs):
     """(format, layers, pages, HKV, page, D) of a cache [pages, HKV, page, D], or of several layers' [layers, pages, ..]."""
-    if kc.dim() == 5:
-        if vc.dim() != 5 or kc.shape != vc.shape or (ks is not None and (ks.dim() != 4 or ks.shape[0] != kc.shape[0])) or (
-                vs is not None and (vs.dim() != 4 or vs.shape[0] != kc.shape[0])):
-            raise RuntimeError(f"kc {tuple(kc.shape)} and vc {tuple(vc.shape)} must be one shape, with scales of its first "
-                               "four sizes")
-        layers, pages = kc.shape[:2]
-        one = [None if t is None else t.flatten(0, 1) if t.is_contiguous() else t for t in (kc, vc, ks, vs)]
-    else:
-        if kc.dim() != 4:
-            raise RuntimeError(f"kc must be [pages, HKV, page, D] or [layers, pages, HKV, page, D], got {tuple(kc.shape)}")
-        layers, pages, one = 1, kc.shape[0], (kc, vc, ks, vs)
-    HKV, D = kc.shape[-3], kc.shape[-1]
-    fmt, _, page = _chk_cache(*one, HKV, D)
-    return fmt, layers, pages, HKV, page, D
+    fmt, shape = _CACHE.get(kc.dtype), kc.shape
+    if fmt is None:
+        raise RuntimeError(f"a cache is torch.bfloat16 or torch.float8_e4m3fn, got {kc.dtype}")
+    _chk_each((kc, "kc", kc.dtype), (vc, "vc", kc.dtype))
+    if len(shape) not in (4, 5) or vc.shape != shape:
+        raise RuntimeError(f"kc {tuple(shape)} and vc {tuple(vc.shape)} must both be [pages, HKV, page, D], or [layers, pages, "
+                           "HKV, page, D]")
+    if fmt == _lib.KV_E4M3:
+        _chk_each((ks, "ks", torch.float32), (vs, "vs", torch.float32))
+        if ks.shape != shape[:-1] or vs.shape != shape[:-1]:
+            raise RuntimeError(f"ks {tuple(ks.shape)} and vs {tuple(vs.shape)} must be {tuple(shape[:-1])}")
+    elif ks is not None or vs is not None:
+        raise RuntimeError("a bf16 cache has no scales")
+    return (fmt, 1, *shape) if len(shape) == 4 else (fmt, *shape)
 
 
 def _chk_table(table, B=None):
-    _chk(table, "table", torch.int32)
-    if table.dim() != 2 or (B is not None and table.shape[0] != B):
-        raise RuntimeError(f"table {tuple(table.shape)} must be [B{'' if B is None else '=' + str(B)}, max_pages]")
-    return table.shape
+    _chk_each((table, "table", torch.int32))
+    shape = table.shape
+    if len(shape) != 2 or (B is not None and shape[0] != B):
+        raise RuntimeError(f"table {tuple(shape)} must be [B{'' if B is None else '=' + str(B)}, max_pages]")
+    return shape
 
 
 def kv_cache_keep(kc, vc, table, ctx, q_ptr, path, count, ks=None, vs=None):
@@ -832,15 +851,11 @@ def kv_cache_keep(kc, vc, table, ctx, q_ptr, path, count, ks=None, vs=None):
     them). The cache as in kv_cache_write, or that of several layers with one table: [layers, pages, HKV, page, D], scales
     [layers, pages, HKV, page]. Add count to ctx afterwards."""
     fmt, layers, pages, HKV, page, D = _chk_layers(kc, vc, ks, vs)
-    if path is None or count is None:
-        raise RuntimeError("path and count must be tensors")
-    _chk(path, "path", torch.int32)
+    _chk_each((q_ptr, "q_ptr", torch.int32), (path, "path", torch.int32), (count, "count", torch.int32),
+              (ctx, "ctx", torch.int32))
     N = path.numel()
-    B = _chk_rows(q_ptr, N, None, path, count)
+    B = _chk_rows(q_ptr, N, (count, "count", False), (ctx, "ctx", False))
     MP = _chk_table(table, B)[1]
-    _chk(ctx, "ctx", torch.int32)
-    if ctx.numel() != B:
-        raise RuntimeError(f"ctx must have B={B} elements, got {ctx.numel()}")
     _one_device(kc, vc, ks, vs, table, ctx, q_ptr, path, count)
     check(lib().ojx_kv_cache_keep(_ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), fmt, layers, pages, HKV, page, D, _ptr(table), MP,
                                   _ptr(ctx), _ptr(q_ptr), _ptr(path), _ptr(count), N, B, _stream()))
@@ -848,10 +863,8 @@ def kv_cache_keep(kc, vc, table, ctx, q_ptr, path, count, ks=None, vs=None):
 
 def _pages_call(table, refs, per_slot, name):
     B, MP = _chk_table(table)
-    _chk(refs, "refs", torch.int32)
-    _chk(per_slot, name, torch.int32)
-    if per_slot.numel() != B:
-        raise RuntimeError(f"{name} must have B={B} elements, got {per_slot.numel()}")
+    _chk_each((refs, "refs", torch.int32), (per_slot, name, torch.int32))
+    _chk_count(per_slot, name, B)
     return B, MP, refs.numel()
 
 
@@ -863,9 +876,7 @@ def kv_pages_resize(table, refs, tokens, page):
     B, MP, pages = _pages_call(table, refs, tokens, "tokens")
     _one_device(table, refs, tokens)
     missing = table.new_empty(B)
-    n = lib().ojx_kv_pages_workspace(B, MP, pages, 0)
-    if n < 0:
-        check(2)
+    n = _work_bytes("ojx_kv_pages_workspace", B, MP, pages, 0)
     ws = _scratch(n, table)
     check(lib().ojx_kv_pages_resize(_ptr(table), MP, _ptr(refs), pages, _ptr(tokens), B, page, _ptr(missing), _ptr(ws), n,
                                     _stream()))
@@ -878,14 +889,11 @@ def kv_pages_fork(table, ctx, refs, src, page):
     pages to copy: kv_pages_copy does that for a layer or several, and has to before anything else writes to the cache or
     takes pages. A slot for which the pool has no page left ends with its last full page (its ctx says so)."""
     B, MP, pages = _pages_call(table, refs, src, "src")
-    _chk(ctx, "ctx", torch.int32)
-    if ctx.numel() != B:
-        raise RuntimeError(f"ctx must have B={B} elements, got {ctx.numel()}")
+    _chk_each((ctx, "ctx", torch.int32))
+    _chk_count(ctx, "ctx", B)
     _one_device(table, ctx, refs, src)
     pairs = table.new_empty((B, 2))
-    n = lib().ojx_kv_pages_workspace(B, MP, pages, 1)
-    if n < 0:
-        check(2)
+    n = _work_bytes("ojx_kv_pages_workspace", B, MP, pages, 1)
     ws = _scratch(n, table)
     check(lib().ojx_kv_pages_fork(_ptr(table), MP, _ptr(ctx), _ptr(refs), pages, _ptr(src), B, page, _ptr(pairs), _ptr(ws),
                                   n, _stream()))
@@ -896,7 +904,7 @@ def kv_pages_copy(kc, vc, pairs, ks=None, vs=None):
     """Copies page pairs[i][0] to page pairs[i][1] (int32 [n, 2], as kv_pages_fork gives them; a pair with a page outside the
     cache is left out) in a cache of one layer or several (see kv_cache_keep). No page may be both read and written."""
     fmt, layers, pages, HKV, page, D = _chk_layers(kc, vc, ks, vs)
-    _chk(pairs, "pairs", torch.int32)
+    _chk_each((pairs, "pairs", torch.int32))
     if pairs.dim() != 2 or pairs.shape[1] != 2:
         raise RuntimeError(f"pairs must be [n, 2], got {tuple(pairs.shape)}")
     _one_device(kc, vc, ks, vs, pairs)

@@ -118,6 +118,13 @@ def test_verify_many_rejections(ext, D, dev, probs):
         _check_verify(D, c, _run_verify(ext, c, dev))
 
 
+@pytest.mark.parametrize("dtype,V,pad", [(BF16, 16500, 3), (F32, 9001, 0)])
+def test_verify_many_rows(ext, D, dev, dtype, V, pad):
+    """Enough rows that a workgroup takes several chunks of one, the last of them alone; unaligned rows."""
+    c = _verify_case([7, 0, 9, 5] * 200, V, dtype, "none", "near", pad, seed=12)
+    _check_verify(D, c, _run_verify(ext, c, dev))
+
+
 @pytest.mark.parametrize("probs", ["none", "bf16", "fp32"])
 def test_verify_temperatures(ext, D, dev, probs):
     temps = [0.0, -1.0, math.nan, math.inf, 1e-3, 1e-40, 50.0, 1.0]
@@ -182,6 +189,28 @@ def test_verify_borders(ext, dev):
     for bad in (0.0, -1.0, math.nan):
         q0 = torch.full((2, 5), bad)
         assert _run_verify(ext, {**c, "probs": q0, "u": torch.tensor([0.3, 0.9])}, dev)[1].tolist() == [2]
+
+
+@pytest.mark.parametrize("V", [9000, 41000])
+def test_verify_chunks_with_nothing_left(ext, dev, V):
+    """A random number of 0 passes over all that is masked, rejected or proposed more often than wanted."""
+    at = [5, 8500, 8600, V - 1]
+    logits = torch.full((2, V), -math.inf)
+    logits[:, at] = 0.0                                                       # 1/4 each
+    c = {"logits": logits, "q_ptr": torch.tensor([0, 2], dtype=I32), "parents": None, "temperature": None}
+    got = _run_verify(ext, {**c, "probs": None, "tokens": torch.tensor([0, 5]), "u": torch.tensor([0.0, 0.25])}, dev)
+    assert got[1].tolist() == [1] and got[2].tolist() == [8500]
+    q = torch.zeros(2, V)
+    q[:, at[:2]] = 0.5
+    tree = torch.tensor([-1, 0], dtype=I32)
+    for parents in (None, tree):
+        d = {**c, "probs": q, "tokens": torch.tensor([0, 8500]), "parents": parents}
+        assert _run_verify(ext, {**d, "u": torch.tensor([0.0, 0.5])}, dev)[2].tolist() == [8600]
+        assert _run_verify(ext, {**d, "u": torch.tensor([0.5, 0.5])}, dev)[2].tolist() == [V - 1]
+        d["probs"] = torch.where(q > 0, 1.0, 0.25 * torch.isfinite(logits))      # as often as wanted, or more: nothing left
+        got = _run_verify(ext, {**d, "u": torch.tensor([0.0, 0.25])}, dev)
+        assert got[1].tolist() == [1] and got[2].tolist() == [5]
+        assert _run_verify(ext, {**d, "u": torch.tensor([0.75, 0.25])}, dev)[2].tolist() == [V - 1]
 
 
 @pytest.mark.parametrize("probs", [False, True])
