@@ -330,7 +330,7 @@ int ojx_kv_cache_keep(void* kc, void* vc, float* ks, float* vs, int32_t fmt, int
  * to the cache or taken from the pool; (-1, -1) where there is none. A slot for which the pool has no page gets (page, -1)
  * and ends with its last full page: ctx says so.
  * ojx_kv_pages_copy: page pairs[i][0] -> page pairs[i][1] of a cache of `layers` layers (see ojx_kv_cache_keep), i < n; pairs
- * with a page outside [0, pages) are left out. Pages written must not be among those read.
+ * with a page outside [0, pages) are left out. Pages written must not be among those read, nor named twice.
  * workspace: ojx_kv_pages_workspace bytes of device memory, 16-byte aligned (fork: 1 for ojx_kv_pages_fork). B at most
  * 65536, B max_pages below 2^31, a copy at most 2^24 pieces of 16 KB, n at most 65535. */
 int64_t ojx_kv_pages_workspace(int64_t B, int64_t max_pages, int64_t pages, int32_t fork);

@@ -968,7 +968,7 @@ int check_work(const char* what, const void* workspace, int64_t have, int64_t ne
 
 int64_t ojx_linattn_tree_workspace(int64_t N, int32_t B, int32_t HV, int32_t HK) {
   if (check_lintree_sizes(N, B, HV, HK) != OJX_OK) return -1;
-  return N * HV * 128 * 4;
+  return ojx::lintree_work_bytes(N, HV);
 }
 
 int ojx_linattn_tree(const void* q, const void* k, const void* v, const float* g, const void* beta, const float* state,

@@ -50,10 +50,11 @@ __device__ __forceinline__ void store4(uint16_t* o, float a, float b, float c, f
   *reinterpret_cast<uint2*>(o) = make_uint2(pack2(a, b), pack2(c, d));
 }
 
-// Row by row, any tree: each row's ancestors from its parent upwards, their u from the workspace. The whole workgroup calls;
-// red: [4][32][12] floats.
-template <bool DELTA>
-__device__ __forceinline__ void by_rows(const LinTreeParams& p, const SeqPlace& at, int64_t slot, int h, int hk, float* red) {
+// Row by row, any tree: each row's ancestors from its parent upwards, their u from LDS (near, where there is room for all the
+// rows') or the workspace. The whole workgroup calls; red: [4][32][12] floats.
+template <bool DELTA, bool NEAR>
+__device__ __forceinline__ void by_rows(const LinTreeParams& p, const SeqPlace& at, int64_t slot, int h, int hk, float* red,
+                                        float4 (*near)[32]) {
   const int c = threadIdx.x & 31, rg = threadIdx.x >> 5;
   const float* const st = p.state + (slot * p.HV + h) * (kHD * kHD) + rg * 16 * kHD + c * 4;
   float4 s[16];
@@ -80,7 +81,7 @@ __device__ __forceinline__ void by_rows(const LinTreeParams& p, const SeqPlace& 
         dk += y[x] * k[x];
         dq += y[x] * q[x];
       }
-      const float4 u = *reinterpret_cast<const float4*>(p.u + (a * p.HV + h) * kHD + c * 4);
+      const float4 u = NEAR ? near[j][c] : *reinterpret_cast<const float4*>(p.u + (a * p.HV + h) * kHD + c * 4);
       dk *= fade;
       dq *= fade;
       f[0] += dk * u.x;
@@ -122,7 +123,8 @@ __device__ __forceinline__ void by_rows(const LinTreeParams& p, const SeqPlace& 
       for (int x = 0; x < 4; ++x) u[x] = beta * (u[x] - f[x]);
     }
     if (rg == 0) {
-      *reinterpret_cast<float4*>(p.u + (row * p.HV + h) * kHD + c * 4) = make_float4(u[0], u[1], u[2], u[3]);
+      (NEAR ? near[i][c] : *reinterpret_cast<float4*>(p.u + (row * p.HV + h) * kHD + c * 4)) =
+          make_float4(u[0], u[1], u[2], u[3]);
       store4(p.o + (row * p.HV + h) * kHD + c * 4, p.scale * (f[4] + f[8] * u[0]), p.scale * (f[5] + f[8] * u[1]),
              p.scale * (f[6] + f[8] * u[2]), p.scale * (f[7] + f[8] * u[3]));
     }
@@ -131,7 +133,8 @@ __device__ __forceinline__ void by_rows(const LinTreeParams& p, const SeqPlace& 
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-constexpr int kTree = 64;  // rows that a sequence may have to be taken at once
+constexpr int kTree = 64;  // rows that are taken at once
+constexpr int kParts = 4;  // as many times as a sequence may have of them
 
 // 16-byte pieces of 16 rows that are read at once spread over the banks.
 __device__ __forceinline__ constexpr int swizzle(int r) { return (r & 7) << 1 | (r >> 3 & 1); }
@@ -180,69 +183,63 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 // LDS reads and writes of all waves are done; global loads stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// A sequence's rows at once, in blocks of 16 (a block's rows are tokens, its columns value dims; with two value dims, 2 c and
-// 2 c + 1 of the wave's 32, for each lane): with
+// What a head's workgroup has in LDS.
+struct TreeShared {
+  f32x4 mats[19][64];
+  bf16x8 rows[2][kTree][16];  // K and Q, piece x of a row r at x ^ swizzle(r)
+  double sums[kTree];         // every wave writes the same there
+  uint64_t seen[kTree];
+  float strength[kTree];
+};
+static_assert(sizeof(TreeShared::mats) >= 4 * 32 * 12 * 4 && sizeof(TreeShared::rows) == kTree * 32 * sizeof(float4),
+              "by_rows' sums and u");
+
+// What parts of a long sequence leave to the later ones, for each row and head: the decays' sum, the ancestors 64 to a word.
+struct TreeLeft {
+  double sum;
+  uint64_t seen[kParts];
+};
+
+// Up to 64 rows of a sequence at once, those from row s0 on, in blocks of 16 (a block's rows are tokens, its columns value
+// dims; with two value dims, 2 c and 2 c + 1 of the wave's 32, for each lane): with
 //   A_ij = beta_i e^(G_i - G_j) k_i . k_j  and  P_ij = e^(G_i - G_j) q_i . k_j  for the ancestors j of i (in P also i itself),
 //   X = diag(beta) (V - diag(e^G) K S0),  U = (I + A)^-1 X,  O = scale (diag(e^G) Q S0 + P U),
 // block row after block row. S0 enters as two bf16 pieces (what it makes is rounded to bf16 in the end), everything else in
 // fp32. A product with a zero in place of a row that is no ancestor is only right for finite numbers: where a U is not finite
-// or a decay is above 1, the head goes row by row instead.
+// or a decay is above 1 (true), the head goes row by row instead.
 // Loads come back in the order in which they were made, so the rows' go first: while the state is on its way the four waves
 // make the blocks of A, P and the inverses of A's diagonal ones, each once, and hand them to each other in LDS as the operands
-// that they are.
-template <bool DELTA>
-__global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
-  __shared__ __attribute__((aligned(16))) f32x4 mats[19][64];
-  __shared__ __attribute__((aligned(16))) bf16x8 rows[2][kTree][16];  // K and Q, piece x of a row r at x ^ swizzle(r)
-  __shared__ double sums[kTree];  // every wave writes the same there
-  __shared__ uint64_t seen[kTree];
-  __shared__ float strength[kTree];
-  float* const red = reinterpret_cast<float*>(mats);  // row by row
-  static_assert(sizeof(mats) >= 4 * 32 * 12 * 4, "by_rows' sums");
-  const int64_t b = blockIdx.x / p.HV;
-  const int h = blockIdx.x - (int)(b * p.HV), hk = h / (p.HV / p.HK);
-  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+// that they are. LONG: the rows before s0 have left their U and TreeLeft in the workspace (a thread reads back the U that it
+// wrote), and these rows leave theirs.
+template <bool DELTA, bool LONG>
+__device__ __forceinline__ bool tree_part(const LinTreeParams& p, TreeShared& lds, int64_t first, int s0, int n, int64_t slot,
+                                          int h, int hk) {
+  auto& mats = lds.mats;
+  auto& rows = lds.rows;
+  auto& sums = lds.sums;
+  auto& seen = lds.seen;
+  auto& strength = lds.strength;
+  int lane = threadIdx.x & 63;
+  if (LONG) asm volatile("" : "+v"(lane));  // a part computes its addresses anew: there are no registers to keep them over a loop
+  const int g = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (b == p.B) {  // rows of no sequence
-    int lo, hi;
-    seq_span(p.q_ptr, p.B, p.N, lo, hi);
-    for (int64_t r = threadIdx.x >> 5; r < p.N; r += 8)
-      if (r < lo || r >= hi)
-        *reinterpret_cast<uint2*>(p.o + (r * p.HV + h) * kHD + (threadIdx.x & 31) * 4) = make_uint2(0u, 0u);
-    return;
-  }
-  const int64_t slot = p.slot[b];
-  SeqPlace at;
-  if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == (int)b; }, at)) return;
-  const int n = at.n;
-  if (n == 0) return;
-  if (slot < 0 || slot >= p.slots) {
-    const uint32_t x = slot < 0 ? 0u : 0x7fc07fc0u;
-    for (int i = threadIdx.x >> 5; i < n; i += 8)
-      *reinterpret_cast<uint2*>(p.o + ((int64_t)(at.first + i) * p.HV + h) * kHD + (threadIdx.x & 31) * 4) = make_uint2(x, x);
-    return;
-  }
-  if (n > kTree) {
-    by_rows<DELTA>(p, at, slot, h, hk, red);
-    return;
-  }
-
+  const int64_t at = first + s0;
   const int dv = w * 32 + c * 2, blocks = (n + 15) >> 4;
   float gate, beta;
   int up;
-  bf16x8 kf[4], qf[4];    // a piece a thread of each block's rows of K and Q
-  uint32_t vw[4][4];   // this lane's values of rows 16 I + 4 g + r
+  bf16x8 kf[4], qf[4];  // a piece a thread of each block's rows of K and Q
+  uint32_t vw[4][4];    // this lane's values of rows 16 I + 4 g + r
   {
-    const int64_t row = at.first + min(lane, n - 1);
+    const int64_t row = at + min(lane, n - 1);
     gate = p.g[row * p.HV + h];
     beta = DELTA ? bf2f(p.beta[row * p.HV + h]) : 1.f;
-    up = p.parents == nullptr ? lane - 1 : p.parents[row];
+    up = p.parents == nullptr ? s0 + lane - 1 : p.parents[row];
   }
 #pragma unroll
   for (int I = 0; I < 4; ++I)
     if (I < blocks) {
-      const int64_t row = at.first + min(I * 16 + ((int)threadIdx.x >> 4), n - 1);
-      const int64_t from = (row * p.HK + hk) * kHD + (threadIdx.x & 15) * 8;
+      const int64_t row = at + min(I * 16 + ((int)threadIdx.x >> 4), n - 1);
+      const int64_t from = (row * p.HK + hk) * kHD + c * 8;
       kf[I] = *reinterpret_cast<const bf16x8*>(p.k + from);
       qf[I] = *reinterpret_cast<const bf16x8*>(p.q + from);
     }
@@ -251,7 +248,7 @@ __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
     if (I < blocks)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t row = at.first + min(I * 16 + g * 4 + r, n - 1);
+        const int64_t row = at + min(I * 16 + g * 4 + r, n - 1);
         vw[I][r] = *reinterpret_cast<const uint32_t*>(p.v + (row * p.HV + h) * kHD + dv);
       }
   asm volatile("" ::: "memory");  // the state's loads stay behind
@@ -266,10 +263,14 @@ __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
   asm volatile("" ::: "memory");
 
   // a row a lane: its ancestors and itself, and the sum of their decays (to base two, in 64 bits: differences of long sums
-  // are taken), by jumps of 1, 2, 4 .. rows up the tree
+  // are taken), by jumps of 1, 2, 4 .. rows up the tree; `above`: the row before s0 that it hangs on
   bool odd = !(gate <= 0.f) || !(fabsf(beta) < INFINITY);
+  uint64_t before[kParts - 1] = {};
+  TreeLeft* const left = reinterpret_cast<TreeLeft*>(p.u + p.N * p.HV * kHD);
   {
-    if (up < 0 || up >= lane || lane >= n) up = -1;
+    if (up < 0 || up >= s0 + lane || lane >= n) up = -1;
+    int above = up < s0 ? up : -1;
+    up = up < s0 ? -1 : up - s0;
     // e^-200 is 0 in fp32: -infinity does no worse, and differences of sums stay numbers
     double G = lane < n ? (double)fmaxf(gate, -200.f) * 0x1.71547652b82fep+0 : 0.0;
     uint64_t path = lane < n ? 1ull << lane : 0ull;
@@ -277,11 +278,27 @@ __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
       const int from = up < 0 ? lane : up;
       const double more = __shfl(G, from);
       const uint64_t rest = __shfl((unsigned long long)path, from);
-      const int next = __shfl(up, from);
+      const int next = __shfl(up, from), last = LONG ? __shfl(above, from) : -1;
       if (up >= 0) {
         G += more;
         path |= rest;
         up = next;
+        above = last;
+      }
+    }
+    if (LONG) {
+      if (above >= 0) {
+        const TreeLeft& l = left[(first + above) * p.HV + h];
+        G += l.sum;
+#pragma unroll
+        for (int m = 0; m < kParts - 1; ++m) before[m] = l.seen[m];
+      }
+      if (w == 0 && lane < n) {
+        TreeLeft& l = left[(at + lane) * p.HV + h];
+        l.sum = G;
+#pragma unroll
+        for (int m = 0; m < kParts; ++m)
+          l.seen[m] = m * kTree == s0 ? path : m < kParts - 1 && m * kTree < s0 ? before[m] : 0ull;
       }
     }
     sums[lane] = G;
@@ -291,7 +308,7 @@ __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
 #pragma unroll
   for (int I = 0; I < 4; ++I)
     if (I < blocks) {
-      const int r = (int)threadIdx.x >> 4, x = (threadIdx.x & 15) ^ swizzle(r);
+      const int r = w * 4 + g, x = c ^ swizzle(r);
       rows[0][I * 16 + r][x] = kf[I];
       rows[1][I * 16 + r][x] = qf[I];
     }
@@ -362,28 +379,20 @@ __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
 #pragma unroll
     for (int I = 0; I < 4; ++I) {
       if (I >= blocks) break;
-      const bf16x8 kf = operand(0, I, s), qf = operand(1, I, s);
+      const bf16x8 ki = operand(0, I, s), qi = operand(1, I, s);
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         const bf16x8 sh = __builtin_bit_cast(bf16x8, make_uint4(hi[f][0], hi[f][1], hi[f][2], hi[f][3]));
         const bf16x8 sl = __builtin_bit_cast(bf16x8, make_uint4(lo[f][0], lo[f][1], lo[f][2], lo[f][3]));
-        if (DELTA) u[I][f] = mfma(kf, sl, mfma(kf, sh, u[I][f]));
-        o[I][f] = mfma(qf, sl, mfma(qf, sh, o[I][f]));
+        if (DELTA) u[I][f] = mfma(ki, sl, mfma(ki, sh, u[I][f]));
+        o[I][f] = mfma(qi, sl, mfma(qi, sh, o[I][f]));
       }
     }
   }
-
-  f32x4* const late = reinterpret_cast<f32x4*>(rows);
-  if (DELTA && blocks == 4) {
-    lds_barrier();
-    if (w == 3) late[lane] = fourth;
-    lds_barrier();
-  }
-
+  // X in place of K S0, Q S0 decayed
 #pragma unroll
   for (int I = 0; I < 4; ++I) {
     if (I >= blocks) break;
-    f32x4 x[2];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = I * 16 + g * 4 + r;
@@ -391,25 +400,68 @@ __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         const float v = __uint_as_float(f == 0 ? vw[I][r] << 16 : vw[I][r] & 0xffff0000u);
-        x[f][r] = i < n ? (DELTA ? by * (v - since * u[I][f][r]) : v) : 0.f;
+        u[I][f][r] = i < n ? (DELTA ? by * (v - since * u[I][f][r]) : v) : 0.f;
         o[I][f][r] *= since;
       }
     }
+  }
+  f32x4* const late = reinterpret_cast<f32x4*>(rows);
+
+#pragma unroll
+  for (int I = 0; I < 4; ++I) {
+    if (I >= blocks) break;
+    // the rows before s0, 16 at a time
+    if (LONG)
+#pragma unroll 1
+      for (int j0 = 0; j0 < s0; j0 += 16) {
+        asm volatile("" ::: "memory");  // LDS is read where it is needed: there are no registers to hold its rows
+        const uint64_t word = j0 < kTree ? before[0] : j0 < 2 * kTree ? before[1] : before[2];
+        const uint64_t path = __shfl((unsigned long long)word, I * 16 + c) >> (j0 & (kTree - 1));
+        f32x4 kk = {}, qk = {}, uj[2];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const bf16x8 kj =
+              *reinterpret_cast<const bf16x8*>(p.k + ((first + j0 + c) * p.HK + hk) * kHD + s * 32 + g * 8);
+          if (DELTA) kk = mfma(kj, operand(0, I, s), kk);
+          qk = mfma(kj, operand(1, I, s), qk);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t row = (first + j0 + g * 4 + r) * p.HV + h;
+          const f32x2 x = *reinterpret_cast<const f32x2*>(p.u + row * kHD + dv);
+          uj[0][r] = x.x;
+          uj[1][r] = x.y;
+          const bool in = path >> (g * 4 + r) & 1;
+          const float e = in ? fade(sums[I * 16 + c], left[row].sum) : 0.f;
+          kk[r] = in ? -strength[I * 16 + c] * e * kk[r] : 0.f;
+          qk[r] = in ? e * qk[r] : 0.f;
+        }
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          if (DELTA) u[I][f] = times(kk, uj[f], u[I][f]);
+          o[I][f] = times(qk, uj[f], o[I][f]);
+        }
+      }
 #pragma unroll
     for (int J = 0; J < I; ++J) {
       const int pair = I * (I - 1) / 2 + J;
       const f32x4 a = mats[7 + pair][lane], pj = mats[13 + pair][lane];
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        if (DELTA) x[f] = times(a, u[J][f], x[f]);
+        if (DELTA) u[I][f] = times(a, u[J][f], u[I][f]);
         o[I][f] = times(pj, u[J][f], o[I][f]);
       }
+    }
+    if (DELTA && I == 3) {
+      lds_barrier();
+      if (w == 3) late[lane] = fourth;
+      lds_barrier();
     }
     const f32x4 pi = mats[3 + I][lane];
     const f32x4 t = !DELTA ? f32x4{} : I < 3 ? mats[I][lane] : late[lane];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
-      u[I][f] = DELTA ? times(t, x[f], f32x4{}) : x[f];
+      if (DELTA) u[I][f] = times(t, u[I][f], f32x4{});
       o[I][f] = times(pi, u[I][f], o[I][f]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) odd |= !(fabsf(u[I][f][r]) < INFINITY);
@@ -417,12 +469,66 @@ __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = I * 16 + g * 4 + r;
-      if (i < n)
-        *reinterpret_cast<uint32_t*>(p.o + ((int64_t)(at.first + i) * p.HV + h) * kHD + dv) =
-            cvt_pk2(p.scale * o[I][0][r], p.scale * o[I][1][r]);
+      const int64_t row = (at + i) * p.HV + h;
+      if (i < n) {
+        *reinterpret_cast<uint32_t*>(p.o + row * kHD + dv) = cvt_pk2(p.scale * o[I][0][r], p.scale * o[I][1][r]);
+        if (LONG) *reinterpret_cast<f32x2*>(p.u + row * kHD + dv) = f32x2{u[I][0][r], u[I][1][r]};
+      }
     }
   }
-  if (__syncthreads_or(odd)) by_rows<DELTA>(p, at, slot, h, hk, red);
+  return odd;
+}
+
+template <bool DELTA>
+__global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
+  __shared__ __attribute__((aligned(16))) TreeShared lds;
+  float* const red = reinterpret_cast<float*>(lds.mats);  // row by row
+  const int64_t b = blockIdx.x / p.HV;
+  const int h = blockIdx.x - (int)(b * p.HV), hk = h / (p.HV / p.HK);
+  if (b == p.B) {  // rows of no sequence
+    int lo, hi;
+    seq_span(p.q_ptr, p.B, p.N, lo, hi);
+    for (int64_t r = threadIdx.x >> 5; r < p.N; r += 8)
+      if (r < lo || r >= hi)
+        *reinterpret_cast<uint2*>(p.o + (r * p.HV + h) * kHD + (threadIdx.x & 31) * 4) = make_uint2(0u, 0u);
+    return;
+  }
+  const int64_t slot = p.slot[b];
+  SeqPlace at;
+  if (!seq_find(p.q_ptr, p.B, p.N, [](int, int) { return 0; }, [=](int i, int) { return i == (int)b; }, at)) return;
+  const int n = at.n;
+  if (n == 0) return;
+  if (slot < 0 || slot >= p.slots) {
+    const uint32_t x = slot < 0 ? 0u : 0x7fc07fc0u;
+    for (int i = threadIdx.x >> 5; i < n; i += 8)
+      *reinterpret_cast<uint2*>(p.o + ((int64_t)(at.first + i) * p.HV + h) * kHD + (threadIdx.x & 31) * 4) = make_uint2(x, x);
+    return;
+  }
+  if (n > kTree) return;  // lintree_long_k's
+  if (__syncthreads_or(tree_part<DELTA, false>(p, lds, at.first, 0, n, slot, h, hk)))
+    by_rows<DELTA, true>(p, at, slot, h, hk, red, reinterpret_cast<float4(*)[32]>(lds.rows));
+}
+
+// The sequences with more rows than that, part after part; a workgroup for each that there can be, and head. (A kernel of its
+// own: in one with the other form, the registers that this one wants cost that one a third more time.)
+template <bool DELTA>
+__global__ void __launch_bounds__(256, 2) lintree_long_k(LinTreeParams p) {
+  __shared__ __attribute__((aligned(16))) TreeShared lds;
+  const int which = blockIdx.x / (uint32_t)p.HV, h = blockIdx.x - which * p.HV, hk = h / (p.HV / p.HK);
+  SeqPlace at;
+  if (!seq_find(p.q_ptr, p.B, p.N, [](int, int n) { return (int)(n > kTree); }, [=](int, int upto) { return upto > which; },
+                at))
+    return;
+  const int64_t slot = p.slot[at.seq];
+  if (slot < 0 || slot >= p.slots) return;  // lintree_k has seen to these
+  bool odd = at.n > kTree * kParts;
+  if (!odd)
+#pragma unroll 1
+    for (int s0 = 0; s0 < at.n; s0 += kTree) {
+      odd |= tree_part<DELTA, true>(p, lds, at.first, s0, min(kTree, at.n - s0), slot, h, hk);
+      __syncthreads();  // what it leaves is there for the next one, and LDS is free
+    }
+  if (__syncthreads_or(odd)) by_rows<DELTA, false>(p, at, slot, h, hk, reinterpret_cast<float*>(lds.mats), nullptr);
 }
 
 // x summed over the four groups of 16 lanes, in all of them.
@@ -523,9 +629,16 @@ __global__ void __launch_bounds__(128) linattn_keep_k(LinTreeParams p) {
 
 }  // namespace
 
+// Sequences longer than what a workgroup takes at once leave their u in memory.
+int64_t lintree_work_bytes(int64_t N, int HV) { return N > kTree ? N * HV * (kHD * 4 + (int64_t)sizeof(TreeLeft)) : 0; }
+
 hipError_t launch_linattn_tree(const LinTreeParams& p, hipStream_t st) {
   hipLaunchKernelGGL(p.beta != nullptr ? lintree_k<true> : lintree_k<false>,
                      dim3((unsigned)((p.B + 1LL) * p.HV)), dim3(256), 0, st, p);
+  const int64_t longs = std::min<int64_t>(p.B, p.N / (kTree + 1));  // at most
+  if (longs > 0)
+    hipLaunchKernelGGL(p.beta != nullptr ? lintree_long_k<true> : lintree_long_k<false>, dim3((unsigned)(longs * p.HV)),
+                       dim3(256), 0, st, p);
   return hipGetLastError();
 }
 

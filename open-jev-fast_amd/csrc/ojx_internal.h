@@ -336,6 +336,7 @@ struct LinTreeParams {
   int B, HV, HK;
   float scale;
 };
+int64_t lintree_work_bytes(int64_t N, int HV);
 hipError_t launch_linattn_tree(const LinTreeParams& p, hipStream_t st);
 hipError_t launch_linattn_keep(const LinTreeParams& p, hipStream_t st);
 

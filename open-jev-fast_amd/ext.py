@@ -902,7 +902,8 @@ def kv_pages_fork(table, ctx, refs, src, page):
 
 def kv_pages_copy(kc, vc, pairs, ks=None, vs=None):
     """Copies page pairs[i][0] to page pairs[i][1] (int32 [n, 2], as kv_pages_fork gives them; a pair with a page outside the
-    cache is left out) in a cache of one layer or several (see kv_cache_keep). No page may be both read and written."""
+    cache is left out) in a cache of one layer or several (see kv_cache_keep). No page may be both read and written, or written
+    twice."""
     fmt, layers, pages, HKV, page, D = _chk_layers(kc, vc, ks, vs)
     _chk_each((pairs, "pairs", torch.int32))
     if pairs.dim() != 2 or pairs.shape[1] != 2:

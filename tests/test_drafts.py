@@ -147,7 +147,9 @@ def test_lintree_refusals(pkg, p):
         assert tree(**bad) == 1, bad
     for bad in (dict(path=None), dict(count=None), dict(path=mis), dict(count=mis)):
         assert keep(**bad) == 1, bad
-    assert tree(ws=None) == 3 and tree(nws=16) == 3 and tree(ws=mis) == 3
+    for bad in (dict(ws=None), dict(nws=16), dict(ws=mis)):
+        assert tree(N=65, **bad) == 3, bad            # longer sequences than a workgroup takes at once
+    assert L.ojx_linattn_tree_workspace(64, 2, 6, 2) == 0 and L.ojx_linattn_tree_workspace(65, 2, 6, 2) == 65 * 6 * 552
     assert tree(N=0, k=None, q=None) == 0 and keep(N=0, k=None) == 0
 
 
