@@ -18,6 +18,11 @@
 //                   rejection, all it needs being in draft_rows_k's few numbers, and sums w over the chunk
 //   draft_next_k    a workgroup per sequence: the whole walk, the accepted rows, the next token
 // The two in the middle are launched with q and more than a few chunks; otherwise draft_next_k does their work.
+//
+// What bounds it: 64 sequences of up to 12 rows of 131072 bf16 logits (71 million, 142 MB) with a draft model's probabilities
+// take 106 us. The chunks are 50 to 54 of them, the vector unit's: 18 operations a logit, issued 79% of the time, where memory
+// would allow 27 us. Each launch of draft_sums_k is 4 us with nothing to do, 8 with a few sequences left and 15 with all of
+// them (50 MB); draft_rows_k 5, draft_next_k 9: latency. Few rows are latency alone: 17 us for 6 rows of 32000 in two launches.
 #include "ojx_internal.h"
 
 #include <algorithm>
@@ -231,7 +236,8 @@ __device__ __forceinline__ int owner(const DraftParams& p, int64_t r, SeqPlace& 
                                                                                                               : -1;
 }
 
-// `each` chunks of a row for a workgroup, the next one's logits on their way while one is summed.
+// `each` chunks of a row for a workgroup, the next one's logits on their way while one is summed. (Workgroups of 512 and 1024
+// threads, with 16 and 8 logits a thread in place of 32: 6% and 29% more time for the largest case.)
 template <typename T>
 __global__ void __launch_bounds__(256) draft_chunks_k(DraftParams p, int each, int groups) {
   __shared__ float tops[4], temp;

@@ -1,7 +1,8 @@
 // What becomes of a paged cache around drafted tokens: accepted rows moved together, pages taken, given back, shared and
 // copied. A table row names a sequence's pages, refs counts the table entries that name each page; a page with none is free.
 //
-// All of it is whole numbers and copies. Tables and counts are small: what bounds them is the chain of launches and loads.
+// All of it is whole numbers and copies. Tables and counts are small: what bounds them is the chain of launches and loads (4.6
+// and 6.0 us for a resize and a fork in one launch each).
 #include "ojx_internal.h"
 
 #include <algorithm>
@@ -16,7 +17,8 @@ namespace {
 // may take its 16 bytes of every entry in order, four read and then written, with no barrier between.
 //
 // A workgroup looks a sequence's places up once, 128 entries at a time, and then moves them for 256 / L heads' keys or values
-// of some layer at once, a row being L lanes of 16 bytes.
+// of some layer at once, a row being L lanes of 16 bytes. What bounds it: the chain pointers, path, table, rows, 3.1 us for one
+// sequence and layer; 64 sequences of up to 6 rows in 16 layers, 9 MB, 6.2 us (27 with a look-up for every head and layer).
 template <int ROW>  // bytes of a row
 __global__ void __launch_bounds__(256) kv_keep_k(KeepParams p, int parts) {
   constexpr int L = ROW / 16, G = 256 / L, kList = 128;
@@ -375,6 +377,7 @@ __device__ __forceinline__ void store_past(uint4* p, uint4 x) {
 }
 
 // A workgroup moves 16 KB of one page of one layer, keys or values (then a part of its scales): four loads a lane in flight.
+// What bounds it: the writes (56 pages of 16 layers from 8, 235 MB: 39 to 43 us, 5.5 to 6 TB/s).
 __global__ void __launch_bounds__(256) pages_copy_k(CopyParams p) {
   const int64_t pair = blockIdx.y, from = p.pairs[2 * pair], to = p.pairs[2 * pair + 1];
   if (from < 0 || from >= p.pages || to < 0 || to >= p.pages || from == to) return;

@@ -401,6 +401,24 @@ def test_tree_odd_parents_slots_and_pointers(ext, D, dev, n, delta):
     _check_tree(D, args, state, slot, ptr, parents, 128 ** -0.5, got)
 
 
+@pytest.mark.parametrize("delta", [True, False])
+def test_tree_long_sequences_among_others(ext, D, dev, delta):
+    """Sequences of more than 64 rows beside short, empty, idle ones and one whose state is not there; falling pointers."""
+    g = torch.Generator().manual_seed(6)
+    lengths = [70, 3, 0, 130, 64, 90, 65]
+    N = sum(lengths) + 5
+    args = _lin_case(N, 1, 2, delta, seed=6)
+    parents = torch.cat([_parents(lengths, "near", g), torch.zeros(5, dtype=I32)])
+    parents[69], parents[80] = -1, 500
+    state = 0.3 * torch.randn(3, 2, 128, 128, generator=g)
+    slot = torch.tensor([1, -1, 0, 0, 2, 7, 2], dtype=I32)
+    for ptr in (_ptr(lengths), torch.tensor([2, 70, 60, 260, 200, 380, 390, 5], dtype=I32)):
+        d = _put(dev, *args, state, slot, ptr, parents)
+        got = ext.linattn_tree(*d)
+        assert torch.equal(got, ext.linattn_tree(*d)) or bool(torch.isnan(got).any())
+        _check_tree(D, args, state, slot, ptr, parents, 128 ** -0.5, got)
+
+
 def _below(parents, n, j):
     """Rows of a sequence that hang on row j, itself among them."""
     out = {j}
