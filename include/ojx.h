@@ -329,6 +329,8 @@ int ojx_kv_cache_keep(void* kc, void* vc, float* ks, float* vs, int32_t fmt, int
  * (the other's last page, the new one), to be copied by ojx_kv_pages_copy in every layer before anything else is written
  * to the cache or taken from the pool; (-1, -1) where there is none. A slot for which the pool has no page gets (page, -1)
  * and ends with its last full page: ctx says so.
+ * A shared page is full: a sequence goes on behind it, on pages of its own. One that is cut back into a shared page must not
+ * be written there.
  * ojx_kv_pages_copy: page pairs[i][0] -> page pairs[i][1] of a cache of `layers` layers (see ojx_kv_cache_keep), i < n; pairs
  * with a page outside [0, pages) are left out. Pages written must not be among those read, nor named twice.
  * workspace: ojx_kv_pages_workspace bytes of device memory, 16-byte aligned (fork: 1 for ojx_kv_pages_fork). B at most
