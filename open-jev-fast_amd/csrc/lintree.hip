@@ -205,8 +205,8 @@ struct TreeLeft {
 //   A_ij = beta_i e^(G_i - G_j) k_i . k_j  and  P_ij = e^(G_i - G_j) q_i . k_j  for the ancestors j of i (in P also i itself),
 //   X = diag(beta) (V - diag(e^G) K S0),  U = (I + A)^-1 X,  O = scale (diag(e^G) Q S0 + P U),
 // block row after block row. S0 enters as two bf16 pieces (what it makes is rounded to bf16 in the end), everything else in
-// fp32. A product with a zero in place of a row that is no ancestor is only right for finite numbers: where a U is not finite
-// or a decay is above 1 (true), the head goes row by row instead.
+// fp32. A product with a zero in place of a row that is no ancestor is only right for finite numbers: where a U or an O is
+// not finite (a state's two pieces have no infinity) or a decay is above 1 (true), the head goes row by row instead.
 // Loads come back in the order in which they were made, so the rows' go first: while the state is on its way the four waves
 // make the blocks of A, P and the inverses of A's diagonal ones, each once, and hand them to each other in LDS as the operands
 // that they are. LONG: the rows before s0 have left their U and TreeLeft in the workspace (a thread reads back the U that it
@@ -464,7 +464,7 @@ __device__ __forceinline__ bool tree_part(const LinTreeParams& p, TreeShared& ld
       if (DELTA) u[I][f] = times(t, u[I][f], f32x4{});
       o[I][f] = times(pi, u[I][f], o[I][f]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) odd |= !(fabsf(u[I][f][r]) < INFINITY);
+      for (int r = 0; r < 4; ++r) odd |= !(fabsf(u[I][f][r]) < INFINITY) || !(fabsf(o[I][f][r]) < INFINITY);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {

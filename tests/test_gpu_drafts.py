@@ -490,6 +490,22 @@ def test_tree_state_not_finite(ext, D, dev):
     assert bool((got[:, 1, others].float() - clean[:, 1, others].float()).abs().max() <= 0.02)
 
 
+@pytest.mark.parametrize("n", [1, 20, 90])
+def test_tree_state_past_16_bits(ext, D, dev, n):
+    """Without the delta rule too, infinities in a state come out as such, and what rounds to one in 16 bits as it is."""
+    g = torch.Generator().manual_seed(n)
+    args = _lin_case(n, 1, 2, False, seed=n)
+    parents, slot, ptr = _parents([n], "near", g), torch.zeros(1, dtype=I32), _ptr([n])
+    state = 0.3 * torch.randn(1, 2, 128, 128, generator=g)
+    state[0, 1, 90, 77], state[0, 1, 3, 20] = math.inf, torch.finfo(F32).max
+    got = ext.linattn_tree(*_put(dev, *args, state, slot, ptr, parents)).cpu().double().reshape(n, 2, 128)
+    o, bo = D.linattn_tree(*args, state, [0], [0, n], parents, 128 ** -0.5)
+    assert bool(torch.isinf(o[:, 1, 77]).all()) and torch.equal(got[:, 1, 77], o[:, 1, 77])
+    fine = torch.isfinite(o)
+    assert int(fine.sum()) == n * (256 - 1)
+    assert bool(((got - o).abs() <= bo)[fine].all())
+
+
 @pytest.mark.parametrize("delta", [True, False])
 def test_tree_decays_above_one(ext, D, dev, delta):
     q, k, v, gate, beta = _lin_case(24, 1, 2, delta, seed=8)
