@@ -297,8 +297,8 @@ int ojx_linattn_keep(const void* k, const void* v, const float* g, const void* b
  * path int32 [N]: of each sequence the accepted rows in order, row 0 first, then -1; count int32 [B]: how many; next int64
  * [B]. A sequence without rows gives count 0 and next -1. A row with a NaN or +infinity among its logits, or none above
  * -infinity, accepts nothing and gives next -1. path is -1 in rows of no sequence.
- * workspace: ojx_verify_drafts_workspace bytes of device memory, 16-byte aligned. V at most 2^22; V / 8192 + 1 times N below 2^24,
- * times B below 2^22, B at most 65536 (OJX_ERR_SHAPE otherwise; -1 from the workspace's size). */
+ * workspace: ojx_verify_drafts_workspace bytes of device memory, 16-byte aligned. V at most 2^22; (V + 8198) / 8192 times N below
+ * 2^24, times B below 2^22, B at most 65536 (OJX_ERR_SHAPE otherwise; -1 from the workspace's size). */
 enum { OJX_F32 = 0, OJX_BF16 = 1 };
 int64_t ojx_verify_drafts_workspace(int64_t N, int32_t B, int64_t V, int32_t has_probs);
 int ojx_verify_drafts(const void* logits, int32_t logits_type, int64_t ldl, const int64_t* tokens, const int32_t* q_ptr,
