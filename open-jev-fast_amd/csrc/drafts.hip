@@ -786,20 +786,24 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
 
 int64_t draft_chunks(int64_t V) { return (V + 7 + kPiece - 1) / kPiece; }
 
+// Rejections of a sequence whose sums are launches of their own. In a line of tokens nothing follows a rejection but the next
+// token. A few chunks are summed by one workgroup sooner than by another launch; without rows there is no walk to leave.
+static int draft_rounds(int64_t N, int64_t B, int64_t V, bool probs, bool tree) {
+  return !probs || N == 0 || B == 0 || draft_chunks(V) <= 4 ? 0 : tree ? kDraftRounds : 1;
+}
+
 int64_t draft_work_bytes(int64_t N, int64_t B, int64_t V, bool probs) {
-  const int64_t c = draft_chunks(V);
-  return N * c * (int64_t)sizeof(DraftChunk) + N * (int64_t)sizeof(DraftRow) + (probs ? kDraftRounds * B * (c * 8 + (int64_t)sizeof(DraftWalk)) : 0);
+  const int64_t c = draft_chunks(V), rounds = draft_rounds(N, B, V, probs, true);
+  return N * c * (int64_t)sizeof(DraftChunk) + N * (int64_t)sizeof(DraftRow) + rounds * B * (c * 8 + (int64_t)sizeof(DraftWalk));
 }
 
 hipError_t launch_verify(DraftParams p, bool f32, bool probs_f32, uint8_t* work, hipStream_t st) {
   p.chunks = (int)draft_chunks(p.V);
-  // In a line of tokens nothing follows a rejection but the next token. A few chunks are summed by one workgroup sooner than
-  // by another launch.
-  p.rounds = p.probs == nullptr || p.chunks <= 4 ? 0 : p.parents != nullptr ? kDraftRounds : 1;
+  p.rounds = draft_rounds(p.N, p.B, p.V, p.probs != nullptr, p.parents != nullptr);
   p.parts = reinterpret_cast<DraftChunk*>(work);
   p.rows = reinterpret_cast<DraftRow*>(p.parts + p.N * p.chunks);
   p.walks = reinterpret_cast<DraftWalk*>(p.rows + p.N);
-  p.sums = reinterpret_cast<double*>(p.walks + kDraftRounds * p.B);
+  p.sums = reinterpret_cast<double*>(p.walks + p.rounds * p.B);
   const dim3 wide(256), rows((unsigned)((p.N + 3) / 4));
   if (p.N > 0) {
     // two chunks a workgroup where there are enough of them for the chip twice over: 50 us in place of 53 in the largest case
@@ -807,7 +811,7 @@ hipError_t launch_verify(DraftParams p, bool f32, bool probs_f32, uint8_t* work,
     hipLaunchKernelGGL(f32 ? draft_chunks_k<float> : draft_chunks_k<uint16_t>, dim3((unsigned)(p.N * groups)), wide, 0, st, p,
                        each, groups);
   }
-  if (p.rounds > 0 && p.N > 0 && p.B > 0) {
+  if (p.rounds > 0) {
     const auto rows_k = probs_f32 ? (f32 ? draft_rows_k<float, float> : draft_rows_k<uint16_t, float>)
                                   : (f32 ? draft_rows_k<float, uint16_t> : draft_rows_k<uint16_t, uint16_t>);
     const auto sums_k = probs_f32 ? (f32 ? draft_sums_k<float, float, kSumThreads> : draft_sums_k<uint16_t, float, kSumThreads>)

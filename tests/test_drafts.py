@@ -273,3 +273,14 @@ def test_python_refusals_of_shapes(ext, monkeypatch):
                 lambda: ext.kv_pages_copy(k5, k5, z(2, 2, t=i32), s5)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_verify_without_rows_has_no_walks(pkg):
+    """Walks and sums of rejections are left by launches over rows and sequences: where there are none, no part of a call may
+    count on them, and none is asked for. With at most four chunks (V + 7 places in 8192s) there are no such launches."""
+    L = pkg._lib.lib()
+    size = lambda N, B, V, probs: L.ojx_verify_drafts_workspace(N, B, V, probs)  # noqa: E731
+    for V in (10, 32761, 32762, 41000, 1 << 22):
+        assert size(0, 3, V, 1) == size(0, 3, V, 0) == 0
+        assert size(6, 0, V, 1) == size(6, 0, V, 0) > 0
+        assert (size(6, 3, V, 1) > size(6, 3, V, 0)) == (V > 32761)

@@ -927,3 +927,18 @@ def test_steps_on_streams_at_once(ext, dev):
     for (step, want, side), outs in zip(lots, got):
         for i, (a, b) in enumerate(zip(outs, want)):
             assert torch.equal(a, b), f"output {i}"
+
+
+def test_verify_no_rows_in_c(pkg, dev):
+    """A step without rows, with draft probabilities of a large vocabulary, as a host in C may call it: counts of 0, no next
+    tokens, and a workspace of no bytes."""
+    L = pkg._lib.lib()
+    ptr, some = torch.zeros(4, dtype=I32, device=dev), torch.ones(16, device=dev)
+    for parents in (None, ptr.data_ptr()):
+        for V in (10, 41000, 1 << 22):
+            count, nxt = torch.full((3,), 77, dtype=I32, device=dev), torch.full((3,), 77, device=dev)
+            assert L.ojx_verify_drafts_workspace(0, 3, V, 1) == 0
+            assert L.ojx_verify_drafts(None, 0, V, None, ptr.data_ptr(), None, parents, some.data_ptr(), 0, V, None, 0, 3, V,
+                                       None, count.data_ptr(), nxt.data_ptr(), None, 0, None) == 0
+            torch.cuda.synchronize()
+            assert count.tolist() == [0] * 3 and nxt.tolist() == [-1] * 3, V
