@@ -20,7 +20,7 @@
 // The two in the middle are launched with q and more than a few chunks; otherwise draft_next_k does their work.
 //
 // What bounds it: 64 sequences of up to 12 rows of 131072 bf16 logits (71 million, 142 MB) with a draft model's probabilities
-// take 106 us. The chunks are 50 to 54 of them, the vector unit's: 18 operations a logit, issued 79% of the time, where memory
+// take 112 us. The chunks are 55 to 59 of them, the vector unit's: 20 operations a logit, where memory
 // would allow 27 us. Each launch of draft_sums_k is 4 us with nothing to do, 8 with a few sequences left and 15 with all of
 // them (50 MB); draft_rows_k 5, draft_next_k 9: latency. Few rows are latency alone: 17 us for 6 rows of 32000 in two launches.
 #include "ojx_internal.h"
@@ -141,18 +141,20 @@ __device__ __forceinline__ float temperature(const DraftParams& p, int b) {
   const float t = p.temp == nullptr ? 1.f : p.temp[b];
   return t > 0.f ? t : 0.f;
 }
-// 2^f for |f| <= 1/2, 1.1e-12 off at most: a polynomial of degree 8, interpolated at Chebyshev's nodes, then its first
-// coefficient made 1 (a degree more: 2e-14). That error moves the borders between tokens by as much: one draw in some 10^7
-// may fall on the other side of one.
+// 2^f for |f| <= 1/2, 3.2e-16 off at most beside the roundings, as much as one and a half of them: a polynomial of degree 10,
+// interpolated at Chebyshev's nodes, its first coefficient 1 (degree 9: 3.8e-14, degree 8: 1.1e-12 and two operations of 16 a
+// logit less: 108 us in place of 112 for the largest case. A caller who is promised 64 bits gets them).
 __device__ __forceinline__ double exp2_part(double f) {
-  double x = 0x1.63d136366db24p-20;
-  x = fma(x, f, 0x1.00dc4a532fb8ep-16);
-  x = fma(x, f, 0x1.4308ac85aa947p-13);
-  x = fma(x, f, 0x1.5d8745a728441p-10);
-  x = fma(x, f, 0x1.3b2ab7181b755p-7);
-  x = fma(x, f, 0x1.c6b08dd6fd234p-5);
-  x = fma(x, f, 0x1.ebfbdff823cedp-3);
-  x = fma(x, f, 0x1.62e42fef84cf0p-1);
+  double x = 0x1.e6063f7217bc6p-28;
+  x = fma(x, f, 0x1.b675bca4eeebbp-24);
+  x = fma(x, f, 0x1.62bfd47773353p-20);
+  x = fma(x, f, 0x1.ffcb54062e698p-17);
+  x = fma(x, f, 0x1.430913096fd9fp-13);
+  x = fma(x, f, 0x1.5d87fe9d7a584p-10);
+  x = fma(x, f, 0x1.3b2ab6fba1ddap-7);
+  x = fma(x, f, 0x1.c6b08d703ce49p-5);
+  x = fma(x, f, 0x1.ebfbdff82c598p-3);
+  x = fma(x, f, 0x1.62e42fefa3a19p-1);
   return fma(x, f, 1.0);
 }
 constexpr double kRound = 0x1.8p52;  // added and taken off again: rounds to a whole number, whose low bits it leaves in the sum
@@ -167,7 +169,7 @@ __device__ __forceinline__ double exp2_down(double y) {
 }
 
 // exp((x - top) / T) = 2^((x - top) c), c = 1 / (T log 2). In the loops over whole rows it is made as 2^(x c - k), k the
-// whole number next to top c, times `rest` = 2^(k - top c): 14 operations a logit instead of 17, where the library's
+// whole number next to top c, times `rest` = 2^(k - top c): 16 operations a logit instead of 19, where the library's
 // exponential would be 40 (the largest case makes 71 million of them, and is bound by them). `plain` says that the sizes do
 // not allow it. A logit of -infinity counts as 2^-990 there, next to nothing.
 struct Scale {

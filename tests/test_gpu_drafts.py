@@ -942,3 +942,46 @@ def test_verify_no_rows_in_c(pkg, dev):
                                        None, count.data_ptr(), nxt.data_ptr(), None, 0, None) == 0
             torch.cuda.synchronize()
             assert count.tolist() == [0] * 3 and nxt.tolist() == [-1] * 3, V
+
+
+def _near_borders(T, least, most, count):
+    """Logits x (beside one of 0) and numbers u, all fp32, with u between `least` and `most` from e^(x/T) / (1 + e^(x/T)) or from
+    the other's share, relative to them: (x, u, below) of each kind. In 80 bits, whose exponential is off by some 1e-19."""
+    import numpy as np
+    x = np.linspace(-12.0, -1e-3, 1 << 22).astype(np.float32)
+    e = np.exp(x.astype(np.longdouble) / np.longdouble(np.float32(T)))
+    out = []
+    for p in (e / (1 + e), 1 / (1 + e)):
+        u = p.astype(np.float32)
+        off = u.astype(np.longdouble) / p - 1
+        at = np.nonzero((np.abs(off) > least) & (np.abs(off) < most))[0][:count]
+        assert len(at) >= min(count, 20)
+        out.append((torch.from_numpy(x[at]), torch.from_numpy(u[at]), (off[at] < 0).tolist()))
+    return out
+
+
+@pytest.mark.parametrize("T", [1.0, 0.7])
+@pytest.mark.parametrize("V,probs", [(2, False), (2, True), (9000, True), (41000, False), (41000, True)])
+def test_verify_decides_in_64_bits(ext, dev, V, probs, T):
+    """Numbers 2e-14 to 1e-12 beside the border of a test and of a draw, a distance that 64 bits tell and fewer do not. A
+    probability is off by the argument's roundings, four times 2^-53 of |x / T| <= 17.2, by the exponential's 3.2e-16 and its
+    rounding, 2^-52, and by those of a sum and quotient of two such: 2 (4 17.2 2^-53 + 3.2e-16 + 2^-52) + 4 2^-53 < 1.8e-14."""
+    test, draw = _near_borders(T, 2e-14, 1e-12, 60)
+    ends = (0, V - 1)
+    for kind, (x, u, below) in (("test", test), ("draw", draw)):
+        B, n = len(x), 2 if kind == "test" else 1
+        logits = torch.full((B * n, V), -math.inf)
+        logits[:, ends[0]] = 0.0
+        logits[:, ends[1]] = x.repeat_interleave(n)
+        q = torch.zeros(B * n, V)
+        q[:, ends[1]] = 1.0
+        tokens = torch.full((B * n,), ends[1])
+        numbers = u if kind == "draw" else torch.stack([torch.full_like(u, 0.5), u], 1).reshape(-1)
+        for tree in (None, torch.tensor([-1, 0][:n] * B, dtype=I32)):
+            got = _run_verify(ext, {"logits": logits, "tokens": tokens, "q_ptr": torch.arange(0, B * n + 1, n, dtype=I32),
+                                    "u": numbers, "parents": tree, "probs": q if probs else None,
+                                    "temperature": torch.full((B,), T)}, dev)
+            if kind == "test":
+                assert got[1].tolist() == [1 + b for b in below]
+            else:
+                assert got[2].tolist() == [ends[0] if b else ends[1] for b in below]
