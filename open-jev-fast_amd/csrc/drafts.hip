@@ -45,7 +45,7 @@ struct DraftRow {
 
 struct DraftWalk {
   int j, cur, count, rejections;  // the next row to look at, the current one, accepted so far
-  double a, t;
+  double a, t;                    // without q a = 1 says that t has to be summed
   int first, n;                   // the sequence's rows, its temperature
   float temp, pad;
 };
@@ -404,8 +404,12 @@ __global__ void __launch_bounds__(256) draft_rows_k(DraftParams p) {
 // Where the walk over a sequence's rows stands.
 using Walk = DraftWalk;
 
-// On to the next rejection with q (true: what is left has to be summed before the walk can go on), or to the end; the whole
-// wave calls, with the walk the same in all lanes. write(i, j): row j is the i-th accepted.
+// Without q what is left after a rejection is one less that token's share, until fewer than three of its digits are: then it is
+// summed, should another token be tested (a = 1: it has to be).
+constexpr double kCancelled = 1e-3;
+
+// On to the next rejection with q or test with a sum that has to be made (true: what is left has to be summed before the walk
+// can go on), or to the end; the whole wave calls, with the walk the same in all lanes. write(i, j): row j is the i-th accepted.
 template <bool PROBS, typename Write>
 __device__ __forceinline__ bool walk_on(const DraftParams& p, Walk& w, Write write) {
   const int lane = threadIdx.x & 63;
@@ -419,6 +423,7 @@ __device__ __forceinline__ bool walk_on(const DraftParams& p, Walk& w, Write wri
       if (__builtin_amdgcn_readlane(above, l) != w.cur) continue;
       const double x = lane_of(rp, l), q = lane_of(rq, l), v = lane_of(u, l);
       if (x < 0.0) continue;
+      if (!PROBS && w.a > 0.0) return true;
       const double left = PROBS && w.temp > 0.f && w.a > 0.0 ? fmax(x - w.a * q, 0.0) : x;
       if (v * q * w.t < left) {
         write(w.count, w.j);
@@ -433,7 +438,10 @@ __device__ __forceinline__ bool walk_on(const DraftParams& p, Walk& w, Write wri
         return true;
       } else {
         ++w.rejections;
-        if (w.temp > 0.f) w.t -= x;
+        if (w.temp > 0.f && x > 0.0) {
+          w.t -= x;
+          w.a = w.t < kCancelled ? 1.0 : 0.0;
+        }
       }
     }
   }
@@ -579,8 +587,9 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     __syncthreads();
   }
 
-  // what is left in four chunks, to all threads; `less`: without the tokens of the row's children, all of them rejected
-  const auto chunk_sums = [&](int64_t r, const Scale& sc, double unit, double a, int c0, int many, bool less) {
+  // what is left in four chunks, to all threads; without the tokens of the row's children before row `upto`, all of them
+  // rejected
+  const auto chunk_sums = [&](int64_t r, const Scale& sc, double unit, double a, int c0, int many, int upto) {
     const int64_t e0 = (int64_t)c0 * kPiece - lead(static_cast<const T*>(p.logits) + r * p.ldl) + threadIdx.x * 8;
     double sum[4];
 #pragma unroll
@@ -594,8 +603,8 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
       }
       double w[8];
       left_of<T, Q, PROBS>(p, r, e, sc, unit, a, w);
-      if (less)
-        for (int j = (int)(r - first) + 1; j < n; ++j) {
+      if (!PROBS)
+        for (int j = (int)(r - first) + 1; j < upto; ++j) {
           const int64_t x = p.rows[first + j].token - e;
           if (p.rows[first + j].above == (int)(r - first) && x >= 0 && x < 8)
 #pragma unroll
@@ -637,12 +646,13 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
     const bool more = need;
     __syncthreads();
     if (!more) break;
-    // a rejection beyond the ones that draft_sums_k was launched for
+    // with q a rejection beyond the ones that draft_sums_k was launched for
     const int64_t r = first + w.cur;
     const Scale sc = scale_of(t, p.rows[r].top);
     const double unit = 1.0 / p.rows[r].sum;
     w.t = 0.0;
-    for (int c = 0; c < p.chunks; c += 4) w.t += chunk_sums(r, sc, unit, w.a, c, min(4, p.chunks - c), false);
+    for (int c = 0; c < p.chunks; c += 4) w.t += chunk_sums(r, sc, unit, w.a, c, min(4, p.chunks - c), w.j);
+    if (!PROBS) w.a = 0.0;
   }
   for (int i = w.count + threadIdx.x; i < n; i += 1024) p.path[first + i] = -1;
   const int64_t r = first + w.cur;
@@ -686,7 +696,7 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
             const int l = __builtin_ctzll(m), at = __builtin_amdgcn_readlane(c, l);
             const double before = chunk_left[at], after = before - lane_of(x, l) * row.sum;
             some = true;
-            if (lane == 0) chunk_left[at] = before < 0.0 || after < 1e-3 * before ? -1.0 : after;
+            if (lane == 0) chunk_left[at] = before < 0.0 || after < kCancelled * before ? -1.0 : after;
           }
         }
         if (lane == 0) need = some;
@@ -696,7 +706,7 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
       if (less)
         for (int c = 0; c < p.chunks; ++c) {
           if (chunk_left[c] >= 0.0) continue;  // the same for the whole workgroup: written before the barriers above
-          chunk_sums(r, sc, unit, a, c, 1, true);
+          chunk_sums(r, sc, unit, a, c, 1, n);
           __syncthreads();
         }
     }

@@ -985,3 +985,30 @@ def test_verify_decides_in_64_bits(ext, dev, V, probs, T):
                 assert got[1].tolist() == [1 + b for b in below]
             else:
                 assert got[2].tolist() == [ends[0] if b else ends[1] for b in below]
+
+
+@pytest.mark.parametrize("V", [7, 9000, 41000])
+def test_verify_little_left_without_probabilities(ext, D, dev, V):
+    """Looked-up tokens that are nearly certain, rejected one after the other: each time some e^-16 of what was there is left,
+    which one less their shares does not give. Then tokens that share the rest alike, tested on both sides of their share."""
+    g = torch.Generator().manual_seed(V)
+    up = 1.0 - 2.0 ** -24
+    lots = []
+    for B in range(24):
+        deep = 1 + B % 3
+        at = torch.randperm(V, generator=g)[:deep + 4].tolist()
+        x = torch.full((V,), -math.inf)
+        for i, a in enumerate(at):
+            x[a] = -16.0 * min(i, deep) + (0.0 if i < deep else 0.1 * (i - deep))
+        share = torch.softmax(x[at[deep:]].double(), 0)
+        first = float(share[0])
+        u = (first * 0.999, first * 1.001)[B // 3 % 2]
+        second = float(share[1]) / (1.0 - first)
+        lots.append((x, [at[0]] + at[:deep] + at[deep:deep + 2], [0.4] + [up] * deep + [u, second * (0.999, 1.001)[B // 6 % 2]]))
+    n = [len(t) for _, t, _ in lots]
+    c = {"logits": torch.cat([x.repeat(k, 1) for (x, _, _), k in zip(lots, n)]),
+         "tokens": torch.tensor([t for _, ts, _ in lots for t in ts]), "q_ptr": _ptr(n),
+         "u": torch.tensor([t for _, _, us in lots for t in us], dtype=F32),
+         "parents": torch.tensor([j for k in n for j in [-1] + [0] * (k - 1)], dtype=I32), "probs": None, "temperature": None}
+    count = _check_verify(D, c, _run_verify(ext, c, dev), least=1e-9)
+    assert set(count) == {1, 2}
