@@ -174,10 +174,12 @@ __device__ __forceinline__ f32x4 inverse(const f32x4& a, const f32x4& at, int g,
   return tt;
 }
 
-// x and y in two bf16 pieces each: hi + lo is x to 16 bits.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  hi = cvt_pk2(x, y);
-  lo = cvt_pk2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+// The bf16 pieces next to element e of x and of y, which become what those leave: three pieces are all 24 bits.
+__device__ __forceinline__ uint32_t take_piece(f32x2& x, f32x2& y, int e) {
+  const uint32_t piece = cvt_pk2(x[e], y[e]);
+  x[e] -= __uint_as_float(piece << 16);
+  y[e] -= __uint_as_float(piece & 0xffff0000u);
+  return piece;
 }
 
 // LDS reads and writes of all waves are done; global loads stay in flight.
@@ -204,9 +206,10 @@ struct TreeLeft {
 // dims; with two value dims, 2 c and 2 c + 1 of the wave's 32, for each lane): with
 //   A_ij = beta_i e^(G_i - G_j) k_i . k_j  and  P_ij = e^(G_i - G_j) q_i . k_j  for the ancestors j of i (in P also i itself),
 //   X = diag(beta) (V - diag(e^G) K S0),  U = (I + A)^-1 X,  O = scale (diag(e^G) Q S0 + P U),
-// block row after block row. S0 enters as two bf16 pieces (what it makes is rounded to bf16 in the end), everything else in
-// fp32. A product with a zero in place of a row that is no ancestor is only right for finite numbers: where a U or an O is
-// not finite (a state's two pieces have no infinity) or a decay is above 1 (true), the head goes row by row instead.
+// block row after block row. S0 enters as three bf16 pieces, all its 24 bits (two, 17 bits: 48 us in place of 50 for the 64
+// sequences below, but outputs in which key dims cancel are 2^-17 of those off), everything else in fp32. A product with a zero
+// in place of a row that is no ancestor is only right for finite numbers: where a U or an O is not finite (a state's pieces have
+// no infinity) or a decay is above 1 (true), the head goes row by row instead.
 // Loads come back in the order in which they were made, so the rows' go first: while the state is on its way the four waves
 // make the blocks of A, P and the inverses of A's diagonal ones, each once, and hand them to each other in LDS as the operands
 // that they are. LONG: the rows before s0 have left their U and TreeLeft in the workspace (a thread reads back the U that it
@@ -243,14 +246,19 @@ __device__ __forceinline__ bool tree_part(const LinTreeParams& p, TreeShared& ld
       kf[I] = *reinterpret_cast<const bf16x8*>(p.k + from);
       qf[I] = *reinterpret_cast<const bf16x8*>(p.q + from);
     }
-#pragma unroll
-  for (int I = 0; I < 4; ++I)
+  // the last block's values come behind the state's first parts: there are no registers to have both (with them spilled, 62 us
+  // for 64 sequences of 12 rows in place of 50)
+  constexpr int kEarly = DELTA && !LONG ? 3 : 4;
+  const auto load_v = [&](int I) {
     if (I < blocks)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int64_t row = at + min(I * 16 + g * 4 + r, n - 1);
         vw[I][r] = *reinterpret_cast<const uint32_t*>(p.v + (row * p.HV + h) * kHD + dv);
       }
+  };
+#pragma unroll
+  for (int I = 0; I < kEarly; ++I) load_v(I);
   asm volatile("" ::: "memory");  // the state's loads stay behind
   f32x2 st[4][8];                 // key dims 32 s + 8 g + j
   {
@@ -370,22 +378,30 @@ __device__ __forceinline__ bool tree_part(const LinTreeParams& p, TreeShared& ld
     for (int f = 0; f < 2; ++f) u[I][f] = o[I][f] = f32x4{};
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
-    uint32_t hi[2][4], lo[2][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      split2(st[s][2 * j].x, st[s][2 * j + 1].x, hi[0][j], lo[0][j]);
-      split2(st[s][2 * j].y, st[s][2 * j + 1].y, hi[1][j], lo[1][j]);
+    if (s == 2 && kEarly < 4) {
+      asm volatile("" ::: "memory");
+      load_v(3);
+      asm volatile("" ::: "memory");
     }
 #pragma unroll
-    for (int I = 0; I < 4; ++I) {
-      if (I >= blocks) break;
-      const bf16x8 ki = operand(0, I, s), qi = operand(1, I, s);
+    for (int f = 0; f < 2; ++f) {
+      bf16x8 piece[3];
 #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const bf16x8 sh = __builtin_bit_cast(bf16x8, make_uint4(hi[f][0], hi[f][1], hi[f][2], hi[f][3]));
-        const bf16x8 sl = __builtin_bit_cast(bf16x8, make_uint4(lo[f][0], lo[f][1], lo[f][2], lo[f][3]));
-        if (DELTA) u[I][f] = mfma(ki, sl, mfma(ki, sh, u[I][f]));
-        o[I][f] = mfma(qi, sl, mfma(qi, sh, o[I][f]));
+      for (int x = 0; x < 3; ++x) {
+        uint32_t at[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) at[j] = take_piece(st[s][2 * j], st[s][2 * j + 1], f);
+        piece[x] = __builtin_bit_cast(bf16x8, make_uint4(at[0], at[1], at[2], at[3]));
+      }
+#pragma unroll
+      for (int I = 0; I < 4; ++I) {
+        if (I >= blocks) break;
+        const bf16x8 ki = operand(0, I, s), qi = operand(1, I, s);
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+          if (DELTA) u[I][f] = mfma(ki, piece[x], u[I][f]);
+          o[I][f] = mfma(qi, piece[x], o[I][f]);
+        }
       }
     }
   }

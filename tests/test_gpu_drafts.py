@@ -1012,3 +1012,34 @@ def test_verify_little_left_without_probabilities(ext, D, dev, V):
          "parents": torch.tensor([j for k in n for j in [-1] + [0] * (k - 1)], dtype=I32), "probs": None, "temperature": None}
     count = _check_verify(D, c, _run_verify(ext, c, dev), least=1e-9)
     assert set(count) == {1, 2}
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("n", [1, 20, 64, 100, 300])
+def test_tree_states_in_fp32(ext, D, dev, n, delta):
+    """States enter as exactly as fp32 products take them: keys and queries that read the difference of two key dims which agree
+    to 13 bits. Every row follows the state. With the delta rule a row's query reads its own key alone, so that its output is
+    -(x - y) of its key, otherwise x - y of its query. Bound: a sum of six pieces' products, each off by two fp32 roundings of
+    the magnitudes, and the output's rounding to bf16, beside which four fp32 roundings of the output."""
+    g = torch.Generator().manual_seed(n)
+    HV = 2
+    state = torch.randn(1, HV, 128, 128, generator=g)
+    state[:, :, 1:126:3] = state[:, :, 0:126:3] * (1 + 2.0 ** -13 * torch.randn(1, HV, 42, 128, generator=g))
+    state[:, :, 2:126:3] = 0.0
+    i = torch.arange(n)
+    x = 3 * (i % 42)
+    pick = torch.zeros(n, 128)
+    pick[i, x], pick[i, x + 1] = 1.0, -1.0
+    q, k = pick.clone(), torch.zeros(n, 128)
+    if delta:
+        q, k = torch.zeros(n, 128), pick.clone()
+        q[i, x + 2] = k[i, x + 2] = 1.0
+    args = (q.bfloat16(), k.bfloat16(), torch.zeros(n, HV * 128, dtype=BF16), torch.zeros(n, HV),
+            torch.ones(n, HV, dtype=BF16) if delta else None)
+    parents, slot, ptr = torch.full((n,), -1, dtype=I32), torch.zeros(1, dtype=I32), _ptr([n])
+    o = D.linattn_tree(*args, state, [0], [0, n], parents, 1.0)[0]
+    got = ext.linattn_tree(*_put(dev, *args, state, slot, ptr, parents), scale=1.0).cpu().double().reshape(o.shape)
+    a, b = state[0][:, x].double().abs().transpose(0, 1), state[0][:, x + 1].double().abs().transpose(0, 1)
+    bound = 12 * 2.0 ** -24 * (a + b) + (2.0 ** -8 + 4 * 2.0 ** -24) * o.abs()
+    _say(f"  out {((got - o).abs() / bound).max().item():.3f} of its bound")
+    assert bool(((got - o).abs() <= bound).all())
