@@ -525,8 +525,10 @@ __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
     return;
   }
   if (n > kTree) return;  // lintree_long_k's
-  if (__syncthreads_or(tree_part<DELTA, false>(p, lds, at.first, 0, n, slot, h, hk)))
+  if (__syncthreads_or(tree_part<DELTA, false>(p, lds, at.first, 0, n, slot, h, hk))) {
+    __syncthreads();  // outputs that other waves have stored, before they are stored again
     by_rows<DELTA, true>(p, at, slot, h, hk, red, reinterpret_cast<float4(*)[32]>(lds.rows));
+  }
 }
 
 // The sequences with more rows than that, part after part; a workgroup for each that there can be, and head. (A kernel of its

@@ -1043,3 +1043,30 @@ def test_tree_states_in_fp32(ext, D, dev, n, delta):
     bound = 12 * 2.0 ** -24 * (a + b) + (2.0 ** -8 + 4 * 2.0 ** -24) * o.abs()
     _say(f"  out {((got - o).abs() / bound).max().item():.3f} of its bound")
     assert bool(((got - o).abs() <= bound).all())
+
+
+def _bits(t):
+    return _raw(t.contiguous()).cpu()
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_tree_repeats_itself(ext, dev, delta):
+    """Two calls give the same bits, NaN among them: short and long sequences, heads that go row by row after their outputs were
+    stored once, sequences whose state is not there."""
+    g = torch.Generator().manual_seed(16)
+    lengths = [70, 3, 0, 130, 64, 90, 256, 300, 12, 64]
+    N, B = sum(lengths), len(lengths)
+    q, k, v, gate, beta = _lin_case(N, 1, 3, delta, seed=16)
+    parents, ptr = _parents(lengths, "near", g), _ptr(lengths)
+    v[int(ptr[3]) + 70, 5], v[int(ptr[4]) + 1, 130] = math.inf, math.nan
+    gate[int(ptr[9]) + 2, 1], gate[int(ptr[8]), 0] = 0.5, math.nan
+    state = 0.3 * torch.randn(4, 3, 128, 128, generator=g)
+    state[3, 2, 4, 4] = math.inf
+    slot = torch.tensor([1, -1, 0, 0, 2, 7, 2, 1, 3, 3], dtype=I32)
+    d = _put(dev, q, k, v, gate, beta, state, slot, ptr, parents)
+    first = _bits(ext.linattn_tree(*d))
+    assert int((first != 0).sum()) > 0
+    for i in range(20):
+        other = torch.full((1 << 22,), i + 0.5, device=dev)      # the workspace's former contents differ from call to call
+        del other
+        assert torch.equal(_bits(ext.linattn_tree(*d)), first), i
