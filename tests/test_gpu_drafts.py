@@ -1070,3 +1070,172 @@ def test_tree_repeats_itself(ext, dev, delta):
         other = torch.full((1 << 22,), i + 0.5, device=dev)      # the workspace's former contents differ from call to call
         del other
         assert torch.equal(_bits(ext.linattn_tree(*d)), first), i
+
+
+# ------------------------------------------------- verification with launches of their own for the first rejections' sums
+def _has_walks(pkg, V):
+    """Whether calls with draft probabilities of V tokens have such launches: their workspace holds the walks then."""
+    size = pkg._lib.lib().ojx_verify_drafts_workspace
+    return size(8, 2, V, 1) > size(8, 2, V, 0)
+
+
+@pytest.mark.parametrize("kind", ["line", "near", "star", "wide"])
+@pytest.mark.parametrize("probs", ["bf16", "fp32"])
+@pytest.mark.parametrize("dtype,V,pad", [(BF16, 32761, 0), (BF16, 32762, 3), (F32, 32762, 0), (BF16, 41000, 0), (F32, 41003, 5),
+                                         (BF16, 65539, 1)])
+def test_verify_walks(ext, pkg, D, dev, dtype, V, pad, probs, kind):
+    """Vocabularies around the smallest with such launches and above, rows of any alignment, greedy sequences and empty ones
+    among others."""
+    assert _has_walks(pkg, V) == (V > 32761)
+    _say(f"case walks {V} {dtype} probs={probs} {kind}")
+    c = _verify_case([6, 0, 9, 1, 5, 12, 4], V, dtype, probs, kind, pad, seed=V + len(kind), near=1.5)
+    _say(f"  accepted {_check_verify(D, c, _run_verify(ext, c, dev))}")
+
+
+def _rejections(V, patterns, dtype, seed):
+    """Sequences in which the first pattern[0] children of row 0 are rejected, then one is accepted, the first pattern[1] of its
+    own are, and so on; behind the last ones nothing is accepted. The drafts' distributions are on the even tokens but for one in
+    a hundred, the target's on the odd ones but for one in a thousand."""
+    g = torch.Generator().manual_seed(seed)
+    n = [1 + sum(p) + len(p) - 1 for p in patterns]
+    N = sum(n)
+    raw = 2.0 * torch.randn(N, V, generator=g)
+    odd = (torch.arange(V) % 2).bool()
+
+    def half(mask, weight):
+        e = torch.exp(raw) * mask
+        return weight * e / e.sum(-1, keepdim=True)
+
+    p = half(odd, 0.999) + half(~odd, 0.001)
+    raw = 2.0 * torch.randn(N, V, generator=g)
+    q = half(~odd, 0.99) + half(odd, 0.01)
+    tokens, parents, u = [], [], []
+    for b, pattern in enumerate(patterns):
+        at, cur, j = len(tokens), 0, 1
+        tokens.append(0), parents.append(-1), u.append(0.1 + 0.8 * float(torch.rand(1, generator=g)))
+        for i, k in enumerate(pattern):
+            for r in range(k + (i + 1 < len(pattern))):
+                here = q[at + cur] * ~odd if r < k else p[at + cur] * odd
+                tokens.append(int(torch.multinomial(here, 1, generator=g)))
+                parents.append(cur)
+                # rejected: q of the even tokens is hundreds of times p; accepted: p of the odd ones hundreds of times q
+                u.append(0.9 if r < k else 0.1)
+            j += k + 1
+            cur = j - 1
+    return {"logits": torch.log(p).to(dtype), "tokens": torch.tensor(tokens), "q_ptr": _ptr(n), "u": torch.tensor(u),
+            "parents": torch.tensor(parents, dtype=I32), "probs": q, "temperature": None}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [9000, 33000, 70001])
+def test_verify_counted_rejections(ext, pkg, D, dev, V, dtype):
+    """One to dozens of rejections, accepted rows before, between and behind them, so that walks are handed on at every number
+    of rejections and taken up by the last kernel before, at and behind the last launch."""
+    assert _has_walks(pkg, V) == (V > 32761)
+    patterns = [[k] for k in range(0, 10)] + [[0, k] for k in range(0, 9)] + [[k, 0] for k in range(1, 9)]
+    patterns += [[2, 3], [5, 1], [6, 1], [7, 2], [1, 6], [3, 3], [3, 4], [1, 1, 1, 1, 1, 1], [1, 1, 1, 1, 1, 1, 1], [2, 2, 2, 0],
+                 [2, 2, 2, 1], [0, 0, 6, 0, 1], [12, 12], [30], [70], [66, 3], [1, 70, 1], [0, 0, 0, 0]]
+    c = _rejections(V, patterns, dtype, seed=V)
+    count = _check_verify(D, c, _run_verify(ext, c, dev))
+    hits = sum(x == len(p) for x, p in zip(count, patterns))
+    assert hits >= len(patterns) - 3, (hits, len(patterns))
+
+
+def test_verify_walks_temperatures(ext, pkg, D, dev):
+    assert _has_walks(pkg, 33000)
+    temps = [0.0, -1.0, math.nan, math.inf, 1e-3, 1e-40, 50.0, 1.0]
+    for kind in ("near", "star", "line"):
+        c = _verify_case([7] * 8, 33000, BF16, "fp32", kind, seed=5, temps=temps, near=3.0)
+        _check_verify(D, c, _run_verify(ext, c, dev))
+    c = _verify_case([7] * 8, 33000, F32, "bf16", "star", seed=6, temps=[0.0] * 8)       # nobody has sums to make
+    _check_verify(D, c, _run_verify(ext, c, dev))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_verify_walks_masks(ext, pkg, D, dev, dtype):
+    """test_verify_masks in a vocabulary with such launches: masked, lowest, infinite and NaN logits, probabilities that are
+    none, tokens and parents that are none."""
+    V = 33003
+    assert _has_walks(pkg, V)
+    low = torch.finfo(dtype).min
+    for seed in range(4):
+        c = _verify_case([7] * 14, V, dtype, "fp32", "near", seed=seed, temps=[1.0, 0.0, 0.8, 1.5, 1.0, 0.9, 0.0] * 2, near=3.0)
+        x, P, q = c["logits"], c["parents"], c["probs"]
+        x[0:28, 20000:] = -math.inf
+        x[7:14, ::2] = low
+        x[14:21, 50:] = low
+        x[21 + seed, :] = -math.inf
+        x[28 + seed, V - 1] = math.nan
+        x[35 + seed, 3] = math.inf
+        x[42, :] = -math.inf
+        x[49, :] = math.nan
+        x[56, :] = low
+        x[63:70] = -math.inf
+        x[63:70, V - 2] = low
+        c["tokens"][70:77] = torch.tensor([0, -1, V, 1 << 40, -(1 << 40), V - 1, 0])
+        P[77:84] = torch.tensor([5, 1, 7, -3, 0, 100, 3])
+        q[84:91, ::3], q[84:91, 1::3] = -1.0, math.nan
+        q[91:98] = 0.0
+        _check_verify(D, c, _run_verify(ext, c, dev))
+
+
+def test_verify_walks_rows_of_no_sequence(ext, pkg, D, dev):
+    assert _has_walks(pkg, 33000)
+    c = _verify_case([3, 4, 0, 8], 33000, BF16, "fp32", "star", seed=2, lead=2, spare=5, near=4.0)
+    _check_verify(D, c, _run_verify(ext, c, dev))
+    for ptr in ([9, 2, 5, 5, 12], [-4, 3, 2, 18, 19], [0, 100, 3, 5, 7], [2, 2, 2, 2, 2], [22, 22, 22, 22, 22]):
+        c["q_ptr"] = torch.tensor(ptr, dtype=I32)
+        _check_verify(D, c, _run_verify(ext, c, dev))
+
+
+def test_verify_walks_past_32_bits(ext, pkg, D, dev):
+    assert _has_walks(pkg, 33000)
+    c = _verify_case([6], 33000, BF16, "fp32", "star", seed=6, temps=[0.9], near=4.0)
+    want = _run_verify(ext, c, dev)
+    _check_verify(D, c, want)
+    ld = (1 << 29) + 17
+    d = {x: None if t is None else t.to(dev) for x, t in c.items()}
+    for name in ("logits", "probs"):
+        back = torch.empty(5 * ld + 33000, dtype=d[name].dtype, device=dev)
+        far = back.as_strided((6, 33000), (ld, 1))
+        far.copy_(d[name])
+        d[name] = far
+    got = ext.verify_drafts(d["logits"], d["tokens"], d["q_ptr"], d["u"], d["parents"], d["probs"], d["temperature"])
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu(), b)
+
+
+def test_verify_walks_in_graphs_and_on_streams(ext, pkg, D, dev):
+    """Two captured calls replayed in turn and at once on two streams, with other numbers each time, and eager work between."""
+    V = 40000
+    assert _has_walks(pkg, V)
+    lots = []
+    for seed in (1, 2):
+        c = _rejections(V, [[k, 9 - k, 2] for k in range(10)], BF16, seed)
+        d = {x: None if t is None else t.to(dev) for x, t in c.items()}
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            ext.verify_drafts(**d)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = ext.verify_drafts(**d)
+        lots.append((c, d, graph, out, side))
+    for turn in range(4):
+        for c, d, *_ in lots:
+            g = torch.Generator().manual_seed(turn)
+            c["u"] = torch.where(torch.rand(len(c["u"]), generator=g) < 0.5, c["u"], torch.rand(len(c["u"]), generator=g))
+            d["u"].copy_(c["u"])
+        torch.cuda.synchronize()
+        for c, d, graph, out, side in lots:
+            with torch.cuda.stream(side):
+                graph.replay()
+            if turn < 2:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        for c, d, graph, out, side in lots:
+            got = [t.cpu() for t in out]
+            _check_verify(D, c, got)
+            for a, b in zip(got, ext.verify_drafts(**d)):
+                assert torch.equal(a, b.cpu())
