@@ -20,9 +20,9 @@
 // The two in the middle are launched with q and more than a few chunks; otherwise draft_next_k does their work.
 //
 // What bounds it: 64 sequences of up to 12 rows of 131072 bf16 logits (71 million, 142 MB) with a draft model's probabilities
-// take 112 us. The chunks are 55 to 59 of them, the vector unit's: 20 operations a logit, where memory
-// would allow 27 us. Each launch of draft_sums_k is 4 us with nothing to do, 8 with a few sequences left and 15 with all of
-// them (50 MB); draft_rows_k 5, draft_next_k 9: latency. Few rows are latency alone: 17 us for 6 rows of 32000 in two launches.
+// take 108 to 112 us. The chunks are 55 to 60 of them, the vector unit's: 20 operations a logit, issued 80% of the time, where
+// memory would allow 27 us. Each launch of draft_sums_k is 4 us with nothing to do, 7 with a few sequences left and 14 with all
+// of them (50 MB); draft_rows_k 5, draft_next_k 9: latency. Few rows are latency alone: 17 us for 6 rows of 32000 in two launches.
 #include "ojx_internal.h"
 
 #include <algorithm>
@@ -799,7 +799,9 @@ __global__ void __launch_bounds__(1024) draft_next_k(DraftParams p) {
 int64_t draft_chunks(int64_t V) { return (V + 7 + kPiece - 1) / kPiece; }
 
 // Rejections of a sequence whose sums are launches of their own. In a line of tokens nothing follows a rejection but the next
-// token. A few chunks are summed by one workgroup sooner than by another launch; without rows there is no walk to leave.
+// token. A few chunks are summed by one workgroup sooner than by other launches: with them and without, trees of 64 x 6 rows
+// take 43 and 33 us for 2 chunks, 46 and 44 for 4, 52 and 63 for 5; of one sequence of 6, 28 and 17, 32 and 27, 30 and 22 (33 and
+// 34 for 7); lines of 64 x 6 29 and 26, 33 and 34, 35 and 38. Without rows there is no walk to leave.
 static int draft_rounds(int64_t N, int64_t B, int64_t V, bool probs, bool tree) {
   return !probs || N == 0 || B == 0 || draft_chunks(V) <= 4 ? 0 : tree ? kDraftRounds : 1;
 }

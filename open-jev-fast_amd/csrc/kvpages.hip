@@ -1,8 +1,10 @@
 // What becomes of a paged cache around drafted tokens: accepted rows moved together, pages taken, given back, shared and
 // copied. A table row names a sequence's pages, refs counts the table entries that name each page; a page with none is free.
 //
-// All of it is whole numbers and copies. Tables and counts are small: what bounds them is the chain of launches and loads (4.6
-// and 6.0 us for a resize and a fork in one launch each).
+// All of it is whole numbers and copies. Tables and counts are small: what bounds them is the chain of launches and loads. For 64
+// sequences of 16 entries a resize that gives each a page and one that takes it back are 7.7 us, one that changes nothing 3.3, a
+// fork of every other sequence 6.6, in one launch each. Where free pages are rare the scan for them counts: 256 sequences of
+// 2048 entries get a page each from the 300 free ones of 389000, and give it back, in 155 us.
 #include "ojx_internal.h"
 
 #include <algorithm>
@@ -110,6 +112,8 @@ __device__ __forceinline__ int block_before(int x, int* red, int& all) {
 // A call has three parts: what sequences give back (and what they want), the free pages that are taken, where they go. With
 // large tables each is a launch, the first and the last with a workgroup per sequence. A table of up to kSmall entries is one
 // workgroup's, an entry a thread at a time, in one launch.
+// In one launch and in three, the two resizes above take 7.7 and 17 us for 64 x 16 entries, 15.9 and 17.1 for 64 x 64, 29 and 18
+// for 128 x 64; forks 6.6 and 10.2, 11.5 and 10.8, 19.6 and 10.9.
 constexpr int kSmall = 4096;
 
 // Pages behind what a sequence wants are given back; what it lacks is counted.

@@ -496,9 +496,10 @@ __device__ __forceinline__ bool tree_part(const LinTreeParams& p, TreeShared& ld
 }
 
 // A workgroup per sequence and value head. What bounds it: the states, read once. 64 sequences of 12 rows and 48 heads, 216 MB,
-// take 45 us: 4.8 TB/s, where a copy reaches 5.1 and a stream that is only read 5.8. (Two workgroups a CU: 50 us; the rows' loads
-// behind the state's, three workgroups: 57; row by row: 134.) Few sequences of 64 rows are bound by their chain, loads, the
-// inverses, K S0, four blocks in turn: 8 of them 21 us (row by row 356), one 14; one of 8 rows 7.5 us.
+// take 48 us: 4.5 TB/s, where a copy reaches 5.1 and a stream that is only read 5.8. (With states in two pieces 45 us; then two
+// workgroups a CU: 50; the rows' loads behind the state's, three workgroups: 57; row by row: 134.) Few sequences of 64 rows are
+// bound by their chain, loads, the inverses, K S0, four blocks in turn: 8 of them 25 us (row by row 356), one 15.6; one of 8 rows
+// 8.1 us.
 template <bool DELTA>
 __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
   __shared__ __attribute__((aligned(16))) TreeShared lds;
@@ -533,8 +534,8 @@ __global__ void __launch_bounds__(256, 3) lintree_k(LinTreeParams p) {
 
 // The sequences with more rows than that, part after part; a workgroup for each that there can be, and head. (A kernel of its
 // own: in one with the other form, the registers that this one wants cost that one 6 to 110% more time, as it was put; its
-// launch costs 2.3 us where no sequence is so long.) One sequence of 65 rows takes 28 us, of 128 rows 52; row by row 313 and
-// 1098.
+// launch costs 2.3 to 4.6 us where no sequence is so long.) One sequence of 65 rows takes 30 us, of 128 rows 55; row by row 313
+// and 1098.
 template <bool DELTA>
 __global__ void __launch_bounds__(256, 2) lintree_long_k(LinTreeParams p) {
   __shared__ __attribute__((aligned(16))) TreeShared lds;
