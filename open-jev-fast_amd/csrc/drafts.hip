@@ -404,8 +404,8 @@ __global__ void __launch_bounds__(256) draft_rows_k(DraftParams p) {
 // Where the walk over a sequence's rows stands.
 using Walk = DraftWalk;
 
-// Without q what is left after a rejection is one less that token's share, until fewer than three of its digits are: then it is
-// summed, should another token be tested (a = 1: it has to be).
+// Without q what is left is one less the rejected tokens' shares, as long as that is more than this; where more digits than three
+// have cancelled it is summed, should another token be tested (a = 1: it has to be).
 constexpr double kCancelled = 1e-3;
 
 // On to the next rejection with q or test with a sum that has to be made (true: what is left has to be summed before the walk
